@@ -8,7 +8,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libdfine_hip.so")
 ARCH = "gfx950"
 COMMON = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
-          "-Wno-pass-failed"]
+          "-Wno-pass-failed",
+          # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms give wrong results now and then
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file flags: the gather's f32 atomics must lower to global_atomic_add_f32; the assignment
 # kernel's float64 arithmetic must not be contracted into FMAs (bit-exact vs SciPy)
 SOURCES = {
