@@ -1,0 +1,937 @@
+// A2 / A6 - differential attention of the token streams, forward and backward.
+//
+// Next to the softmax attention of attn.hip (src/d_fine/arch/hybrid_encoder.py:243-290, src/d_fine/arch/dfine_decoder.py:200,233-255): every head
+// has two query and two key vectors per token, and reads its values through the DIFFERENCE of two softmax maps,
+//   A_t = softmax(scale q_t k_t^T + mask), t = 0, 1 (a row that sees no key: 0),   U = A_0 V - l_h A_1 V,
+//   l_h = exp(x0 . x1) - exp(x2 . x3) + init (the head's learned vectors),          Y = (1 - init) norm(U) g   (or Y = U without a norm weight),
+// norm(U) = U r, r = rsqrt(mean U^2 + eps) over the head's dv channels.  Backward, with D_t = dU . (A_t V):
+//   dU = (1 - init) r (g dY - U r^2 mean(U g dY)), dP = dU V^T, dS_0 = A_0 (dP - D_0), dS_1 = -l A_1 (dP - D_1),
+//   dq_t = scale dS_t k_t, dk_t = scale dS_t^T q_t, dV = (A_0 - l A_1)^T dU, dl = - sum D_1, dx0 = dl exp(x0 . x1) x1 and its like.
+//
+// Rows.  The G = H / Hk query heads of a shared key head read the same keys: their rows (query i, head g) form one list r = i G + g, and a wave takes 32
+// rows of it.  One token of G heads therefore fills G columns of one matrix tile, and the gradients of a shared key head add up in registers.
+// Products (32 x 32 matrix instructions).  Forward and dQ: S^T = K Q^T puts ONE row of the list (a lane's column) against 16 keys per lane and tile in the
+// order 8 a + 4 h + b (h = lane / 32, a and b the register), which is the order the transposed read of V delivers the second product's other operand in, so
+// the probabilities go from registers to the matrix unit as they are.  dK and dV: S = Q K^T, one KEY per lane, the same way with dU and Q transposed.
+// LDS tiles hold rows of 16-byte units, unit u of row r at u ^ f(r) (da_swz): 8 lanes with one u and consecutive rows, and the 4 rows x 2 units of a
+// transposed read, fall on different banks without padding.
+// Types: bf16 (v_mfma_f32_32x32x16_bf16; probabilities and dS are rounded to bf16 for the second products, as the values they meet are) and fp32
+// (v_mfma_f32_32x32x2_f32).  Scores, softmax statistics, sums and norms are 32-bit.  Head dims up to 64 with values up to 128, multiples of 8, run on the
+// next of three sizes with zero-filled tiles.
+#include "common.h"
+
+namespace dfine {
+
+typedef __attribute__((ext_vector_type(16))) float da_f16v;
+typedef __attribute__((ext_vector_type(8))) __bf16 da_bf16x8;
+typedef short da_tr4 __attribute__((ext_vector_type(4)));
+typedef short da_tr8 __attribute__((ext_vector_type(8)));
+
+constexpr int kDaThreads = 256;
+
+struct DiffArgs {
+    const void *q, *k, *v;                      // [B, N, H, 2, d], [B, M, Hk, 2, d], [B, M, Hk, dv]
+    const void *lam, *weight;                   // [4, H or 1, d], [dv] or null
+    const uint64_t *rowbits, *colbits, *live;   // mask forms (1 = may attend): [Bm][N][M64], [Bm][M][N64], [Bm][M64]; null: no mask
+    const uint8_t *tiles;                       // [Bm][N64][M64] 0 free, 1 mixed, 2 blocked
+    const int *kvlen, *qstart_dev;              // [B] or null
+    void *out, *u, *o2;                         // [B, N, H, dv]; u, o2 (null: not kept) are read by the backward pass
+    float *stats;                               // [3][B, H, N]: lse of the two maps in the exp2 domain (+inf: an empty row), r
+    int64_t qs[4], ks[4], vs[3];                // strides (batch, token, head, map)
+    int64_t mask_b;                             // 0: one mask for the batch
+    int64_t qstart;
+    int B, N, M, H, Hk, G, d, dv, causal, lam_heads, lam_bf16, w_bf16;
+    float scale, scale_log2e, init, post, eps;  // post = 1 - init with a norm weight
+    // backward
+    const void *dy;
+    int64_t dys[3];
+    void *du, *dq, *dk, *dvv;
+    float *delta, *lpart, *wpart;               // [2][B, H, N]; per workgroup of the first kernel: sum of D_1, sums of dg
+};
+
+template <typename T> struct Da;
+template <> struct Da<uint16_t> {
+    static constexpr int KPF = 16;              // contraction length of one fragment (16 bytes per lane)
+    static __device__ __forceinline__ da_f16v mma(uint4 a, uint4 b, da_f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(da_bf16x8, a), __builtin_bit_cast(da_bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Da<float> {
+    static constexpr int KPF = 8;
+    static __device__ __forceinline__ da_f16v mma(uint4 a, uint4 b, da_f16v c) {
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+    }
+};
+
+// sizes of one instantiation: DK channels per map, 2 DK value channels
+template <typename T, int DK> struct DaCfg {
+    static constexpr int ES = sizeof(T), DV = 2 * DK, ROWB = 2 * DK * ES, U = ROWB / 16, NF = DK / Da<T>::KPF, NFV = DV / Da<T>::KPF, MT = DV / 32 ? DV / 32 : 1,
+                         MTK = DK / 32 ? DK / 32 : 1, FPT = 32 / Da<T>::KPF;      // fragments per 32 keys
+    static_assert(DV % 32 == 0, "a value tile is 32 channels");
+};
+
+template <int U> __device__ __forceinline__ int da_swz(int row) { return U >= 16 ? (row & 7) << 1 : U == 8 ? ((row >> 1) & 3) << 1 : ((row >> 2) & 1) << 1; }
+
+// one lane's 16 bytes of a row-major operand: row `row`, fragment f (channels f KPF ..), starting at unit u0 of the row
+template <int U> __device__ __forceinline__ uint4 da_frag(const char *tile, int row, int u) {
+    return *reinterpret_cast<const uint4 *>(tile + row * U * 16 + ((u ^ da_swz<U>(row)) << 4));
+}
+
+// transposed operand: contraction over the tile's rows r0 .. r0 + KPF - 1 in the order 8 a + 4 h + b, this lane's column c0 + lane % 32
+template <typename T, int U> __device__ __forceinline__ uint4 da_frag_tr(const char *tile, int r0, int c0, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        const int i16 = lane & 15, row = r0 + 4 * h + (i16 >> 2), u = (c0 >> 3) + ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1);
+        const char *p = tile + row * U * 16 + ((u ^ da_swz<U>(row)) << 4) + 8 * (i16 & 1);
+        const da_tr4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_tr4 __attribute__((address_space(3))) *)p);
+        const da_tr4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_tr4 __attribute__((address_space(3))) *)(p + 8 * U * 16));
+        return __builtin_bit_cast(uint4, (da_tr8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+        const int col = c0 + (lane & 31), u = col >> 2;
+        uint32_t r[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int row = r0 + 4 * h + b;
+            r[b] = *reinterpret_cast<const uint32_t *>(tile + row * U * 16 + ((u ^ da_swz<U>(row)) << 4) + (col & 3) * 4);
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
+    }
+}
+
+// Two floats to bf16 as a conversion the compiler sees (common.h's pack_bf16x2 is inline assembly): it has to put two wait states between the
+// conversion and a matrix instruction that reads it, which it does not do behind assembly.
+typedef __attribute__((ext_vector_type(2))) float da_f2;
+typedef __attribute__((ext_vector_type(2))) __bf16 da_bf2;
+__device__ __forceinline__ uint32_t da_pk(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((da_f2){a, b}, da_bf2)); }
+
+// fragment f of 32 values per lane pair (accumulator order) as a matrix operand
+template <typename T> __device__ __forceinline__ uint4 da_pack(const da_f16v &p, int f) {
+    if constexpr (sizeof(T) == 2)
+        return make_uint4(da_pk(p[8 * f], p[8 * f + 1]), da_pk(p[8 * f + 2], p[8 * f + 3]), da_pk(p[8 * f + 4], p[8 * f + 5]),
+                          da_pk(p[8 * f + 6], p[8 * f + 7]));
+    else
+        return make_uint4(__float_as_uint(p[4 * f]), __float_as_uint(p[4 * f + 1]), __float_as_uint(p[4 * f + 2]), __float_as_uint(p[4 * f + 3]));
+}
+
+__device__ __forceinline__ float da_exp2(float x) { return __builtin_amdgcn_exp2f(x); }     // arguments <= 0 or -inf: no range handling needed
+__device__ __forceinline__ float da_load1(const void *p, int64_t i, int bf16) {
+    return bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i]) : reinterpret_cast<const float *>(p)[i];
+}
+template <typename T> __device__ __forceinline__ void da_store4(T *p, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+    else *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d);
+}
+template <typename T> __device__ __forceinline__ void da_load4(const T *p, float *f) {
+    if constexpr (sizeof(T) == 2) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(p);
+        f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
+        f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
+    } else {
+        const float4 u = *reinterpret_cast<const float4 *>(p);
+        f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+    }
+}
+
+// exp(x0 . x1) and exp(x2 . x3) of a head
+__device__ __forceinline__ void da_lambda_parts(const DiffArgs &a, int h, float &e1, float &e2) {
+    const int64_t hh = a.lam_heads == 1 ? 0 : h, st = (int64_t)a.lam_heads * a.d;
+    float s1 = 0.f, s2 = 0.f;
+    for (int j = 0; j < a.d; ++j) {
+        const int64_t o = hh * a.d + j;
+        s1 += da_load1(a.lam, o, a.lam_bf16) * da_load1(a.lam, st + o, a.lam_bf16);
+        s2 += da_load1(a.lam, 2 * st + o, a.lam_bf16) * da_load1(a.lam, 3 * st + o, a.lam_bf16);
+    }
+    e1 = expf(s1); e2 = expf(s2);
+}
+
+// keys that row i of batch b may look at end here
+__device__ __forceinline__ int da_limit(const DiffArgs &a, int len, int64_t start, int i) {
+    if (!a.causal) return len;
+    const int64_t e = start + i + 1;
+    return e < 0 ? 0 : e < len ? (int)e : len;
+}
+__device__ __forceinline__ int da_len(const DiffArgs &a, int b) { return a.kvlen ? min(max(a.kvlen[b], 0), a.M) : a.M; }
+__device__ __forceinline__ int64_t da_start(const DiffArgs &a, int b) { return a.qstart_dev ? (int64_t)a.qstart_dev[b] : a.qstart; }
+
+// global -> LDS, `rows` rows of 2 DK channels: k-like (two maps of d channels) or v-like (dv channels); dead rows and channels become zeros
+template <typename T, int DK>
+__device__ __forceinline__ void da_stage(char *dst, const T *src, int64_t ld, int64_t map, int nch, bool maps, int rows, int valid, uint64_t live, int tid) {
+    using C = DaCfg<T, DK>;
+    constexpr int CH = 16 / C::ES;                           // channels per unit
+    for (int it = tid; it < rows * C::U; it += kDaThreads) {
+        const int r = it / C::U, u = it % C::U;
+        const int t = maps ? u / (C::U / 2) : 0, c = (maps ? u % (C::U / 2) : u) * CH;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < valid && ((live >> r) & 1) && c < nch) x = *reinterpret_cast<const uint4 *>(src + (int64_t)r * ld + t * map + c);
+        *reinterpret_cast<uint4 *>(dst + r * C::U * 16 + ((u ^ da_swz<C::U>(r)) << 4)) = x;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// forward: workgroup = (batch, key head, 128 rows), a wave owns 32 rows; 64 keys at a time
+template <typename T, int DK>
+__global__ __launch_bounds__(kDaThreads) void diff_attn_fwd_kernel(const DiffArgs a) {
+    using C = DaCfg<T, DK>;
+    constexpr int KB = 64, NT = KB / 32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char *sK = lds, *sV = lds + KB * C::ROWB;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h2 = lane >> 5, l32 = lane & 31;
+    const int bh = blockIdx.x % (a.B * a.Hk), blk = blockIdx.x / (a.B * a.Hk), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int64_t R = (int64_t)a.N * a.G;
+    const int64_t row = (int64_t)blk * 128 + wave * 32 + l32;
+    const bool rlive = row < R;
+    const int i = rlive ? (int)(row / a.G) : 0, g = rlive ? (int)(row - (int64_t)i * a.G) : 0, head = hk * a.G + g;
+    const int len = da_len(a, b);
+    const int64_t start = da_start(a, b);
+    const int limit = rlive ? da_limit(a, len, start, i) : 0;
+    const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
+    // queries of this wave / workgroup: the rows' range in i
+    const int64_t w0 = (int64_t)blk * 128 + wave * 32, wl = min(w0 + 31, R - 1);
+    const bool wlive = w0 < R;
+    const int i_lo = wlive ? (int)(w0 / a.G) : 0, i_hi = wlive ? (int)(wl / a.G) : 0;
+    const int blk_hi = (int)(min((int64_t)blk * 128 + 127, R - 1) / a.G);
+    const int wg_end = da_limit(a, len, start, blk_hi);
+
+    uint4 qf[2][C::NF];
+    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.qs[0] + i * a.qs[1] + head * a.qs[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int f = 0; f < C::NF; ++f) {
+            const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
+            qf[t][f] = rlive && c < a.d ? *reinterpret_cast<const uint4 *>(qp + t * a.qs[3] + c) : make_uint4(0, 0, 0, 0);
+        }
+    da_f16v o[2][C::MT];
+    float m[2], l[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        m[t] = -INFINITY; l[t] = 0.f;
+#pragma unroll
+        for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[t][x][r] = 0.f;
+    }
+    const T *kp = reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2];
+    const T *vp = reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2];
+    const int64_t mb = a.mask_b ? b : 0;
+
+    for (int k0 = 0; k0 < wg_end; k0 += KB) {
+        const int kt = k0 >> 6;
+        const uint64_t live = a.live ? a.live[mb * M64 + kt] : ~0ull;
+        __syncthreads();
+        da_stage<T, DK>(sK, kp + (int64_t)k0 * a.ks[1], a.ks[1], a.ks[3], a.d, true, KB, min(KB, len - k0), live, tid);
+        da_stage<T, DK>(sV, vp + (int64_t)k0 * a.vs[1], a.vs[1], 0, a.dv, false, KB, min(KB, len - k0), live, tid);
+        __syncthreads();
+        // this wave's tile: nothing visible / everything visible / some
+        if (!wlive) continue;
+        int code = 0;
+        if (a.tiles) {
+            const uint8_t *tp = a.tiles + mb * N64 * M64 + kt;
+            const int c0 = tp[(int64_t)(i_lo >> 6) * M64], c1 = tp[(int64_t)(i_hi >> 6) * M64];
+            code = c0 == c1 ? c0 : 1;
+        }
+        if (code == 2 || k0 >= da_limit(a, len, start, i_hi)) continue;
+        const bool cut = k0 + KB > da_limit(a, len, start, i_lo) || !wlive || wl - w0 < 31;
+        uint64_t vis = ~0ull;
+        if (code == 1 && rlive) vis = a.rowbits[(mb * a.N + i) * M64 + kt];
+        if (cut) vis &= limit <= k0 ? 0ull : limit >= k0 + 64 ? ~0ull : (1ull << (limit - k0)) - 1;
+        const bool masked = cut || code == 1;
+
+        uint4 pf[2][NT][C::FPT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            da_f16v s[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[nt][r] = 0.f;
+#pragma unroll
+                for (int f = 0; f < C::NF; ++f) s[nt] = Da<T>::mma(da_frag<C::U>(sK, nt * 32 + l32, t * (C::U / 2) + 2 * f + h2), qf[t][f], s[nt]);
+            }
+            if (masked) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!((vis >> (nt * 32 + 8 * (r >> 2) + 4 * h2 + (r & 3))) & 1)) s[nt][r] = -INFINITY;
+            }
+            float bm = -INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) bm = fmaxf(bm, s[nt][r]);
+            bm = fmaxf(bm, __shfl_xor(bm, 32));
+            const float mn = fmaxf(m[t], bm), mu = mn == -INFINITY ? 0.f : mn * a.scale_log2e;
+            const float alpha = da_exp2(fmaf(m[t], a.scale_log2e, -mu));
+            m[t] = mn;
+            float sum = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[nt][r] = da_exp2(fmaf(s[nt][r], a.scale_log2e, -mu));
+                    sum += s[nt][r];
+                }
+#pragma unroll
+                for (int f = 0; f < C::FPT; ++f) pf[t][nt][f] = da_pack<T>(s[nt], f);
+            }
+            l[t] = l[t] * alpha + sum;                       // this lane's half of the keys; the halves meet at the end
+#pragma unroll
+            for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[t][x][r] *= alpha;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int f = 0; f < C::FPT; ++f)
+#pragma unroll
+                for (int x = 0; x < C::MT; ++x) {
+                    const uint4 vf = da_frag_tr<T, C::U>(sV, nt * 32 + f * Da<T>::KPF, x * 32, lane);
+                    o[0][x] = Da<T>::mma(vf, pf[0][nt][f], o[0][x]);
+                    o[1][x] = Da<T>::mma(vf, pf[1][nt][f], o[1][x]);
+                }
+    }
+    if (!rlive) return;                                      // (both lanes of a row go together)
+    float e1, e2;
+    da_lambda_parts(a, head, e1, e2);
+    const float lam = e1 - e2 + a.init;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) l[t] += __shfl_xor(l[t], 32);
+    const float inv0 = l[0] > 0.f ? 1.f / l[0] : l[0], inv1 = l[1] > 0.f ? 1.f / l[1] : l[1];       // (a sum that is not a number stays one)
+    float ss = 0.f;
+#pragma unroll
+    for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            o[1][x][r] *= inv1;
+            o[0][x][r] = o[0][x][r] * inv0 - lam * o[1][x][r];
+            ss += o[0][x][r] * o[0][x][r];
+        }
+    ss += __shfl_xor(ss, 32);
+    const float rn = a.weight ? rsqrtf(ss / (float)a.dv + a.eps) : 1.f;
+    const int64_t orow = (((int64_t)b * a.N + i) * a.H + head) * a.dv;
+#pragma unroll
+    for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const int c = x * 32 + 8 * q4 + 4 * h2;
+            if (c >= a.dv) continue;
+            float w[4] = {1.f, 1.f, 1.f, 1.f};
+            if (a.weight)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = da_load1(a.weight, c + j, a.w_bf16) * a.post * rn;
+            const float u0 = o[0][x][4 * q4], u1 = o[0][x][4 * q4 + 1], u2 = o[0][x][4 * q4 + 2], u3 = o[0][x][4 * q4 + 3];
+            da_store4(reinterpret_cast<T *>(a.out) + orow + c, u0 * w[0], u1 * w[1], u2 * w[2], u3 * w[3]);
+            if (a.u) {
+                if (a.weight) da_store4(reinterpret_cast<T *>(a.u) + orow + c, u0, u1, u2, u3);
+                da_store4(reinterpret_cast<T *>(a.o2) + orow + c, o[1][x][4 * q4], o[1][x][4 * q4 + 1], o[1][x][4 * q4 + 2], o[1][x][4 * q4 + 3]);
+            }
+        }
+    if (a.stats && h2 == 0) {
+        const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + head) * a.N + i;
+        a.stats[at] = l[0] > 0.f ? m[0] * a.scale_log2e + log2f(l[0]) : l[0] == 0.f ? INFINITY : l[0];
+        a.stats[bhn + at] = l[1] > 0.f ? m[1] * a.scale_log2e + log2f(l[1]) : l[1] == 0.f ? INFINITY : l[1];
+        a.stats[2 * bhn + at] = rn;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// mask [Bm][N][M] bytes (strides mb, mn; non-zero = blocked) -> the forms the kernels read.  Workgroup = (batch, 64 keys), all queries: a wave takes every
+// fourth tile of 64 queries; lane = key, one ballot per query
+__global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sn, int N, int M, uint64_t *__restrict__ rowbits,
+                                                             uint64_t *__restrict__ colbits, uint64_t *__restrict__ live, uint8_t *__restrict__ tiles) {
+    const int M64 = (M + 63) >> 6, N64 = (N + 63) >> 6;
+    const int kt = blockIdx.x % M64;
+    const int64_t b = blockIdx.x / M64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, key = kt * 64 + lane;
+    const uint64_t inside = M - kt * 64 >= 64 ? ~0ull : (1ull << (M - kt * 64)) - 1;
+    __shared__ uint64_t any_s[4];
+    uint64_t any = 0;
+    for (int nt = wave; nt < N64; nt += 4) {
+        uint64_t col = 0, all = inside, some = 0, mine = 0;
+        const int n1 = min(64, N - nt * 64);
+        for (int n = 0; n < n1; ++n) {
+            const bool see = key < M && mask[b * sb + (int64_t)(nt * 64 + n) * sn + key] == 0;
+            const uint64_t bits = __ballot(see);
+            if (see) col |= 1ull << n;
+            if (n == lane) mine = bits;
+            all &= bits;
+            some |= bits;
+        }
+        if (lane < n1) rowbits[(b * N + nt * 64 + lane) * M64 + kt] = mine;
+        if (key < M) colbits[(b * M + key) * N64 + nt] = col;
+        if (lane == 0) tiles[(b * N64 + nt) * M64 + kt] = some == 0 ? 2 : all == inside ? 0 : 1;
+        any |= some;
+    }
+    if (lane == 0) any_s[wave] = any;
+    __syncthreads();
+    if (threadIdx.x == 0) live[b * M64 + kt] = any_s[0] | any_s[1] | any_s[2] | any_s[3];
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// backward, first: dU (rounded to the type it is multiplied in), D_0, D_1 of every row and the partial sums of dl and dg.  Workgroup = (head, run of
+// (batch, query) rows); LPR lanes of 4 channels each per row
+template <typename T>
+__global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, int nrun) {
+    const int head = blockIdx.x % a.H, run = blockIdx.x / a.H;
+    const int lane = threadIdx.x & 31, rr = threadIdx.x >> 5;                       // 32 lanes x 4 channels cover dv <= 128
+    const int c = lane * 4;
+    const bool ok = c < a.dv;
+    float e1, e2;
+    da_lambda_parts(a, head, e1, e2);
+    const float lam = e1 - e2 + a.init;
+    float w[4], dw[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = !ok ? 0.f : a.weight ? a.post * da_load1(a.weight, c + j, a.w_bf16) : 1.f;
+    const int64_t rows = (int64_t)a.B * a.N, bhn = rows * a.H;
+    for (int64_t r = (int64_t)run * 8 + rr; r < rows; r += (int64_t)nrun * 8) {
+        const int b = (int)(r / a.N), i = (int)(r - (int64_t)b * a.N);
+        const int64_t at = ((int64_t)b * a.H + head) * a.N + i, orow = (r * a.H + head) * a.dv + c;
+        float dy[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f}, o2[4] = {0.f, 0.f, 0.f, 0.f};
+        if (ok) {
+            da_load4(reinterpret_cast<const T *>(a.dy) + b * a.dys[0] + i * a.dys[1] + head * a.dys[2] + c, dy);
+            da_load4(reinterpret_cast<const T *>(a.weight ? a.u : a.out) + orow, u);
+            da_load4(reinterpret_cast<const T *>(a.o2) + orow, o2);
+        }
+        const bool empty = a.stats[at] == INFINITY;                                            // sees no key: no gradient, whatever dY holds
+        const float rn = a.weight ? a.stats[2 * bhn + at] : 1.f;
+        float dot = 0.f, du[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dot += u[j] * w[j] * dy[j];
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) dot += __shfl_xor(dot, x);
+        dot *= rn * rn / (float)a.dv;
+        float d0 = 0.f, d1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (a.weight) {
+                du[j] = rn * (w[j] * dy[j] - u[j] * dot);
+                if (!empty) dw[j] += a.post * rn * u[j] * dy[j];
+            } else {
+                du[j] = dy[j];
+            }
+            if (empty) du[j] = 0.f;
+            d0 += du[j] * (u[j] + lam * o2[j]);
+            d1 += du[j] * o2[j];
+        }
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) { d0 += __shfl_xor(d0, x); d1 += __shfl_xor(d1, x); }
+        if (empty) d0 = d1 = 0.f;
+        if (ok) da_store4(reinterpret_cast<T *>(a.du) + orow, du[0], du[1], du[2], du[3]);
+        if (lane == 0) {
+            a.delta[at] = d0;
+            a.delta[bhn + at] = d1;
+        }
+        dsum += d1;
+    }
+    __shared__ float sw[8][128], sd[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sw[rr][c + j] = dw[j];
+    if (lane == 0) sd[rr] = dsum;
+    __syncthreads();
+    if (threadIdx.x < a.dv && a.weight) {
+        float v = 0.f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v += sw[x][threadIdx.x];
+        a.wpart[(int64_t)blockIdx.x * a.dv + threadIdx.x] = v;
+    }
+    if (threadIdx.x == 0) {
+        float v = 0.f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v += sd[x];
+        a.lpart[blockIdx.x] = v;
+    }
+}
+
+// gradients of the learned vectors and of the norm weight from the first kernel's partial sums (one workgroup per head / per 16 channels; in order)
+__global__ __launch_bounds__(256) void diff_attn_param_kernel(const DiffArgs a, int nrun, void *dlam, void *dw) {
+    const int tid = threadIdx.x;
+    __shared__ float s[16][17];
+    __shared__ float dl_s[256];
+    const int nh = a.lam_heads == 1 ? 1 : a.H;
+    if ((int)blockIdx.x < nh) {
+        if (!dlam) return;
+        // sum over runs (and over all heads where they share the vectors; their exponentials are then one pair)
+        float v = 0.f;
+        const int h0 = a.lam_heads == 1 ? 0 : blockIdx.x, h1 = a.lam_heads == 1 ? a.H : h0 + 1;
+        for (int x = tid; x < nrun * (h1 - h0); x += 256) v += a.lpart[(x / (h1 - h0)) * a.H + h0 + x % (h1 - h0)];
+        dl_s[tid] = v;
+        __syncthreads();
+        for (int x = 128; x > 0; x >>= 1) {
+            if (tid < x) dl_s[tid] += dl_s[tid + x];
+            __syncthreads();
+        }
+        const float dl = -dl_s[0];
+        float e1, e2;
+        da_lambda_parts(a, h0, e1, e2);
+        const int64_t st = (int64_t)a.lam_heads * a.d, o = (a.lam_heads == 1 ? 0 : (int64_t)h0 * a.d);
+        for (int x = tid; x < 4 * a.d; x += 256) {
+            const int vec = x / a.d, j = x - vec * a.d;
+            const float other = da_load1(a.lam, (vec ^ 1) * st + o + j, a.lam_bf16), gr = dl * (vec < 2 ? e1 : -e2) * other;
+            if (a.lam_bf16) reinterpret_cast<uint16_t *>(dlam)[vec * st + o + j] = f32_to_bf16(gr);
+            else reinterpret_cast<float *>(dlam)[vec * st + o + j] = gr;
+        }
+        return;
+    }
+    if (!dw) return;
+    const int col = tid & 15, r0 = tid >> 4, ch = (blockIdx.x - nh) * 16 + col, rows = nrun * a.H;
+    float v = 0.f;
+    if (ch < a.dv)
+        for (int r = r0; r < rows; r += 16) v += a.wpart[(int64_t)r * a.dv + ch];
+    s[r0][col] = v;
+    __syncthreads();
+    if (r0 || ch >= a.dv) return;
+#pragma unroll
+    for (int r = 1; r < 16; ++r) v += s[r][col];
+    if (a.w_bf16) reinterpret_cast<uint16_t *>(dw)[ch] = f32_to_bf16(v);
+    else reinterpret_cast<float *>(dw)[ch] = v;
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// backward, dQ: the forward's decomposition; probabilities from the saved statistics
+template <typename T, int DK>
+__global__ __launch_bounds__(kDaThreads) void diff_attn_dq_kernel(const DiffArgs a) {
+    using C = DaCfg<T, DK>;
+    constexpr int KB = 64, NT = KB / 32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char *sK = lds, *sV = lds + KB * C::ROWB;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h2 = lane >> 5, l32 = lane & 31;
+    const int bh = blockIdx.x % (a.B * a.Hk), blk = blockIdx.x / (a.B * a.Hk), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int64_t R = (int64_t)a.N * a.G;
+    const int64_t row = (int64_t)blk * 128 + wave * 32 + l32;
+    const bool rlive = row < R;
+    const int i = rlive ? (int)(row / a.G) : 0, g = rlive ? (int)(row - (int64_t)i * a.G) : 0, head = hk * a.G + g;
+    const int len = da_len(a, b);
+    const int64_t start = da_start(a, b);
+    const int limit = rlive ? da_limit(a, len, start, i) : 0;
+    const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
+    const int64_t w0 = (int64_t)blk * 128 + wave * 32, wl = min(w0 + 31, R - 1);
+    const bool wlive = w0 < R;
+    const int i_lo = wlive ? (int)(w0 / a.G) : 0, i_hi = wlive ? (int)(wl / a.G) : 0;
+    const int wg_end = da_limit(a, len, start, (int)(min((int64_t)blk * 128 + 127, R - 1) / a.G));
+
+    float e1, e2;
+    da_lambda_parts(a, head, e1, e2);
+    const float lam = e1 - e2 + a.init;
+    const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + head) * a.N + i;
+    uint4 qf[2][C::NF], uf[C::NFV];
+    float lse[2], dl[2];
+    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.qs[0] + i * a.qs[1] + head * a.qs[2];
+    const T *up = reinterpret_cast<const T *>(a.du) + (((int64_t)b * a.N + i) * a.H + head) * a.dv;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        lse[t] = rlive ? a.stats[t * bhn + at] : INFINITY;
+        dl[t] = rlive ? a.delta[t * bhn + at] : 0.f;
+    }
+    const bool empty = lse[0] == INFINITY;                   // sees no key: its query may hold anything
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int f = 0; f < C::NF; ++f) {
+            const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
+            qf[t][f] = rlive && !empty && c < a.d ? *reinterpret_cast<const uint4 *>(qp + t * a.qs[3] + c) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+    for (int f = 0; f < C::NFV; ++f) {
+        const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
+        uf[f] = rlive && c < a.dv ? *reinterpret_cast<const uint4 *>(up + c) : make_uint4(0, 0, 0, 0);
+    }
+    da_f16v dq[2][C::MTK];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < C::MTK; ++x)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dq[t][x][r] = 0.f;
+    const T *kp = reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2];
+    const T *vp = reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2];
+    const int64_t mb = a.mask_b ? b : 0;
+
+    for (int k0 = 0; k0 < wg_end; k0 += KB) {
+        const int kt = k0 >> 6;
+        const uint64_t live = a.live ? a.live[mb * M64 + kt] : ~0ull;
+        __syncthreads();
+        da_stage<T, DK>(sK, kp + (int64_t)k0 * a.ks[1], a.ks[1], a.ks[3], a.d, true, KB, min(KB, len - k0), live, tid);
+        da_stage<T, DK>(sV, vp + (int64_t)k0 * a.vs[1], a.vs[1], 0, a.dv, false, KB, min(KB, len - k0), live, tid);
+        __syncthreads();
+        if (!wlive) continue;
+        int code = 0;
+        if (a.tiles) {
+            const uint8_t *tp = a.tiles + mb * N64 * M64 + kt;
+            const int c0 = tp[(int64_t)(i_lo >> 6) * M64], c1 = tp[(int64_t)(i_hi >> 6) * M64];
+            code = c0 == c1 ? c0 : 1;
+        }
+        if (code == 2 || k0 >= da_limit(a, len, start, i_hi)) continue;
+        const bool cut = k0 + KB > da_limit(a, len, start, i_lo) || wl - w0 < 31;
+        uint64_t vis = ~0ull;
+        if (code == 1 && rlive) vis = a.rowbits[(mb * a.N + i) * M64 + kt];
+        if (cut) vis &= limit <= k0 ? 0ull : limit >= k0 + 64 ? ~0ull : (1ull << (limit - k0)) - 1;
+        const bool masked = cut || code == 1;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            da_f16v dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+#pragma unroll
+            for (int f = 0; f < C::NFV; ++f) dp = Da<T>::mma(da_frag<C::U>(sV, nt * 32 + l32, 2 * f + h2), uf[f], dp);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                da_f16v s;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+                for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sK, nt * 32 + l32, t * (C::U / 2) + 2 * f + h2), qf[t][f], s);
+                const float fac = t ? -lam : 1.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float p = da_exp2(fmaf(s[r], a.scale_log2e, -lse[t])) * fac;
+                    if (masked && !((vis >> (nt * 32 + 8 * (r >> 2) + 4 * h2 + (r & 3))) & 1)) p = 0.f;
+                    s[r] = p == 0.f ? 0.f : p * (dp[r] - dl[t]);
+                }
+#pragma unroll
+                for (int f = 0; f < C::FPT; ++f) {
+                    const uint4 sf = da_pack<T>(s, f);
+#pragma unroll
+                    for (int x = 0; x < C::MTK; ++x)
+                        dq[t][x] = Da<T>::mma(da_frag_tr<T, C::U>(sK, nt * 32 + f * Da<T>::KPF, DK < 32 ? 0 : t * DK + x * 32, lane), sf, dq[t][x]);
+                }
+            }
+        }
+    }
+    if (!rlive) return;
+    T *dst = reinterpret_cast<T *>(a.dq) + (((int64_t)b * a.N + i) * a.H + head) * 2 * a.d;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < C::MTK; ++x)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                int c = x * 32 + 8 * q4 + 4 * h2;
+                if (DK < 32) {                                // one tile holds both maps' channels: this map's half
+                    if (c / DK != t) continue;
+                    c -= t * DK;
+                }
+                if (c >= a.d) continue;
+                da_store4(dst + t * a.d + c, dq[t][x][4 * q4] * a.scale, dq[t][x][4 * q4 + 1] * a.scale, dq[t][x][4 * q4 + 2] * a.scale,
+                          dq[t][x][4 * q4 + 3] * a.scale);
+            }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// backward, dK and dV: workgroup = (batch, key head, 128 keys), a wave owns 32 keys; all rows that may see them, 32 queries of one head at a time
+template <typename T, int DK>
+__global__ __launch_bounds__(kDaThreads) void diff_attn_dkdv_kernel(const DiffArgs a) {
+    using C = DaCfg<T, DK>;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char *sQ = lds, *sU = lds + 32 * C::ROWB;
+    __shared__ __attribute__((aligned(16))) float sL[2][32], sD[2][32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h2 = lane >> 5, l32 = lane & 31;
+    const int bh = blockIdx.x % (a.B * a.Hk), blk = blockIdx.x / (a.B * a.Hk), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int len = da_len(a, b);
+    const int64_t start = da_start(a, b);
+    const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
+    const int kw0 = blk * 128 + wave * 32, key = kw0 + l32;
+    const int64_t mb = a.mask_b ? b : 0, bhn = (int64_t)a.B * a.H * a.N;
+    bool klive = key < len;
+    if (klive && a.live) klive = (a.live[mb * M64 + (key >> 6)] >> (key & 63)) & 1;
+    const bool wlive = kw0 < len;
+
+    uint4 kf[2][C::NF], vf[C::NFV];
+    const T *kp = reinterpret_cast<const T *>(a.k) + b * a.ks[0] + (int64_t)key * a.ks[1] + hk * a.ks[2];
+    const T *vp = reinterpret_cast<const T *>(a.v) + b * a.vs[0] + (int64_t)key * a.vs[1] + hk * a.vs[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int f = 0; f < C::NF; ++f) {
+            const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
+            kf[t][f] = klive && c < a.d ? *reinterpret_cast<const uint4 *>(kp + t * a.ks[3] + c) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+    for (int f = 0; f < C::NFV; ++f) {
+        const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
+        vf[f] = klive && c < a.dv ? *reinterpret_cast<const uint4 *>(vp + c) : make_uint4(0, 0, 0, 0);
+    }
+    da_f16v dk[2][C::MTK], dv[C::MT];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < C::MTK; ++x) dk[t][x][r] = 0.f;
+#pragma unroll
+        for (int x = 0; x < C::MT; ++x) dv[x][r] = 0.f;
+    }
+    // first query that may see a key of this workgroup
+    int i_first = 0;
+    if (a.causal) {
+        const int64_t f = (int64_t)blk * 128 - start;
+        i_first = f <= 0 ? 0 : f >= a.N ? a.N : (int)f;
+    }
+    if (blk * 128 >= len) i_first = a.N;
+    for (int g = 0; g < a.G; ++g) {
+        const int head = hk * a.G + g;
+        float e1, e2;
+        da_lambda_parts(a, head, e1, e2);
+        const float lam = e1 - e2 + a.init;
+        const int64_t hrow = ((int64_t)b * a.H + head) * a.N;
+        for (int i0 = i_first & ~31; i0 < a.N; i0 += 32) {
+            const int valid = min(32, a.N - i0);
+            __syncthreads();
+            uint64_t rows = ~0ull;                            // rows that see nothing: their queries may hold anything
+            if (tid < 64) {
+                const int t = tid >> 5, r = tid & 31;
+                const float ls = r < valid ? a.stats[t * bhn + hrow + i0 + r] : INFINITY;
+                sL[t][r] = ls;
+                sD[t][r] = r < valid ? a.delta[t * bhn + hrow + i0 + r] : 0.f;
+            }
+            __syncthreads();
+            rows = __ballot(sL[0][l32] != INFINITY) & 0xffffffffull;
+            da_stage<T, DK>(sQ, reinterpret_cast<const T *>(a.q) + b * a.qs[0] + (int64_t)i0 * a.qs[1] + head * a.qs[2], a.qs[1], a.qs[3], a.d, true, 32, valid, rows, tid);
+            da_stage<T, DK>(sU, reinterpret_cast<const T *>(a.du) + (((int64_t)b * a.N + i0) * a.H + head) * a.dv, (int64_t)a.H * a.dv, 0, a.dv, false, 32, valid, rows,
+                            tid);
+            __syncthreads();
+            if (!wlive) continue;
+            int code = 0;
+            if (a.tiles) code = a.tiles[(mb * N64 + (i0 >> 6)) * M64 + (kw0 >> 6)];
+            if (code == 2 || (a.causal && start + i0 + valid <= kw0)) continue;
+            const bool cut = a.causal && start + i0 < kw0 + 31;
+            uint32_t vis = ~0u;
+            if (code == 1 && klive) vis = (uint32_t)(a.colbits[(mb * a.M + key) * N64 + (i0 >> 6)] >> (i0 & 32));
+            if (cut) {                                        // query i0 + n sees this key from n >= key - start - i0 on
+                const int64_t n0 = (int64_t)key - start - i0;
+                vis &= n0 <= 0 ? ~0u : n0 >= 32 ? 0u : ~0u << n0;
+            }
+            const bool masked = cut || code == 1;
+            da_f16v dp, p0, s;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+#pragma unroll
+            for (int f = 0; f < C::NFV; ++f) dp = Da<T>::mma(da_frag<C::U>(sU, l32, 2 * f + h2), vf[f], dp);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+                for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sQ, l32, t * (C::U / 2) + 2 * f + h2), kf[t][f], s);
+                const float fac = t ? -lam : 1.f;
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const float4 ls = *reinterpret_cast<const float4 *>(&sL[t][8 * q4 + 4 * h2]), dd = *reinterpret_cast<const float4 *>(&sD[t][8 * q4 + 4 * h2]);
+                    const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv4[4] = {dd.x, dd.y, dd.z, dd.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = 4 * q4 + j;
+                        float p = da_exp2(fmaf(s[r], a.scale_log2e, -lv[j])) * fac;
+                        if (masked && !((vis >> (8 * q4 + 4 * h2 + j)) & 1)) p = 0.f;
+                        p0[r] = t ? p0[r] + p : p;
+                        s[r] = p == 0.f ? 0.f : p * (dp[r] - dv4[j]);
+                    }
+                }
+#pragma unroll
+                for (int f = 0; f < C::FPT; ++f) {
+                    const uint4 sf = da_pack<T>(s, f);
+#pragma unroll
+                    for (int x = 0; x < C::MTK; ++x)
+                        dk[t][x] = Da<T>::mma(da_frag_tr<T, C::U>(sQ, f * Da<T>::KPF, DK < 32 ? 0 : t * DK + x * 32, lane), sf, dk[t][x]);
+                }
+            }
+#pragma unroll
+            for (int f = 0; f < C::FPT; ++f) {
+                const uint4 pf = da_pack<T>(p0, f);
+#pragma unroll
+                for (int x = 0; x < C::MT; ++x) dv[x] = Da<T>::mma(da_frag_tr<T, C::U>(sU, f * Da<T>::KPF, x * 32, lane), pf, dv[x]);
+            }
+        }
+    }
+    if (key >= a.M) return;
+    const int64_t krow = ((int64_t)b * a.M + key) * a.Hk + hk;
+    T *dkp = reinterpret_cast<T *>(a.dk) + krow * 2 * a.d, *dvp = reinterpret_cast<T *>(a.dvv) + krow * a.dv;
+    const float keep = klive ? a.scale : 0.f;
+#pragma unroll
+    for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const int c = x * 32 + 8 * q4 + 4 * h2;
+            if (c >= a.dv) continue;
+            if (klive) da_store4(dvp + c, dv[x][4 * q4], dv[x][4 * q4 + 1], dv[x][4 * q4 + 2], dv[x][4 * q4 + 3]);
+            else da_store4(dvp + c, 0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < C::MTK; ++x)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                int c = x * 32 + 8 * q4 + 4 * h2;
+                if (DK < 32) {
+                    if (c / DK != t) continue;
+                    c -= t * DK;
+                }
+                if (c >= a.d) continue;
+                if (klive) da_store4(dkp + t * a.d + c, dk[t][x][4 * q4] * keep, dk[t][x][4 * q4 + 1] * keep, dk[t][x][4 * q4 + 2] * keep, dk[t][x][4 * q4 + 3] * keep);
+                else da_store4(dkp + t * a.d + c, 0.f, 0.f, 0.f, 0.f);
+            }
+}
+
+}  // namespace dfine
+
+using namespace dfine;
+
+extern "C" {
+
+static int diff_attn_setup(DiffArgs &a, const int64_t *s, float scale, float init, float eps) {
+    // shape: see include/dfine_hip.h
+    const int64_t B = s[0], N = s[1], M = s[2], H = s[3], Hk = s[4], d = s[5], dv = s[6], dt = s[7];
+    if (B < 0 || N < 0 || M < 0 || B > 0xffffff || N > 0x3fffffff || M > 0x3fffffff || H < 1 || Hk < 1 || H > 4096 || H % Hk || d < 8 || d > 64 || d % 8 || dv < 8 ||
+        dv > 128 || dv % 8 || (dt != 0 && dt != 1) || !(scale > 0.f) || !(eps >= 0.f))
+        return DFINE_E_BADARG;
+    if (s[8] != 1 && s[8] != H) return DFINE_E_BADARG;                               // heads of the learned vectors
+    if (N * (H / Hk) > (int64_t)1 << 36 || B * Hk > 0xffffff) return DFINE_E_BADARG;
+    a.B = (int)B; a.N = (int)N; a.M = (int)M; a.H = (int)H; a.Hk = (int)Hk; a.G = (int)(H / Hk); a.d = (int)d; a.dv = (int)dv;
+    a.lam_heads = (int)s[8]; a.lam_bf16 = s[9] != 0; a.w_bf16 = s[10] != 0;
+    a.causal = s[11] != 0; a.qstart = s[12]; a.mask_b = s[13];
+    const int unit = dt == 0 ? 4 : 8;                                                // elements of a 16-byte load
+    for (int j = 0; j < 4; ++j) { a.qs[j] = s[14 + j]; a.ks[j] = s[18 + j]; if (j < 3) { a.vs[j] = s[22 + j]; a.dys[j] = s[25 + j]; } }
+    for (int j = 14; j < 28; ++j) if (s[j] % unit) return DFINE_E_BADARG;
+    a.scale = scale; a.scale_log2e = scale * 1.44269504088896340736f; a.init = init; a.eps = eps;
+    return DFINE_OK;
+}
+
+static bool diff_attn_aligned(const void *p) { return p && ((uintptr_t)p & 15) == 0; }
+
+int64_t dfine_diff_attn_mask_words(int64_t batches, int64_t N, int64_t M) {
+    if (batches < 0 || N < 0 || M < 0) return -1;
+    const int64_t M64 = (M + 63) / 64, N64 = (N + 63) / 64;
+    return batches * (N * M64 + M * N64 + M64 + (N64 * M64 + 7) / 8);
+}
+
+static void diff_attn_forms(DiffArgs &a, const uint64_t *forms, int64_t batches) {
+    if (!forms) return;
+    const int64_t M64 = (a.M + 63) / 64, N64 = (a.N + 63) / 64;
+    a.rowbits = forms;
+    a.colbits = forms + batches * a.N * M64;
+    a.live = a.colbits + batches * a.M * N64;
+    a.tiles = reinterpret_cast<const uint8_t *>(a.live + batches * M64);
+}
+
+int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_t M, int64_t stride_b, int64_t stride_n, uint64_t *forms, void *stream) {
+    if (batches < 0 || N < 0 || M < 0 || N > 0x3fffffff || M > 0x3fffffff || batches > 0xffffff) return DFINE_E_BADARG;
+    if (batches == 0 || N == 0 || M == 0) return DFINE_OK;
+    if (!mask || !forms) return DFINE_E_BADARG;
+    const int64_t M64 = (M + 63) / 64, N64 = (N + 63) / 64;
+    if (batches * M64 > 0x7fffffff) return DFINE_E_BADARG;
+    uint64_t *col = forms + batches * N * M64, *live = col + batches * M * N64;
+    hipLaunchKernelGGL(diff_attn_mask_kernel, dim3((unsigned)(batches * M64)), dim3(256), 0, (hipStream_t)stream, mask, stride_b, stride_n, (int)N, (int)M, forms, col, live,
+                       reinterpret_cast<uint8_t *>(live + batches * M64));
+    return check_launch();
+}
+
+// the smallest of the three sizes that holds the head (values are twice as wide as a map's channels)
+static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <= 32 && dv <= 64 ? 32 : 64; }
+
+#define DA_DISPATCH(KERNEL, GRID, LDSROWS)                                                                                                                       \
+    {                                                                                                                                                            \
+        const int dk_ = diff_attn_size(a.d, a.dv);                                                                                                               \
+        const dim3 grid_(GRID);                                                                                                                                  \
+        hipStream_t st_ = (hipStream_t)stream;                                                                                                                   \
+        if (shape[7] == 0) {                                                                                                                                     \
+            if (dk_ == 16) hipLaunchKernelGGL((KERNEL<float, 16>), grid_, dim3(kDaThreads), 2 * LDSROWS * 128, st_, a);                                          \
+            else if (dk_ == 32) hipLaunchKernelGGL((KERNEL<float, 32>), grid_, dim3(kDaThreads), 2 * LDSROWS * 256, st_, a);                                     \
+            else hipLaunchKernelGGL((KERNEL<float, 64>), grid_, dim3(kDaThreads), 2 * LDSROWS * 512, st_, a);                                                    \
+        } else {                                                                                                                                                 \
+            if (dk_ == 16) hipLaunchKernelGGL((KERNEL<uint16_t, 16>), grid_, dim3(kDaThreads), 2 * LDSROWS * 64, st_, a);                                        \
+            else if (dk_ == 32) hipLaunchKernelGGL((KERNEL<uint16_t, 32>), grid_, dim3(kDaThreads), 2 * LDSROWS * 128, st_, a);                                  \
+            else hipLaunchKernelGGL((KERNEL<uint16_t, 64>), grid_, dim3(kDaThreads), 2 * LDSROWS * 256, st_, a);                                                 \
+        }                                                                                                                                                        \
+    }
+
+int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms, const int *kv_len,
+                        const int *q_start, void *out, void *u, void *o2, float *stats, const int64_t *shape, float scale, float init, float eps, void *stream) {
+    if (!shape) return DFINE_E_BADARG;
+    DiffArgs a{};
+    if (int e = diff_attn_setup(a, shape, scale, init, eps)) return e;
+    if (a.B == 0 || a.N == 0) return DFINE_OK;
+    if (!diff_attn_aligned(q) || !diff_attn_aligned(out) || !lam || (a.M && (!diff_attn_aligned(k) || !diff_attn_aligned(v)))) return DFINE_E_BADARG;
+    if ((o2 != nullptr) != (stats != nullptr) || (u && !o2) || (o2 && weight && !u)) return DFINE_E_BADARG;
+    a.q = q; a.k = k; a.v = v; a.lam = lam; a.weight = weight; a.kvlen = kv_len; a.qstart_dev = q_start;
+    a.out = out; a.u = o2 ? (u ? u : out) : nullptr; a.o2 = o2; a.stats = stats;
+    a.post = weight ? 1.f - init : 1.f;
+    diff_attn_forms(a, mask_forms, a.mask_b ? a.B : 1);
+    const int64_t blocks = ((int64_t)a.N * a.G + 127) / 128 * a.B * a.Hk;
+    if (blocks > 0x7fffffff) return DFINE_E_BADARG;
+    DA_DISPATCH(diff_attn_fwd_kernel, (unsigned)blocks, 64)
+    return check_launch();
+}
+
+static int diff_attn_runs(const DiffArgs &a) {                  // workgroups per head of the first backward kernel: 1024 in all, 8 rows each at least
+    const int64_t rows = ((int64_t)a.B * a.N + 7) / 8;
+    int64_t n = 1024 / a.H;
+    if (n < 1) n = 1;
+    return (int)(n < rows ? n : rows < 1 ? 1 : rows);
+}
+
+// workspace of the backward pass in bytes: dU, D_0 and D_1, the partial sums
+static int64_t da_up(int64_t x) { return (x + 255) / 256 * 256; }
+int64_t dfine_diff_attn_bwd_ws_bytes(const int64_t *shape) {
+    DiffArgs a{};
+    if (!shape || diff_attn_setup(a, shape, 1.f, 0.f, 0.f)) return -1;
+    const int64_t rows = (int64_t)a.B * a.N * a.H, n = (int64_t)diff_attn_runs(a) * a.H;
+    return da_up(rows * a.dv * (shape[7] ? 2 : 4)) + da_up(rows * 8) + da_up(n * 4) + da_up(n * a.dv * 4);
+}
+
+int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms, const int *kv_len,
+                        const int *q_start, const void *out, const void *u, const void *o2, const float *stats, const void *dy, void *dq, void *dk, void *dv,
+                        void *dlam, void *dweight, void *ws, const int64_t *shape, float scale, float init, float eps, void *stream) {
+    if (!shape) return DFINE_E_BADARG;
+    DiffArgs a{};
+    if (int e = diff_attn_setup(a, shape, scale, init, eps)) return e;
+    if (!lam || !ws || ((uintptr_t)ws & 255)) return DFINE_E_BADARG;
+    const bool rows_ = a.B && a.N, keys_ = a.B && a.M;
+    if (rows_ && (!diff_attn_aligned(q) || !diff_attn_aligned(out) || !diff_attn_aligned(o2) || !stats || !diff_attn_aligned(dy) || (dq && !diff_attn_aligned(dq)) ||
+                  (weight && !diff_attn_aligned(u))))
+        return DFINE_E_BADARG;
+    if ((dk == nullptr) != (dv == nullptr)) return DFINE_E_BADARG;
+    if (keys_ && (!diff_attn_aligned(k) || !diff_attn_aligned(v) || (dk && (!diff_attn_aligned(dk) || !diff_attn_aligned(dv))))) return DFINE_E_BADARG;
+    a.q = q; a.k = k; a.v = v; a.lam = lam; a.weight = weight; a.kvlen = kv_len; a.qstart_dev = q_start;
+    a.out = const_cast<void *>(out); a.u = const_cast<void *>(u); a.o2 = const_cast<void *>(o2); a.stats = const_cast<float *>(stats);
+    a.dy = dy; a.dq = dq; a.dk = dk; a.dvv = dv;
+    a.post = weight ? 1.f - init : 1.f;
+    diff_attn_forms(a, mask_forms, a.mask_b ? a.B : 1);
+    const int nrun = diff_attn_runs(a);
+    const int64_t rows = (int64_t)a.B * a.N * a.H, n = (int64_t)nrun * a.H;
+    char *p = reinterpret_cast<char *>(ws);
+    a.du = p; p += da_up(rows * a.dv * (shape[7] ? 2 : 4));
+    a.delta = reinterpret_cast<float *>(p); p += da_up(rows * 8);
+    a.lpart = reinterpret_cast<float *>(p); p += da_up(n * 4);
+    a.wpart = reinterpret_cast<float *>(p);
+    hipStream_t st = (hipStream_t)stream;
+    if (n > 0x7fffffff) return DFINE_E_BADARG;
+    if (shape[7] == 0) hipLaunchKernelGGL(diff_attn_prep_kernel<float>, dim3((unsigned)n), dim3(256), 0, st, a, nrun);
+    else hipLaunchKernelGGL(diff_attn_prep_kernel<uint16_t>, dim3((unsigned)n), dim3(256), 0, st, a, nrun);
+    if (int e = check_launch()) return e;
+    if (dlam || dweight) {
+        const int nh = a.lam_heads == 1 ? 1 : a.H;
+        hipLaunchKernelGGL(diff_attn_param_kernel, dim3(nh + (a.dv + 15) / 16), dim3(256), 0, st, a, nrun, dlam, weight ? dweight : nullptr);
+        if (int e = check_launch()) return e;
+    }
+    if (rows_ && dq) {
+        const int64_t blocks = ((int64_t)a.N * a.G + 127) / 128 * a.B * a.Hk;
+        if (blocks > 0x7fffffff) return DFINE_E_BADARG;
+        DA_DISPATCH(diff_attn_dq_kernel, (unsigned)blocks, 64)
+        if (int e = check_launch()) return e;
+    }
+    if (keys_ && dk) {
+        const int64_t blocks = ((int64_t)a.M + 127) / 128 * a.B * a.Hk;
+        if (blocks > 0x7fffffff) return DFINE_E_BADARG;
+        DA_DISPATCH(diff_attn_dkdv_kernel, (unsigned)blocks, 32)
+        if (int e = check_launch()) return e;
+    }
+    return DFINE_OK;
+}
+#undef DA_DISPATCH
+
+}  // extern "C"

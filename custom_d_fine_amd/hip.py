@@ -13,7 +13,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DFINE_HIP_LIB") or os.path.join(_HERE, "csrc", "libdfine_hip.so")     # (override: A/B of two builds on one box)
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 if not os.path.exists(LIB_PATH):
     raise ImportError(
@@ -117,6 +117,14 @@ _SIGNATURES = {
     "dfine_attn_fwd_ms": (c_int, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P]),
     "dfine_attn_bwd_ms": (c_int, [_P] * 13 + [_I] * 12 + [_F, _P]),
     "dfine_attn_mask_bits_words": (_L, [_I]),
+    "dfine_qk_norm_rotate_ws_floats": (_L, [_P]),
+    "dfine_qk_norm_rotate_fwd": (c_int, [_P] * 10 + [_F, _P]),
+    "dfine_qk_norm_rotate_bwd": (c_int, [_P] * 15 + [_F, _P]),
+    "dfine_diff_attn_mask_words": (_L, [_L, _L, _L]),
+    "dfine_diff_attn_mask": (c_int, [_P, _L, _L, _L, _L, _L, _P, _P]),
+    "dfine_diff_attn_bwd_ws_bytes": (_L, [_P]),
+    "dfine_diff_attn_fwd": (c_int, [_P] * 13 + [_F, _F, _F, _P]),
+    "dfine_diff_attn_bwd": (c_int, [_P] * 20 + [_F, _F, _F, _P]),
     "dfine_attn_mask_bits": (c_int, [_P, _I, _P, _P]),
     "dfine_groupnorm_ws_floats": (_L, [_I, _I, _I]),
     "dfine_groupnorm_fwd": (c_int, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P]),
@@ -1510,6 +1518,135 @@ def attn_backward(q, k, v, o, dout, lse2, num_heads, dq, dk, dv, mask=None):
         _check(_lib.dfine_attn_bwd_ms(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dout), _ptr(lse2), _ptr(mask), _ptr(mbits), _ptr(msum), _ptr(dq),
                                       _ptr(dk), _ptr(dv), _ptr(delta), B, L, num_heads, hd, _ld(q), _ld(k), _ld(v), _ld(o), _ld(dout),
                                       _ld(dq), _ld(dk), _ld(dv), float(hd) ** -0.5, _stream()), "dfine_attn_bwd_ms")
+
+
+# ------------------------------------------------------------------------------------- attention block: norms + rotation, differential attention
+_QKN_SHAPE, _DA_SHAPE = c_int64 * 25, c_int64 * 28
+
+
+def _rows16(t):
+    """`t` as the kernels read it - unit stride in the last dimension, every row on a 16-byte border - and its other strides; a copy where it is not."""
+    unit = 16 // t.element_size()
+    shape, st = t.shape, t.stride()
+    ok = (st[-1] == 1 or shape[-1] == 1) and t.data_ptr() % 16 == 0
+    out = []
+    for n, s in zip(shape[:-1], st[:-1]):
+        out.append(s if n > 1 else 0)                       # (a dimension of one row carries any stride)
+        ok = ok and (n <= 1 or s % unit == 0)
+    if ok:
+        return t, out
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, [s if n > 1 else 0 for n, s in zip(shape[:-1], t.stride()[:-1])]
+
+
+def _on_device(fn):
+    """The launcher on its first tensor's device: the stream and the new tensors are that device's."""
+    def launch(t, *args):
+        if t.device.index == torch.cuda.current_device():
+            return fn(t, *args)
+        with torch.cuda.device(t.device):
+            return fn(t, *args)
+    return launch
+
+
+def _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks, dqs=(0, 0, 0), dks=(0, 0, 0)):
+    B, L, Hq, D = q.shape
+    return _QKN_SHAPE(B, L, Hq, 0 if k is None else k.shape[2], D, 0 if cos is None else 2 * cos.shape[1], 0 if cos is None else cos.shape[0], _DTYPE[q.dtype],
+                      paired, positions is not None and positions.dtype == torch.int64, L if positions is not None and positions.dim() == 2 else 0,
+                      wq is not None and wq.dtype == torch.bfloat16, wk is not None and wk.dtype == torch.bfloat16, *qs, *ks, *dqs, *dks)
+
+
+@_on_device
+def qk_norm_rotate_forward(q, k, wq, wk, cos, sin, positions, eps, paired):
+    """q [B, L, Hq, D], k [B, L, Hk, D] or None -> the normed and rotated queries and keys (contiguous), and q, k as the kernel read them."""
+    q, qs = _rows16(q)
+    ks = (0, 0, 0)
+    if k is not None:
+        k, ks = _rows16(k)
+    yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    yk = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
+    with _timed("qk_norm_rotate", 2.0 * q.element_size() * (q.numel() + (0 if k is None else k.numel()))):
+        _check(_lib.dfine_qk_norm_rotate_fwd(_ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(yq), _ptr(yk),
+                                             _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks), eps, _stream()), "dfine_qk_norm_rotate_fwd")
+    return yq, yk, q, k
+
+
+@_on_device
+def qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions, eps, paired, dyq, dyk, want_wq, want_wk):
+    q, qs = _rows16(q)
+    dyq, dqs = _rows16(dyq)
+    ks = dks = (0, 0, 0)
+    if k is not None:
+        k, ks = _rows16(k)
+        dyk, dks = _rows16(dyk)
+    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    dk = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
+    dwq = torch.empty_like(wq) if want_wq else None
+    dwk = torch.empty_like(wk) if want_wk else None
+    shape = _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks, dqs, dks)
+    ws = torch.empty(max(1, int(_lib.dfine_qk_norm_rotate_ws_floats(shape))), device=q.device, dtype=torch.float32)
+    with _timed("qk_norm_rotate", 3.0 * q.element_size() * (q.numel() + (0 if k is None else k.numel()))):
+        _check(_lib.dfine_qk_norm_rotate_bwd(_ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(dyq), _ptr(dyk), _ptr(dq),
+                                             _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(ws), shape, eps, _stream()), "dfine_qk_norm_rotate_bwd")
+    return dq, dk, dwq, dwk
+
+
+@_on_device
+def diff_attn_mask_forms(mask):
+    """mask [1 or B, N, M] bool (True = may not attend) -> the packed forms of dfine_diff_attn_mask, one int64 tensor."""
+    if mask.stride(2) != 1 and mask.shape[2] > 1:
+        mask = mask.contiguous()
+    nb, N, M = mask.shape
+    forms = torch.empty(max(1, int(_lib.dfine_diff_attn_mask_words(nb, N, M))), device=mask.device, dtype=torch.int64)
+    _check(_lib.dfine_diff_attn_mask(_ptr(mask), nb, N, M, mask.stride(0), mask.stride(1), _ptr(forms), _stream()), "dfine_diff_attn_mask")
+    return forms
+
+
+def _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys=(0, 0, 0)):
+    B, N, H, _, d = q.shape
+    return _DA_SHAPE(B, N, k.shape[1], H, k.shape[2], d, v.shape[3], _DTYPE[q.dtype], 1 if lam.dim() == 2 else H, lam.dtype == torch.bfloat16,
+                     weight is not None and weight.dtype == torch.bfloat16, causal, start if isinstance(start, int) else 0, mask_batches, *qs, *ks, *vs, *dys)
+
+
+@_on_device
+def diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, keep):
+    """-> out [B, N, H, dv], and with `keep` what the backward pass reads: q, k, v as the kernel read them, u, o2, stats (else None)."""
+    q, qs = _rows16(q)
+    k, ks = _rows16(k)
+    v, vs = _rows16(v)
+    B, N, H, _, d = q.shape
+    M, dv = k.shape[1], v.shape[3]
+    out = torch.empty(B, N, H, dv, device=q.device, dtype=q.dtype)
+    u = o2 = stats = None
+    if keep:
+        u = torch.empty_like(out) if weight is not None else None
+        o2 = torch.empty_like(out)
+        stats = torch.empty(3, B, H, N, device=q.device, dtype=torch.float32)
+    with _timed("diff_attention", 4.0 * B * H * N * M * (d + dv), io=float(q.element_size()) * (q.numel() + k.numel() + v.numel() + out.numel())):
+        _check(_lib.dfine_diff_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(weight), _ptr(forms), _ptr(kv_len),
+                                        None if isinstance(start, int) else _ptr(start), _ptr(out), _ptr(u), _ptr(o2), _ptr(stats),
+                                        _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs), scale, init, eps, _stream()), "dfine_diff_attn_fwd")
+    return out, q, k, v, u, o2, stats
+
+
+@_on_device
+def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, out, u, o2, stats, dy, want):
+    """`want`: which of dq, (dk, dv), dlam, dweight are needed -> (dq, dk, dv, dlam, dweight)."""
+    q, qs = _rows16(q)
+    k, ks = _rows16(k)
+    v, vs = _rows16(v)
+    dy, dys = _rows16(dy)
+    new = lambda t, on: torch.empty(t.shape, device=t.device, dtype=t.dtype) if on else None  # noqa: E731
+    dq, dk, dv, dlam = new(q, want[0]), new(k, want[1]), new(v, want[1]), new(lam, want[2])
+    dweight = None if weight is None else new(weight, want[3])
+    shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys)
+    ws = torch.empty(max(256, int(_lib.dfine_diff_attn_bwd_ws_bytes(shape))), device=q.device, dtype=torch.uint8)
+    B, N, H, _, d = q.shape
+    with _timed("diff_attention", 4.0 * B * H * N * k.shape[1] * (3 * d + 2 * v.shape[3]), io=2.0 * q.element_size() * (q.numel() + k.numel() + v.numel() + out.numel())):
+        _check(_lib.dfine_diff_attn_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(weight), _ptr(forms), _ptr(kv_len),
+                                        None if isinstance(start, int) else _ptr(start), _ptr(out), _ptr(u), _ptr(o2), _ptr(stats), _ptr(dy), _ptr(dq), _ptr(dk),
+                                        _ptr(dv), _ptr(dlam), _ptr(dweight), _ptr(ws), shape, scale, init, eps, _stream()), "dfine_diff_attn_bwd")
+    return dq, dk, dv, dlam, dweight
 
 
 # ------------------------------------------------------------------------------------- linear wgrad

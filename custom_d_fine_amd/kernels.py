@@ -2490,6 +2490,176 @@ def self_attention(qk, value, in_w, in_b, out_w, out_b, num_heads: int, attn_mas
     return linear(o.transpose(1, 2).reshape(b, l, e), out_w, out_b)
 
 
+# =============================================================================================
+# attention block with normed, rotated heads and differential attention
+# =============================================================================================
+def _need(ok, what, kind=ValueError):
+    if not ok:
+        raise kind(f"custom_d_fine_amd.kernels.{what}")
+
+
+def _float_tensor(op, name, t, dtypes, device):
+    _need(isinstance(t, torch.Tensor) and t.dtype in dtypes, f"{op}: {name} is a {' or '.join(str(d)[6:] for d in dtypes)} tensor, got "
+          f"{getattr(t, 'dtype', type(t).__name__)}", TypeError)
+    _need(device is None or t.device == device, f"{op}: {name} is on {t.device}, the queries on {device}")
+
+
+_ACT_DTYPES = (torch.float32, torch.bfloat16)
+
+
+class _QKNormRotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, paired):
+        yq, yk, qr, kr = _hip().qk_norm_rotate_forward(q, k, wq, wk, cos, sin, positions, eps, paired)
+        ctx.save_for_backward(qr, kr, wq, wk, cos, sin, positions)
+        ctx.meta = (eps, paired)
+        return yq, yk
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dyq, dyk):
+        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dwq, dwk = _hip().qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions, *ctx.meta, dyq, dyk, need[2] and wq is not None,
+                                                         need[3] and wk is not None)
+        return dq, dk, dwq, dwk, None, None, None, None, None
+
+
+def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, positions=None, eps: float = 1e-6, interleaved: bool = False):
+    """RMS norm of every head's queries and keys and the rotation by the token's position, one pass each way.
+
+    q [B, L, heads, D], k [B, L, key heads, D] or None, float32 / bfloat16, any strides (rows that are not on 16-byte borders are copied);
+    D and 2 * cos.shape[1] multiples of 8, D <= 256.  q_weight, k_weight [D] (None: ones).  cos, sin float32 [T, R / 2] (None: no rotation):
+    channels (j, j + R / 2) - with `interleaved` (2j, 2j + 1) - turn by row positions[.., l] of the table (None: row l); channels from R on
+    pass.  positions: int32 / int64 [L] or [B, L]; a position outside the table gives NaN.  Gradients for q, k and the weights.
+    -> (q', k'), contiguous, of q's type (k' None without k).  Under bf16 autocast q and k are cast to bfloat16 first."""
+    op = "qk_norm_rotate"
+    _float_tensor(op, "q", q, _ACT_DTYPES, None)
+    if k is not None:
+        _float_tensor(op, "k", k, _ACT_DTYPES, q.device)
+    if q.is_cuda and _bf16_autocast():
+        q, k = q.to(torch.bfloat16), None if k is None else k.to(torch.bfloat16)
+    _need(q.dim() == 4, f"{op}: q is [batch, tokens, heads, channels], got {tuple(q.shape)}")
+    D = q.shape[3]
+    _need(8 <= D <= 256 and D % 8 == 0, f"{op}: heads of {D} channels (multiples of 8 up to 256)")
+    if k is not None:
+        _need(k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == D, f"{op}: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
+        _need(k.dtype == q.dtype, f"{op}: k is {k.dtype}, q {q.dtype}", TypeError)
+    _need(q.shape[0] * q.shape[1] < 2 ** 31 - 65536 and q.shape[2] <= 4096 and (k is None or k.shape[2] <= 4096), f"{op}: too many tokens or heads")
+    _need(k is not None or k_weight is None, f"{op}: k_weight without k")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _float_tensor(op, name, w, _ACT_DTYPES, q.device)
+            _need(w.shape == (D,), f"{op}: {name} {tuple(w.shape)} for heads of {D} channels")
+    _need((cos is None) == (sin is None), f"{op}: cos and sin come together")
+    _need(positions is None or cos is not None, f"{op}: positions without a table")
+    if cos is not None:
+        for name, t in (("cos", cos), ("sin", sin)):
+            _float_tensor(op, name, t, (torch.float32,), q.device)
+        _need(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] % 4 == 0 and 0 < 2 * cos.shape[1] <= D and cos.shape[0] > 0,
+              f"{op}: tables {tuple(cos.shape)}, {tuple(sin.shape)} for heads of {D} channels (R a multiple of 8, at most {D})")
+        _need(not (cos.requires_grad or sin.requires_grad), f"{op}: the tables take no gradient")
+        if positions is None:
+            _need(q.shape[1] <= cos.shape[0], f"{op}: {q.shape[1]} tokens, {cos.shape[0]} rows in the table")
+        else:
+            _need(isinstance(positions, torch.Tensor) and positions.dtype in (torch.int32, torch.int64), f"{op}: positions are int32 or int64", TypeError)
+            _need(positions.device == q.device, f"{op}: positions are on {positions.device}, the queries on {q.device}")
+            _need(positions.shape in (q.shape[1:2], q.shape[:2]), f"{op}: positions {tuple(positions.shape)} for {tuple(q.shape[:2])} tokens")
+            positions = positions.contiguous()
+        cos, sin = cos.contiguous(), sin.contiguous()
+    eps = float(eps)
+    _need(eps >= 0, f"{op}: eps {eps}")
+    if not q.is_cuda:
+        return _backend_for_cpu(op)(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))
+    wq, wk = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, wq, wk)):
+        return _QKNormRotate.apply(q, k, wq, wk, cos, sin, positions, eps, bool(interleaved))
+    return _hip().qk_norm_rotate_forward(q, k, wq, wk, cos, sin, positions, eps, bool(interleaved))[:2]
+
+
+class _DiffAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps):
+        out, qr, kr, vr, u, o2, stats = _hip().diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, True)
+        at = None if isinstance(start, int) else start
+        ctx.save_for_backward(qr, kr, vr, lam, weight, forms, kv_len, at, out if weight is None else None, u, o2, stats)
+        ctx.meta = (mask_batches, causal, start if at is None else None, scale, init, eps)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        q, k, v, lam, weight, forms, kv_len, at, out, u, o2, stats = ctx.saved_tensors
+        mask_batches, causal, start, scale, init, eps = ctx.meta
+        n = ctx.needs_input_grad
+        dq, dk, dv, dlam, dw = _hip().diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start if at is None else at, scale, init, eps,
+                                                         u if out is None else out, u, o2, stats, dy, (n[0], n[1] or n[2], n[3], n[4]))
+        return (dq, dk if n[1] else None, dv if n[2] else None, dlam, dw) + (None,) * 8
+
+
+def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None, norm_eps: float = 1e-5, attn_mask=None, kv_lengths=None, causal: bool = False,
+                   query_start=0, scale: Optional[float] = None):
+    """Differential attention: every head reads its values through the difference of two softmax maps,
+    U = (softmax(scale q_0 k_0^T) - l softmax(scale q_1 k_1^T)) v with l = exp(x_0 . x_1) - exp(x_2 . x_3) + lambda_init, and with `norm_weight`
+    returns (1 - lambda_init) * U / sqrt(mean U^2 + norm_eps) * norm_weight (the norm of each head's result), without it U.
+
+    q [B, N, H, 2, d], k [B, M, Hk, 2, d], v [B, M, Hk, dv] (H a multiple of Hk: head h reads key head h // (H / Hk)), float32 / bfloat16, any strides;
+    d <= 64, dv <= 128, multiples of 8.  lambda_vectors: the learned x_0 .. x_3, [4, H, d] or shared by the heads [4, d].  norm_weight [dv].
+    Which keys query i of sequence b sees: those `attn_mask` (bool [N, M] or [B, N, M], True = may not attend) lets it, j < kv_lengths[b] (int [B]: a
+    padded batch or a cache that is not full; keys from there on are never read), and when `causal` j <= query_start + i (an int, or int [B]: the position
+    of the first query among the keys).  A query that sees no key gives 0 and takes no gradient.  Keys that some query sees hold finite numbers; keys that
+    the mask hides from every query, and keys behind kv_lengths, may hold anything.
+    Gradients for q, k, v, lambda_vectors and norm_weight, added up in a fixed order.  -> [B, N, H, dv], contiguous, of q's type.  Under bf16 autocast
+    q, k, v are cast to bfloat16 first.  scale: d ** -0.5 by default."""
+    op = "diff_attention"
+    _float_tensor(op, "q", q, _ACT_DTYPES, None)
+    for name, t in (("k", k), ("v", v)):
+        _float_tensor(op, name, t, _ACT_DTYPES, q.device)
+    if q.is_cuda and _bf16_autocast():
+        q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
+    _need(q.dtype == k.dtype == v.dtype, f"{op}: q is {q.dtype}, k {k.dtype}, v {v.dtype}", TypeError)
+    _need(q.dim() == 5 and q.shape[3] == 2, f"{op}: q is [batch, queries, heads, 2, channels], got {tuple(q.shape)}")
+    B, N, H, _, d = q.shape
+    _need(k.dim() == 5 and k.shape[0] == B and k.shape[3:] == (2, d), f"{op}: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
+    M, Hk = k.shape[1:3]
+    _need(v.dim() == 4 and v.shape[:3] == k.shape[:3], f"{op}: v {tuple(v.shape)} does not go with k {tuple(k.shape)}")
+    dv = v.shape[3]
+    _need(8 <= d <= 64 and d % 8 == 0 and 8 <= dv <= 128 and dv % 8 == 0, f"{op}: heads of 2 x {d} channels with values of {dv} (multiples of 8 up to 64, 128)")
+    _need(1 <= Hk <= H <= 4096 and H % Hk == 0, f"{op}: {H} heads on {Hk} key heads")
+    _need(N < 2 ** 30 and M < 2 ** 30 and B < 2 ** 24 and B * Hk < 2 ** 24, f"{op}: {B} sequences of {N} queries and {M} keys")
+    _float_tensor(op, "lambda_vectors", lambda_vectors, _ACT_DTYPES, q.device)
+    _need(lambda_vectors.shape in ((4, d), (4, H, d)), f"{op}: lambda_vectors {tuple(lambda_vectors.shape)} for {H} heads of 2 x {d} channels")
+    if norm_weight is not None:
+        _float_tensor(op, "norm_weight", norm_weight, _ACT_DTYPES, q.device)
+        _need(norm_weight.shape == (dv,), f"{op}: norm_weight {tuple(norm_weight.shape)} for values of {dv} channels")
+    if attn_mask is not None:
+        _need(isinstance(attn_mask, torch.Tensor) and attn_mask.dtype == torch.bool, f"{op}: attn_mask is a bool tensor, True = may not attend", TypeError)
+        _need(attn_mask.device == q.device, f"{op}: attn_mask is on {attn_mask.device}, the queries on {q.device}")
+        _need(attn_mask.shape in ((N, M), (B, N, M)), f"{op}: attn_mask {tuple(attn_mask.shape)} for {N} queries and {M} keys of {B} sequences")
+    starts = isinstance(query_start, torch.Tensor)
+    for name, t in (("kv_lengths", kv_lengths), ("query_start", query_start if starts else None)):
+        if t is not None:
+            _need(isinstance(t, torch.Tensor) and t.dtype in (torch.int32, torch.int64), f"{op}: {name} is an int32 or int64 tensor", TypeError)
+            _need(t.device == q.device and t.shape == (B,), f"{op}: {name} {tuple(t.shape)} on {t.device} for {B} sequences on {q.device}")
+    _need(causal or (not starts and query_start == 0), f"{op}: query_start goes with causal")
+    _need(starts or -(2 ** 31) < int(query_start) < 2 ** 31, f"{op}: query_start {query_start}")
+    scale, init, eps = d ** -0.5 if scale is None else float(scale), float(lambda_init), float(norm_eps)
+    _need(0 < scale < float("inf"), f"{op}: scale {scale}")
+    _need(eps >= 0, f"{op}: norm_eps {eps}")
+    if not q.is_cuda:
+        return _backend_for_cpu(op)(q, k, v, lambda_vectors, init, norm_weight, eps, attn_mask, kv_lengths, bool(causal), query_start, scale)
+    lam, weight = lambda_vectors.contiguous(), None if norm_weight is None else norm_weight.contiguous()
+    kv_len = None if kv_lengths is None else kv_lengths.to(torch.int32).contiguous()
+    start = query_start.to(torch.int32).contiguous() if starts else int(query_start)
+    forms = None
+    if attn_mask is not None:
+        forms = _hip().diff_attn_mask_forms(attn_mask if attn_mask.dim() == 3 else attn_mask[None])
+    batches = attn_mask is not None and attn_mask.dim() == 3 and B > 1
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, lam, weight)):
+        return _DiffAttention.apply(q, k, v, lam, weight, forms, batches, kv_len, bool(causal), start, scale, init, eps)
+    return _hip().diff_attn_forward(q, k, v, lam, weight, forms, batches, kv_len, bool(causal), start, scale, init, eps, False)[0]
+
+
 # BatchNorm bookkeeping: nn.BatchNorm2d bumps `num_batches_tracked` (an int64 device scalar) every forward -
 # 133 tiny launches per step.  A train loop may defer them and flush once per step with one multi-tensor add.
 _BN_DEFER = False

@@ -809,6 +809,46 @@ int64_t dfine_mask_bits_words(int64_t HW);
 int dfine_mask_pack_bits(const void *masks, int dtype, float thresh, int N, int64_t HW, void *bits, void *stream);
 int dfine_mask_iou_bits(const void *pred_bits, const void *gt_bits, int Np, int Ng, int64_t words, float *iou, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * A2 / A6  Norms of queries and keys for each head with the position rotation in the same pass, next to the attention of
+ * src/d_fine/arch/hybrid_encoder.py:243-290 and src/d_fine/arch/dfine_decoder.py:200,233-255 (no counterpart there).
+ * q [B, L, Hq, D], k [B, L, Hk, D] (Hq or Hk may be 0: that operand is left out); y = rot(x rsqrt(mean_D x^2 + eps) w): pairs of the
+ * first R channels are turned by the token's row of cosv / sinv fp32 [T, R / 2] - pairs (j, j + R / 2), or (2j, 2j + 1) when paired -
+ * the rest passes.  pos int32 / int64 [B or 1, L]: the row of each token (NULL: its index; outside the table: NaN).  wq, wk [D] or NULL.
+ * shape (host int64): B, L, Hq, Hk, D, R, T, dtype (0 fp32, 1 bf16), paired, pos is int64, batch stride of pos, wq bf16, wk bf16, then the
+ * strides (batch, token, head; elements, 16-byte rows) of q, of k, of dyq, of dyk.  Results are contiguous.  D, R multiples of 8, D <= 256.
+ * Backward: dwq, dwk (the weights' types; NULL: not wanted); ws dfine_qk_norm_rotate_ws_floats(shape) floats. */
+int64_t dfine_qk_norm_rotate_ws_floats(const int64_t *shape);
+int dfine_qk_norm_rotate_fwd(const void *q, const void *k, const void *wq, const void *wk, const float *cosv, const float *sinv,
+                             const void *pos, void *yq, void *yk, const int64_t *shape, float eps, void *stream);
+int dfine_qk_norm_rotate_bwd(const void *q, const void *k, const void *wq, const void *wk, const float *cosv, const float *sinv,
+                             const void *pos, const void *dyq, const void *dyk, void *dq, void *dk, void *dwq, void *dwk, float *ws,
+                             const int64_t *shape, float eps, void *stream);
+
+/* Differential attention of the token streams: out = (1 - init) norm((A_0 - l A_1) V) weight per head, A_t = softmax(scale q_t k_t^T +
+ * mask), l = exp(x0 . x1) - exp(x2 . x3) + init from lam [4, H or 1, d]; without weight: out = (A_0 - l A_1) V.  A query that sees no key
+ * gives 0 and takes no gradient.
+ * q [B, N, H, 2, d], k [B, M, Hk, 2, d], v [B, M, Hk, dv] (H a multiple of Hk), out [B, N, H, dv] contiguous; d <= 64, dv <= 128, multiples of 8.
+ * What query i of batch b sees: keys j < kv_len[b] (NULL: M; keys from there on are not read), j <= q_start[b] + i when causal (q_start NULL:
+ * one start for all in shape), and where the mask lets it: mask_forms = the dfine_diff_attn_mask_words(batches, N, M) words that
+ * dfine_diff_attn_mask makes of bytes [batches, N, M] (non-zero = may not attend; strides in bytes), batches 1 or B.
+ * Forward for training keeps u, o2 (out's shape and type; u NULL without weight) and stats fp32 [3, B, H, N].
+ * shape (host int64): B, N, M, H, Hk, d, dv, dtype (0 fp32, 1 bf16), heads of lam, lam bf16, weight bf16, causal, q_start, mask has batches, then the
+ * strides (batch, token, head, map) of q, of k, (batch, token, head) of v, of dy (elements; 16-byte rows).
+ * Backward: dq, dk, dv contiguous (dq, or dk and dv, NULL: not wanted), dlam, dweight of lam's and weight's types (NULL: not wanted);
+ * ws: dfine_diff_attn_bwd_ws_bytes(shape) bytes, 256-byte aligned.  Deterministic. */
+int64_t dfine_diff_attn_mask_words(int64_t batches, int64_t N, int64_t M);
+int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_t M, int64_t stride_b, int64_t stride_n, uint64_t *forms,
+                         void *stream);
+int64_t dfine_diff_attn_bwd_ws_bytes(const int64_t *shape);
+int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms,
+                        const int *kv_len, const int *q_start, void *out, void *u, void *o2, float *stats, const int64_t *shape,
+                        float scale, float init, float eps, void *stream);
+int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms,
+                        const int *kv_len, const int *q_start, const void *out, const void *u, const void *o2, const float *stats,
+                        const void *dy, void *dq, void *dk, void *dv, void *dlam, void *dweight, void *ws, const int64_t *shape,
+                        float scale, float init, float eps, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

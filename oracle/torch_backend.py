@@ -111,6 +111,57 @@ def preprocess_frames(frames, out_hw, resized_hw, top_left=(0, 0), pad_value=114
     return (t.float() / 255.0).to(dtype)
 
 
+def qk_norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    """RMS norm per head, then the rotation of channel pairs by the token's table row."""
+    def one(x, w):
+        if x is None:
+            return None
+        y = x.float()
+        y = y / torch.sqrt((y ** 2).mean(-1, keepdim=True) + eps)
+        if w is not None:
+            y = y * w.float()
+        if cos is not None:
+            rows = torch.arange(x.shape[1]) if positions is None else positions.long()
+            c, s = cos[rows].unsqueeze(-2), sin[rows].unsqueeze(-2)
+            r = 2 * cos.shape[1]
+            first, second = (slice(0, r, 2), slice(1, r, 2)) if interleaved else (slice(0, r // 2), slice(r // 2, r))
+            out = y.clone()
+            out[..., first] = y[..., first] * c - y[..., second] * s
+            out[..., second] = y[..., second] * c + y[..., first] * s
+            y = out
+        return y.to(x.dtype)
+    return one(q, q_weight), one(k, k_weight)
+
+
+def diff_attention(q, k, v, lam, init, weight, eps, mask, kv_lengths, causal, start, scale):
+    """The difference of two softmax maps over the values, normed per head; rows that see nothing give 0."""
+    B, N, H, _, d = q.shape
+    M, Hk = k.shape[1:3]
+    seen = torch.ones(B, N, M, dtype=torch.bool)
+    if mask is not None:
+        seen &= ~mask
+    if kv_lengths is not None:
+        seen &= torch.arange(M) < kv_lengths.long()[:, None, None]
+    if causal:
+        first = start.long()[:, None, None] if isinstance(start, torch.Tensor) else start
+        seen &= torch.arange(M) <= first + torch.arange(N)[:, None]
+    share = torch.arange(H) // (H // Hk)
+    kh, vh = k.float()[:, :, share], v.float()[:, :, share].transpose(1, 2)
+    used = seen.any(1)[:, None, :, None]
+    vh = torch.where(used, vh, 0.0)
+    score = torch.where(seen[:, None, None], torch.einsum("bnhtd,bmhtd->bhtnm", q.float(), kh) * scale, -torch.inf)
+    top = score.detach().amax(-1, keepdim=True)
+    p = torch.exp(score - torch.where(torch.isinf(top), 0.0, top))
+    total = p.sum(-1, keepdim=True)
+    a = p / torch.where(total == 0, 1.0, total)
+    x = lam.float() if lam.dim() == 3 else lam.float()[:, None].expand(4, H, d)
+    l = (x[0] * x[1]).sum(-1).exp() - (x[2] * x[3]).sum(-1).exp() + init
+    u = ((a[:, :, 0] - l[:, None, None] * a[:, :, 1]) @ vh).transpose(1, 2)
+    if weight is not None:
+        u = (1 - init) * u / torch.sqrt((u ** 2).mean(-1, keepdim=True) + eps) * weight.float()
+    return u.to(q.dtype)
+
+
 def install():
     """Route CPU tensors of the HIP-backed operators to this module (tests / cpu baseline)."""
     import sys
