@@ -36,7 +36,7 @@ struct DiffArgs {
     const uint8_t *tiles;                       // [Bm][N64][M64] 0 free, 1 mixed, 2 blocked
     const int *kvlen, *qstart_dev;              // [B] or null
     void *out, *u, *o2;                         // [B, N, H, dv]; u, o2 (null: not kept) are read by the backward pass
-    float *stats;                               // [3][B, H, N]: lse of the two maps in the exp2 domain (+inf: an empty row), r
+    float *stats;                               // [4][B, H, N]: lse of the two maps in the exp2 domain (+inf: an empty row), r, beta
     int64_t qs[4], ks[4], vs[3];                // strides (batch, token, head, map)
     int64_t mask_b;                             // 0: one mask for the batch
     int64_t qstart;
@@ -124,6 +124,7 @@ template <typename T> __device__ __forceinline__ void da_store4(T *p, float a, f
     if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
     else *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d);
 }
+template <typename T> __device__ __forceinline__ float da_round(float v) { return sizeof(T) == 2 ? bf16_to_f32(f32_to_bf16(v)) : v; }
 template <typename T> __device__ __forceinline__ void da_load4(const T *p, float *f) {
     if constexpr (sizeof(T) == 2) {
         const uint2 u = *reinterpret_cast<const uint2 *>(p);
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_fwd_kernel(const DiffArg
 #pragma unroll
     for (int t = 0; t < 2; ++t) l[t] += __shfl_xor(l[t], 32);
     const float inv0 = l[0] > 0.f ? 1.f / l[0] : l[0], inv1 = l[1] > 0.f ? 1.f / l[1] : l[1];       // (a sum that is not a number stays one)
-    float ss = 0.f;
+    float ss = 0.f, us = 0.f;
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
 #pragma unroll
@@ -310,8 +311,11 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_fwd_kernel(const DiffArg
             o[1][x][r] *= inv1;
             o[0][x][r] = o[0][x][r] * inv0 - lam * o[1][x][r];
             ss += o[0][x][r] * o[0][x][r];
+            us += o[0][x][r] * o[1][x][r];
         }
     ss += __shfl_xor(ss, 32);
+    us += __shfl_xor(us, 32);
+    const float beta = a.weight && ss > 0.f ? us / ss : 0.f;     // what is kept of A_1 V is its part at right angles to U (diff_attn_prep_kernel)
     const float rn = a.weight ? rsqrtf(ss / (float)a.dv + a.eps) : 1.f;
     const int64_t orow = (((int64_t)b * a.N + i) * a.H + head) * a.dv;
 #pragma unroll
@@ -328,7 +332,8 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_fwd_kernel(const DiffArg
             da_store4(reinterpret_cast<T *>(a.out) + orow + c, u0 * w[0], u1 * w[1], u2 * w[2], u3 * w[3]);
             if (a.u) {
                 if (a.weight) da_store4(reinterpret_cast<T *>(a.u) + orow + c, u0, u1, u2, u3);
-                da_store4(reinterpret_cast<T *>(a.o2) + orow + c, o[1][x][4 * q4], o[1][x][4 * q4 + 1], o[1][x][4 * q4 + 2], o[1][x][4 * q4 + 3]);
+                da_store4(reinterpret_cast<T *>(a.o2) + orow + c, o[1][x][4 * q4] - beta * u0, o[1][x][4 * q4 + 1] - beta * u1, o[1][x][4 * q4 + 2] - beta * u2,
+                          o[1][x][4 * q4 + 3] - beta * u3);
             }
         }
     if (a.stats && h2 == 0) {
@@ -336,6 +341,7 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_fwd_kernel(const DiffArg
         a.stats[at] = l[0] > 0.f ? m[0] * a.scale_log2e + log2f(l[0]) : l[0] == 0.f ? INFINITY : l[0];
         a.stats[bhn + at] = l[1] > 0.f ? m[1] * a.scale_log2e + log2f(l[1]) : l[1] == 0.f ? INFINITY : l[1];
         a.stats[2 * bhn + at] = rn;
+        a.stats[3 * bhn + at] = beta;
     }
 }
 
@@ -374,7 +380,11 @@ __global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__re
 
 // ------------------------------------------------------------------------------------------------------------------
 // backward, first: dU (rounded to the type it is multiplied in), D_0, D_1 of every row and the partial sums of dl and dg.  Workgroup = (head, run of
-// (batch, query) rows); LPR lanes of 4 channels each per row
+// (batch, query) rows); 32 lanes of 4 channels each per row.
+// With a norm dU stands at right angles to U up to eps: dU . U = r (t . U) eps r^2 with t = (1 - init) g dY.  A_1 V mostly points along U (both are
+// near the mean of the values where the maps are flat), so dU . (A_1 V) of rounded vectors would be a small difference of large products.  The forward
+// pass therefore keeps W = A_1 V - beta U, beta = (A_1 V . U) / (U . U), and D_1 = r (t . W) + beta (dU . U), D_0 = dU . U + l D_1 (long rows, bf16: error of dl
+// and dq against 64 bits 0.0046 with A_1 V itself).  dP is made from the ROUNDED dU: what the rounding adds to D is added here too.
 template <typename T>
 __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, int nrun) {
     const int head = blockIdx.x % a.H, run = blockIdx.x / a.H;
@@ -399,32 +409,44 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
         }
         const bool empty = a.stats[at] == INFINITY;                                            // sees no key: no gradient, whatever dY holds
         const float rn = a.weight ? a.stats[2 * bhn + at] : 1.f;
-        float dot = 0.f, du[4];
+        const float beta = a.weight ? a.stats[3 * bhn + at] : 0.f;
+        float dot = 0.f, d1 = 0.f, e1r = 0.f, e2r = 0.f, du[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dot += u[j] * w[j] * dy[j];
+        for (int j = 0; j < 4; ++j) {
+            dot += u[j] * w[j] * dy[j];
+            d1 += w[j] * dy[j] * o2[j];
+        }
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) dot += __shfl_xor(dot, x);
-        dot *= rn * rn / (float)a.dv;
-        float d0 = 0.f, d1 = 0.f;
+        for (int x = 1; x < 32; x <<= 1) { dot += __shfl_xor(dot, x); d1 += __shfl_xor(d1, x); }
+        float uu = dot;                                                                        // dU . U
+        if (a.weight) {
+            uu = rn * dot * a.eps * rn * rn;
+            d1 = rn * d1 + beta * uu;
+            dot *= rn * rn / (float)a.dv;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (a.weight) {
                 du[j] = rn * (w[j] * dy[j] - u[j] * dot);
                 if (!empty) dw[j] += a.post * rn * u[j] * dy[j];
+                const float lost = da_round<T>(du[j]) - du[j];
+                e1r += lost * u[j];
+                e2r += lost * (o2[j] + beta * u[j]);
             } else {
                 du[j] = dy[j];
             }
             if (empty) du[j] = 0.f;
-            d0 += du[j] * (u[j] + lam * o2[j]);
-            d1 += du[j] * o2[j];
         }
+        if (sizeof(T) == 2 && a.weight) {
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) { d0 += __shfl_xor(d0, x); d1 += __shfl_xor(d1, x); }
-        if (empty) d0 = d1 = 0.f;
+            for (int x = 1; x < 32; x <<= 1) { e1r += __shfl_xor(e1r, x); e2r += __shfl_xor(e2r, x); }
+        }
+        float d0 = uu + lam * d1;
+        if (empty) d0 = d1 = e1r = e2r = 0.f;
         if (ok) da_store4(reinterpret_cast<T *>(a.du) + orow, du[0], du[1], du[2], du[3]);
         if (lane == 0) {
-            a.delta[at] = d0;
-            a.delta[bhn + at] = d1;
+            a.delta[at] = d0 + e1r + lam * e2r;
+            a.delta[bhn + at] = d1 + e2r;
         }
         dsum += d1;
     }

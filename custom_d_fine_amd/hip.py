@@ -1621,7 +1621,7 @@ def diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal,
     if keep:
         u = torch.empty_like(out) if weight is not None else None
         o2 = torch.empty_like(out)
-        stats = torch.empty(3, B, H, N, device=q.device, dtype=torch.float32)
+        stats = torch.empty(4, B, H, N, device=q.device, dtype=torch.float32)
     with _timed("diff_attention", 4.0 * B * H * N * M * (d + dv), io=float(q.element_size()) * (q.numel() + k.numel() + v.numel() + out.numel())):
         _check(_lib.dfine_diff_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(weight), _ptr(forms), _ptr(kv_len),
                                         None if isinstance(start, int) else _ptr(start), _ptr(out), _ptr(u), _ptr(o2), _ptr(stats),

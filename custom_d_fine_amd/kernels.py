@@ -2493,18 +2493,19 @@ def self_attention(qk, value, in_w, in_b, out_w, out_b, num_heads: int, attn_mas
 # =============================================================================================
 # attention block with normed, rotated heads and differential attention
 # =============================================================================================
-def _need(ok, what, kind=ValueError):
-    if not ok:
-        raise kind(f"custom_d_fine_amd.kernels.{what}")
-
-
-def _float_tensor(op, name, t, dtypes, device):
-    _need(isinstance(t, torch.Tensor) and t.dtype in dtypes, f"{op}: {name} is a {' or '.join(str(d)[6:] for d in dtypes)} tensor, got "
-          f"{getattr(t, 'dtype', type(t).__name__)}", TypeError)
-    _need(device is None or t.device == device, f"{op}: {name} is on {t.device}, the queries on {device}")
-
-
 _ACT_DTYPES = (torch.float32, torch.bfloat16)
+_INDEX_DTYPES = (torch.int32, torch.int64)
+
+
+def _refuse(what, kind=ValueError):
+    raise kind(f"custom_d_fine_amd.kernels.{what}")
+
+
+def _float_operand(op, name, t, device, dtypes=_ACT_DTYPES):
+    if not (isinstance(t, torch.Tensor) and t.dtype in dtypes):
+        _refuse(f"{op}: {name} is a {' or '.join(str(d)[6:] for d in dtypes)} tensor, got {getattr(t, 'dtype', type(t).__name__)}", TypeError)
+    if t.device != device:
+        _refuse(f"{op}: {name} is on {t.device}, the queries on {device}")
 
 
 class _QKNormRotate(torch.autograd.Function):
@@ -2534,41 +2535,58 @@ def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, posit
     pass.  positions: int32 / int64 [L] or [B, L]; a position outside the table gives NaN.  Gradients for q, k and the weights.
     -> (q', k'), contiguous, of q's type (k' None without k).  Under bf16 autocast q and k are cast to bfloat16 first."""
     op = "qk_norm_rotate"
-    _float_tensor(op, "q", q, _ACT_DTYPES, None)
+    device = q.device if isinstance(q, torch.Tensor) else None
+    _float_operand(op, "q", q, device)
     if k is not None:
-        _float_tensor(op, "k", k, _ACT_DTYPES, q.device)
-    if q.is_cuda and _bf16_autocast():
+        _float_operand(op, "k", k, device)
+    if q.is_cuda and torch.is_autocast_enabled() and _bf16_autocast():
         q, k = q.to(torch.bfloat16), None if k is None else k.to(torch.bfloat16)
-    _need(q.dim() == 4, f"{op}: q is [batch, tokens, heads, channels], got {tuple(q.shape)}")
-    D = q.shape[3]
-    _need(8 <= D <= 256 and D % 8 == 0, f"{op}: heads of {D} channels (multiples of 8 up to 256)")
+    if q.dim() != 4:
+        _refuse(f"{op}: q is [batch, tokens, heads, channels], got {tuple(q.shape)}")
+    B, L, H, D = q.shape
+    if not 8 <= D <= 256 or D % 8:
+        _refuse(f"{op}: heads of {D} channels (multiples of 8 up to 256)")
     if k is not None:
-        _need(k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == D, f"{op}: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
-        _need(k.dtype == q.dtype, f"{op}: k is {k.dtype}, q {q.dtype}", TypeError)
-    _need(q.shape[0] * q.shape[1] < 2 ** 31 - 65536 and q.shape[2] <= 4096 and (k is None or k.shape[2] <= 4096), f"{op}: too many tokens or heads")
-    _need(k is not None or k_weight is None, f"{op}: k_weight without k")
+        if k.dim() != 4 or k.shape[0] != B or k.shape[1] != L or k.shape[3] != D:
+            _refuse(f"{op}: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
+        if k.dtype != q.dtype:
+            _refuse(f"{op}: k is {k.dtype}, q {q.dtype}", TypeError)
+    if B * L >= 2 ** 31 - 65536 or H > 4096 or (k is not None and k.shape[2] > 4096):
+        _refuse(f"{op}: too many tokens or heads")
+    if k is None and k_weight is not None:
+        _refuse(f"{op}: k_weight without k")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None:
-            _float_tensor(op, name, w, _ACT_DTYPES, q.device)
-            _need(w.shape == (D,), f"{op}: {name} {tuple(w.shape)} for heads of {D} channels")
-    _need((cos is None) == (sin is None), f"{op}: cos and sin come together")
-    _need(positions is None or cos is not None, f"{op}: positions without a table")
-    if cos is not None:
-        for name, t in (("cos", cos), ("sin", sin)):
-            _float_tensor(op, name, t, (torch.float32,), q.device)
-        _need(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] % 4 == 0 and 0 < 2 * cos.shape[1] <= D and cos.shape[0] > 0,
-              f"{op}: tables {tuple(cos.shape)}, {tuple(sin.shape)} for heads of {D} channels (R a multiple of 8, at most {D})")
-        _need(not (cos.requires_grad or sin.requires_grad), f"{op}: the tables take no gradient")
+            _float_operand(op, name, w, device)
+            if w.shape != (D,):
+                _refuse(f"{op}: {name} {tuple(w.shape)} for heads of {D} channels")
+    if (cos is None) != (sin is None):
+        _refuse(f"{op}: cos and sin come together")
+    if cos is None:
+        if positions is not None:
+            _refuse(f"{op}: positions without a table")
+    else:
+        _float_operand(op, "cos", cos, device, (torch.float32,))
+        _float_operand(op, "sin", sin, device, (torch.float32,))
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] % 4 or not 0 < 2 * cos.shape[1] <= D or cos.shape[0] == 0:
+            _refuse(f"{op}: tables {tuple(cos.shape)}, {tuple(sin.shape)} for heads of {D} channels (R a multiple of 8, at most {D})")
+        if cos.requires_grad or sin.requires_grad:
+            _refuse(f"{op}: the tables take no gradient")
         if positions is None:
-            _need(q.shape[1] <= cos.shape[0], f"{op}: {q.shape[1]} tokens, {cos.shape[0]} rows in the table")
+            if L > cos.shape[0]:
+                _refuse(f"{op}: {L} tokens, {cos.shape[0]} rows in the table")
         else:
-            _need(isinstance(positions, torch.Tensor) and positions.dtype in (torch.int32, torch.int64), f"{op}: positions are int32 or int64", TypeError)
-            _need(positions.device == q.device, f"{op}: positions are on {positions.device}, the queries on {q.device}")
-            _need(positions.shape in (q.shape[1:2], q.shape[:2]), f"{op}: positions {tuple(positions.shape)} for {tuple(q.shape[:2])} tokens")
+            if not isinstance(positions, torch.Tensor) or positions.dtype not in _INDEX_DTYPES:
+                _refuse(f"{op}: positions are int32 or int64", TypeError)
+            if positions.device != device:
+                _refuse(f"{op}: positions are on {positions.device}, the queries on {device}")
+            if positions.shape != (B, L) and positions.shape != (L,):
+                _refuse(f"{op}: positions {tuple(positions.shape)} for {(B, L)} tokens")
             positions = positions.contiguous()
         cos, sin = cos.contiguous(), sin.contiguous()
     eps = float(eps)
-    _need(eps >= 0, f"{op}: eps {eps}")
+    if not eps >= 0:
+        _refuse(f"{op}: eps {eps}")
     if not q.is_cuda:
         return _backend_for_cpu(op)(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))
     wq, wk = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
@@ -2612,40 +2630,59 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
     Gradients for q, k, v, lambda_vectors and norm_weight, added up in a fixed order.  -> [B, N, H, dv], contiguous, of q's type.  Under bf16 autocast
     q, k, v are cast to bfloat16 first.  scale: d ** -0.5 by default."""
     op = "diff_attention"
-    _float_tensor(op, "q", q, _ACT_DTYPES, None)
-    for name, t in (("k", k), ("v", v)):
-        _float_tensor(op, name, t, _ACT_DTYPES, q.device)
-    if q.is_cuda and _bf16_autocast():
+    device = q.device if isinstance(q, torch.Tensor) else None
+    _float_operand(op, "q", q, device)
+    _float_operand(op, "k", k, device)
+    _float_operand(op, "v", v, device)
+    if q.is_cuda and torch.is_autocast_enabled() and _bf16_autocast():
         q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
-    _need(q.dtype == k.dtype == v.dtype, f"{op}: q is {q.dtype}, k {k.dtype}, v {v.dtype}", TypeError)
-    _need(q.dim() == 5 and q.shape[3] == 2, f"{op}: q is [batch, queries, heads, 2, channels], got {tuple(q.shape)}")
+    if not q.dtype == k.dtype == v.dtype:
+        _refuse(f"{op}: q is {q.dtype}, k {k.dtype}, v {v.dtype}", TypeError)
+    if q.dim() != 5 or q.shape[3] != 2:
+        _refuse(f"{op}: q is [batch, queries, heads, 2, channels], got {tuple(q.shape)}")
     B, N, H, _, d = q.shape
-    _need(k.dim() == 5 and k.shape[0] == B and k.shape[3:] == (2, d), f"{op}: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
-    M, Hk = k.shape[1:3]
-    _need(v.dim() == 4 and v.shape[:3] == k.shape[:3], f"{op}: v {tuple(v.shape)} does not go with k {tuple(k.shape)}")
+    if k.dim() != 5 or k.shape[0] != B or k.shape[3] != 2 or k.shape[4] != d:
+        _refuse(f"{op}: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
+    M, Hk = k.shape[1], k.shape[2]
+    if v.dim() != 4 or v.shape[:3] != k.shape[:3]:
+        _refuse(f"{op}: v {tuple(v.shape)} does not go with k {tuple(k.shape)}")
     dv = v.shape[3]
-    _need(8 <= d <= 64 and d % 8 == 0 and 8 <= dv <= 128 and dv % 8 == 0, f"{op}: heads of 2 x {d} channels with values of {dv} (multiples of 8 up to 64, 128)")
-    _need(1 <= Hk <= H <= 4096 and H % Hk == 0, f"{op}: {H} heads on {Hk} key heads")
-    _need(N < 2 ** 30 and M < 2 ** 30 and B < 2 ** 24 and B * Hk < 2 ** 24, f"{op}: {B} sequences of {N} queries and {M} keys")
-    _float_tensor(op, "lambda_vectors", lambda_vectors, _ACT_DTYPES, q.device)
-    _need(lambda_vectors.shape in ((4, d), (4, H, d)), f"{op}: lambda_vectors {tuple(lambda_vectors.shape)} for {H} heads of 2 x {d} channels")
+    if not 8 <= d <= 64 or d % 8 or not 8 <= dv <= 128 or dv % 8:
+        _refuse(f"{op}: heads of 2 x {d} channels with values of {dv} (multiples of 8 up to 64, 128)")
+    if not 1 <= Hk <= H <= 4096 or H % Hk:
+        _refuse(f"{op}: {H} heads on {Hk} key heads")
+    if N >= 2 ** 30 or M >= 2 ** 30 or B * Hk >= 2 ** 24:
+        _refuse(f"{op}: {B} sequences of {N} queries and {M} keys")
+    _float_operand(op, "lambda_vectors", lambda_vectors, device)
+    if lambda_vectors.shape != (4, d) and lambda_vectors.shape != (4, H, d):
+        _refuse(f"{op}: lambda_vectors {tuple(lambda_vectors.shape)} for {H} heads of 2 x {d} channels")
     if norm_weight is not None:
-        _float_tensor(op, "norm_weight", norm_weight, _ACT_DTYPES, q.device)
-        _need(norm_weight.shape == (dv,), f"{op}: norm_weight {tuple(norm_weight.shape)} for values of {dv} channels")
+        _float_operand(op, "norm_weight", norm_weight, device)
+        if norm_weight.shape != (dv,):
+            _refuse(f"{op}: norm_weight {tuple(norm_weight.shape)} for values of {dv} channels")
     if attn_mask is not None:
-        _need(isinstance(attn_mask, torch.Tensor) and attn_mask.dtype == torch.bool, f"{op}: attn_mask is a bool tensor, True = may not attend", TypeError)
-        _need(attn_mask.device == q.device, f"{op}: attn_mask is on {attn_mask.device}, the queries on {q.device}")
-        _need(attn_mask.shape in ((N, M), (B, N, M)), f"{op}: attn_mask {tuple(attn_mask.shape)} for {N} queries and {M} keys of {B} sequences")
+        if not isinstance(attn_mask, torch.Tensor) or attn_mask.dtype != torch.bool:
+            _refuse(f"{op}: attn_mask is a bool tensor, True = may not attend", TypeError)
+        if attn_mask.device != device:
+            _refuse(f"{op}: attn_mask is on {attn_mask.device}, the queries on {device}")
+        if attn_mask.shape != (N, M) and attn_mask.shape != (B, N, M):
+            _refuse(f"{op}: attn_mask {tuple(attn_mask.shape)} for {N} queries and {M} keys of {B} sequences")
     starts = isinstance(query_start, torch.Tensor)
     for name, t in (("kv_lengths", kv_lengths), ("query_start", query_start if starts else None)):
         if t is not None:
-            _need(isinstance(t, torch.Tensor) and t.dtype in (torch.int32, torch.int64), f"{op}: {name} is an int32 or int64 tensor", TypeError)
-            _need(t.device == q.device and t.shape == (B,), f"{op}: {name} {tuple(t.shape)} on {t.device} for {B} sequences on {q.device}")
-    _need(causal or (not starts and query_start == 0), f"{op}: query_start goes with causal")
-    _need(starts or -(2 ** 31) < int(query_start) < 2 ** 31, f"{op}: query_start {query_start}")
+            if not isinstance(t, torch.Tensor) or t.dtype not in _INDEX_DTYPES:
+                _refuse(f"{op}: {name} is an int32 or int64 tensor", TypeError)
+            if t.device != device or t.shape != (B,):
+                _refuse(f"{op}: {name} {tuple(t.shape)} on {t.device} for {B} sequences on {device}")
+    if not causal and (starts or query_start != 0):
+        _refuse(f"{op}: query_start goes with causal")
+    if not starts and not -(2 ** 31) < int(query_start) < 2 ** 31:
+        _refuse(f"{op}: query_start {query_start}")
     scale, init, eps = d ** -0.5 if scale is None else float(scale), float(lambda_init), float(norm_eps)
-    _need(0 < scale < float("inf"), f"{op}: scale {scale}")
-    _need(eps >= 0, f"{op}: norm_eps {eps}")
+    if not 0 < scale < float("inf"):
+        _refuse(f"{op}: scale {scale}")
+    if not eps >= 0:
+        _refuse(f"{op}: norm_eps {eps}")
     if not q.is_cuda:
         return _backend_for_cpu(op)(q, k, v, lambda_vectors, init, norm_weight, eps, attn_mask, kv_lengths, bool(causal), query_start, scale)
     lam, weight = lambda_vectors.contiguous(), None if norm_weight is None else norm_weight.contiguous()

@@ -832,7 +832,7 @@ int dfine_qk_norm_rotate_bwd(const void *q, const void *k, const void *wq, const
  * What query i of batch b sees: keys j < kv_len[b] (NULL: M; keys from there on are not read), j <= q_start[b] + i when causal (q_start NULL:
  * one start for all in shape), and where the mask lets it: mask_forms = the dfine_diff_attn_mask_words(batches, N, M) words that
  * dfine_diff_attn_mask makes of bytes [batches, N, M] (non-zero = may not attend; strides in bytes), batches 1 or B.
- * Forward for training keeps u, o2 (out's shape and type; u NULL without weight) and stats fp32 [3, B, H, N].
+ * Forward for training keeps u, o2 (out's shape and type; u NULL without weight) and stats fp32 [4, B, H, N].
  * shape (host int64): B, N, M, H, Hk, d, dv, dtype (0 fp32, 1 bf16), heads of lam, lam bf16, weight bf16, causal, q_start, mask has batches, then the
  * strides (batch, token, head, map) of q, of k, (batch, token, head) of v, of dy (elements; 16-byte rows).
  * Backward: dq, dk, dv contiguous (dq, or dk and dv, NULL: not wanted), dlam, dweight of lam's and weight's types (NULL: not wanted);
