@@ -171,178 +171,511 @@ __device__ __forceinline__ void da_stage(char *dst, const T *src, int64_t ld, in
     }
 }
 
-// ------------------------------------------------------------------------------------------------------------------
-// forward: workgroup = (batch, key head, 128 rows), a wave owns 32 rows; 64 keys at a time
-template <typename T, int DK>
-__global__ __launch_bounds__(kDaThreads) void diff_attn_fwd_kernel(const DiffArgs a) {
+// 16 bytes global -> LDS without registers; the LDS side is lane-linear from lds_addr (wave-uniform).  Inline assembly, waited for by hand (da_wait_copies):
+// behind the builtin the compiler waits for every copy in front of the next LDS read, which would end the overlap of copies and products.
+__device__ __forceinline__ void da_copy16(const void *src, uint32_t lds_addr) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(lds_addr) : "memory");
+}
+template <int N> __device__ __forceinline__ void da_wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void da_lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __attribute__((aligned(16))) uint32_t da_zero_page[4];            // what rows and channels that are not there are copied from
+
+// One operand's way into LDS: `ROWS` rows of U units by NT threads (a workgroup or a wave), this thread's part
+template <typename T, int DK, int ROWS, int NT> struct DaCopy {
     using C = DaCfg<T, DK>;
-    constexpr int KB = 64, NT = KB / 32;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *sK = lds, *sV = lds + KB * C::ROWB;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h2 = lane >> 5, l32 = lane & 31;
-    const int bh = blockIdx.x % (a.B * a.Hk), blk = blockIdx.x / (a.B * a.Hk), b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int64_t R = (int64_t)a.N * a.G;
-    const int64_t row = (int64_t)blk * 128 + wave * 32 + l32;
-    const bool rlive = row < R;
-    const int i = rlive ? (int)(row / a.G) : 0, g = rlive ? (int)(row - (int64_t)i * a.G) : 0, head = hk * a.G + g;
-    const int len = da_len(a, b);
-    const int64_t start = da_start(a, b);
-    const int limit = rlive ? da_limit(a, len, start, i) : 0;
-    const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
-    // queries of this wave / workgroup: the rows' range in i
-    const int64_t w0 = (int64_t)blk * 128 + wave * 32, wl = min(w0 + 31, R - 1);
-    const bool wlive = w0 < R;
-    const int i_lo = wlive ? (int)(w0 / a.G) : 0, i_hi = wlive ? (int)(wl / a.G) : 0;
-    const int blk_hi = (int)(min((int64_t)blk * 128 + 127, R - 1) / a.G);
-    const int wg_end = da_limit(a, len, start, blk_hi);
-
-    uint4 qf[2][C::NF];
-    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.qs[0] + i * a.qs[1] + head * a.qs[2];
+    static constexpr int J = ROWS * C::U / NT, STEP = NT / C::U, P = STEP >= 8 ? 1 : 8 / STEP;       // the swizzle repeats every 8 rows
+    static_assert(J >= 1 && STEP >= 1 && J % P == 0, "");
+    const T *base[P];                                   // row r0 of the tile at hand, this thread's channels
+    bool ok[P];
+    int r0;
+    __device__ __forceinline__ void init(const T *src, int64_t ld, int64_t map, int nch, bool maps, int t) {
+        r0 = t / C::U;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int f = 0; f < C::NF; ++f) {
-            const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
-            qf[t][f] = rlive && c < a.d ? *reinterpret_cast<const uint4 *>(qp + t * a.qs[3] + c) : make_uint4(0, 0, 0, 0);
+        for (int p = 0; p < P; ++p) {
+            const int u = (t % C::U) ^ da_swz<C::U>(r0 + p * STEP), half = maps ? u / (C::U / 2) : 0;
+            const int c = (maps ? u % (C::U / 2) : u) * (16 / C::ES);
+            ok[p] = c < nch;
+            base[p] = src + (int64_t)(r0 + p * STEP) * ld + half * map + c;
         }
-    da_f16v o[2][C::MT];
-    float m[2], l[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        m[t] = -INFINITY; l[t] = 0.f;
-#pragma unroll
-        for (int x = 0; x < C::MT; ++x)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[t][x][r] = 0.f;
     }
-    const T *kp = reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2];
-    const T *vp = reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2];
-    const int64_t mb = a.mask_b ? b : 0;
-
-    for (int k0 = 0; k0 < wg_end; k0 += KB) {
-        const int kt = k0 >> 6;
-        const uint64_t live = a.live ? a.live[mb * M64 + kt] : ~0ull;
-        __syncthreads();
-        da_stage<T, DK>(sK, kp + (int64_t)k0 * a.ks[1], a.ks[1], a.ks[3], a.d, true, KB, min(KB, len - k0), live, tid);
-        da_stage<T, DK>(sV, vp + (int64_t)k0 * a.vs[1], a.vs[1], 0, a.dv, false, KB, min(KB, len - k0), live, tid);
-        __syncthreads();
-        // this wave's tile: nothing visible / everything visible / some
-        if (!wlive) continue;
-        int code = 0;
-        if (a.tiles) {
-            const uint8_t *tp = a.tiles + mb * N64 * M64 + kt;
-            const int c0 = tp[(int64_t)(i_lo >> 6) * M64], c1 = tp[(int64_t)(i_hi >> 6) * M64];
-            code = c0 == c1 ? c0 : 1;
+    // rows [row0, row0 + ROWS) of the source into the tile at lds (this wave's first byte); rows >= valid and rows whose live bit is 0 become zeros
+    __device__ __forceinline__ void run(uint32_t lds, int64_t row0, int64_t ld, int valid, uint64_t live, bool whole) const {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const T *p = base[j % P] + (row0 + (j / P) * P * STEP) * ld;
+            if (!whole) {
+                const int r = r0 + j * STEP;
+                if (!(ok[j % P] && r < valid && ((live >> r) & 1))) p = reinterpret_cast<const T *>(da_zero_page);
+            }
+            da_copy16(p, __builtin_amdgcn_readfirstlane(lds + j * NT * 16));
         }
-        if (code == 2 || k0 >= da_limit(a, len, start, i_hi)) continue;
-        const bool cut = k0 + KB > da_limit(a, len, start, i_lo) || !wlive || wl - w0 < 31;
-        uint64_t vis = ~0ull;
-        if (code == 1 && rlive) vis = a.rowbits[(mb * a.N + i) * M64 + kt];
-        if (cut) vis &= limit <= k0 ? 0ull : limit >= k0 + 64 ? ~0ull : (1ull << (limit - k0)) - 1;
-        const bool masked = cut || code == 1;
+    }
+};
 
-        uint4 pf[2][NT][C::FPT];
+__device__ __forceinline__ float da_other_half_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float da_both_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// the rows of a wave: what the forward pass knows about the lane's row and the wave's range of queries
+struct DaRows {
+    int64_t row;
+    int i, head, limit, lim_lo, lim_hi, q_lo, q_hi;           // lim_*: ends of the first and last query's keys; q_*: their 64-query tiles
+    bool live, alive, ragged;                                 // this row / any row of the wave exists; some do not
+};
+__device__ __forceinline__ DaRows da_rows(const DiffArgs &a, int hk, int64_t w0, int l32, int len, int64_t start) {
+    DaRows w;
+    const int64_t R = (int64_t)a.N * a.G, wl = w0 + 31 < R - 1 ? w0 + 31 : R - 1;
+    w.row = w0 + l32;
+    w.live = w.row < R;
+    w.alive = w0 < R;
+    w.ragged = wl - w0 < 31;
+    w.i = w.live ? (int)(w.row / a.G) : 0;
+    w.head = hk * a.G + (w.live ? (int)(w.row - (int64_t)w.i * a.G) : 0);
+    w.limit = w.live ? da_limit(a, len, start, w.i) : 0;
+    const int i_lo = w.alive ? (int)(w0 / a.G) : 0, i_hi = w.alive ? (int)(wl / a.G) : 0;
+    w.lim_lo = da_limit(a, len, start, i_lo);
+    w.lim_hi = w.alive ? da_limit(a, len, start, i_hi) : 0;
+    w.q_lo = i_lo >> 6; w.q_hi = i_hi >> 6;
+    return w;
+}
+// what the mask says about (this wave's rows, 64 keys kt): 0 all free, 1 mixed, 2 all hidden
+__device__ __forceinline__ int da_tile_code(const DiffArgs &a, const DaRows &w, int64_t mb, int kt, int M64, int N64) {
+    if (!a.tiles) return 0;
+    const uint8_t *tp = a.tiles + mb * N64 * M64 + kt;
+    const int c0 = tp[(int64_t)w.q_lo * M64], c1 = tp[(int64_t)w.q_hi * M64];
+    return __builtin_amdgcn_readfirstlane(c0 == c1 ? c0 : 1);
+}
+
+template <typename T, int DK> struct DaState {
+    using C = DaCfg<T, DK>;
+    da_f16v o[2][C::MT];
+    float m[2], l[2];                                         // running maximum (exp2 domain) and this lane's part of the sum
+    __device__ __forceinline__ void init() {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            da_f16v s[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[nt][r] = 0.f;
-#pragma unroll
-                for (int f = 0; f < C::NF; ++f) s[nt] = Da<T>::mma(da_frag<C::U>(sK, nt * 32 + l32, t * (C::U / 2) + 2 * f + h2), qf[t][f], s[nt]);
-            }
-            if (masked) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (!((vis >> (nt * 32 + 8 * (r >> 2) + 4 * h2 + (r & 3))) & 1)) s[nt][r] = -INFINITY;
-            }
-            float bm = -INFINITY;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) bm = fmaxf(bm, s[nt][r]);
-            bm = fmaxf(bm, __shfl_xor(bm, 32));
-            const float mn = fmaxf(m[t], bm), mu = mn == -INFINITY ? 0.f : mn * a.scale_log2e;
-            const float alpha = da_exp2(fmaf(m[t], a.scale_log2e, -mu));
-            m[t] = mn;
-            float sum = 0.f;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[nt][r] = da_exp2(fmaf(s[nt][r], a.scale_log2e, -mu));
-                    sum += s[nt][r];
-                }
-#pragma unroll
-                for (int f = 0; f < C::FPT; ++f) pf[t][nt][f] = da_pack<T>(s[nt], f);
-            }
-            l[t] = l[t] * alpha + sum;                       // this lane's half of the keys; the halves meet at the end
+            m[t] = -INFINITY; l[t] = 0.f;
 #pragma unroll
             for (int x = 0; x < C::MT; ++x)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[t][x][r] *= alpha;
+                for (int r = 0; r < 16; ++r) o[t][x][r] = 0.f;
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int f = 0; f < C::FPT; ++f)
-#pragma unroll
-                for (int x = 0; x < C::MT; ++x) {
-                    const uint4 vf = da_frag_tr<T, C::U>(sV, nt * 32 + f * Da<T>::KPF, x * 32, lane);
-                    o[0][x] = Da<T>::mma(vf, pf[0][nt][f], o[0][x]);
-                    o[1][x] = Da<T>::mma(vf, pf[1][nt][f], o[1][x]);
-                }
     }
-    if (!rlive) return;                                      // (both lanes of a row go together)
-    float e1, e2;
-    da_lambda_parts(a, head, e1, e2);
-    const float lam = e1 - e2 + a.init;
+};
+
+template <typename T, int DK> __device__ __forceinline__ void da_load_q(const DiffArgs &a, const DaRows &w, int b, int h2, uint4 (*qf)[DaCfg<T, DK>::NF]) {
+    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.qs[0] + w.i * a.qs[1] + w.head * a.qs[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) l[t] += __shfl_xor(l[t], 32);
-    const float inv0 = l[0] > 0.f ? 1.f / l[0] : l[0], inv1 = l[1] > 0.f ? 1.f / l[1] : l[1];       // (a sum that is not a number stays one)
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int f = 0; f < DaCfg<T, DK>::NF; ++f) {
+            const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
+            qf[t][f] = w.live && c < a.d ? *reinterpret_cast<const uint4 *>(qp + t * a.qs[3] + c) : make_uint4(0, 0, 0, 0);
+        }
+}
+
+// 32 keys (rows r0 .. of the tiles in LDS) against the wave's 32 rows.  vis: bit per key of the lane's row, looked at where `masked`.
+// The running maximum moves only when some row's grows by more than 2^8 (in the exp2 domain, 8): the accumulators are then rescaled; below that the
+// probabilities are at most 256 times what the true maximum would give, which 32-bit sums and bf16's exponent hold without loss.
+template <typename T, int DK>
+__device__ __forceinline__ void da_fwd_tile(DaState<T, DK> &st, const uint4 (*qf)[DaCfg<T, DK>::NF], const char *sK, const char *sV, int r0, bool masked, uint32_t vis,
+                                            float c, int lane) {
+    using C = DaCfg<T, DK>;
+    const int h2 = lane >> 5, l32 = lane & 31;
+    uint4 pf[2][C::FPT];
+    vis >>= 4 * h2;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        da_f16v s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sK, r0 + l32, t * (C::U / 2) + 2 * f + h2), qf[t][f], s);
+        if (masked) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)vis, 8 * (r >> 2) + (r & 3), 1);
+                s[r] = __uint_as_float((__float_as_uint(s[r]) & on) | (0xff800000u & ~on));
+            }
+        }
+        float bm = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
+        bm = da_other_half_max(bm) * c;
+        if (__any(bm > st.m[t] + 8.f)) {
+            const float mn = fmaxf(st.m[t], bm), alpha = mn == -INFINITY ? 1.f : da_exp2(st.m[t] - mn);
+            st.m[t] = mn;
+            st.l[t] *= alpha;
+#pragma unroll
+            for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) st.o[t][x][r] *= alpha;
+        }
+        const float mu = st.m[t] == -INFINITY ? 0.f : st.m[t];
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = da_exp2(fmaf(s[r], c, -mu));
+            sum += s[r];
+        }
+        st.l[t] += sum;
+#pragma unroll
+        for (int f = 0; f < C::FPT; ++f) pf[t][f] = da_pack<T>(s, f);
+        if (C::ROWB > 256) __builtin_amdgcn_sched_barrier(0); // (fp32 heads of 64: all fragments asked for at once would not fit the registers)
+    }
+#pragma unroll
+    for (int f = 0; f < C::FPT; ++f)
+#pragma unroll
+        for (int x = 0; x < C::MT; ++x) {
+            if (C::ROWB > 256) __builtin_amdgcn_sched_barrier(0);
+            const uint4 vf = da_frag_tr<T, C::U>(sV, r0 + f * Da<T>::KPF, x * 32, lane);
+            st.o[0][x] = Da<T>::mma(vf, pf[0][f], st.o[0][x]);
+            st.o[1][x] = Da<T>::mma(vf, pf[1][f], st.o[1][x]);
+        }
+}
+
+__device__ __forceinline__ float da_inv(float l) { return l > 0.f ? 1.f / l : l; }                 // an empty row: 0; not a number stays that
+__device__ __forceinline__ float da_lse(float m, float l) { return l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l; }
+
+// ------------------------------------------------------------------------------------------------------------------
+// forward, many rows: workgroup = (batch, key head, 128 rows), a wave owns 32 rows; the keys stream through two LDS buffers of KB, copied while the block
+// in front is worked on (one barrier per block)
+template <typename T, int DK>
+__global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) void diff_attn_fwd_kernel(const DiffArgs a) {
+    using C = DaCfg<T, DK>;
+    constexpr int KB = sizeof(T) == 2 ? 64 : 32, TILE = KB * C::ROWB;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
+    const int bh = blockIdx.x % (a.B * a.Hk), blk = blockIdx.x / (a.B * a.Hk), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int len = da_len(a, b);
+    const int64_t start = da_start(a, b), R = (int64_t)a.N * a.G, blk0 = (int64_t)blk * 128;
+    const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
+    const int64_t mb = a.mask_b ? b : 0;
+    const DaRows w = da_rows(a, hk, blk0 + wave * 32, l32, len, start);
+    const int i_end = (int)((blk0 + 127 < R - 1 ? blk0 + 127 : R - 1) / a.G);
+    const int wg_end = da_limit(a, len, start, i_end), qt0 = (int)(blk0 / a.G) >> 6, qt1 = i_end >> 6;
+
+    uint4 qf[2][C::NF];
+    da_load_q<T, DK>(a, w, b, h2, qf);
+    DaState<T, DK> st;
+    st.init();
+    DaCopy<T, DK, KB, kDaThreads> ck, cv;
+    ck.init(reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.ks[3], a.d, true, tid);
+    cv.init(reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, a.dv, false, tid);
+    const bool full = a.d == DK && a.dv == C::DV;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 1024;
+    auto next = [&](int k0) {                                 // the next block that any row of the workgroup may see part of
+        for (; k0 < wg_end && a.tiles; k0 += KB) {
+            bool hidden = true;
+            for (int qt = qt0; qt <= qt1; ++qt) hidden = hidden && a.tiles[(mb * N64 + qt) * M64 + (k0 >> 6)] == 2;
+            if (!hidden) break;
+        }
+        return k0;
+    };
+    auto issue = [&](int k0, int buf) {
+        const int valid = len - k0;
+        const uint64_t live = a.live ? a.live[mb * M64 + (k0 >> 6)] >> (k0 & 63) : ~0ull;
+        const bool whole = full && valid >= KB && live == ~0ull;
+        ck.run(lds0 + buf * 2 * TILE, k0, a.ks[1], valid, live, whole);
+        cv.run(lds0 + buf * 2 * TILE + TILE, k0, a.vs[1], valid, live, whole);
+    };
+    int k0 = next(0), buf = 0;
+    if (k0 < wg_end) issue(k0, 0);
+    while (k0 < wg_end) {
+        const int kn = next(k0 + KB), code = da_tile_code(a, w, mb, k0 >> 6, M64, N64);
+        uint64_t vis = ~0ull;                                 // (loaded in front of the next copies: the wait for it would be a wait for them)
+        if (code == 1 && w.live) vis = a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63);
+        da_wait_copies<0>();
+        da_lds_done();
+        __builtin_amdgcn_s_barrier();                         // block k0 is there for every wave, and every wave is done with the buffer in front
+        if (kn < wg_end) issue(kn, buf ^ 1);
+        if (code != 2 && k0 < w.lim_hi) {
+            const bool cut = k0 + KB > w.lim_lo || w.ragged, masked = cut || code == 1;
+            if (cut) vis &= w.limit <= k0 ? 0ull : w.limit >= k0 + 64 ? ~0ull : (1ull << (w.limit - k0)) - 1;
+            const char *sK = lds + buf * 2 * TILE, *sV = sK + TILE;
+#pragma unroll 1
+            for (int nt = 0; nt < KB / 32; ++nt) da_fwd_tile<T, DK>(st, qf, sK, sV, nt * 32, masked, (uint32_t)(vis >> (32 * nt)), a.scale_log2e, lane);
+        }
+        k0 = kn;
+        buf ^= 1;
+    }
+    if (!w.live) return;                                      // (both lanes of a row go together)
+    float e1, e2;
+    da_lambda_parts(a, w.head, e1, e2);
+    const float lam = e1 - e2 + a.init;
+    const float l0 = da_both_halves(st.l[0]), l1 = da_both_halves(st.l[1]), inv0 = da_inv(l0), inv1 = da_inv(l1);
     float ss = 0.f, us = 0.f;
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            o[1][x][r] *= inv1;
-            o[0][x][r] = o[0][x][r] * inv0 - lam * o[1][x][r];
-            ss += o[0][x][r] * o[0][x][r];
-            us += o[0][x][r] * o[1][x][r];
+            st.o[1][x][r] *= inv1;
+            st.o[0][x][r] = st.o[0][x][r] * inv0 - lam * st.o[1][x][r];
+            ss += st.o[0][x][r] * st.o[0][x][r];
+            us += st.o[0][x][r] * st.o[1][x][r];
         }
-    ss += __shfl_xor(ss, 32);
-    us += __shfl_xor(us, 32);
-    const float beta = a.weight && ss > 0.f ? us / ss : 0.f;     // what is kept of A_1 V is its part at right angles to U (diff_attn_prep_kernel)
+    ss = da_both_halves(ss);
+    us = da_both_halves(us);
+    const float beta = a.weight && ss > 0.f ? us / ss : 0.f;  // what is kept of A_1 V is its part at right angles to U (diff_attn_prep_kernel)
     const float rn = a.weight ? rsqrtf(ss / (float)a.dv + a.eps) : 1.f;
-    const int64_t orow = (((int64_t)b * a.N + i) * a.H + head) * a.dv;
+    const int64_t orow = (((int64_t)b * a.N + w.i) * a.H + w.head) * a.dv;
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
             const int c = x * 32 + 8 * q4 + 4 * h2;
             if (c >= a.dv) continue;
-            float w[4] = {1.f, 1.f, 1.f, 1.f};
+            float g[4] = {1.f, 1.f, 1.f, 1.f};
             if (a.weight)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = da_load1(a.weight, c + j, a.w_bf16) * a.post * rn;
-            const float u0 = o[0][x][4 * q4], u1 = o[0][x][4 * q4 + 1], u2 = o[0][x][4 * q4 + 2], u3 = o[0][x][4 * q4 + 3];
-            da_store4(reinterpret_cast<T *>(a.out) + orow + c, u0 * w[0], u1 * w[1], u2 * w[2], u3 * w[3]);
-            if (a.u) {
+                for (int j = 0; j < 4; ++j) g[j] = da_load1(a.weight, c + j, a.w_bf16) * a.post * rn;
+            const float u0 = st.o[0][x][4 * q4], u1 = st.o[0][x][4 * q4 + 1], u2 = st.o[0][x][4 * q4 + 2], u3 = st.o[0][x][4 * q4 + 3];
+            da_store4(reinterpret_cast<T *>(a.out) + orow + c, u0 * g[0], u1 * g[1], u2 * g[2], u3 * g[3]);
+            if (a.o2) {
                 if (a.weight) da_store4(reinterpret_cast<T *>(a.u) + orow + c, u0, u1, u2, u3);
-                da_store4(reinterpret_cast<T *>(a.o2) + orow + c, o[1][x][4 * q4] - beta * u0, o[1][x][4 * q4 + 1] - beta * u1, o[1][x][4 * q4 + 2] - beta * u2,
-                          o[1][x][4 * q4 + 3] - beta * u3);
+                da_store4(reinterpret_cast<T *>(a.o2) + orow + c, st.o[1][x][4 * q4] - beta * u0, st.o[1][x][4 * q4 + 1] - beta * u1, st.o[1][x][4 * q4 + 2] - beta * u2,
+                          st.o[1][x][4 * q4 + 3] - beta * u3);
             }
         }
     if (a.stats && h2 == 0) {
-        const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + head) * a.N + i;
-        a.stats[at] = l[0] > 0.f ? m[0] * a.scale_log2e + log2f(l[0]) : l[0] == 0.f ? INFINITY : l[0];
-        a.stats[bhn + at] = l[1] > 0.f ? m[1] * a.scale_log2e + log2f(l[1]) : l[1] == 0.f ? INFINITY : l[1];
+        const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + w.head) * a.N + w.i;
+        a.stats[at] = da_lse(st.m[0], l0);
+        a.stats[bhn + at] = da_lse(st.m[1], l1);
         a.stats[2 * bhn + at] = rn;
         a.stats[3 * bhn + at] = beta;
     }
+}
+
+// One row of the result from its two maps' sums in plain order: LPR neighbouring lanes of NE channels each (c0: the lane's first), O normalised
+template <typename T, int NE, int LPR>
+__device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, int head, int c0, float *o0, float *o1, float lse0, float lse1, bool first) {
+    float e1, e2;
+    da_lambda_parts(a, head, e1, e2);
+    const float lam = e1 - e2 + a.init;
+    float ss = 0.f, us = 0.f;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+        o0[j] -= lam * o1[j];
+        ss += o0[j] * o0[j];
+        us += o0[j] * o1[j];
+    }
+#pragma unroll
+    for (int x = 1; x < LPR; x <<= 1) { ss += __shfl_xor(ss, x); us += __shfl_xor(us, x); }
+    const float beta = a.weight && ss > 0.f ? us / ss : 0.f;
+    const float rn = a.weight ? rsqrtf(ss / (float)a.dv + a.eps) : 1.f;
+    const int64_t orow = (((int64_t)b * a.N + i) * a.H + head) * a.dv;
+#pragma unroll
+    for (int j = 0; j < NE; j += 4) {
+        const int c = c0 + j;
+        if (c >= a.dv) continue;
+        float g[4] = {1.f, 1.f, 1.f, 1.f};
+        if (a.weight)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) g[x] = da_load1(a.weight, c + x, a.w_bf16) * a.post * rn;
+        da_store4(reinterpret_cast<T *>(a.out) + orow + c, o0[j] * g[0], o0[j + 1] * g[1], o0[j + 2] * g[2], o0[j + 3] * g[3]);
+        if (a.o2) {
+            if (a.weight) da_store4(reinterpret_cast<T *>(a.u) + orow + c, o0[j], o0[j + 1], o0[j + 2], o0[j + 3]);
+            da_store4(reinterpret_cast<T *>(a.o2) + orow + c, o1[j] - beta * o0[j], o1[j + 1] - beta * o0[j + 1], o1[j + 2] - beta * o0[j + 2], o1[j + 3] - beta * o0[j + 3]);
+        }
+    }
+    if (a.stats && first) {
+        const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + head) * a.N + i;
+        a.stats[at] = lse0;
+        a.stats[bhn + at] = lse1;
+        a.stats[2 * bhn + at] = rn;
+        a.stats[3 * bhn + at] = beta;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// forward, few rows: workgroup = (batch, key head, 32 rows, one of nsplit runs of the keys), its waves take every fourth tile of 32 keys of the run, each
+// through two LDS buffers of its own (no barrier until the end).  The waves' sums meet in LDS; with one run the rows are finished here, else the run's sums
+// go to `part` (rows x nsplit x 2 DV, with maxima and sums in `ml`) for diff_attn_join_kernel.
+template <typename T, int DK>
+__global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(const DiffArgs a, int nsplit, float *__restrict__ part, float4 *__restrict__ ml) {
+    using C = DaCfg<T, DK>;
+    constexpr int TILE = 32 * C::ROWB, NE = C::DV / 8, UO = 2 * C::DV / 4;
+    constexpr int NBUF = C::ROWB > 256 ? 1 : 2;               // (fp32 heads of 64: two buffers for four waves would not fit LDS)
+    constexpr int WBYTES = NBUF * 2 * TILE;                   // a wave's buffers, later its sums
+    static_assert(WBYTES >= 32 * 2 * C::DV * 4, "");
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ float sM[2][4][32], sS[2][4][32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
+    const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, rest = blockIdx.x / nbh, sp = rest % nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int64_t blk = rest / nsplit, R = (int64_t)a.N * a.G;
+    const int len = da_len(a, b);
+    const int64_t start = da_start(a, b);
+    const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
+    const int64_t mb = a.mask_b ? b : 0;
+    const DaRows w = da_rows(a, hk, blk * 32, l32, len, start);
+    const int tiles = (w.lim_hi + 31) >> 5, per = (tiles + nsplit - 1) / nsplit, t_end = min(tiles, (sp + 1) * per);
+
+    uint4 qf[2][C::NF];
+    da_load_q<T, DK>(a, w, b, h2, qf);
+    DaState<T, DK> st;
+    st.init();
+    DaCopy<T, DK, 32, 64> ck, cv;
+    constexpr int NCOPY = 2 * DaCopy<T, DK, 32, 64>::J;
+    ck.init(reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.ks[3], a.d, true, lane);
+    cv.init(reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, a.dv, false, lane);
+    const bool full = a.d == DK && a.dv == C::DV;
+    char *mine = lds + wave * WBYTES;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)mine;
+    auto next = [&](int t) {
+        while (t < t_end && da_tile_code(a, w, mb, t >> 1, M64, N64) == 2) t += 4;
+        return t;
+    };
+    auto issue = [&](int t, int buf) {
+        const int k0 = t * 32, valid = len - k0;
+        const uint64_t live = a.live ? a.live[mb * M64 + (k0 >> 6)] >> (k0 & 63) : ~0ull;
+        const bool whole = full && valid >= 32 && (uint32_t)live == ~0u;
+        ck.run(lds0 + buf * 2 * TILE, k0, a.ks[1], valid, live, whole);
+        cv.run(lds0 + buf * 2 * TILE + TILE, k0, a.vs[1], valid, live, whole);
+    };
+    int t = next(sp * per + wave), buf = 0;
+    if (t < t_end && NBUF == 2) issue(t, 0);
+    while (t < t_end) {
+        const int tn = next(t + 4), k0 = t * 32, code = da_tile_code(a, w, mb, k0 >> 6, M64, N64);
+        uint32_t vis = ~0u;                                   // (loaded in front of the next copies: the wait for it would be a wait for them)
+        if (code == 1 && w.live) vis = (uint32_t)(a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63));
+        asm volatile("" : "+v"(vis));
+        da_lds_done();                                        // the buffer in front has been read
+        if (NBUF == 1) {
+            issue(t, 0);
+            da_wait_copies<0>();
+        } else if (tn < t_end) {
+            issue(tn, buf ^ 1);
+            da_wait_copies<NCOPY>();                          // tile t is there; tile tn may be on its way
+        } else {
+            da_wait_copies<0>();
+        }
+        const bool cut = k0 + 32 > w.lim_lo || w.ragged, masked = cut || code == 1;
+        if (cut) vis &= w.limit <= k0 ? 0u : w.limit >= k0 + 32 ? ~0u : (1u << (w.limit - k0)) - 1;
+        da_fwd_tile<T, DK>(st, qf, mine + buf * 2 * TILE, mine + buf * 2 * TILE + TILE, 0, masked, vis, a.scale_log2e, lane);
+        t = tn;
+        buf ^= NBUF - 1;
+    }
+    // the four waves' sums: common maximum, then every wave's share of it through LDS (unit u of row r at u ^ (r % 16))
+    da_lds_done();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const float l = da_both_halves(st.l[x]);
+        if (h2 == 0) { sM[x][wave][l32] = st.m[x]; sS[x][wave][l32] = l; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        float mx = sM[x][0][l32];
+#pragma unroll
+        for (int v = 1; v < 4; ++v) mx = fmaxf(mx, sM[x][v][l32]);
+        const float f = mx == -INFINITY ? 1.f : da_exp2(st.m[x] - mx);
+#pragma unroll
+        for (int y = 0; y < C::MT; ++y)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                const int u = (x * C::DV + y * 32 + 8 * q4 + 4 * h2) >> 2;
+                const da_f16v &o = st.o[x][y];
+                *reinterpret_cast<float4 *>(mine + l32 * UO * 16 + ((u ^ (l32 & 15)) << 4)) = make_float4(o[4 * q4] * f, o[4 * q4 + 1] * f, o[4 * q4 + 2] * f, o[4 * q4 + 3] * f);
+            }
+    }
+    __syncthreads();
+    const int r = tid >> 3, c0 = (tid & 7) * NE;
+    const int64_t row = blk * 32 + r;
+    if (row >= R) return;
+    float o[2][NE], lse[2], mx[2], sum[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        mx[x] = fmaxf(fmaxf(sM[x][0][r], sM[x][1][r]), fmaxf(sM[x][2][r], sM[x][3][r]));
+        sum[x] = 0.f;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sum[x] += mx[x] == -INFINITY ? sS[x][v][r] : sS[x][v][r] * da_exp2(sM[x][v][r] - mx[x]);
+        lse[x] = da_lse(mx[x], sum[x]);
+#pragma unroll
+        for (int j = 0; j < NE; j += 4) {
+            const int u = (x * C::DV + c0 + j) >> 2;
+            float4 s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float4 z = *reinterpret_cast<const float4 *>(lds + v * WBYTES + r * UO * 16 + ((u ^ (r & 15)) << 4));
+                s4.x += z.x; s4.y += z.y; s4.z += z.z; s4.w += z.w;
+            }
+            o[x][j] = s4.x; o[x][j + 1] = s4.y; o[x][j + 2] = s4.z; o[x][j + 3] = s4.w;
+        }
+    }
+    const int i = (int)(row / a.G), head = hk * a.G + (int)(row - (int64_t)i * a.G);
+    if (nsplit == 1) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const float inv = da_inv(sum[x]);
+#pragma unroll
+            for (int j = 0; j < NE; ++j) o[x][j] *= inv;
+        }
+        da_finish_row<T, NE, 8>(a, b, i, head, c0, o[0], o[1], lse[0], lse[1], (tid & 7) == 0);
+        return;
+    }
+    const int64_t at = ((int64_t)bh * R + row) * nsplit + sp;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int j = 0; j < NE; j += 4) *reinterpret_cast<float4 *>(part + (at * 2 + x) * C::DV + c0 + j) = make_float4(o[x][j], o[x][j + 1], o[x][j + 2], o[x][j + 3]);
+    if ((tid & 7) == 0) ml[at] = make_float4(mx[0], sum[0], mx[1], sum[1]);
+}
+
+// joins the runs of a row: a wave per row, 8 lanes x DV / 8 channels, 8 runs side by side, in a fixed order
+template <typename T, int DV>
+__global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffArgs a, int nsplit, const float *__restrict__ part, const float4 *__restrict__ ml) {
+    constexpr int NE = DV / 8;
+    const int lane = threadIdx.x & 63, sg = lane >> 3, c0 = (lane & 7) * NE;
+    const int64_t R = (int64_t)a.N * a.G, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= R * a.B * a.Hk) return;
+    const int bh = (int)(at / R), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int64_t row = at - (int64_t)bh * R;
+    const int i = (int)(row / a.G), head = hk * a.G + (int)(row - (int64_t)i * a.G);
+    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, o[2][NE];
+    for (int s = lane; s < nsplit; s += 64) {
+        const float4 v = ml[at * nsplit + s];
+        mx[0] = fmaxf(mx[0], v.x);
+        mx[1] = fmaxf(mx[1], v.z);
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) { mx[0] = fmaxf(mx[0], __shfl_xor(mx[0], x)); mx[1] = fmaxf(mx[1], __shfl_xor(mx[1], x)); }
+#pragma unroll
+    for (int j = 0; j < NE; ++j) o[0][j] = o[1][j] = 0.f;
+    for (int s = sg; s < nsplit; s += 8) {
+        const float4 v = ml[at * nsplit + s];
+        const float f[2] = {mx[0] == -INFINITY ? 1.f : da_exp2(v.x - mx[0]), mx[1] == -INFINITY ? 1.f : da_exp2(v.z - mx[1])};
+        sum[0] += v.y * f[0];
+        sum[1] += v.w * f[1];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int j = 0; j < NE; j += 4) {
+                const float4 z = *reinterpret_cast<const float4 *>(part + ((at * nsplit + s) * 2 + x) * DV + c0 + j);
+                o[x][j] += z.x * f[x]; o[x][j + 1] += z.y * f[x]; o[x][j + 2] += z.z * f[x]; o[x][j + 3] += z.w * f[x];
+            }
+    }
+#pragma unroll
+    for (int y = 8; y < 64; y <<= 1)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            sum[x] += __shfl_xor(sum[x], y);
+#pragma unroll
+            for (int j = 0; j < NE; ++j) o[x][j] += __shfl_xor(o[x][j], y);
+        }
+    if (sg) return;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const float inv = da_inv(sum[x]);
+#pragma unroll
+        for (int j = 0; j < NE; ++j) o[x][j] *= inv;
+    }
+    da_finish_row<T, NE, 8>(a, b, i, head, c0, o[0], o[1], da_lse(mx[0], sum[0]), da_lse(mx[1], sum[1]), lane == 0);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -855,24 +1188,58 @@ int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_
 // the smallest of the three sizes that holds the head (values are twice as wide as a map's channels)
 static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <= 32 && dv <= 64 ? 32 : 64; }
 
-#define DA_DISPATCH(KERNEL, GRID, LDSROWS)                                                                                                                       \
+// dispatch on type and size; ROWS16, ROWS32: rows of 2 DK channels in LDS; DA_ARGS: the kernel's arguments
+#define DA_LAUNCH(K_, BYTES)                                                                                                                                      \
+    {                                                                                                                                                            \
+        const int by_ = (int)(BYTES);                                                                                                                            \
+        if (by_ > 64 * 1024) {                                                                                                                                   \
+            if (hipError_t e_ = hipFuncSetAttribute(reinterpret_cast<const void *>(K_), hipFuncAttributeMaxDynamicSharedMemorySize, by_); e_ != hipSuccess) {    \
+                set_last_error(e_);                                                                                                                              \
+                return DFINE_E_LAUNCH;                                                                                                                           \
+            }                                                                                                                                                    \
+        }                                                                                                                                                        \
+        hipLaunchKernelGGL(K_, grid_, block_, by_, st_, DA_ARGS);                                                                                                \
+    }
+#define DA_DISPATCH(KERNEL, GRID, ROWS16, ROWS32)                                                                                                                 \
     {                                                                                                                                                            \
         const int dk_ = diff_attn_size(a.d, a.dv);                                                                                                               \
-        const dim3 grid_(GRID);                                                                                                                                  \
+        const dim3 grid_(GRID), block_(kDaThreads);                                                                                                              \
         hipStream_t st_ = (hipStream_t)stream;                                                                                                                   \
         if (shape[7] == 0) {                                                                                                                                     \
-            if (dk_ == 16) hipLaunchKernelGGL((KERNEL<float, 16>), grid_, dim3(kDaThreads), 2 * LDSROWS * 128, st_, a);                                          \
-            else if (dk_ == 32) hipLaunchKernelGGL((KERNEL<float, 32>), grid_, dim3(kDaThreads), 2 * LDSROWS * 256, st_, a);                                     \
-            else hipLaunchKernelGGL((KERNEL<float, 64>), grid_, dim3(kDaThreads), 2 * LDSROWS * 512, st_, a);                                                    \
+            if (dk_ == 16) DA_LAUNCH((KERNEL<float, 16>), (ROWS32) * 128)                                                                                        \
+            else if (dk_ == 32) DA_LAUNCH((KERNEL<float, 32>), (ROWS32) * 256)                                                                                   \
+            else DA_LAUNCH((KERNEL<float, 64>), (ROWS32) * 512)                                                                                                  \
         } else {                                                                                                                                                 \
-            if (dk_ == 16) hipLaunchKernelGGL((KERNEL<uint16_t, 16>), grid_, dim3(kDaThreads), 2 * LDSROWS * 64, st_, a);                                        \
-            else if (dk_ == 32) hipLaunchKernelGGL((KERNEL<uint16_t, 32>), grid_, dim3(kDaThreads), 2 * LDSROWS * 128, st_, a);                                  \
-            else hipLaunchKernelGGL((KERNEL<uint16_t, 64>), grid_, dim3(kDaThreads), 2 * LDSROWS * 256, st_, a);                                                 \
+            if (dk_ == 16) DA_LAUNCH((KERNEL<uint16_t, 16>), (ROWS16) * 64)                                                                                      \
+            else if (dk_ == 32) DA_LAUNCH((KERNEL<uint16_t, 32>), (ROWS16) * 128)                                                                                \
+            else DA_LAUNCH((KERNEL<uint16_t, 64>), (ROWS16) * 256)                                                                                               \
         }                                                                                                                                                        \
     }
 
+// Runs of the keys a forward pass is cut into: 0 = the kernel for many rows (128 rows per workgroup, all keys), n >= 1 = the kernel for few (32 rows per
+// workgroup, n runs).
+static int diff_attn_splits(const DiffArgs &a) {
+    const int64_t R = (int64_t)a.N * a.G, bh = (int64_t)a.B * a.Hk;
+    if ((R + 127) / 128 * bh >= 256) return 0;
+    const int64_t wgs = (R + 31) / 32 * bh, most = ((int64_t)a.M + 255) / 256;           // a run has 256 keys (two tiles per wave) at least
+    int64_t n = 1024 / wgs;
+    if (n > most) n = most;
+    if (n > 256) n = 256;
+    return (int)(n < 1 ? 1 : n);
+}
+
+static int64_t da_up(int64_t x) { return (x + 255) / 256 * 256; }
+static int64_t diff_attn_rows(const DiffArgs &a) { return (int64_t)a.N * a.G * a.B * a.Hk; }
+int64_t dfine_diff_attn_fwd_ws_bytes(const int64_t *shape) {
+    DiffArgs a{};
+    if (!shape || diff_attn_setup(a, shape, 1.f, 0.f, 0.f)) return -1;
+    if (a.B == 0 || a.N == 0) return 0;
+    const int n = diff_attn_splits(a);
+    return n <= 1 ? 0 : da_up(diff_attn_rows(a) * n * 16) + diff_attn_rows(a) * n * 16 * diff_attn_size(a.d, a.dv);
+}
+
 int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms, const int *kv_len,
-                        const int *q_start, void *out, void *u, void *o2, float *stats, const int64_t *shape, float scale, float init, float eps, void *stream) {
+                        const int *q_start, void *out, void *u, void *o2, float *stats, void *ws, const int64_t *shape, float scale, float init, float eps, void *stream) {
     if (!shape) return DFINE_E_BADARG;
     DiffArgs a{};
     if (int e = diff_attn_setup(a, shape, scale, init, eps)) return e;
@@ -880,12 +1247,35 @@ int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void 
     if (!diff_attn_aligned(q) || !diff_attn_aligned(out) || !lam || (a.M && (!diff_attn_aligned(k) || !diff_attn_aligned(v)))) return DFINE_E_BADARG;
     if ((o2 != nullptr) != (stats != nullptr) || (u && !o2) || (o2 && weight && !u)) return DFINE_E_BADARG;
     a.q = q; a.k = k; a.v = v; a.lam = lam; a.weight = weight; a.kvlen = kv_len; a.qstart_dev = q_start;
-    a.out = out; a.u = o2 ? (u ? u : out) : nullptr; a.o2 = o2; a.stats = stats;
+    a.out = out; a.u = u; a.o2 = o2; a.stats = stats;
     a.post = weight ? 1.f - init : 1.f;
     diff_attn_forms(a, mask_forms, a.mask_b ? a.B : 1);
-    const int64_t blocks = ((int64_t)a.N * a.G + 127) / 128 * a.B * a.Hk;
+    const int n = diff_attn_splits(a);
+    const int64_t R = (int64_t)a.N * a.G, blocks = n ? (R + 31) / 32 * a.B * a.Hk * n : (R + 127) / 128 * a.B * a.Hk;
     if (blocks > 0x7fffffff) return DFINE_E_BADARG;
-    DA_DISPATCH(diff_attn_fwd_kernel, (unsigned)blocks, 64)
+    if (n == 0) {
+        #define DA_ARGS a
+        DA_DISPATCH(diff_attn_fwd_kernel, (unsigned)blocks, 256, 128)
+#undef DA_ARGS
+        return check_launch();
+    }
+    if (n > 1 && (!ws || ((uintptr_t)ws & 255))) return DFINE_E_BADARG;
+    float4 *ml = reinterpret_cast<float4 *>(ws);
+    float *part = n > 1 ? reinterpret_cast<float *>(reinterpret_cast<char *>(ws) + da_up(diff_attn_rows(a) * n * 16)) : nullptr;
+#define DA_ARGS a, n, part, ml
+    DA_DISPATCH(diff_attn_fwd_split_kernel, (unsigned)blocks, 512, dk_ == 64 ? 256 : 512)
+#undef DA_ARGS
+    if (int e = check_launch()) return e;
+    if (n == 1) return DFINE_OK;
+    const int64_t joins = (diff_attn_rows(a) + 3) / 4;
+    if (joins > 0x7fffffff) return DFINE_E_BADARG;
+    const int dk = diff_attn_size(a.d, a.dv);
+    const dim3 grid((unsigned)joins), block(kDaThreads);
+    hipStream_t st = (hipStream_t)stream;
+#define DA_JOIN(T_, DV_) hipLaunchKernelGGL((diff_attn_join_kernel<T_, DV_>), grid, block, 0, st, a, n, (const float *)part, (const float4 *)ml)
+    if (shape[7] == 0) { if (dk == 16) DA_JOIN(float, 32); else if (dk == 32) DA_JOIN(float, 64); else DA_JOIN(float, 128); }
+    else { if (dk == 16) DA_JOIN(uint16_t, 32); else if (dk == 32) DA_JOIN(uint16_t, 64); else DA_JOIN(uint16_t, 128); }
+#undef DA_JOIN
     return check_launch();
 }
 
@@ -897,7 +1287,6 @@ static int diff_attn_runs(const DiffArgs &a) {                  // workgroups pe
 }
 
 // workspace of the backward pass in bytes: dU, D_0 and D_1, the partial sums
-static int64_t da_up(int64_t x) { return (x + 255) / 256 * 256; }
 int64_t dfine_diff_attn_bwd_ws_bytes(const int64_t *shape) {
     DiffArgs a{};
     if (!shape || diff_attn_setup(a, shape, 1.f, 0.f, 0.f)) return -1;
@@ -905,6 +1294,7 @@ int64_t dfine_diff_attn_bwd_ws_bytes(const int64_t *shape) {
     return da_up(rows * a.dv * (shape[7] ? 2 : 4)) + da_up(rows * 8) + da_up(n * 4) + da_up(n * a.dv * 4);
 }
 
+#define DA_ARGS a
 int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms, const int *kv_len,
                         const int *q_start, const void *out, const void *u, const void *o2, const float *stats, const void *dy, void *dq, void *dk, void *dv,
                         void *dlam, void *dweight, void *ws, const int64_t *shape, float scale, float init, float eps, void *stream) {
@@ -943,17 +1333,19 @@ int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void 
     if (rows_ && dq) {
         const int64_t blocks = ((int64_t)a.N * a.G + 127) / 128 * a.B * a.Hk;
         if (blocks > 0x7fffffff) return DFINE_E_BADARG;
-        DA_DISPATCH(diff_attn_dq_kernel, (unsigned)blocks, 64)
+        DA_DISPATCH(diff_attn_dq_kernel, (unsigned)blocks, 128, 128)
         if (int e = check_launch()) return e;
     }
     if (keys_ && dk) {
         const int64_t blocks = ((int64_t)a.M + 127) / 128 * a.B * a.Hk;
         if (blocks > 0x7fffffff) return DFINE_E_BADARG;
-        DA_DISPATCH(diff_attn_dkdv_kernel, (unsigned)blocks, 32)
+        DA_DISPATCH(diff_attn_dkdv_kernel, (unsigned)blocks, 64, 64)
         if (int e = check_launch()) return e;
     }
     return DFINE_OK;
 }
+#undef DA_ARGS
 #undef DA_DISPATCH
+#undef DA_LAUNCH
 
 }  // extern "C"

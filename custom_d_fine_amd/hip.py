@@ -122,8 +122,9 @@ _SIGNATURES = {
     "dfine_qk_norm_rotate_bwd": (c_int, [_P] * 15 + [_F, _P]),
     "dfine_diff_attn_mask_words": (_L, [_L, _L, _L]),
     "dfine_diff_attn_mask": (c_int, [_P, _L, _L, _L, _L, _L, _P, _P]),
+    "dfine_diff_attn_fwd_ws_bytes": (_L, [_P]),
     "dfine_diff_attn_bwd_ws_bytes": (_L, [_P]),
-    "dfine_diff_attn_fwd": (c_int, [_P] * 13 + [_F, _F, _F, _P]),
+    "dfine_diff_attn_fwd": (c_int, [_P] * 14 + [_F, _F, _F, _P]),
     "dfine_diff_attn_bwd": (c_int, [_P] * 20 + [_F, _F, _F, _P]),
     "dfine_attn_mask_bits": (c_int, [_P, _I, _P, _P]),
     "dfine_groupnorm_ws_floats": (_L, [_I, _I, _I]),
@@ -1622,10 +1623,13 @@ def diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal,
         u = torch.empty_like(out) if weight is not None else None
         o2 = torch.empty_like(out)
         stats = torch.empty(4, B, H, N, device=q.device, dtype=torch.float32)
+    shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs)
+    nws = _lib.dfine_diff_attn_fwd_ws_bytes(shape)
+    ws = torch.empty(nws, device=q.device, dtype=torch.uint8) if nws > 0 else None
     with _timed("diff_attention", 4.0 * B * H * N * M * (d + dv), io=float(q.element_size()) * (q.numel() + k.numel() + v.numel() + out.numel())):
         _check(_lib.dfine_diff_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(weight), _ptr(forms), _ptr(kv_len),
-                                        None if isinstance(start, int) else _ptr(start), _ptr(out), _ptr(u), _ptr(o2), _ptr(stats),
-                                        _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs), scale, init, eps, _stream()), "dfine_diff_attn_fwd")
+                                        None if isinstance(start, int) else _ptr(start), _ptr(out), _ptr(u), _ptr(o2), _ptr(stats), _ptr(ws), shape, scale, init,
+                                        eps, _stream()), "dfine_diff_attn_fwd")
     return out, q, k, v, u, o2, stats
 
 

@@ -59,7 +59,7 @@ def test_c_entries_refuse_without_a_gpu():
     """Bad arguments come back as a status before anything touches a device."""
     from custom_d_fine_amd import hip
     shape = hip._DA_SHAPE(*([2, 5, 7, 4, 2, 16, 32, 1, 4, 1, 1, 0, 0, 0] + [8] * 14))
-    call = lambda s, scale=0.25, q=None: hip._lib.dfine_diff_attn_fwd(q, q, q, q, None, None, None, None, q, None, None, None, s, scale, 0.1, 1e-5, None)  # noqa: E731
+    call = lambda s, scale=0.25, q=None: hip._lib.dfine_diff_attn_fwd(q, q, q, q, None, None, None, None, q, None, None, None, None, s, scale, 0.1, 1e-5, None)  # noqa: E731
     assert call(shape) == -1                                                            # null pointers
     assert call(None) == -1
     for at, bad in ((3, 3), (5, 12), (5, 72), (6, 130), (7, 2), (8, 3), (14, 4)):
