@@ -46,7 +46,10 @@ struct DiffArgs {
     const void *dy;
     int64_t dys[3];
     void *du, *dq, *dk, *dvv;
-    float *delta, *lpart, *wpart;               // [2][B, H, N]; per workgroup of the first kernel: sum of D_1, sums of dg
+    float *rowstat;                             // [4][B, H, N]: lse_0, lse_1 - log2 |l|, D_0, sign(l) D_1 (diff_attn_prep_kernel)
+    float *lpart, *wpart;                       // per workgroup of the first kernel: sum of D_1, sums of dg
+    float *kvpart;                              // dK | dV sums of each run of the rows, fp32 [runs][B, M, Hk, 2 d + dv] (null: one run)
+    int kvruns;
 };
 
 template <typename T> struct Da;
@@ -136,16 +139,48 @@ template <typename T> __device__ __forceinline__ void da_load4(const T *p, float
     }
 }
 
-// exp(x0 . x1) and exp(x2 . x3) of a head
+// sum over the 64 lanes, the same in every lane
+__device__ __forceinline__ float da_wave_sum(float v) {
+#define DA_DPP(ctrl) __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, true))
+    v += DA_DPP(0xB1);                          // lane ^ 1
+    v += DA_DPP(0x4E);                          // lane ^ 2
+    v += DA_DPP(0x141);                         // mirrored in 8
+    v += DA_DPP(0x140);                         // mirrored in 16
+#undef DA_DPP
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// exp(x0 . x1) and exp(x2 . x3) of a head, by a whole wave: one channel per lane
 __device__ __forceinline__ void da_lambda_parts(const DiffArgs &a, int h, float &e1, float &e2) {
-    const int64_t hh = a.lam_heads == 1 ? 0 : h, st = (int64_t)a.lam_heads * a.d;
+    const int j = threadIdx.x & 63;
+    const int64_t st = (int64_t)a.lam_heads * a.d, o = (a.lam_heads == 1 ? 0 : (int64_t)h * a.d) + j;
     float s1 = 0.f, s2 = 0.f;
-    for (int j = 0; j < a.d; ++j) {
-        const int64_t o = hh * a.d + j;
-        s1 += da_load1(a.lam, o, a.lam_bf16) * da_load1(a.lam, st + o, a.lam_bf16);
-        s2 += da_load1(a.lam, 2 * st + o, a.lam_bf16) * da_load1(a.lam, 3 * st + o, a.lam_bf16);
+    if (j < a.d) {
+        const float x0 = da_load1(a.lam, o, a.lam_bf16), x1 = da_load1(a.lam, st + o, a.lam_bf16), x2 = da_load1(a.lam, 2 * st + o, a.lam_bf16),
+                    x3 = da_load1(a.lam, 3 * st + o, a.lam_bf16);
+        s1 = x0 * x1;
+        s2 = x2 * x3;
     }
-    e1 = expf(s1); e2 = expf(s2);
+    e1 = expf(da_wave_sum(s1));
+    e2 = expf(da_wave_sum(s2));
+}
+__device__ __forceinline__ float da_lambda(const DiffArgs &a, int h) {
+    float e1, e2;
+    da_lambda_parts(a, h, e1, e2);
+    return e1 - e2 + a.init;
+}
+// l of each lane's own head, for a wave whose rows start at w0: its rows' heads are min(G, 32) in a row (a whole wave calls this)
+__device__ __forceinline__ float da_lambda_rows(const DiffArgs &a, int hk, int64_t w0, int head) {
+    if (a.lam_heads == 1) return da_lambda(a, 0);
+    const int g0 = (int)(w0 % a.G), n = min(a.G, 32);
+    float lam = 0.f;
+    for (int x = 0; x < n; ++x) {
+        const int h = hk * a.G + (g0 + x) % a.G;
+        const float l = da_lambda(a, h);
+        if (h == head) lam = l;
+    }
+    return lam;
 }
 
 // keys that row i of batch b may look at end here
@@ -156,20 +191,6 @@ __device__ __forceinline__ int da_limit(const DiffArgs &a, int len, int64_t star
 }
 __device__ __forceinline__ int da_len(const DiffArgs &a, int b) { return a.kvlen ? min(max(a.kvlen[b], 0), a.M) : a.M; }
 __device__ __forceinline__ int64_t da_start(const DiffArgs &a, int b) { return a.qstart_dev ? (int64_t)a.qstart_dev[b] : a.qstart; }
-
-// global -> LDS, `rows` rows of 2 DK channels: k-like (two maps of d channels) or v-like (dv channels); dead rows and channels become zeros
-template <typename T, int DK>
-__device__ __forceinline__ void da_stage(char *dst, const T *src, int64_t ld, int64_t map, int nch, bool maps, int rows, int valid, uint64_t live, int tid) {
-    using C = DaCfg<T, DK>;
-    constexpr int CH = 16 / C::ES;                           // channels per unit
-    for (int it = tid; it < rows * C::U; it += kDaThreads) {
-        const int r = it / C::U, u = it % C::U;
-        const int t = maps ? u / (C::U / 2) : 0, c = (maps ? u % (C::U / 2) : u) * CH;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < valid && ((live >> r) & 1) && c < nch) x = *reinterpret_cast<const uint4 *>(src + (int64_t)r * ld + t * map + c);
-        *reinterpret_cast<uint4 *>(dst + r * C::U * 16 + ((u ^ da_swz<C::U>(r)) << 4)) = x;
-    }
-}
 
 // 16 bytes global -> LDS without registers; the LDS side is lane-linear from lds_addr (wave-uniform).  Inline assembly, waited for by hand (da_wait_copies):
 // behind the builtin the compiler waits for every copy in front of the next LDS read, which would end the overlap of copies and products.
@@ -352,7 +373,8 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     constexpr int KB = sizeof(T) == 2 ? 64 : 32, TILE = KB * C::ROWB;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
-    const int bh = blockIdx.x % (a.B * a.Hk), blk = blockIdx.x / (a.B * a.Hk), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, nblk = gridDim.x / nbh, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int blk = a.causal ? nblk - 1 - (int)(blockIdx.x / nbh) : (int)(blockIdx.x / nbh);          // causal: the longest first
     const int len = da_len(a, b);
     const int64_t start = da_start(a, b), R = (int64_t)a.N * a.G, blk0 = (int64_t)blk * 128;
     const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
@@ -387,6 +409,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     };
     int k0 = next(0), buf = 0;
     if (k0 < wg_end) issue(k0, 0);
+    const float lam = da_lambda_rows(a, hk, blk0 + wave * 32, w.head);
     while (k0 < wg_end) {
         const int kn = next(k0 + KB), code = da_tile_code(a, w, mb, k0 >> 6, M64, N64);
         uint64_t vis = ~0ull;                                 // (loaded in front of the next copies: the wait for it would be a wait for them)
@@ -406,9 +429,6 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         buf ^= 1;
     }
     if (!w.live) return;                                      // (both lanes of a row go together)
-    float e1, e2;
-    da_lambda_parts(a, w.head, e1, e2);
-    const float lam = e1 - e2 + a.init;
     const float l0 = da_both_halves(st.l[0]), l1 = da_both_halves(st.l[1]), inv0 = da_inv(l0), inv1 = da_inv(l1);
     float ss = 0.f, us = 0.f;
 #pragma unroll
@@ -454,10 +474,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
 
 // One row of the result from its two maps' sums in plain order: LPR neighbouring lanes of NE channels each (c0: the lane's first), O normalised
 template <typename T, int NE, int LPR>
-__device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, int head, int c0, float *o0, float *o1, float lse0, float lse1, bool first) {
-    float e1, e2;
-    da_lambda_parts(a, head, e1, e2);
-    const float lam = e1 - e2 + a.init;
+__device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, int head, float lam, int c0, float *o0, float *o1, float lse0, float lse1, bool first) {
     float ss = 0.f, us = 0.f;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
@@ -505,7 +522,7 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
     constexpr int WBYTES = NBUF * 2 * TILE;                   // a wave's buffers, later its sums
     static_assert(WBYTES >= 32 * 2 * C::DV * 4, "");
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ float sM[2][4][32], sS[2][4][32];
+    __shared__ float sM[2][4][32], sS[2][4][32], sLam[32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, rest = blockIdx.x / nbh, sp = rest % nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int64_t blk = rest / nsplit, R = (int64_t)a.N * a.G;
@@ -540,6 +557,10 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
     };
     int t = next(sp * per + wave), buf = 0;
     if (t < t_end && NBUF == 2) issue(t, 0);
+    if (wave == 0 && nsplit == 1) {
+        const float lam = da_lambda_rows(a, hk, blk * 32, w.head);
+        if (h2 == 0) sLam[l32] = lam;
+    }
     while (t < t_end) {
         const int tn = next(t + 4), k0 = t * 32, code = da_tile_code(a, w, mb, k0 >> 6, M64, N64);
         uint32_t vis = ~0u;                                   // (loaded in front of the next copies: the wait for it would be a wait for them)
@@ -616,7 +637,7 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
 #pragma unroll
             for (int j = 0; j < NE; ++j) o[x][j] *= inv;
         }
-        da_finish_row<T, NE, 8>(a, b, i, head, c0, o[0], o[1], lse[0], lse[1], (tid & 7) == 0);
+        da_finish_row<T, NE, 8>(a, b, i, head, sLam[r], c0, o[0], o[1], lse[0], lse[1], (tid & 7) == 0);
         return;
     }
     const int64_t at = ((int64_t)bh * R + row) * nsplit + sp;
@@ -637,6 +658,7 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
     const int bh = (int)(at / R), b = bh / a.Hk, hk = bh - b * a.Hk;
     const int64_t row = at - (int64_t)bh * R;
     const int i = (int)(row / a.G), head = hk * a.G + (int)(row - (int64_t)i * a.G);
+    const float lam = da_lambda(a, head);
     float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, o[2][NE];
     for (int s = lane; s < nsplit; s += 64) {
         const float4 v = ml[at * nsplit + s];
@@ -647,6 +669,7 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
     for (int x = 1; x < 64; x <<= 1) { mx[0] = fmaxf(mx[0], __shfl_xor(mx[0], x)); mx[1] = fmaxf(mx[1], __shfl_xor(mx[1], x)); }
 #pragma unroll
     for (int j = 0; j < NE; ++j) o[0][j] = o[1][j] = 0.f;
+#pragma unroll 2
     for (int s = sg; s < nsplit; s += 8) {
         const float4 v = ml[at * nsplit + s];
         const float f[2] = {mx[0] == -INFINITY ? 1.f : da_exp2(v.x - mx[0]), mx[1] == -INFINITY ? 1.f : da_exp2(v.z - mx[1])};
@@ -675,31 +698,40 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
 #pragma unroll
         for (int j = 0; j < NE; ++j) o[x][j] *= inv;
     }
-    da_finish_row<T, NE, 8>(a, b, i, head, c0, o[0], o[1], da_lse(mx[0], sum[0]), da_lse(mx[1], sum[1]), lane == 0);
+    da_finish_row<T, NE, 8>(a, b, i, head, lam, c0, o[0], o[1], da_lse(mx[0], sum[0]), da_lse(mx[1], sum[1]), lane == 0);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// mask [Bm][N][M] bytes (strides mb, mn; non-zero = blocked) -> the forms the kernels read.  Workgroup = (batch, 64 keys), all queries: a wave takes every
-// fourth tile of 64 queries; lane = key, one ballot per query
-__global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sn, int N, int M, uint64_t *__restrict__ rowbits,
-                                                             uint64_t *__restrict__ colbits, uint64_t *__restrict__ live, uint8_t *__restrict__ tiles) {
+// mask [Bm][N][M] bytes (strides sb, sn; non-zero = blocked) -> the forms the kernels read.  Workgroup = (batch, 64 keys), all queries: each of its 16 waves
+// takes every 16th tile of 64 queries; lane = key, one ballot per query, 16 loads in flight
+__global__ __launch_bounds__(1024) void diff_attn_mask_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sn, int N, int M, uint64_t *__restrict__ rowbits,
+                                                              uint64_t *__restrict__ colbits, uint64_t *__restrict__ live, uint8_t *__restrict__ tiles) {
     const int M64 = (M + 63) >> 6, N64 = (N + 63) >> 6;
     const int kt = blockIdx.x % M64;
     const int64_t b = blockIdx.x / M64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, key = kt * 64 + lane;
     const uint64_t inside = M - kt * 64 >= 64 ? ~0ull : (1ull << (M - kt * 64)) - 1;
-    __shared__ uint64_t any_s[4];
+    const uint8_t *col_p = mask + b * sb + min(key, M - 1);
+    __shared__ uint64_t any_s[16];
     uint64_t any = 0;
-    for (int nt = wave; nt < N64; nt += 4) {
+    for (int nt = wave; nt < N64; nt += 16) {
         uint64_t col = 0, all = inside, some = 0, mine = 0;
         const int n1 = min(64, N - nt * 64);
-        for (int n = 0; n < n1; ++n) {
-            const bool see = key < M && mask[b * sb + (int64_t)(nt * 64 + n) * sn + key] == 0;
-            const uint64_t bits = __ballot(see);
-            if (see) col |= 1ull << n;
-            if (n == lane) mine = bits;
-            all &= bits;
-            some |= bits;
+        for (int n0 = 0; n0 < n1; n0 += 16) {
+            uint8_t v[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) v[x] = col_p[(int64_t)min(nt * 64 + n0 + x, N - 1) * sn];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const int n = n0 + x;
+                if (n >= n1) break;
+                const bool see = key < M && v[x] == 0;
+                const uint64_t bits = __ballot(see);
+                if (see) col |= 1ull << n;
+                if (n == lane) mine = bits;
+                all &= bits;
+                some |= bits;
+            }
         }
         if (lane < n1) rowbits[(b * N + nt * 64 + lane) * M64 + kt] = mine;
         if (key < M) colbits[(b * M + key) * N64 + nt] = col;
@@ -708,7 +740,11 @@ __global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__re
     }
     if (lane == 0) any_s[wave] = any;
     __syncthreads();
-    if (threadIdx.x == 0) live[b * M64 + kt] = any_s[0] | any_s[1] | any_s[2] | any_s[3];
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int x = 1; x < 16; ++x) any |= any_s[x];
+        live[b * M64 + kt] = any;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -718,15 +754,14 @@ __global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__re
 // near the mean of the values where the maps are flat), so dU . (A_1 V) of rounded vectors would be a small difference of large products.  The forward
 // pass therefore keeps W = A_1 V - beta U, beta = (A_1 V . U) / (U . U), and D_1 = r (t . W) + beta (dU . U), D_0 = dU . U + l D_1 (long rows, bf16: error of dl
 // and dq against 64 bits 0.0046 with A_1 V itself).  dP is made from the ROUNDED dU: what the rounding adds to D is added here too.
+// The other kernels read the rows' statistics with l worked in: exp2(s - (lse_1 - log2 |l|)) is |l| A_1, and its sign goes with D_1 and dP.
 template <typename T>
 __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, int nrun) {
     const int head = blockIdx.x % a.H, run = blockIdx.x / a.H;
     const int lane = threadIdx.x & 31, rr = threadIdx.x >> 5;                       // 32 lanes x 4 channels cover dv <= 128
     const int c = lane * 4;
     const bool ok = c < a.dv;
-    float e1, e2;
-    da_lambda_parts(a, head, e1, e2);
-    const float lam = e1 - e2 + a.init;
+    const float lam = da_lambda(a, head), log2l = log2f(fabsf(lam)), sign = lam < 0.f ? -1.f : 1.f;
     float w[4], dw[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = !ok ? 0.f : a.weight ? a.post * da_load1(a.weight, c + j, a.w_bf16) : 1.f;
@@ -778,8 +813,10 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
         if (empty) d0 = d1 = e1r = e2r = 0.f;
         if (ok) da_store4(reinterpret_cast<T *>(a.du) + orow, du[0], du[1], du[2], du[3]);
         if (lane == 0) {
-            a.delta[at] = d0 + e1r + lam * e2r;
-            a.delta[bhn + at] = d1 + e2r;
+            a.rowstat[at] = a.stats[at];
+            a.rowstat[bhn + at] = a.stats[bhn + at] - log2l;
+            a.rowstat[2 * bhn + at] = d0 + e1r + lam * e2r;
+            a.rowstat[3 * bhn + at] = (d1 + e2r) * sign;
         }
         dsum += d1;
     }
@@ -802,98 +839,150 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
     }
 }
 
-// gradients of the learned vectors and of the norm weight from the first kernel's partial sums (one workgroup per head / per 16 channels; in order)
-__global__ __launch_bounds__(256) void diff_attn_param_kernel(const DiffArgs a, int nrun, void *dlam, void *dw) {
+// gradients of the learned vectors and of the norm weight from the first kernel's partial sums, in a fixed order: one workgroup per head (or one for shared
+// vectors), then one per 32 channels of the weight (32 interleaved runs of the partial rows, 8 loads in flight)
+__global__ __launch_bounds__(1024) void diff_attn_param_kernel(const DiffArgs a, int nrun, void *dlam, void *dw) {
     const int tid = threadIdx.x;
-    __shared__ float s[16][17];
-    __shared__ float dl_s[256];
+    __shared__ float s[32][33];
     const int nh = a.lam_heads == 1 ? 1 : a.H;
     if ((int)blockIdx.x < nh) {
         if (!dlam) return;
         // sum over runs (and over all heads where they share the vectors; their exponentials are then one pair)
+        const int h0 = a.lam_heads == 1 ? 0 : blockIdx.x, nhead = a.lam_heads == 1 ? a.H : 1;
         float v = 0.f;
-        const int h0 = a.lam_heads == 1 ? 0 : blockIdx.x, h1 = a.lam_heads == 1 ? a.H : h0 + 1;
-        for (int x = tid; x < nrun * (h1 - h0); x += 256) v += a.lpart[(x / (h1 - h0)) * a.H + h0 + x % (h1 - h0)];
-        dl_s[tid] = v;
-        __syncthreads();
-        for (int x = 128; x > 0; x >>= 1) {
-            if (tid < x) dl_s[tid] += dl_s[tid + x];
-            __syncthreads();
-        }
-        const float dl = -dl_s[0];
+        for (int x = tid; x < nrun * nhead; x += 1024) v += a.lpart[(x / nhead) * a.H + h0 + x % nhead];
+        v = da_wave_sum(v);
+        if ((tid & 63) == 0) s[0][tid >> 6] = v;
         float e1, e2;
         da_lambda_parts(a, h0, e1, e2);
+        __syncthreads();
+        float dl = 0.f;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) dl -= s[0][x];
         const int64_t st = (int64_t)a.lam_heads * a.d, o = (a.lam_heads == 1 ? 0 : (int64_t)h0 * a.d);
-        for (int x = tid; x < 4 * a.d; x += 256) {
-            const int vec = x / a.d, j = x - vec * a.d;
-            const float other = da_load1(a.lam, (vec ^ 1) * st + o + j, a.lam_bf16), gr = dl * (vec < 2 ? e1 : -e2) * other;
-            if (a.lam_bf16) reinterpret_cast<uint16_t *>(dlam)[vec * st + o + j] = f32_to_bf16(gr);
-            else reinterpret_cast<float *>(dlam)[vec * st + o + j] = gr;
-        }
+        if (tid >= 4 * a.d) return;
+        const int vec = tid / a.d, j = tid - vec * a.d;
+        const float other = da_load1(a.lam, (vec ^ 1) * st + o + j, a.lam_bf16), gr = dl * (vec < 2 ? e1 : -e2) * other;
+        if (a.lam_bf16) reinterpret_cast<uint16_t *>(dlam)[vec * st + o + j] = f32_to_bf16(gr);
+        else reinterpret_cast<float *>(dlam)[vec * st + o + j] = gr;
         return;
     }
     if (!dw) return;
-    const int col = tid & 15, r0 = tid >> 4, ch = (blockIdx.x - nh) * 16 + col, rows = nrun * a.H;
+    const int col = tid & 31, r0 = tid >> 5, ch = (blockIdx.x - nh) * 32 + col, rows = nrun * a.H;
     float v = 0.f;
-    if (ch < a.dv)
-        for (int r = r0; r < rows; r += 16) v += a.wpart[(int64_t)r * a.dv + ch];
+    if (ch < a.dv) {
+#pragma unroll 8
+        for (int r = r0; r < rows; r += 32) v += a.wpart[(int64_t)r * a.dv + ch];
+    }
     s[r0][col] = v;
     __syncthreads();
     if (r0 || ch >= a.dv) return;
 #pragma unroll
-    for (int r = 1; r < 16; ++r) v += s[r][col];
+    for (int r = 1; r < 32; ++r) v += s[r][col];
     if (a.w_bf16) reinterpret_cast<uint16_t *>(dw)[ch] = f32_to_bf16(v);
     else reinterpret_cast<float *>(dw)[ch] = v;
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// backward, dQ: the forward's decomposition; probabilities from the saved statistics
+// backward, dQ: the forward's decomposition and copies; probabilities from the saved statistics
 template <typename T, int DK>
-__global__ __launch_bounds__(kDaThreads) void diff_attn_dq_kernel(const DiffArgs a) {
+__device__ __forceinline__ void da_dq_tile(const DiffArgs &a, da_f16v (*dq)[DaCfg<T, DK>::MTK], const uint4 (*qf)[DaCfg<T, DK>::NF], const uint4 *uf, const float *lse, const float *dl, float sign,
+                                           const char *sK, const char *sV, int r0, bool masked, uint32_t vis, int lane) {
     using C = DaCfg<T, DK>;
-    constexpr int KB = 64, NT = KB / 32;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *sK = lds, *sV = lds + KB * C::ROWB;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h2 = lane >> 5, l32 = lane & 31;
-    const int bh = blockIdx.x % (a.B * a.Hk), blk = blockIdx.x / (a.B * a.Hk), b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int64_t R = (int64_t)a.N * a.G;
-    const int64_t row = (int64_t)blk * 128 + wave * 32 + l32;
-    const bool rlive = row < R;
-    const int i = rlive ? (int)(row / a.G) : 0, g = rlive ? (int)(row - (int64_t)i * a.G) : 0, head = hk * a.G + g;
-    const int len = da_len(a, b);
-    const int64_t start = da_start(a, b);
-    const int limit = rlive ? da_limit(a, len, start, i) : 0;
-    const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
-    const int64_t w0 = (int64_t)blk * 128 + wave * 32, wl = min(w0 + 31, R - 1);
-    const bool wlive = w0 < R;
-    const int i_lo = wlive ? (int)(w0 / a.G) : 0, i_hi = wlive ? (int)(wl / a.G) : 0;
-    const int wg_end = da_limit(a, len, start, (int)(min((int64_t)blk * 128 + 127, R - 1) / a.G));
-
-    float e1, e2;
-    da_lambda_parts(a, head, e1, e2);
-    const float lam = e1 - e2 + a.init;
-    const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + head) * a.N + i;
-    uint4 qf[2][C::NF], uf[C::NFV];
-    float lse[2], dl[2];
-    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.qs[0] + i * a.qs[1] + head * a.qs[2];
-    const T *up = reinterpret_cast<const T *>(a.du) + (((int64_t)b * a.N + i) * a.H + head) * a.dv;
+    const int h2 = lane >> 5, l32 = lane & 31;
+    const float c = a.scale_log2e;
+    vis >>= 4 * h2;
+    da_f16v dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+#pragma unroll
+    for (int f = 0; f < C::NFV; ++f) dp = Da<T>::mma(da_frag<C::U>(sV, r0 + l32, 2 * f + h2), uf[f], dp);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        lse[t] = rlive ? a.stats[t * bhn + at] : INFINITY;
-        dl[t] = rlive ? a.delta[t * bhn + at] : 0.f;
+        da_f16v s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sK, r0 + l32, t * (C::U / 2) + 2 * f + h2), qf[t][f], s);
+        const float fac = t ? -sign : 1.f, dd = t ? dl[1] : -dl[0];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = da_exp2(fmaf(s[r], c, -lse[t])) * fmaf(dp[r], fac, dd);
+        if (masked) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __uint_as_float(__float_as_uint(s[r]) & (uint32_t)__builtin_amdgcn_sbfe((int)vis, 8 * (r >> 2) + (r & 3), 1));
+        }
+#pragma unroll
+        for (int f = 0; f < C::FPT; ++f) {
+            const uint4 sf = da_pack<T>(s, f);
+#pragma unroll
+            for (int x = 0; x < C::MTK; ++x)
+                dq[t][x] = Da<T>::mma(da_frag_tr<T, C::U>(sK, r0 + f * Da<T>::KPF, DK < 32 ? 0 : t * DK + x * 32, lane), sf, dq[t][x]);
+        }
     }
-    const bool empty = lse[0] == INFINITY;                   // sees no key: its query may hold anything
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) void diff_attn_dq_kernel(const DiffArgs a) {
+    using C = DaCfg<T, DK>;
+    constexpr int KB = sizeof(T) == 2 ? 64 : 32, TILE = KB * C::ROWB;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
+    const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, nblk = gridDim.x / nbh, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int blk = a.causal ? nblk - 1 - (int)(blockIdx.x / nbh) : (int)(blockIdx.x / nbh);          // causal: the longest first
+    const int len = da_len(a, b);
+    const int64_t start = da_start(a, b), R = (int64_t)a.N * a.G, blk0 = (int64_t)blk * 128;
+    const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
+    const int64_t mb = a.mask_b ? b : 0;
+    const DaRows w = da_rows(a, hk, blk0 + wave * 32, l32, len, start);
+    const int i_end = (int)((blk0 + 127 < R - 1 ? blk0 + 127 : R - 1) / a.G);
+    const int wg_end = da_limit(a, len, start, i_end), qt0 = (int)(blk0 / a.G) >> 6, qt1 = i_end >> 6;
+
+    DaCopy<T, DK, KB, kDaThreads> ck, cv;
+    ck.init(reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.ks[3], a.d, true, tid);
+    cv.init(reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, a.dv, false, tid);
+    const bool full = a.d == DK && a.dv == C::DV;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 1024;
+    auto next = [&](int k0) {
+        for (; k0 < wg_end && a.tiles; k0 += KB) {
+            bool hidden = true;
+            for (int qt = qt0; qt <= qt1; ++qt) hidden = hidden && a.tiles[(mb * N64 + qt) * M64 + (k0 >> 6)] == 2;
+            if (!hidden) break;
+        }
+        return k0;
+    };
+    auto issue = [&](int k0, int buf) {
+        const int valid = len - k0;
+        const uint64_t live = a.live ? a.live[mb * M64 + (k0 >> 6)] >> (k0 & 63) : ~0ull;
+        const bool whole = full && valid >= KB && live == ~0ull;
+        ck.run(lds0 + buf * 2 * TILE, k0, a.ks[1], valid, live, whole);
+        cv.run(lds0 + buf * 2 * TILE + TILE, k0, a.vs[1], valid, live, whole);
+    };
+    int k0 = next(0), buf = 0;
+    if (k0 < wg_end) issue(k0, 0);
+
+    const float lam = da_lambda_rows(a, hk, blk0 + wave * 32, w.head), sign = lam < 0.f ? -1.f : 1.f;
+    const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + w.head) * a.N + w.i;
+    uint4 qf[2][C::NF], uf[C::NFV];
+    float lse[2], dl[2];
+    const T *qp = reinterpret_cast<const T *>(a.q) + b * a.qs[0] + w.i * a.qs[1] + w.head * a.qs[2];
+    const T *up = reinterpret_cast<const T *>(a.du) + (((int64_t)b * a.N + w.i) * a.H + w.head) * a.dv;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        lse[t] = w.live ? a.rowstat[t * bhn + at] : INFINITY;
+        dl[t] = w.live ? a.rowstat[(2 + t) * bhn + at] : 0.f;
+    }
+    const bool empty = lse[0] == INFINITY;                    // sees no key: its query may hold anything
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int f = 0; f < C::NF; ++f) {
             const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
-            qf[t][f] = rlive && !empty && c < a.d ? *reinterpret_cast<const uint4 *>(qp + t * a.qs[3] + c) : make_uint4(0, 0, 0, 0);
+            qf[t][f] = w.live && !empty && c < a.d ? *reinterpret_cast<const uint4 *>(qp + t * a.qs[3] + c) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
     for (int f = 0; f < C::NFV; ++f) {
         const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
-        uf[f] = rlive && c < a.dv ? *reinterpret_cast<const uint4 *>(up + c) : make_uint4(0, 0, 0, 0);
+        uf[f] = w.live && c < a.dv ? *reinterpret_cast<const uint4 *>(up + c) : make_uint4(0, 0, 0, 0);
     }
     da_f16v dq[2][C::MTK];
 #pragma unroll
@@ -902,63 +991,28 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_dq_kernel(const DiffArgs
         for (int x = 0; x < C::MTK; ++x)
 #pragma unroll
             for (int r = 0; r < 16; ++r) dq[t][x][r] = 0.f;
-    const T *kp = reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2];
-    const T *vp = reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2];
-    const int64_t mb = a.mask_b ? b : 0;
 
-    for (int k0 = 0; k0 < wg_end; k0 += KB) {
-        const int kt = k0 >> 6;
-        const uint64_t live = a.live ? a.live[mb * M64 + kt] : ~0ull;
-        __syncthreads();
-        da_stage<T, DK>(sK, kp + (int64_t)k0 * a.ks[1], a.ks[1], a.ks[3], a.d, true, KB, min(KB, len - k0), live, tid);
-        da_stage<T, DK>(sV, vp + (int64_t)k0 * a.vs[1], a.vs[1], 0, a.dv, false, KB, min(KB, len - k0), live, tid);
-        __syncthreads();
-        if (!wlive) continue;
-        int code = 0;
-        if (a.tiles) {
-            const uint8_t *tp = a.tiles + mb * N64 * M64 + kt;
-            const int c0 = tp[(int64_t)(i_lo >> 6) * M64], c1 = tp[(int64_t)(i_hi >> 6) * M64];
-            code = c0 == c1 ? c0 : 1;
+    while (k0 < wg_end) {
+        const int kn = next(k0 + KB), code = da_tile_code(a, w, mb, k0 >> 6, M64, N64);
+        uint64_t vis = ~0ull;                                 // (loaded in front of the next copies: the wait for it would be a wait for them)
+        if (code == 1 && w.live) vis = a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63);
+        da_wait_copies<0>();
+        da_lds_done();
+        __builtin_amdgcn_s_barrier();
+        if (kn < wg_end) issue(kn, buf ^ 1);
+        if (code != 2 && k0 < w.lim_hi) {
+            const bool cut = k0 + KB > w.lim_lo || w.ragged, masked = cut || code == 1;
+            if (cut) vis &= w.limit <= k0 ? 0ull : w.limit >= k0 + 64 ? ~0ull : (1ull << (w.limit - k0)) - 1;
+            const char *sK = lds + buf * 2 * TILE, *sV = sK + TILE;
+#pragma unroll 1
+            for (int nt = 0; nt < KB / 32; ++nt)
+                da_dq_tile<T, DK>(a, dq, qf, uf, lse, dl, sign, sK, sV, nt * 32, masked, (uint32_t)(vis >> (32 * nt)), lane);
         }
-        if (code == 2 || k0 >= da_limit(a, len, start, i_hi)) continue;
-        const bool cut = k0 + KB > da_limit(a, len, start, i_lo) || wl - w0 < 31;
-        uint64_t vis = ~0ull;
-        if (code == 1 && rlive) vis = a.rowbits[(mb * a.N + i) * M64 + kt];
-        if (cut) vis &= limit <= k0 ? 0ull : limit >= k0 + 64 ? ~0ull : (1ull << (limit - k0)) - 1;
-        const bool masked = cut || code == 1;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            da_f16v dp;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) dp[r] = 0.f;
-#pragma unroll
-            for (int f = 0; f < C::NFV; ++f) dp = Da<T>::mma(da_frag<C::U>(sV, nt * 32 + l32, 2 * f + h2), uf[f], dp);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                da_f16v s;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-                for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sK, nt * 32 + l32, t * (C::U / 2) + 2 * f + h2), qf[t][f], s);
-                const float fac = t ? -lam : 1.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float p = da_exp2(fmaf(s[r], a.scale_log2e, -lse[t])) * fac;
-                    if (masked && !((vis >> (nt * 32 + 8 * (r >> 2) + 4 * h2 + (r & 3))) & 1)) p = 0.f;
-                    s[r] = p == 0.f ? 0.f : p * (dp[r] - dl[t]);
-                }
-#pragma unroll
-                for (int f = 0; f < C::FPT; ++f) {
-                    const uint4 sf = da_pack<T>(s, f);
-#pragma unroll
-                    for (int x = 0; x < C::MTK; ++x)
-                        dq[t][x] = Da<T>::mma(da_frag_tr<T, C::U>(sK, nt * 32 + f * Da<T>::KPF, DK < 32 ? 0 : t * DK + x * 32, lane), sf, dq[t][x]);
-                }
-            }
-        }
+        k0 = kn;
+        buf ^= 1;
     }
-    if (!rlive) return;
-    T *dst = reinterpret_cast<T *>(a.dq) + (((int64_t)b * a.N + i) * a.H + head) * 2 * a.d;
+    if (!w.live) return;
+    T *dst = reinterpret_cast<T *>(a.dq) + (((int64_t)b * a.N + w.i) * a.H + w.head) * 2 * a.d;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -977,15 +1031,71 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_dq_kernel(const DiffArgs
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// backward, dK and dV: workgroup = (batch, key head, 128 keys), a wave owns 32 keys; all rows that may see them, 32 queries of one head at a time
+// backward, dK and dV: workgroup = (batch, key head, 128 keys, one of kvruns runs of the rows), a wave owns 32 keys with both operands in registers; the
+// queries of the group's heads stream through two LDS buffers of QB rows (Q | dU | four statistics), copied while the block in front is worked on
 template <typename T, int DK>
-__global__ __launch_bounds__(kDaThreads) void diff_attn_dkdv_kernel(const DiffArgs a) {
+__device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[DaCfg<T, DK>::MTK], da_f16v *dv, const uint4 (*kf)[DaCfg<T, DK>::NF], const uint4 *vf, float sign, const char *sQ,
+                                             const char *sU, const float *stat, int stat_ld, int r0, bool masked, uint32_t vis, int lane) {
     using C = DaCfg<T, DK>;
+    const int h2 = lane >> 5, l32 = lane & 31;
+    const float c = a.scale_log2e;
+    vis >>= 4 * h2;
+    da_f16v dp, p;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+#pragma unroll
+    for (int f = 0; f < C::NFV; ++f) dp = Da<T>::mma(da_frag<C::U>(sU, r0 + l32, 2 * f + h2), vf[f], dp);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        da_f16v s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sQ, r0 + l32, t * (C::U / 2) + 2 * f + h2), kf[t][f], s);
+        const float fac = t ? -sign : 1.f;
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const float4 ls = *reinterpret_cast<const float4 *>(stat + t * stat_ld + r0 + 8 * q4 + 4 * h2);
+            const float4 dd = *reinterpret_cast<const float4 *>(stat + (2 + t) * stat_ld + r0 + 8 * q4 + 4 * h2);
+            const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dl[4] = {dd.x, dd.y, dd.z, dd.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = 4 * q4 + j;
+                float e = da_exp2(fmaf(s[r], c, -lv[j]));
+                if (masked) e = __uint_as_float(__float_as_uint(e) & (uint32_t)__builtin_amdgcn_sbfe((int)vis, 8 * q4 + j, 1));
+                p[r] = t ? fmaf(e, fac, p[r]) : e;
+                s[r] = e * (t ? fmaf(dp[r], fac, dl[j]) : dp[r] - dl[j]);
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < C::FPT; ++f) {
+            const uint4 sf = da_pack<T>(s, f);
+#pragma unroll
+            for (int x = 0; x < C::MTK; ++x)
+                dk[t][x] = Da<T>::mma(da_frag_tr<T, C::U>(sQ, r0 + f * Da<T>::KPF, DK < 32 ? 0 : t * DK + x * 32, lane), sf, dk[t][x]);
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < C::FPT; ++f) {
+        const uint4 pf = da_pack<T>(p, f);
+#pragma unroll
+        for (int x = 0; x < C::MT; ++x) dv[x] = Da<T>::mma(da_frag_tr<T, C::U>(sU, r0 + f * Da<T>::KPF, x * 32, lane), pf, dv[x]);
+    }
+}
+
+__device__ __attribute__((aligned(16))) float da_no_row[4] = {__builtin_huge_valf(), __builtin_huge_valf(), 0.f, 0.f};     // statistics of a row that is not there
+__device__ __forceinline__ void da_copy4(const void *src, uint32_t lds_addr) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(lds_addr) : "memory");
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2) ? 2 : 1) void diff_attn_dkdv_kernel(const DiffArgs a) {
+    using C = DaCfg<T, DK>;
+    constexpr int QB = 64, TILE = QB * C::ROWB, BUF = 2 * TILE + 4 * QB * 4;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *sQ = lds, *sU = lds + 32 * C::ROWB;
-    __shared__ __attribute__((aligned(16))) float sL[2][32], sD[2][32];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h2 = lane >> 5, l32 = lane & 31;
-    const int bh = blockIdx.x % (a.B * a.Hk), blk = blockIdx.x / (a.B * a.Hk), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
+    const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, rest = blockIdx.x / nbh, run = rest % a.kvruns, blk = rest / a.kvruns, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int len = da_len(a, b);
     const int64_t start = da_start(a, b);
     const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
@@ -1020,100 +1130,103 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_dkdv_kernel(const DiffAr
 #pragma unroll
         for (int x = 0; x < C::MT; ++x) dv[x][r] = 0.f;
     }
-    // first query that may see a key of this workgroup
-    int i_first = 0;
+    // blocks of QB queries that may see a key of this workgroup, head after head: this run's share
+    int qt_first = 0;
     if (a.causal) {
         const int64_t f = (int64_t)blk * 128 - start;
-        i_first = f <= 0 ? 0 : f >= a.N ? a.N : (int)f;
+        qt_first = f <= 0 ? 0 : f >= a.N ? N64 : (int)f / QB;
     }
-    if (blk * 128 >= len) i_first = a.N;
-    for (int g = 0; g < a.G; ++g) {
-        const int head = hk * a.G + g;
-        float e1, e2;
-        da_lambda_parts(a, head, e1, e2);
-        const float lam = e1 - e2 + a.init;
-        const int64_t hrow = ((int64_t)b * a.H + head) * a.N;
-        for (int i0 = i_first & ~31; i0 < a.N; i0 += 32) {
-            const int valid = min(32, a.N - i0);
-            __syncthreads();
-            uint64_t rows = ~0ull;                            // rows that see nothing: their queries may hold anything
-            if (tid < 64) {
-                const int t = tid >> 5, r = tid & 31;
-                const float ls = r < valid ? a.stats[t * bhn + hrow + i0 + r] : INFINITY;
-                sL[t][r] = ls;
-                sD[t][r] = r < valid ? a.delta[t * bhn + hrow + i0 + r] : 0.f;
-            }
-            __syncthreads();
-            rows = __ballot(sL[0][l32] != INFINITY) & 0xffffffffull;
-            da_stage<T, DK>(sQ, reinterpret_cast<const T *>(a.q) + b * a.qs[0] + (int64_t)i0 * a.qs[1] + head * a.qs[2], a.qs[1], a.qs[3], a.d, true, 32, valid, rows, tid);
-            da_stage<T, DK>(sU, reinterpret_cast<const T *>(a.du) + (((int64_t)b * a.N + i0) * a.H + head) * a.dv, (int64_t)a.H * a.dv, 0, a.dv, false, 32, valid, rows,
-                            tid);
-            __syncthreads();
-            if (!wlive) continue;
-            int code = 0;
-            if (a.tiles) code = a.tiles[(mb * N64 + (i0 >> 6)) * M64 + (kw0 >> 6)];
-            if (code == 2 || (a.causal && start + i0 + valid <= kw0)) continue;
-            const bool cut = a.causal && start + i0 < kw0 + 31;
-            uint32_t vis = ~0u;
-            if (code == 1 && klive) vis = (uint32_t)(a.colbits[(mb * a.M + key) * N64 + (i0 >> 6)] >> (i0 & 32));
-            if (cut) {                                        // query i0 + n sees this key from n >= key - start - i0 on
-                const int64_t n0 = (int64_t)key - start - i0;
-                vis &= n0 <= 0 ? ~0u : n0 >= 32 ? 0u : ~0u << n0;
-            }
-            const bool masked = cut || code == 1;
-            da_f16v dp, p0, s;
+    if (blk * 128 >= len) qt_first = N64;
+    const int per_head = N64 - qt_first, total = per_head * a.G;
+    const int u0 = (int)((int64_t)total * run / a.kvruns), u1 = (int)((int64_t)total * (run + 1) / a.kvruns);
+    const int kt0 = blk * 2, kt1 = min(kt0 + 1, M64 - 1);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    const bool full = a.d == DK && a.dv == C::DV;
+    DaCopy<T, DK, QB, kDaThreads> cq, cu;
+    cq.init(reinterpret_cast<const T *>(a.q) + b * a.qs[0], a.qs[1], a.qs[3], a.d, true, tid);
+    cu.init(reinterpret_cast<const T *>(a.du) + (int64_t)b * a.N * a.H * a.dv, (int64_t)a.H * a.dv, 0, a.dv, false, tid);
+    auto next = [&](int u) {
+        for (; u < u1 && a.tiles; ++u) {
+            const uint8_t *tp = a.tiles + (mb * N64 + qt_first + u % per_head) * M64;
+            if (tp[kt0] != 2 || tp[kt1] != 2) break;
+        }
+        return u;
+    };
+    auto row_lse = [&](int u) {                               // lse of this lane's row of block u: +inf where it sees nothing or is not there
+        if (u >= u1) return INFINITY;
+        const int g = u / per_head, i = (qt_first + u - g * per_head) * QB + lane;
+        return i < a.N ? a.rowstat[((int64_t)b * a.H + hk * a.G + g) * a.N + i] : INFINITY;
+    };
+    auto issue = [&](int u, int buf, float lse) {
+        const int g = u / per_head, i0 = (qt_first + u - g * per_head) * QB, head = hk * a.G + g, valid = a.N - i0;
+        const uint64_t rows = __ballot(lse != INFINITY);      // rows that see nothing: their queries may hold anything, zeros are copied
+        const bool whole = full && rows == ~0ull;
+        const uint32_t to = lds0 + buf * BUF;
+        DaCopy<T, DK, QB, kDaThreads> q2 = cq, u2 = cu;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) dp[r] = 0.f;
-#pragma unroll
-            for (int f = 0; f < C::NFV; ++f) dp = Da<T>::mma(da_frag<C::U>(sU, l32, 2 * f + h2), vf[f], dp);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-                for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sQ, l32, t * (C::U / 2) + 2 * f + h2), kf[t][f], s);
-                const float fac = t ? -lam : 1.f;
-#pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    const float4 ls = *reinterpret_cast<const float4 *>(&sL[t][8 * q4 + 4 * h2]), dd = *reinterpret_cast<const float4 *>(&sD[t][8 * q4 + 4 * h2]);
-                    const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv4[4] = {dd.x, dd.y, dd.z, dd.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = 4 * q4 + j;
-                        float p = da_exp2(fmaf(s[r], a.scale_log2e, -lv[j])) * fac;
-                        if (masked && !((vis >> (8 * q4 + 4 * h2 + j)) & 1)) p = 0.f;
-                        p0[r] = t ? p0[r] + p : p;
-                        s[r] = p == 0.f ? 0.f : p * (dp[r] - dv4[j]);
-                    }
+        for (int p = 0; p < DaCopy<T, DK, QB, kDaThreads>::P; ++p) { q2.base[p] += head * a.qs[2]; u2.base[p] += (int64_t)head * a.dv; }
+        q2.run(to + wave * 1024, i0, a.qs[1], valid, rows, whole);
+        u2.run(to + TILE + wave * 1024, i0, (int64_t)a.H * a.dv, valid, rows, whole);
+        const float *sp = i0 + lane < a.N ? a.rowstat + wave * bhn + ((int64_t)b * a.H + head) * a.N + i0 + lane : da_no_row + wave;     // wave = which statistic
+        da_copy4(sp, __builtin_amdgcn_readfirstlane(to + 2 * TILE + wave * QB * 4));
+    };
+    int u = next(u0), buf = 0, g_now = -1;
+    float sign = 1.f;
+    if (u < u1) issue(u, 0, row_lse(u));
+    int un = next(u + 1);
+    float lse_n = row_lse(un);
+    while (u < u1) {
+        const int g = u / per_head, i0 = (qt_first + u - g * per_head) * QB;
+        if (g != g_now) {
+            sign = da_lambda(a, hk * a.G + g) < 0.f ? -1.f : 1.f;
+            g_now = g;
+        }
+        int code = 0;
+        uint64_t vis = ~0ull;
+        if (a.tiles && wlive) {
+            code = a.tiles[(mb * N64 + (i0 >> 6)) * M64 + (kw0 >> 6)];
+            if (code == 1 && klive) vis = a.colbits[(mb * a.M + key) * N64 + (i0 >> 6)];
+        }
+        const int unn = next(un + 1);
+        const float lse_nn = row_lse(unn);                    // (one block ahead of its use: the rows that the next copies leave out)
+        da_wait_copies<0>();
+        da_lds_done();
+        __builtin_amdgcn_s_barrier();                         // block u is there for every wave, and every wave is done with the buffer in front
+        if (un < u1) issue(un, buf ^ 1, lse_n);
+        if (wlive && code != 2) {
+            const char *sQ = lds + buf * BUF, *sU = sQ + TILE;
+            const float *stat = reinterpret_cast<const float *>(sU + TILE);
+#pragma unroll 1
+            for (int nt = 0; nt < QB / 32; ++nt) {
+                const int i1 = i0 + nt * 32;
+                if (i1 >= a.N || (a.causal && start + i1 + 31 < kw0)) continue;
+                const bool cut = a.causal && start + i1 < kw0 + 31;
+                uint32_t v = (uint32_t)(vis >> (32 * nt));
+                if (cut) {                                    // query i1 + n sees this key from n >= key - start - i1 on
+                    const int64_t n0 = (int64_t)key - start - i1;
+                    v &= n0 <= 0 ? ~0u : n0 >= 32 ? 0u : ~0u << n0;
                 }
-#pragma unroll
-                for (int f = 0; f < C::FPT; ++f) {
-                    const uint4 sf = da_pack<T>(s, f);
-#pragma unroll
-                    for (int x = 0; x < C::MTK; ++x)
-                        dk[t][x] = Da<T>::mma(da_frag_tr<T, C::U>(sQ, f * Da<T>::KPF, DK < 32 ? 0 : t * DK + x * 32, lane), sf, dk[t][x]);
-                }
-            }
-#pragma unroll
-            for (int f = 0; f < C::FPT; ++f) {
-                const uint4 pf = da_pack<T>(p0, f);
-#pragma unroll
-                for (int x = 0; x < C::MT; ++x) dv[x] = Da<T>::mma(da_frag_tr<T, C::U>(sU, f * Da<T>::KPF, x * 32, lane), pf, dv[x]);
+                da_dkdv_tile<T, DK>(a, dk, dv, kf, vf, sign, sQ, sU, stat, QB, nt * 32, cut || code == 1, v, lane);
             }
         }
+        u = un; un = unn; lse_n = lse_nn;
+        buf ^= 1;
     }
     if (key >= a.M) return;
     const int64_t krow = ((int64_t)b * a.M + key) * a.Hk + hk;
+    const int w = 2 * a.d + a.dv;
+    float *part = a.kvpart ? a.kvpart + ((int64_t)run * a.B * a.M * a.Hk + krow) * w : nullptr;
     T *dkp = reinterpret_cast<T *>(a.dk) + krow * 2 * a.d, *dvp = reinterpret_cast<T *>(a.dvv) + krow * a.dv;
-    const float keep = klive ? a.scale : 0.f;
+    const bool keep = klive;                                  // keys that nobody sees: zeros, whatever their lanes met
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
             const int c = x * 32 + 8 * q4 + 4 * h2;
             if (c >= a.dv) continue;
-            if (klive) da_store4(dvp + c, dv[x][4 * q4], dv[x][4 * q4 + 1], dv[x][4 * q4 + 2], dv[x][4 * q4 + 3]);
-            else da_store4(dvp + c, 0.f, 0.f, 0.f, 0.f);
+            const float v0 = keep ? dv[x][4 * q4] : 0.f, v1 = keep ? dv[x][4 * q4 + 1] : 0.f, v2 = keep ? dv[x][4 * q4 + 2] : 0.f, v3 = keep ? dv[x][4 * q4 + 3] : 0.f;
+            if (part) da_store4(part + 2 * a.d + c, v0, v1, v2, v3);
+            else da_store4(dvp + c, v0, v1, v2, v3);
         }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -1127,9 +1240,28 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_dkdv_kernel(const DiffAr
                     c -= t * DK;
                 }
                 if (c >= a.d) continue;
-                if (klive) da_store4(dkp + t * a.d + c, dk[t][x][4 * q4] * keep, dk[t][x][4 * q4 + 1] * keep, dk[t][x][4 * q4 + 2] * keep, dk[t][x][4 * q4 + 3] * keep);
-                else da_store4(dkp + t * a.d + c, 0.f, 0.f, 0.f, 0.f);
+                const float v0 = keep ? dk[t][x][4 * q4] * a.scale : 0.f, v1 = keep ? dk[t][x][4 * q4 + 1] * a.scale : 0.f, v2 = keep ? dk[t][x][4 * q4 + 2] * a.scale : 0.f,
+                            v3 = keep ? dk[t][x][4 * q4 + 3] * a.scale : 0.f;
+                if (part) da_store4(part + t * a.d + c, v0, v1, v2, v3);
+                else da_store4(dkp + t * a.d + c, v0, v1, v2, v3);
             }
+}
+
+// dK and dV from the runs' sums, in order: a thread per 4 channels
+template <typename T> __global__ __launch_bounds__(256) void diff_attn_kv_sum_kernel(const DiffArgs a) {
+    const int w4 = (2 * a.d + a.dv) / 4;
+    const int64_t rows = (int64_t)a.B * a.M * a.Hk, n = rows * w4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / w4;
+        const int c = (int)(i - row * w4) * 4;
+        float4 v = *reinterpret_cast<const float4 *>(a.kvpart + i * 4);
+        for (int r = 1; r < a.kvruns; ++r) {
+            const float4 z = *reinterpret_cast<const float4 *>(a.kvpart + (r * n + i) * 4);
+            v.x += z.x; v.y += z.y; v.z += z.z; v.w += z.w;
+        }
+        if (c < 2 * a.d) da_store4(reinterpret_cast<T *>(a.dk) + row * 2 * a.d + c, v.x, v.y, v.z, v.w);
+        else da_store4(reinterpret_cast<T *>(a.dvv) + row * a.dv + c - 2 * a.d, v.x, v.y, v.z, v.w);
+    }
 }
 
 }  // namespace dfine
@@ -1180,7 +1312,7 @@ int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_
     const int64_t M64 = (M + 63) / 64, N64 = (N + 63) / 64;
     if (batches * M64 > 0x7fffffff) return DFINE_E_BADARG;
     uint64_t *col = forms + batches * N * M64, *live = col + batches * M * N64;
-    hipLaunchKernelGGL(diff_attn_mask_kernel, dim3((unsigned)(batches * M64)), dim3(256), 0, (hipStream_t)stream, mask, stride_b, stride_n, (int)N, (int)M, forms, col, live,
+    hipLaunchKernelGGL(diff_attn_mask_kernel, dim3((unsigned)(batches * M64)), dim3(1024), 0, (hipStream_t)stream, mask, stride_b, stride_n, (int)N, (int)M, forms, col, live,
                        reinterpret_cast<uint8_t *>(live + batches * M64));
     return check_launch();
 }
@@ -1188,7 +1320,7 @@ int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_
 // the smallest of the three sizes that holds the head (values are twice as wide as a map's channels)
 static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <= 32 && dv <= 64 ? 32 : 64; }
 
-// dispatch on type and size; ROWS16, ROWS32: rows of 2 DK channels in LDS; DA_ARGS: the kernel's arguments
+// dispatch on type and size; ROWS16, ROWS32: rows of 2 DK channels in LDS, MORE: bytes beside them; DA_ARGS: the kernel's arguments
 #define DA_LAUNCH(K_, BYTES)                                                                                                                                      \
     {                                                                                                                                                            \
         const int by_ = (int)(BYTES);                                                                                                                            \
@@ -1200,19 +1332,19 @@ static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <
         }                                                                                                                                                        \
         hipLaunchKernelGGL(K_, grid_, block_, by_, st_, DA_ARGS);                                                                                                \
     }
-#define DA_DISPATCH(KERNEL, GRID, ROWS16, ROWS32)                                                                                                                 \
+#define DA_DISPATCH(KERNEL, GRID, ROWS16, ROWS32, MORE)                                                                                                                \
     {                                                                                                                                                            \
         const int dk_ = diff_attn_size(a.d, a.dv);                                                                                                               \
         const dim3 grid_(GRID), block_(kDaThreads);                                                                                                              \
         hipStream_t st_ = (hipStream_t)stream;                                                                                                                   \
         if (shape[7] == 0) {                                                                                                                                     \
-            if (dk_ == 16) DA_LAUNCH((KERNEL<float, 16>), (ROWS32) * 128)                                                                                        \
-            else if (dk_ == 32) DA_LAUNCH((KERNEL<float, 32>), (ROWS32) * 256)                                                                                   \
-            else DA_LAUNCH((KERNEL<float, 64>), (ROWS32) * 512)                                                                                                  \
+            if (dk_ == 16) DA_LAUNCH((KERNEL<float, 16>), (ROWS32) * 128 + (MORE))                                                                                        \
+            else if (dk_ == 32) DA_LAUNCH((KERNEL<float, 32>), (ROWS32) * 256 + (MORE))                                                                                   \
+            else DA_LAUNCH((KERNEL<float, 64>), (ROWS32) * 512 + (MORE))                                                                                                  \
         } else {                                                                                                                                                 \
-            if (dk_ == 16) DA_LAUNCH((KERNEL<uint16_t, 16>), (ROWS16) * 64)                                                                                      \
-            else if (dk_ == 32) DA_LAUNCH((KERNEL<uint16_t, 32>), (ROWS16) * 128)                                                                                \
-            else DA_LAUNCH((KERNEL<uint16_t, 64>), (ROWS16) * 256)                                                                                               \
+            if (dk_ == 16) DA_LAUNCH((KERNEL<uint16_t, 16>), (ROWS16) * 64 + (MORE))                                                                                      \
+            else if (dk_ == 32) DA_LAUNCH((KERNEL<uint16_t, 32>), (ROWS16) * 128 + (MORE))                                                                                \
+            else DA_LAUNCH((KERNEL<uint16_t, 64>), (ROWS16) * 256 + (MORE))                                                                                               \
         }                                                                                                                                                        \
     }
 
@@ -1255,7 +1387,7 @@ int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void 
     if (blocks > 0x7fffffff) return DFINE_E_BADARG;
     if (n == 0) {
         #define DA_ARGS a
-        DA_DISPATCH(diff_attn_fwd_kernel, (unsigned)blocks, 256, 128)
+        DA_DISPATCH(diff_attn_fwd_kernel, (unsigned)blocks, 256, 128, 0)
 #undef DA_ARGS
         return check_launch();
     }
@@ -1263,7 +1395,7 @@ int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void 
     float4 *ml = reinterpret_cast<float4 *>(ws);
     float *part = n > 1 ? reinterpret_cast<float *>(reinterpret_cast<char *>(ws) + da_up(diff_attn_rows(a) * n * 16)) : nullptr;
 #define DA_ARGS a, n, part, ml
-    DA_DISPATCH(diff_attn_fwd_split_kernel, (unsigned)blocks, 512, dk_ == 64 ? 256 : 512)
+    DA_DISPATCH(diff_attn_fwd_split_kernel, (unsigned)blocks, 512, dk_ == 64 ? 256 : 512, 0)
 #undef DA_ARGS
     if (int e = check_launch()) return e;
     if (n == 1) return DFINE_OK;
@@ -1287,11 +1419,21 @@ static int diff_attn_runs(const DiffArgs &a) {                  // workgroups pe
 }
 
 // workspace of the backward pass in bytes: dU, D_0 and D_1, the partial sums
+// runs of the rows that dK and dV are summed in: more where (batch, key head, 128 keys) are fewer workgroups than the chip holds at once
+static int diff_attn_kvruns(const DiffArgs &a) {
+    const int64_t wgs = ((int64_t)a.M + 127) / 128 * a.B * a.Hk, units = ((int64_t)a.N + 63) / 64 * a.G;
+    if (wgs == 0 || wgs >= 512) return 1;
+    int64_t n = 1024 / wgs;
+    if (n > 8) n = 8;
+    if (n > units / 4) n = units / 4;
+    return (int)(n < 1 ? 1 : n);
+}
 int64_t dfine_diff_attn_bwd_ws_bytes(const int64_t *shape) {
     DiffArgs a{};
     if (!shape || diff_attn_setup(a, shape, 1.f, 0.f, 0.f)) return -1;
-    const int64_t rows = (int64_t)a.B * a.N * a.H, n = (int64_t)diff_attn_runs(a) * a.H;
-    return da_up(rows * a.dv * (shape[7] ? 2 : 4)) + da_up(rows * 8) + da_up(n * 4) + da_up(n * a.dv * 4);
+    const int64_t rows = (int64_t)a.B * a.N * a.H, n = (int64_t)diff_attn_runs(a) * a.H, runs = diff_attn_kvruns(a);
+    return da_up(rows * a.dv * (shape[7] ? 2 : 4)) + da_up(rows * 16) + da_up(n * 4) + da_up(n * a.dv * 4) +
+           (runs > 1 ? runs * a.B * a.M * a.Hk * (2 * a.d + a.dv) * 4 : 0);
 }
 
 #define DA_ARGS a
@@ -1317,9 +1459,11 @@ int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void 
     const int64_t rows = (int64_t)a.B * a.N * a.H, n = (int64_t)nrun * a.H;
     char *p = reinterpret_cast<char *>(ws);
     a.du = p; p += da_up(rows * a.dv * (shape[7] ? 2 : 4));
-    a.delta = reinterpret_cast<float *>(p); p += da_up(rows * 8);
+    a.rowstat = reinterpret_cast<float *>(p); p += da_up(rows * 16);
     a.lpart = reinterpret_cast<float *>(p); p += da_up(n * 4);
-    a.wpart = reinterpret_cast<float *>(p);
+    a.wpart = reinterpret_cast<float *>(p); p += da_up(n * a.dv * 4);
+    a.kvruns = diff_attn_kvruns(a);
+    a.kvpart = a.kvruns > 1 ? reinterpret_cast<float *>(p) : nullptr;
     hipStream_t st = (hipStream_t)stream;
     if (n > 0x7fffffff) return DFINE_E_BADARG;
     if (shape[7] == 0) hipLaunchKernelGGL(diff_attn_prep_kernel<float>, dim3((unsigned)n), dim3(256), 0, st, a, nrun);
@@ -1327,20 +1471,26 @@ int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void 
     if (int e = check_launch()) return e;
     if (dlam || dweight) {
         const int nh = a.lam_heads == 1 ? 1 : a.H;
-        hipLaunchKernelGGL(diff_attn_param_kernel, dim3(nh + (a.dv + 15) / 16), dim3(256), 0, st, a, nrun, dlam, weight ? dweight : nullptr);
+        hipLaunchKernelGGL(diff_attn_param_kernel, dim3(nh + (a.dv + 31) / 32), dim3(1024), 0, st, a, nrun, dlam, weight ? dweight : nullptr);
         if (int e = check_launch()) return e;
     }
     if (rows_ && dq) {
         const int64_t blocks = ((int64_t)a.N * a.G + 127) / 128 * a.B * a.Hk;
         if (blocks > 0x7fffffff) return DFINE_E_BADARG;
-        DA_DISPATCH(diff_attn_dq_kernel, (unsigned)blocks, 128, 128)
+        DA_DISPATCH(diff_attn_dq_kernel, (unsigned)blocks, 256, 128, 0)
         if (int e = check_launch()) return e;
     }
     if (keys_ && dk) {
-        const int64_t blocks = ((int64_t)a.M + 127) / 128 * a.B * a.Hk;
+        const int64_t blocks = ((int64_t)a.M + 127) / 128 * a.B * a.Hk * a.kvruns;
         if (blocks > 0x7fffffff) return DFINE_E_BADARG;
-        DA_DISPATCH(diff_attn_dkdv_kernel, (unsigned)blocks, 64, 64)
+        DA_DISPATCH(diff_attn_dkdv_kernel, (unsigned)blocks, 256, 256, 2 * 4 * 64 * 4)
         if (int e = check_launch()) return e;
+        if (a.kvruns > 1) {
+            const int64_t grid = ((int64_t)a.B * a.M * a.Hk * (2 * a.d + a.dv) / 4 + 255) / 256;
+            if (shape[7] == 0) hipLaunchKernelGGL(diff_attn_kv_sum_kernel<float>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, st, a);
+            else hipLaunchKernelGGL(diff_attn_kv_sum_kernel<uint16_t>, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, st, a);
+            if (int e = check_launch()) return e;
+        }
     }
     return DFINE_OK;
 }

@@ -26,7 +26,7 @@ struct QkNormArgs {
     float *part;                          // backward: [grid][2][D]
     int64_t xs[2][3], ds[2][3];           // strides (batch, token, head) of x and dy in elements; y is contiguous
     int64_t pos_b;
-    int heads[2], B, L, D, R, T, pos64, wbf16[2], paired;
+    int heads[2], B, L, D, R, T, pos64, wbf16[2], wvec[2], paired;
     int lpr, hs, hchunk;                  // lanes per head, heads side by side, heads per workgroup column
     float eps;
 };
@@ -87,10 +87,30 @@ __device__ __forceinline__ float qk_row_sum(float v, int lpr) {
     return v;
 }
 
-template <int V> __device__ __forceinline__ void qk_weights(const void *w, int bf16, int e, int D, float *f) {
+// V weights from channel e on (0 past D; 1 without weights): one or two 16-byte loads where the pointer allows it
+template <int V> __device__ __forceinline__ void qk_weights(const void *w, int bf16, bool vec, int e, int D, float *f) {
+    if (!w || e >= D || e < 0) {
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-        f[j] = e + j >= D ? 0.f : !w ? 1.f : bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(w)[e + j]) : reinterpret_cast<const float *>(w)[e + j];
+        for (int j = 0; j < V; ++j) f[j] = e >= D || e < 0 ? 0.f : 1.f;
+    } else if (vec && bf16) {
+        const uint2 *p = reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(w) + e);
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const uint2 u = p[j / 4];
+            f[j] = __uint_as_float(u.x << 16); f[j + 1] = __uint_as_float(u.x & 0xffff0000u);
+            f[j + 2] = __uint_as_float(u.y << 16); f[j + 3] = __uint_as_float(u.y & 0xffff0000u);
+        }
+    } else if (vec) {
+        const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(w) + e);
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const float4 u = p[j / 4];
+            f[j] = u.x; f[j + 1] = u.y; f[j + 2] = u.z; f[j + 3] = u.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(w)[e + j]) : reinterpret_cast<const float *>(w)[e + j];
+    }
 }
 
 // grid.x: workgroups over tokens (strided), grid.y: chunks of heads
@@ -118,8 +138,8 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rotate_kernel(const QkNorm
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         if (a.heads[s] == 0) continue;
-        qk_weights<V>(a.w[s], a.wbf16[s], e, a.D, w[s]);
-        if (!a.paired) qk_weights<V>(a.w[s], a.wbf16[s], e + (plane - lane) * V, a.D, wp[s]);
+        qk_weights<V>(a.w[s], a.wbf16[s], a.wvec[s], e, a.D, w[s]);
+        if (!a.paired && !BWD) qk_weights<V>(a.w[s], a.wbf16[s], a.wvec[s], e + (plane - lane) * V, a.D, wp[s]);
     }
     float dw[2][V];
 #pragma unroll
@@ -141,12 +161,24 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rotate_kernel(const QkNorm
             const bool inside = p >= 0 && p < a.T;                 // a position outside the table: not a number, never a read outside it
             const float *cr = a.cosv + (inside ? p : 0) * half + tcol, *sr = a.sinv + (inside ? p : 0) * half + tcol;
             const float bad = __int_as_float(0x7fc00000);
-            if (a.paired) {
+            if (a.paired) {                                        // (rows of R / 2 floats, R a multiple of 8: 8-byte loads are on their border)
 #pragma unroll
-                for (int j = 0; j < V / 2; ++j) { c[2 * j] = c[2 * j + 1] = inside ? cr[j] : bad; s[2 * j] = s[2 * j + 1] = inside ? sr[j] : bad; }
+                for (int j = 0; j < V / 2; j += 2) {
+                    const float2 cc = *reinterpret_cast<const float2 *>(cr + j), ss = *reinterpret_cast<const float2 *>(sr + j);
+                    c[2 * j] = c[2 * j + 1] = cc.x; c[2 * j + 2] = c[2 * j + 3] = cc.y;
+                    s[2 * j] = s[2 * j + 1] = ss.x; s[2 * j + 2] = s[2 * j + 3] = ss.y;
+                }
             } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) { c[j] = inside ? cr[j] : bad; s[j] = inside ? sr[j] : bad; }
+                for (int j = 0; j < V; j += 4) {
+                    const float4 cc = *reinterpret_cast<const float4 *>(cr + j), ss = *reinterpret_cast<const float4 *>(sr + j);
+                    c[j] = cc.x; c[j + 1] = cc.y; c[j + 2] = cc.z; c[j + 3] = cc.w;
+                    s[j] = ss.x; s[j + 1] = ss.y; s[j + 2] = ss.z; s[j + 3] = ss.w;
+                }
+            }
+            if (!inside) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) c[j] = s[j] = bad;
             }
         }
 #pragma unroll
@@ -233,18 +265,20 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rotate_kernel(const QkNorm
     }
 }
 
-// dw[set][ch] = sum over the partial rows, 16 channels per workgroup, rows in 16 interleaved runs
-__global__ __launch_bounds__(256) void qk_dw_kernel(const float *__restrict__ part, void *dwq, void *dwk, int qbf16, int kbf16, int rows, int D) {
-    __shared__ float s[16][17];
-    const int col = threadIdx.x & 15, run = threadIdx.x >> 4, i = blockIdx.x * 16 + col;
+// dw[set][ch] = sum over the partial rows: 32 channels per workgroup, the rows in 32 interleaved runs, 8 loads in flight
+__global__ __launch_bounds__(1024) void qk_dw_kernel(const float *__restrict__ part, void *dwq, void *dwk, int qbf16, int kbf16, int rows, int D) {
+    __shared__ float s[32][33];
+    const int col = threadIdx.x & 31, run = threadIdx.x >> 5, i = blockIdx.x * 32 + col;
     float v = 0.f;
-    if (i < 2 * D)
-        for (int r = run; r < rows; r += 16) v += part[(int64_t)r * 2 * D + i];
+    if (i < 2 * D) {
+#pragma unroll 8
+        for (int r = run; r < rows; r += 32) v += part[(int64_t)r * 2 * D + i];
+    }
     s[run][col] = v;
     __syncthreads();
     if (run || i >= 2 * D) return;
 #pragma unroll
-    for (int r = 1; r < 16; ++r) v += s[r][col];
+    for (int r = 1; r < 32; ++r) v += s[r][col];
     const bool k = i >= D;
     void *dst = k ? dwk : dwq;
     if (!dst) return;
@@ -266,7 +300,7 @@ static int qk_norm_setup(QkNormArgs &a, const int64_t *s, const float *cosv, con
     if (B < 0 || L < 0 || Hq < 0 || Hk < 0 || B > 0x7fffffff || L > 0x7fffffff || B * L > 0x7fffffff - 0x10000 || Hq > 4096 || Hk > 4096 || D < 8 || D > 256 || D % 8 || R < 0 || R > D || R % 8 ||
         (dt != 0 && dt != 1))
         return DFINE_E_BADARG;
-    if (R && (!cosv || !sinv || T < 1 || (!pos && T < L))) return DFINE_E_BADARG;
+    if (R && (!cosv || !sinv || ((uintptr_t)cosv | (uintptr_t)sinv) & 15 || T < 1 || (!pos && T < L))) return DFINE_E_BADARG;
     a.B = (int)B; a.L = (int)L; a.D = (int)D; a.R = (int)R; a.T = (int)(T > 0x7fffffff ? 0x7fffffff : T);
     a.heads[0] = (int)Hq; a.heads[1] = (int)Hk;
     a.paired = s[8] != 0; a.pos64 = s[9] != 0; a.pos_b = s[10];
@@ -294,10 +328,15 @@ static int qk_norm_setup(QkNormArgs &a, const int64_t *s, const float *cosv, con
     return DFINE_OK;
 }
 
+static void qk_norm_weights(QkNormArgs &a, const void *wq, const void *wk) {
+    a.w[0] = wq; a.w[1] = wk;
+    for (int i = 0; i < 2; ++i) a.wvec[i] = ((uintptr_t)a.w[i] & (a.wbf16[i] ? 7 : 15)) == 0;
+}
+
 int64_t dfine_qk_norm_rotate_ws_floats(const int64_t *shape) {
     QkNormArgs a{};
     int vec, gx, gy;
-    if (!shape || qk_norm_setup(a, shape, (const float *)1, (const float *)1, (const void *)1, 0.f, &vec, &gx, &gy, true)) return -1;
+    if (!shape || qk_norm_setup(a, shape, (const float *)16, (const float *)16, (const void *)1, 0.f, &vec, &gx, &gy, true)) return -1;
     return (int64_t)gx * gy * 2 * a.D;
 }
 
@@ -314,7 +353,8 @@ int dfine_qk_norm_rotate_fwd(const void *q, const void *k, const void *wq, const
     if (int e = qk_norm_setup(a, shape, cosv, sinv, pos, eps, &vec, &gx, &gy, false)) return e;
     if (shape[0] == 0 || shape[1] == 0 || shape[2] + shape[3] == 0) return DFINE_OK;
     if ((a.heads[0] && (!q || !yq)) || (a.heads[1] && (!k || !yk))) return DFINE_E_BADARG;
-    a.x[0] = q; a.x[1] = k; a.y[0] = yq; a.y[1] = yk; a.w[0] = wq; a.w[1] = wk;
+    a.x[0] = q; a.x[1] = k; a.y[0] = yq; a.y[1] = yk;
+    qk_norm_weights(a, wq, wk);
     QK_LAUNCH(false)
     return check_launch();
 }
@@ -332,12 +372,13 @@ int dfine_qk_norm_rotate_bwd(const void *q, const void *k, const void *wq, const
         rows = 0;                                                   // no rows: the weights' gradients are zero
     } else {
         if ((a.heads[0] && (!q || !dyq || !dq)) || (a.heads[1] && (!k || !dyk || !dk))) return DFINE_E_BADARG;
-        a.x[0] = q; a.x[1] = k; a.dy[0] = dyq; a.dy[1] = dyk; a.y[0] = dq; a.y[1] = dk; a.w[0] = wq; a.w[1] = wk; a.part = ws;
+        a.x[0] = q; a.x[1] = k; a.dy[0] = dyq; a.dy[1] = dyk; a.y[0] = dq; a.y[1] = dk; a.part = ws;
+        qk_norm_weights(a, wq, wk);
         QK_LAUNCH(true)
         if (int e = check_launch()) return e;
     }
     if (!dwq && !dwk) return DFINE_OK;
-    hipLaunchKernelGGL(qk_dw_kernel, dim3((2 * a.D + 15) / 16), dim3(256), 0, (hipStream_t)stream, (const float *)ws, dwq, dwk, a.wbf16[0], a.wbf16[1], rows,
+    hipLaunchKernelGGL(qk_dw_kernel, dim3((2 * a.D + 31) / 32), dim3(1024), 0, (hipStream_t)stream, (const float *)ws, dwq, dwk, a.wbf16[0], a.wbf16[1], rows,
                        a.D);
     return check_launch();
 }

@@ -2583,7 +2583,7 @@ def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, posit
             if positions.shape != (B, L) and positions.shape != (L,):
                 _refuse(f"{op}: positions {tuple(positions.shape)} for {(B, L)} tokens")
             positions = positions.contiguous()
-        cos, sin = cos.contiguous(), sin.contiguous()
+        cos, sin = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
     eps = float(eps)
     if not eps >= 0:
         _refuse(f"{op}: eps {eps}")

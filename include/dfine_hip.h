@@ -813,7 +813,7 @@ int dfine_mask_iou_bits(const void *pred_bits, const void *gt_bits, int Np, int 
  * A2 / A6  Norms of queries and keys for each head with the position rotation in the same pass, next to the attention of
  * src/d_fine/arch/hybrid_encoder.py:243-290 and src/d_fine/arch/dfine_decoder.py:200,233-255 (no counterpart there).
  * q [B, L, Hq, D], k [B, L, Hk, D] (Hq or Hk may be 0: that operand is left out); y = rot(x rsqrt(mean_D x^2 + eps) w): pairs of the
- * first R channels are turned by the token's row of cosv / sinv fp32 [T, R / 2] - pairs (j, j + R / 2), or (2j, 2j + 1) when paired -
+ * first R channels are turned by the token's row of cosv / sinv fp32 [T, R / 2] (16-byte aligned) - pairs (j, j + R / 2), or (2j, 2j + 1) when paired -
  * the rest passes.  pos int32 / int64 [B or 1, L]: the row of each token (NULL: its index; outside the table: NaN).  wq, wk [D] or NULL.
  * shape (host int64): B, L, Hq, Hk, D, R, T, dtype (0 fp32, 1 bf16), paired, pos is int64, batch stride of pos, wq bf16, wk bf16, then the
  * strides (batch, token, head; elements, 16-byte rows) of q, of k, of dyq, of dyk.  Results are contiguous.  D, R multiples of 8, D <= 256.
