@@ -32,7 +32,7 @@ constexpr int kDaThreads = 256;
 struct DiffArgs {
     const void *q, *k, *v;                      // [B, N, H, 2, d], [B, M, Hk, 2, d], [B, M, Hk, dv]
     const void *lam, *weight;                   // [4, H or 1, d], [dv] or null
-    const uint64_t *rowbits, *colbits, *live;   // mask forms (1 = may attend): [Bm][N][M64], [Bm][M][N64], [Bm][M64]; null: no mask
+    const uint64_t *rowbits, *colbits, *some;   // mask forms (1 = may attend): [Bm][N][M64], [Bm][M][N64], any of 64 queries [Bm][N64][M64]; null: no mask
     const uint8_t *tiles;                       // [Bm][N64][M64] 0 free, 1 mixed, 2 blocked
     const int *kvlen, *qstart_dev;              // [B] or null
     void *out, *u, *o2;                         // [B, N, H, dv]; u, o2 (null: not kept) are read by the backward pass
@@ -189,8 +189,16 @@ __device__ __forceinline__ int da_limit(const DiffArgs &a, int len, int64_t star
     const int64_t e = start + i + 1;
     return e < 0 ? 0 : e < len ? (int)e : len;
 }
-__device__ __forceinline__ int da_len(const DiffArgs &a, int b) { return a.kvlen ? min(max(a.kvlen[b], 0), a.M) : a.M; }
 __device__ __forceinline__ int64_t da_start(const DiffArgs &a, int b) { return a.qstart_dev ? (int64_t)a.qstart_dev[b] : a.qstart; }
+// keys of batch b that any of its queries may see: what lies behind is never read
+__device__ __forceinline__ int da_len(const DiffArgs &a, int b) {
+    int len = a.kvlen ? min(max(a.kvlen[b], 0), a.M) : a.M;
+    if (a.causal) {
+        const int64_t e = da_start(a, b) + a.N;
+        len = e < 0 ? 0 : e < len ? (int)e : len;
+    }
+    return len;
+}
 
 // 16 bytes global -> LDS without registers; the LDS side is lane-linear from lds_addr (wave-uniform).  Inline assembly, waited for by hand (da_wait_copies):
 // behind the builtin the compiler waits for every copy in front of the next LDS read, which would end the overlap of copies and products.
@@ -266,13 +274,52 @@ __device__ __forceinline__ DaRows da_rows(const DiffArgs &a, int hk, int64_t w0,
     w.q_lo = i_lo >> 6; w.q_hi = i_hi >> 6;
     return w;
 }
-// what the mask says about (this wave's rows, 64 keys kt): 0 all free, 1 mixed, 2 all hidden
-__device__ __forceinline__ int da_tile_code(const DiffArgs &a, const DaRows &w, int64_t mb, int kt, int M64, int N64) {
-    if (!a.tiles) return 0;
-    const uint8_t *tp = a.tiles + mb * N64 * M64 + kt;
-    const int c0 = tp[(int64_t)w.q_lo * M64], c1 = tp[(int64_t)w.q_hi * M64];
-    return __builtin_amdgcn_readfirstlane(c0 == c1 ? c0 : 1);
-}
+// What the mask says about tiles of 64 keys for the 64-query tiles qt0 .. qt1 of a workgroup and q_lo, q_hi of a wave: 64 tiles at a time as bit sets, one tile
+// per lane, so that the loop over the keys reads no mask state but the bits of mixed tiles.
+struct DaWalk {
+    uint64_t need, part, mixed, hide;                         // workgroup: not all hidden, not all free; wave: mixed, all hidden
+    int base;
+    __device__ __forceinline__ void load(const DiffArgs &a, const DaRows &w, int64_t mb, int qt0, int qt1, int chunk, int M64, int N64) {
+        const int kt = chunk * 64 + (threadIdx.x & 63);
+        bool n = false, p = false, x = false, y = true;
+        if (kt < M64) {
+            const uint8_t *tp = a.tiles + mb * N64 * M64 + kt;
+            for (int qt = qt0; qt <= qt1; ++qt) {
+                const int c = tp[(int64_t)qt * M64];
+                n = n || c != 2;
+                p = p || c != 0;
+            }
+            const int c0 = tp[(int64_t)w.q_lo * M64], c1 = tp[(int64_t)w.q_hi * M64];
+            x = c0 != c1 || c0 == 1;
+            y = c0 == 2 && c1 == 2;
+        }
+        need = __ballot(n); part = __ballot(p); mixed = __ballot(x); hide = __ballot(y);
+        base = chunk;
+    }
+    // the first block at or after k0 that any row of the workgroup may see part of
+    __device__ __forceinline__ int next(const DiffArgs &a, const DaRows &w, int64_t mb, int qt0, int qt1, int M64, int N64, int k0, int end) {
+        if (!a.tiles) return k0;
+        while (k0 < end) {
+            const int kt = k0 >> 6;
+            if (kt >> 6 != base) load(a, w, mb, qt0, qt1, kt >> 6, M64, N64);
+            const uint64_t m = need >> (kt & 63);
+            if (m & 1) break;
+            k0 = m ? (kt + __builtin_ctzll(m)) << 6 : ((kt >> 6) + 1) << 12;
+        }
+        return k0;
+    }
+    __device__ __forceinline__ int code(const DiffArgs &a, int k0) const {
+        const int x = (k0 >> 6) & 63;
+        return !a.tiles ? 0 : (mixed >> x) & 1 ? 1 : (hide >> x) & 1 ? 2 : 0;
+    }
+    // keys (from k0 on) that some query of the workgroup's tiles may see: the others are copied as zeros
+    __device__ __forceinline__ uint64_t live(const DiffArgs &a, int64_t mb, int qt0, int qt1, int M64, int N64, int k0) const {
+        if (!a.tiles || !((part >> ((k0 >> 6) & 63)) & 1)) return ~0ull;
+        uint64_t m = 0;
+        for (int qt = qt0; qt <= qt1; ++qt) m |= a.some[(mb * N64 + qt) * M64 + (k0 >> 6)];
+        return m >> (k0 & 63);
+    }
+};
 
 template <typename T, int DK> struct DaState {
     using C = DaCfg<T, DK>;
@@ -392,31 +439,34 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     cv.init(reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, a.dv, false, tid);
     const bool full = a.d == DK && a.dv == C::DV;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 1024;
-    auto next = [&](int k0) {                                 // the next block that any row of the workgroup may see part of
-        for (; k0 < wg_end && a.tiles; k0 += KB) {
-            bool hidden = true;
-            for (int qt = qt0; qt <= qt1; ++qt) hidden = hidden && a.tiles[(mb * N64 + qt) * M64 + (k0 >> 6)] == 2;
-            if (!hidden) break;
-        }
-        return k0;
-    };
+    DaWalk walk;
+    walk.base = -1;
+    auto next = [&](int k0) { return walk.next(a, w, mb, qt0, qt1, M64, N64, k0, wg_end); };
     auto issue = [&](int k0, int buf) {
         const int valid = len - k0;
-        const uint64_t live = a.live ? a.live[mb * M64 + (k0 >> 6)] >> (k0 & 63) : ~0ull;
-        const bool whole = full && valid >= KB && live == ~0ull;
+        const uint64_t live = walk.live(a, mb, qt0, qt1, M64, N64, k0), all = KB == 64 ? ~0ull : 0xffffffffull;
+        const bool whole = full && valid >= KB && (live & all) == all;
         ck.run(lds0 + buf * 2 * TILE, k0, a.ks[1], valid, live, whole);
         cv.run(lds0 + buf * 2 * TILE + TILE, k0, a.vs[1], valid, live, whole);
     };
-    int k0 = next(0), buf = 0;
-    if (k0 < wg_end) issue(k0, 0);
+    auto bits = [&](int k0) {                                 // a mixed tile's keys as this lane's row sees them
+        return w.live ? a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63) : 0ull;
+    };
+    int k0 = next(0), buf = 0, code = 0;
+    uint64_t vis = ~0ull;
+    if (k0 < wg_end) {
+        code = walk.code(a, k0);
+        if (code == 1) vis = bits(k0);
+        issue(k0, 0);
+    }
     const float lam = da_lambda_rows(a, hk, blk0 + wave * 32, w.head);
     while (k0 < wg_end) {
-        const int kn = next(k0 + KB), code = da_tile_code(a, w, mb, k0 >> 6, M64, N64);
-        uint64_t vis = ~0ull;                                 // (loaded in front of the next copies: the wait for it would be a wait for them)
-        if (code == 1 && w.live) vis = a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63);
+        const int kn = next(k0 + KB), code_n = kn < wg_end ? walk.code(a, kn) : 0;
+        uint64_t vis_n = ~0ull;
         da_wait_copies<0>();
         da_lds_done();
         __builtin_amdgcn_s_barrier();                         // block k0 is there for every wave, and every wave is done with the buffer in front
+        if (code_n == 1) vis_n = bits(kn);                    // (in front of the copies: the wait for it is a wait for what comes before it)
         if (kn < wg_end) issue(kn, buf ^ 1);
         if (code != 2 && k0 < w.lim_hi) {
             const bool cut = k0 + KB > w.lim_lo || w.ragged, masked = cut || code == 1;
@@ -426,6 +476,8 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
             for (int nt = 0; nt < KB / 32; ++nt) da_fwd_tile<T, DK>(st, qf, sK, sV, nt * 32, masked, (uint32_t)(vis >> (32 * nt)), a.scale_log2e, lane);
         }
         k0 = kn;
+        code = code_n;
+        vis = vis_n;
         buf ^= 1;
     }
     if (!w.live) return;                                      // (both lanes of a row go together)
@@ -544,33 +596,45 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
     const bool full = a.d == DK && a.dv == C::DV;
     char *mine = lds + wave * WBYTES;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)mine;
+    DaWalk walk;
+    walk.base = -1;
     auto next = [&](int t) {
-        while (t < t_end && da_tile_code(a, w, mb, t >> 1, M64, N64) == 2) t += 4;
+        for (; a.tiles && t < t_end; t += 4) {
+            if (t >> 7 != walk.base) walk.load(a, w, mb, w.q_lo, w.q_hi, t >> 7, M64, N64);
+            if (walk.code(a, t * 32) != 2) break;
+        }
         return t;
     };
+    auto bits = [&](int t) { return w.live ? (uint32_t)(a.rowbits[(mb * a.N + w.i) * M64 + (t >> 1)] >> (t & 1 ? 32 : 0)) : 0u; };
     auto issue = [&](int t, int buf) {
         const int k0 = t * 32, valid = len - k0;
-        const uint64_t live = a.live ? a.live[mb * M64 + (k0 >> 6)] >> (k0 & 63) : ~0ull;
+        const uint64_t live = walk.live(a, mb, w.q_lo, w.q_hi, M64, N64, k0);
         const bool whole = full && valid >= 32 && (uint32_t)live == ~0u;
         ck.run(lds0 + buf * 2 * TILE, k0, a.ks[1], valid, live, whole);
         cv.run(lds0 + buf * 2 * TILE + TILE, k0, a.vs[1], valid, live, whole);
     };
-    int t = next(sp * per + wave), buf = 0;
-    if (t < t_end && NBUF == 2) issue(t, 0);
+    int t = next(sp * per + wave), buf = 0, code = 0;
+    uint32_t vis = ~0u;
+    if (t < t_end) {
+        code = walk.code(a, t * 32);
+        if (code == 1) vis = bits(t);
+        if (NBUF == 2) issue(t, 0);
+    }
     if (wave == 0 && nsplit == 1) {
         const float lam = da_lambda_rows(a, hk, blk * 32, w.head);
         if (h2 == 0) sLam[l32] = lam;
     }
     while (t < t_end) {
-        const int tn = next(t + 4), k0 = t * 32, code = da_tile_code(a, w, mb, k0 >> 6, M64, N64);
-        uint32_t vis = ~0u;                                   // (loaded in front of the next copies: the wait for it would be a wait for them)
-        if (code == 1 && w.live) vis = (uint32_t)(a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63));
-        asm volatile("" : "+v"(vis));
-        da_lds_done();                                        // the buffer in front has been read
         if (NBUF == 1) {
+            da_lds_done();
             issue(t, 0);
-            da_wait_copies<0>();
-        } else if (tn < t_end) {
+        }
+        const int tn = next(t + 4), code_n = tn < t_end ? walk.code(a, tn * 32) : 0, k0 = t * 32;
+        uint32_t vis_n = ~0u;
+        if (code_n == 1) vis_n = bits(tn);                    // (in front of the copies: the wait for it is a wait for what comes before it)
+        asm volatile("" : "+v"(vis), "+v"(vis_n));
+        da_lds_done();                                        // the buffer in front has been read
+        if (NBUF == 2 && tn < t_end) {
             issue(tn, buf ^ 1);
             da_wait_copies<NCOPY>();                          // tile t is there; tile tn may be on its way
         } else {
@@ -580,6 +644,8 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
         if (cut) vis &= w.limit <= k0 ? 0u : w.limit >= k0 + 32 ? ~0u : (1u << (w.limit - k0)) - 1;
         da_fwd_tile<T, DK>(st, qf, mine + buf * 2 * TILE, mine + buf * 2 * TILE + TILE, 0, masked, vis, a.scale_log2e, lane);
         t = tn;
+        code = code_n;
+        vis = vis_n;
         buf ^= NBUF - 1;
     }
     // the four waves' sums: common maximum, then every wave's share of it through LDS (unit u of row r at u ^ (r % 16))
@@ -702,90 +768,90 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// mask [Bm][N][M] bytes (strides sb, sn; non-zero = blocked) -> the forms the kernels read.  Workgroup = (batch, 64 keys), all queries: each of its 16 waves
-// takes every 16th tile of 64 queries; lane = key, one ballot per query, 16 loads in flight
-__global__ __launch_bounds__(1024) void diff_attn_mask_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sn, int N, int M, uint64_t *__restrict__ rowbits,
-                                                              uint64_t *__restrict__ colbits, uint64_t *__restrict__ live, uint8_t *__restrict__ tiles) {
+// mask [Bm][N][M] bytes (strides sb, sn; non-zero = blocked) -> the forms the kernels read.  A wave per tile of 64 queries x 64 keys; lane = key, one ballot
+// per query, 32 loads in flight
+__global__ __launch_bounds__(64) void diff_attn_mask_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sn, int N, int M, uint64_t *__restrict__ rowbits,
+                                                            uint64_t *__restrict__ colbits, uint64_t *__restrict__ some_, uint8_t *__restrict__ tiles) {
     const int M64 = (M + 63) >> 6, N64 = (N + 63) >> 6;
     const int kt = blockIdx.x % M64;
-    const int64_t b = blockIdx.x / M64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, key = kt * 64 + lane;
+    const int64_t rest = blockIdx.x / M64;
+    const int nt = (int)(rest % N64), lane = threadIdx.x, key = kt * 64 + lane, n1 = min(64, N - nt * 64);
+    const int64_t b = rest / N64;
     const uint64_t inside = M - kt * 64 >= 64 ? ~0ull : (1ull << (M - kt * 64)) - 1;
-    const uint8_t *col_p = mask + b * sb + min(key, M - 1);
-    __shared__ uint64_t any_s[16];
-    uint64_t any = 0;
-    for (int nt = wave; nt < N64; nt += 16) {
-        uint64_t col = 0, all = inside, some = 0, mine = 0;
-        const int n1 = min(64, N - nt * 64);
-        for (int n0 = 0; n0 < n1; n0 += 16) {
-            uint8_t v[16];
+    const uint8_t *p = mask + b * sb + (int64_t)nt * 64 * sn + min(key, M - 1);
+    uint64_t all = inside, some = 0, mine = 0;
+    uint32_t col[2];
 #pragma unroll
-            for (int x = 0; x < 16; ++x) v[x] = col_p[(int64_t)min(nt * 64 + n0 + x, N - 1) * sn];
+    for (int half = 0; half < 2; ++half) {
+        uint32_t v[32], c = 0;
 #pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const int n = n0 + x;
-                if (n >= n1) break;
-                const bool see = key < M && v[x] == 0;
-                const uint64_t bits = __ballot(see);
-                if (see) col |= 1ull << n;
-                if (n == lane) mine = bits;
-                all &= bits;
-                some |= bits;
-            }
+        for (int x = 0; x < 32; ++x) v[x] = p[(int64_t)min(half * 32 + x, n1 - 1) * sn];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+            const int n = half * 32 + x;
+            const bool see = v[x] == 0 && key < M && n < n1;
+            const uint64_t bits = __ballot(see);
+            c |= see ? 1u << x : 0u;
+            mine = n == lane ? bits : mine;
+            all &= n < n1 ? bits : ~0ull;
+            some |= bits;
         }
-        if (lane < n1) rowbits[(b * N + nt * 64 + lane) * M64 + kt] = mine;
-        if (key < M) colbits[(b * M + key) * N64 + nt] = col;
-        if (lane == 0) tiles[(b * N64 + nt) * M64 + kt] = some == 0 ? 2 : all == inside ? 0 : 1;
-        any |= some;
+        col[half] = c;
     }
-    if (lane == 0) any_s[wave] = any;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-#pragma unroll
-        for (int x = 1; x < 16; ++x) any |= any_s[x];
-        live[b * M64 + kt] = any;
+    if (lane < n1) rowbits[(b * N + nt * 64 + lane) * M64 + kt] = mine;
+    if (key < M) colbits[(b * M + key) * N64 + nt] = (uint64_t)col[1] << 32 | col[0];
+    if (lane == 0) {
+        some_[(b * N64 + nt) * M64 + kt] = some;
+        tiles[(b * N64 + nt) * M64 + kt] = some == 0 ? 2 : all == inside ? 0 : 1;
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
 // backward, first: dU (rounded to the type it is multiplied in), D_0, D_1 of every row and the partial sums of dl and dg.  Workgroup = (head, run of
-// (batch, query) rows); 32 lanes of 4 channels each per row.
+// (batch, query) rows); the lanes of a row sit next to each other.
 // With a norm dU stands at right angles to U up to eps: dU . U = r (t . U) eps r^2 with t = (1 - init) g dY.  A_1 V mostly points along U (both are
 // near the mean of the values where the maps are flat), so dU . (A_1 V) of rounded vectors would be a small difference of large products.  The forward
 // pass therefore keeps W = A_1 V - beta U, beta = (A_1 V . U) / (U . U), and D_1 = r (t . W) + beta (dU . U), D_0 = dU . U + l D_1 (long rows, bf16: error of dl
 // and dq against 64 bits 0.0046 with A_1 V itself).  dP is made from the ROUNDED dU: what the rounding adds to D is added here too.
 // The other kernels read the rows' statistics with l worked in: exp2(s - (lse_1 - log2 |l|)) is |l| A_1, and its sign goes with D_1 and dP.
-template <typename T>
+template <typename T, int LPR>
 __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, int nrun) {
+    constexpr int RW = 256 / LPR;                                                              // rows at a time, LPR lanes of 8 channels each
     const int head = blockIdx.x % a.H, run = blockIdx.x / a.H;
-    const int lane = threadIdx.x & 31, rr = threadIdx.x >> 5;                       // 32 lanes x 4 channels cover dv <= 128
-    const int c = lane * 4;
+    const int tid = threadIdx.x, lane = tid % LPR, rr = tid / LPR, c = lane * 8;
     const bool ok = c < a.dv;
     const float lam = da_lambda(a, head), log2l = log2f(fabsf(lam)), sign = lam < 0.f ? -1.f : 1.f;
-    float w[4], dw[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
+    float w[8], dw[8], dsum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = !ok ? 0.f : a.weight ? a.post * da_load1(a.weight, c + j, a.w_bf16) : 1.f;
+    for (int j = 0; j < 8; ++j) {
+        w[j] = !ok ? 0.f : a.weight ? a.post * da_load1(a.weight, c + j, a.w_bf16) : 1.f;
+        dw[j] = 0.f;
+    }
     const int64_t rows = (int64_t)a.B * a.N, bhn = rows * a.H;
-    for (int64_t r = (int64_t)run * 8 + rr; r < rows; r += (int64_t)nrun * 8) {
+    for (int64_t r = (int64_t)run * RW + rr; r < rows; r += (int64_t)nrun * RW) {
         const int b = (int)(r / a.N), i = (int)(r - (int64_t)b * a.N);
         const int64_t at = ((int64_t)b * a.H + head) * a.N + i, orow = (r * a.H + head) * a.dv + c;
-        float dy[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f}, o2[4] = {0.f, 0.f, 0.f, 0.f};
-        if (ok) {
-            da_load4(reinterpret_cast<const T *>(a.dy) + b * a.dys[0] + i * a.dys[1] + head * a.dys[2] + c, dy);
-            da_load4(reinterpret_cast<const T *>(a.weight ? a.u : a.out) + orow, u);
-            da_load4(reinterpret_cast<const T *>(a.o2) + orow, o2);
-        }
-        const bool empty = a.stats[at] == INFINITY;                                            // sees no key: no gradient, whatever dY holds
-        const float rn = a.weight ? a.stats[2 * bhn + at] : 1.f;
-        const float beta = a.weight ? a.stats[3 * bhn + at] : 0.f;
-        float dot = 0.f, d1 = 0.f, e1r = 0.f, e2r = 0.f, du[4];
+        float dy[8], u[8], o2[8], du[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 8; ++j) dy[j] = u[j] = o2[j] = 0.f;
+        if (ok) {
+            const T *yp = reinterpret_cast<const T *>(a.dy) + b * a.dys[0] + i * a.dys[1] + head * a.dys[2] + c;
+            const T *up = reinterpret_cast<const T *>(a.weight ? a.u : a.out) + orow, *op = reinterpret_cast<const T *>(a.o2) + orow;
+            da_load4(yp, dy); da_load4(yp + 4, dy + 4);
+            da_load4(up, u); da_load4(up + 4, u + 4);
+            da_load4(op, o2); da_load4(op + 4, o2 + 4);
+        }
+        const float lse0 = a.stats[at], lse1 = a.stats[bhn + at];
+        const bool empty = lse0 == INFINITY;                                                   // sees no key: no gradient, whatever dY holds
+        const float rn = a.weight ? a.stats[2 * bhn + at] : 1.f, beta = a.weight ? a.stats[3 * bhn + at] : 0.f;
+        float dot = 0.f, d1 = 0.f, e1r = 0.f, e2r = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
             dot += u[j] * w[j] * dy[j];
             d1 += w[j] * dy[j] * o2[j];
         }
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) { dot += __shfl_xor(dot, x); d1 += __shfl_xor(d1, x); }
+        for (int x = 1; x < LPR; x <<= 1) { dot += __shfl_xor(dot, x); d1 += __shfl_xor(d1, x); }
         float uu = dot;                                                                        // dU . U
         if (a.weight) {
             uu = rn * dot * a.eps * rn * rn;
@@ -793,7 +859,7 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
             dot *= rn * rn / (float)a.dv;
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 8; ++j) {
             if (a.weight) {
                 du[j] = rn * (w[j] * dy[j] - u[j] * dot);
                 if (!empty) dw[j] += a.post * rn * u[j] * dy[j];
@@ -807,36 +873,40 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
         }
         if (sizeof(T) == 2 && a.weight) {
 #pragma unroll
-            for (int x = 1; x < 32; x <<= 1) { e1r += __shfl_xor(e1r, x); e2r += __shfl_xor(e2r, x); }
+            for (int x = 1; x < LPR; x <<= 1) { e1r += __shfl_xor(e1r, x); e2r += __shfl_xor(e2r, x); }
         }
         float d0 = uu + lam * d1;
         if (empty) d0 = d1 = e1r = e2r = 0.f;
-        if (ok) da_store4(reinterpret_cast<T *>(a.du) + orow, du[0], du[1], du[2], du[3]);
+        if (ok) {
+            T *dp = reinterpret_cast<T *>(a.du) + orow;
+            da_store4(dp, du[0], du[1], du[2], du[3]);
+            da_store4(dp + 4, du[4], du[5], du[6], du[7]);
+        }
         if (lane == 0) {
-            a.rowstat[at] = a.stats[at];
-            a.rowstat[bhn + at] = a.stats[bhn + at] - log2l;
+            a.rowstat[at] = lse0;
+            a.rowstat[bhn + at] = lse1 - log2l;
             a.rowstat[2 * bhn + at] = d0 + e1r + lam * e2r;
             a.rowstat[3 * bhn + at] = (d1 + e2r) * sign;
+            dsum += d1;
         }
-        dsum += d1;
     }
-    __shared__ float sw[8][128], sd[8];
+    // this workgroup's sums: lanes of the same channels, then waves, in order
+    __shared__ float sw[4][LPR * 8], sd[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sw[rr][c + j] = dw[j];
-    if (lane == 0) sd[rr] = dsum;
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int x = LPR; x < 64; x <<= 1) dw[j] += __shfl_xor(dw[j], x);
+    }
+    dsum = da_wave_sum(dsum);
+    if ((tid & 63) < LPR) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sw[tid >> 6][c + j] = dw[j];
+        if (lane == 0) sd[tid >> 6] = dsum;
+    }
     __syncthreads();
-    if (threadIdx.x < a.dv && a.weight) {
-        float v = 0.f;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) v += sw[x][threadIdx.x];
-        a.wpart[(int64_t)blockIdx.x * a.dv + threadIdx.x] = v;
-    }
-    if (threadIdx.x == 0) {
-        float v = 0.f;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) v += sd[x];
-        a.lpart[blockIdx.x] = v;
-    }
+    if (a.weight)
+        for (int x = tid; x < a.dv; x += 256) a.wpart[(int64_t)blockIdx.x * a.dv + x] = (sw[0][x] + sw[1][x]) + (sw[2][x] + sw[3][x]);
+    if (tid == 0) a.lpart[blockIdx.x] = (sd[0] + sd[1]) + (sd[2] + sd[3]);
 }
 
 // gradients of the learned vectors and of the norm weight from the first kernel's partial sums, in a fixed order: one workgroup per head (or one for shared
@@ -942,23 +1012,26 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     cv.init(reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, a.dv, false, tid);
     const bool full = a.d == DK && a.dv == C::DV;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 1024;
-    auto next = [&](int k0) {
-        for (; k0 < wg_end && a.tiles; k0 += KB) {
-            bool hidden = true;
-            for (int qt = qt0; qt <= qt1; ++qt) hidden = hidden && a.tiles[(mb * N64 + qt) * M64 + (k0 >> 6)] == 2;
-            if (!hidden) break;
-        }
-        return k0;
-    };
+    DaWalk walk;
+    walk.base = -1;
+    auto next = [&](int k0) { return walk.next(a, w, mb, qt0, qt1, M64, N64, k0, wg_end); };
     auto issue = [&](int k0, int buf) {
         const int valid = len - k0;
-        const uint64_t live = a.live ? a.live[mb * M64 + (k0 >> 6)] >> (k0 & 63) : ~0ull;
-        const bool whole = full && valid >= KB && live == ~0ull;
+        const uint64_t live = walk.live(a, mb, qt0, qt1, M64, N64, k0), all = KB == 64 ? ~0ull : 0xffffffffull;
+        const bool whole = full && valid >= KB && (live & all) == all;
         ck.run(lds0 + buf * 2 * TILE, k0, a.ks[1], valid, live, whole);
         cv.run(lds0 + buf * 2 * TILE + TILE, k0, a.vs[1], valid, live, whole);
     };
-    int k0 = next(0), buf = 0;
-    if (k0 < wg_end) issue(k0, 0);
+    auto bits = [&](int k0) {                                 // a mixed tile's keys as this lane's row sees them
+        return w.live ? a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63) : 0ull;
+    };
+    int k0 = next(0), buf = 0, code = 0;
+    uint64_t vis = ~0ull;
+    if (k0 < wg_end) {
+        code = walk.code(a, k0);
+        if (code == 1) vis = bits(k0);
+        issue(k0, 0);
+    }
 
     const float lam = da_lambda_rows(a, hk, blk0 + wave * 32, w.head), sign = lam < 0.f ? -1.f : 1.f;
     const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + w.head) * a.N + w.i;
@@ -993,12 +1066,12 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
             for (int r = 0; r < 16; ++r) dq[t][x][r] = 0.f;
 
     while (k0 < wg_end) {
-        const int kn = next(k0 + KB), code = da_tile_code(a, w, mb, k0 >> 6, M64, N64);
-        uint64_t vis = ~0ull;                                 // (loaded in front of the next copies: the wait for it would be a wait for them)
-        if (code == 1 && w.live) vis = a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63);
+        const int kn = next(k0 + KB), code_n = kn < wg_end ? walk.code(a, kn) : 0;
+        uint64_t vis_n = ~0ull;
         da_wait_copies<0>();
         da_lds_done();
         __builtin_amdgcn_s_barrier();
+        if (code_n == 1) vis_n = bits(kn);
         if (kn < wg_end) issue(kn, buf ^ 1);
         if (code != 2 && k0 < w.lim_hi) {
             const bool cut = k0 + KB > w.lim_lo || w.ragged, masked = cut || code == 1;
@@ -1009,6 +1082,8 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
                 da_dq_tile<T, DK>(a, dq, qf, uf, lse, dl, sign, sK, sV, nt * 32, masked, (uint32_t)(vis >> (32 * nt)), lane);
         }
         k0 = kn;
+        code = code_n;
+        vis = vis_n;
         buf ^= 1;
     }
     if (!w.live) return;
@@ -1101,8 +1176,8 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
     const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
     const int kw0 = blk * 128 + wave * 32, key = kw0 + l32;
     const int64_t mb = a.mask_b ? b : 0, bhn = (int64_t)a.B * a.H * a.N;
-    bool klive = key < len;
-    if (klive && a.live) klive = (a.live[mb * M64 + (key >> 6)] >> (key & 63)) & 1;
+    const bool klive = key < len;
+    bool seen = false;                                        // some row of this run sees the key; else zeros are written, whatever its lanes met
     const bool wlive = kw0 < len;
 
     uint4 kf[2][C::NF], vf[C::NFV];
@@ -1145,13 +1220,37 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
     DaCopy<T, DK, QB, kDaThreads> cq, cu;
     cq.init(reinterpret_cast<const T *>(a.q) + b * a.qs[0], a.qs[1], a.qs[3], a.d, true, tid);
     cu.init(reinterpret_cast<const T *>(a.du) + (int64_t)b * a.N * a.H * a.dv, (int64_t)a.H * a.dv, 0, a.dv, false, tid);
+    // the mask's tiles along the queries as bit sets, 64 query blocks from qt_first + 64 base on (one per lane): workgroup and wave
+    uint64_t need = ~0ull, mixed = 0, hide = 0;
+    int base = -1;
     auto next = [&](int u) {
-        for (; u < u1 && a.tiles; ++u) {
-            const uint8_t *tp = a.tiles + (mb * N64 + qt_first + u % per_head) * M64;
-            if (tp[kt0] != 2 || tp[kt1] != 2) break;
+        while (u < u1 && a.tiles) {
+            const int x = u % per_head;
+            if (x >> 6 != base) {
+                base = x >> 6;
+                const int qt = qt_first + base * 64 + lane;
+                bool n = false, p = false, y = true;
+                if (qt < N64) {
+                    const uint8_t *tp = a.tiles + (mb * N64 + qt) * M64;
+                    const int c = wlive ? tp[kw0 >> 6] : 2;
+                    n = tp[kt0] != 2 || tp[kt1] != 2;
+                    p = c == 1;
+                    y = c == 2;
+                }
+                need = __ballot(n); mixed = __ballot(p); hide = __ballot(y);
+            }
+            const uint64_t m = need >> (x & 63);
+            if (m & 1) break;
+            u += m ? __builtin_ctzll(m) : min(64 - (x & 63), per_head - x);
         }
         return u;
     };
+    auto code_of = [&](int u) {
+        if (!a.tiles || u >= u1) return 0;
+        const int x = u % per_head & 63;
+        return (int)((mixed >> x) & 1 ? 1 : (hide >> x) & 1 ? 2 : 0);
+    };
+    auto bits = [&](int u) { return klive ? a.colbits[(mb * a.M + key) * N64 + qt_first + u % per_head] : 0ull; };
     auto row_lse = [&](int u) {                               // lse of this lane's row of block u: +inf where it sees nothing or is not there
         if (u >= u1) return INFINITY;
         const int g = u / per_head, i = (qt_first + u - g * per_head) * QB + lane;
@@ -1170,10 +1269,11 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
         const float *sp = i0 + lane < a.N ? a.rowstat + wave * bhn + ((int64_t)b * a.H + head) * a.N + i0 + lane : da_no_row + wave;     // wave = which statistic
         da_copy4(sp, __builtin_amdgcn_readfirstlane(to + 2 * TILE + wave * QB * 4));
     };
-    int u = next(u0), buf = 0, g_now = -1;
+    int u = next(u0), buf = 0, g_now = -1, code = code_of(u);
     float sign = 1.f;
+    uint64_t vis = code == 1 ? bits(u) : ~0ull;
     if (u < u1) issue(u, 0, row_lse(u));
-    int un = next(u + 1);
+    int un = next(u + 1), code_n = code_of(un);
     float lse_n = row_lse(un);
     while (u < u1) {
         const int g = u / per_head, i0 = (qt_first + u - g * per_head) * QB;
@@ -1181,14 +1281,9 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
             sign = da_lambda(a, hk * a.G + g) < 0.f ? -1.f : 1.f;
             g_now = g;
         }
-        int code = 0;
-        uint64_t vis = ~0ull;
-        if (a.tiles && wlive) {
-            code = a.tiles[(mb * N64 + (i0 >> 6)) * M64 + (kw0 >> 6)];
-            if (code == 1 && klive) vis = a.colbits[(mb * a.M + key) * N64 + (i0 >> 6)];
-        }
-        const int unn = next(un + 1);
+        const int unn = next(un + 1), code_nn = code_of(unn);
         const float lse_nn = row_lse(unn);                    // (one block ahead of its use: the rows that the next copies leave out)
+        const uint64_t vis_n = code_n == 1 && un < u1 ? bits(un) : ~0ull;
         da_wait_copies<0>();
         da_lds_done();
         __builtin_amdgcn_s_barrier();                         // block u is there for every wave, and every wave is done with the buffer in front
@@ -1206,10 +1301,13 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
                     const int64_t n0 = (int64_t)key - start - i1;
                     v &= n0 <= 0 ? ~0u : n0 >= 32 ? 0u : ~0u << n0;
                 }
+                seen = seen || v;
                 da_dkdv_tile<T, DK>(a, dk, dv, kf, vf, sign, sQ, sU, stat, QB, nt * 32, cut || code == 1, v, lane);
             }
         }
         u = un; un = unn; lse_n = lse_nn;
+        code = code_n; code_n = code_nn;
+        vis = vis_n;
         buf ^= 1;
     }
     if (key >= a.M) return;
@@ -1217,7 +1315,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
     const int w = 2 * a.d + a.dv;
     float *part = a.kvpart ? a.kvpart + ((int64_t)run * a.B * a.M * a.Hk + krow) * w : nullptr;
     T *dkp = reinterpret_cast<T *>(a.dk) + krow * 2 * a.d, *dvp = reinterpret_cast<T *>(a.dvv) + krow * a.dv;
-    const bool keep = klive;                                  // keys that nobody sees: zeros, whatever their lanes met
+    const bool keep = klive && seen;
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
 #pragma unroll
@@ -1293,7 +1391,7 @@ static bool diff_attn_aligned(const void *p) { return p && ((uintptr_t)p & 15) =
 int64_t dfine_diff_attn_mask_words(int64_t batches, int64_t N, int64_t M) {
     if (batches < 0 || N < 0 || M < 0) return -1;
     const int64_t M64 = (M + 63) / 64, N64 = (N + 63) / 64;
-    return batches * (N * M64 + M * N64 + M64 + (N64 * M64 + 7) / 8);
+    return batches * (N * M64 + M * N64 + N64 * M64) + (batches * N64 * M64 + 7) / 8;
 }
 
 static void diff_attn_forms(DiffArgs &a, const uint64_t *forms, int64_t batches) {
@@ -1301,8 +1399,8 @@ static void diff_attn_forms(DiffArgs &a, const uint64_t *forms, int64_t batches)
     const int64_t M64 = (a.M + 63) / 64, N64 = (a.N + 63) / 64;
     a.rowbits = forms;
     a.colbits = forms + batches * a.N * M64;
-    a.live = a.colbits + batches * a.M * N64;
-    a.tiles = reinterpret_cast<const uint8_t *>(a.live + batches * M64);
+    a.some = a.colbits + batches * a.M * N64;
+    a.tiles = reinterpret_cast<const uint8_t *>(a.some + batches * N64 * M64);
 }
 
 int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_t M, int64_t stride_b, int64_t stride_n, uint64_t *forms, void *stream) {
@@ -1310,10 +1408,10 @@ int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_
     if (batches == 0 || N == 0 || M == 0) return DFINE_OK;
     if (!mask || !forms) return DFINE_E_BADARG;
     const int64_t M64 = (M + 63) / 64, N64 = (N + 63) / 64;
-    if (batches * M64 > 0x7fffffff) return DFINE_E_BADARG;
-    uint64_t *col = forms + batches * N * M64, *live = col + batches * M * N64;
-    hipLaunchKernelGGL(diff_attn_mask_kernel, dim3((unsigned)(batches * M64)), dim3(1024), 0, (hipStream_t)stream, mask, stride_b, stride_n, (int)N, (int)M, forms, col, live,
-                       reinterpret_cast<uint8_t *>(live + batches * M64));
+    if (batches * M64 * N64 > 0x7fffffff) return DFINE_E_BADARG;
+    uint64_t *col = forms + batches * N * M64, *some = col + batches * M * N64;
+    hipLaunchKernelGGL(diff_attn_mask_kernel, dim3((unsigned)(batches * M64 * N64)), dim3(64), 0, (hipStream_t)stream, mask, stride_b, stride_n, (int)N, (int)M, forms, col,
+                       some, reinterpret_cast<uint8_t *>(some + batches * N64 * M64));
     return check_launch();
 }
 
@@ -1411,8 +1509,8 @@ int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void 
     return check_launch();
 }
 
-static int diff_attn_runs(const DiffArgs &a) {                  // workgroups per head of the first backward kernel: 1024 in all, 8 rows each at least
-    const int64_t rows = ((int64_t)a.B * a.N + 7) / 8;
+static int diff_attn_runs(const DiffArgs &a) {                  // workgroups per head of the first backward kernel: 1024 in all, one pass each at least
+    const int64_t rw = 2048 / (2 * diff_attn_size(a.d, a.dv)), rows = ((int64_t)a.B * a.N + rw - 1) / rw;       // rows of one pass of a workgroup
     int64_t n = 1024 / a.H;
     if (n < 1) n = 1;
     return (int)(n < rows ? n : rows < 1 ? 1 : rows);
@@ -1466,8 +1564,11 @@ int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void 
     a.kvpart = a.kvruns > 1 ? reinterpret_cast<float *>(p) : nullptr;
     hipStream_t st = (hipStream_t)stream;
     if (n > 0x7fffffff) return DFINE_E_BADARG;
-    if (shape[7] == 0) hipLaunchKernelGGL(diff_attn_prep_kernel<float>, dim3((unsigned)n), dim3(256), 0, st, a, nrun);
-    else hipLaunchKernelGGL(diff_attn_prep_kernel<uint16_t>, dim3((unsigned)n), dim3(256), 0, st, a, nrun);
+    const int dk_ = diff_attn_size(a.d, a.dv);
+#define DA_PREP(T_, L_) hipLaunchKernelGGL((diff_attn_prep_kernel<T_, L_>), dim3((unsigned)n), dim3(256), 0, st, a, nrun)
+    if (shape[7] == 0) { if (dk_ == 16) DA_PREP(float, 4); else if (dk_ == 32) DA_PREP(float, 8); else DA_PREP(float, 16); }
+    else { if (dk_ == 16) DA_PREP(uint16_t, 4); else if (dk_ == 32) DA_PREP(uint16_t, 8); else DA_PREP(uint16_t, 16); }
+#undef DA_PREP
     if (int e = check_launch()) return e;
     if (dlam || dweight) {
         const int nh = a.lam_heads == 1 ? 1 : a.H;

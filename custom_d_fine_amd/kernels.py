@@ -2626,7 +2626,7 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
     Which keys query i of sequence b sees: those `attn_mask` (bool [N, M] or [B, N, M], True = may not attend) lets it, j < kv_lengths[b] (int [B]: a
     padded batch or a cache that is not full; keys from there on are never read), and when `causal` j <= query_start + i (an int, or int [B]: the position
     of the first query among the keys).  A query that sees no key gives 0 and takes no gradient.  Keys that some query sees hold finite numbers; keys that
-    the mask hides from every query, and keys behind kv_lengths, may hold anything.
+    the mask hides from every query, and keys behind kv_lengths or the last causal position, may hold anything.
     Gradients for q, k, v, lambda_vectors and norm_weight, added up in a fixed order.  -> [B, N, H, dv], contiguous, of q's type.  Under bf16 autocast
     q, k, v are cast to bfloat16 first.  scale: d ** -0.5 by default."""
     op = "diff_attention"

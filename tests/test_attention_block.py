@@ -69,7 +69,7 @@ def test_c_entries_refuse_without_a_gpu():
     assert call(shape, scale=0.0, q=1 << 20) == -1 and call(shape, q=(1 << 20) + 2) == -1
     empty = hip._DA_SHAPE(*([0] + list(shape)[1:]))
     assert call(empty) == 0
-    assert hip._lib.dfine_diff_attn_bwd_ws_bytes(shape) > 0 and hip._lib.dfine_diff_attn_mask_words(1, 65, 130) == 65 * 3 + 130 * 2 + 3 + 1
+    assert hip._lib.dfine_diff_attn_bwd_ws_bytes(shape) > 0 and hip._lib.dfine_diff_attn_mask_words(1, 65, 130) == 65 * 3 + 130 * 2 + 2 * 3 + 1
     assert hip._lib.dfine_diff_attn_mask(None, 1, 5, 5, 0, 5, None, None) == -1
     qkn = hip._QKN_SHAPE(*([2, 5, 4, 2, 16, 8, 9, 1, 0, 0, 0, 0, 0] + [0] * 12))
     for at, bad in ((4, 12), (4, 264), (5, 12), (5, 24), (6, 4), (7, 3), (0, -1)):

@@ -159,6 +159,19 @@ def test_what_is_hidden_may_hold_anything(cuda, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("N", [1, 40])
+def test_a_cache_behind_the_last_causal_position_may_hold_anything(cuda, N):
+    B, M, H, Hk, d, dv = 2, 500, 6, 2, 32, 64
+    q, k, v, lam, w, dy, g = _inputs(cuda, B, N, M, H, Hk, d, dv, torch.bfloat16)
+    start = torch.tensor([101, 333], device=cuda)
+    clean, _ = _run(q, k, v, lam, w, dy, causal=True, query_start=start)
+    for b, n in enumerate((101 + N, 333 + N)):
+        k[b, n:], v[b, n:] = float("nan"), float("nan")
+    dirty, _ = _run(q, k, v, lam, w, dy, causal=True, query_start=start)
+    for a, b in zip(clean, dirty):
+        assert torch.equal(a, b)
+
+
 def test_a_visible_nan_reaches_the_result(cuda):
     q, k, v, lam, w, dy, _ = _inputs(cuda, 1, 40, 40, 6, 6, 32, 64, torch.bfloat16)
     k[0, 3, 2, 0, 1] = float("nan")
