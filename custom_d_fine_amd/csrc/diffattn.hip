@@ -13,8 +13,7 @@
 // Products (32 x 32 matrix instructions).  Forward and dQ: S^T = K Q^T puts ONE row of the list (a lane's column) against 16 keys per lane and tile in the
 // order 8 a + 4 h + b (h = lane / 32, a and b the register), which is the order the transposed read of V delivers the second product's other operand in, so
 // the probabilities go from registers to the matrix unit as they are.  dK and dV: S = Q K^T, one KEY per lane, the same way with dU and Q transposed.
-// LDS tiles hold rows of 16-byte units, unit u of row r at u ^ f(r) (da_swz): 8 lanes with one u and consecutive rows, and the 4 rows x 2 units of a
-// transposed read, fall on different banks without padding.
+// LDS tiles hold rows of 16-byte units, unit u of row r at u ^ f(r) (da_swz): both kinds of reads fall on different banks without padding.
 // Types: bf16 (v_mfma_f32_32x32x16_bf16; probabilities and dS are rounded to bf16 for the second products, as the values they meet are) and fp32
 // (v_mfma_f32_32x32x2_f32).  Scores, softmax statistics, sums and norms are 32-bit.  Head dims up to 64 with values up to 128, multiples of 8, run on the
 // next of three sizes with zero-filled tiles.
@@ -40,6 +39,8 @@ struct DiffArgs {
     int64_t qs[4], ks[4], vs[3];                // strides (batch, token, head, map)
     int64_t mask_b;                             // 0: one mask for the batch
     int64_t qstart;
+    uint32_t g_mul;                             // n / G = umulhi(2 n, g_mul) >> g_shift for n < 2^31
+    int g_shift;
     int B, N, M, H, Hk, G, d, dv, causal, lam_heads, lam_bf16, w_bf16;
     float scale, scale_log2e, init, post, eps;  // post = 1 - init with a norm weight
     // backward
@@ -76,34 +77,84 @@ template <typename T, int DK> struct DaCfg {
     static_assert(DV % 32 == 0, "a value tile is 32 channels");
 };
 
-template <int U> __device__ __forceinline__ int da_swz(int row) { return U >= 16 ? (row & 7) << 1 : U == 8 ? ((row >> 1) & 3) << 1 : ((row >> 2) & 1) << 1; }
-
-// one lane's 16 bytes of a row-major operand: row `row`, fragment f (channels f KPF ..), starting at unit u0 of the row
-template <int U> __device__ __forceinline__ uint4 da_frag(const char *tile, int row, int u) {
-    return *reinterpret_cast<const uint4 *>(tile + row * U * 16 + ((u ^ da_swz<U>(row)) << 4));
+// f(row): a b128 read serves 16 lanes at a time (rows 16 apart in some order, one u), a transposed read 32 lanes (4 rows from a multiple of 4 on, 4 units from a
+// multiple of 4 on): f takes all values over 16 rows and, in its bits from 2 on, over 4 (256 bytes = all banks; rows shorter than that share them).
+// Measured per wave: b128 4 cycles, transposed 3 (plain rows of 256 bytes: 64 and 8; u ^ 2 (row % 8): 8 and 4).  fp32 reads its transposed operand in 4-byte
+// pieces, 32 columns of rows 4 apart: there bit 2 of the row goes on top.
+template <typename T, int U> __device__ __forceinline__ int da_swz(int row) {
+    if (sizeof(T) == 4) return U >= 16 ? ((row >> 2) & 1) << 3 | (row & 3) << 1 | ((row >> 3) & 1) : (row >> 1) & 7;
+    return U >= 16 ? (row & 3) << 2 | ((row >> 2) & 3) : U == 8 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row >> 2) & 3;
 }
 
-// transposed operand: contraction over the tile's rows r0 .. r0 + KPF - 1 in the order 8 a + 4 h + b, this lane's column c0 + lane % 32
-template <typename T, int U> __device__ __forceinline__ uint4 da_frag_tr(const char *tile, int r0, int c0, int lane) {
-    const int h = lane >> 5;
-    if constexpr (sizeof(T) == 2) {
-        const int i16 = lane & 15, row = r0 + 4 * h + (i16 >> 2), u = (c0 >> 3) + ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1);
-        const char *p = tile + row * U * 16 + ((u ^ da_swz<U>(row)) << 4) + 8 * (i16 & 1);
-        const da_tr4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_tr4 __attribute__((address_space(3))) *)p);
-        const da_tr4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_tr4 __attribute__((address_space(3))) *)(p + 8 * U * 16));
-        return __builtin_bit_cast(uint4, (da_tr8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    } else {
-        const int col = c0 + (lane & 31), u = col >> 2;
-        uint32_t r[4];
+typedef __attribute__((ext_vector_type(4))) uint32_t da_u4v;
+typedef __attribute__((address_space(3))) const da_u4v *da_lds_u4;
+typedef __attribute__((address_space(3))) const uint32_t *da_lds_u1;
+
+// A lane's way through a tile of rows of U units (byte addresses in LDS; tiles start on 512-byte borders): everything that depends on the lane is one register
+// per kind of read, the fragment only flips bits of it
+template <typename T, int DK> struct DaLane {
+    using C = DaCfg<T, DK>;
+    uint32_t row, tr[sizeof(T) == 2 ? 1 : 4];
+    __device__ __forceinline__ void init(int lane) {
+        const int h = lane >> 5, l32 = lane & 31;
+        row = l32 * C::ROWB + ((h ^ da_swz<T, C::U>(l32)) << 4);
+        if constexpr (sizeof(T) == 2) {
+            const int i16 = lane & 15, r = 4 * h + (i16 >> 2), u = ((lane >> 4) & 1) * 2 + ((i16 & 3) >> 1);
+            tr[0] = r * C::ROWB + ((u ^ da_swz<T, C::U>(r)) << 4) + 8 * (i16 & 1);
+        } else {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int row = r0 + 4 * h + b;
-            r[b] = *reinterpret_cast<const uint32_t *>(tile + row * U * 16 + ((u ^ da_swz<U>(row)) << 4) + (col & 3) * 4);
+            for (int b = 0; b < 4; ++b) tr[b] = (4 * h + b) * C::ROWB + (((l32 >> 2) ^ da_swz<T, C::U>(4 * h + b)) << 4) + (l32 & 3) * 4;
         }
-        return make_uint4(r[0], r[1], r[2], r[3]);
+    }
+    // row-major operand: row lane % 32 of the 32 rows at `tile`, fragment f
+    __device__ __forceinline__ uint4 frag(uint32_t tile, int f) const { return __builtin_bit_cast(uint4, *(da_lds_u4)(uintptr_t)(tile + (row ^ (f << 5)))); }
+    // transposed operand: contraction over rows KPF f .. of the 32 rows at `tile` in the order 8 a + 4 h + b, column 32 x + lane % 32
+    __device__ __forceinline__ uint4 frag_tr(uint32_t tile, int f, int x) const {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t p = tile + (tr[0] ^ (x << 6)) + f * 16 * C::ROWB, q = tile + (tr[0] ^ (x << 6) ^ 32) + (f * 16 + 8) * C::ROWB;
+            const da_tr4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_tr4 __attribute__((address_space(3))) *)(uintptr_t)p);
+            const da_tr4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_tr4 __attribute__((address_space(3))) *)(uintptr_t)q);
+            return __builtin_bit_cast(uint4, (da_tr8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            uint32_t r[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                r[b] = *(da_lds_u1)(uintptr_t)(tile + (tr[b] ^ (x << 7) ^ (C::U >= 16 && (f & 1) ? 16 : 0) ^ (C::U == 8 && (f & 1) ? 64 : 0)) + f * 8 * C::ROWB);
+            return make_uint4(r[0], r[1], r[2], r[3]);
+        }
+    }
+};
+
+// N fragments through D registers in flight: rd(i) asks for fragment i, use(i, fragment) multiplies.  The order is held against the scheduler, which would
+// ask for each fragment right in front of its product and wait out the LDS latency N times; vector instructions may move across.
+template <int N, int D, class RD, class USE> __device__ __forceinline__ void da_ring(RD rd, USE use) {
+    uint4 fr[D];
+#pragma unroll
+    for (int i = 0; i < D && i < N; ++i) fr[i] = rd(i);
+    __builtin_amdgcn_sched_barrier(0x406);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        use(i, fr[i % D]);
+        if (i + D < N) fr[i % D] = rd(i + D);
+        __builtin_amdgcn_sched_barrier(0x406);
     }
 }
 
+// -1 where bit `pos` of v is set, else 0 (assembly: written as an expression it becomes an and, a compare and a select for each use)
+template <int POS> __device__ __forceinline__ uint32_t da_bit(uint32_t v) {
+    uint32_t r;
+    asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(r) : "v"(v), "n"(POS));
+    return r;
+}
+// scores of keys (rows) that the lane's row (key) does not see: -inf
+template <int R = 0> __device__ __forceinline__ void da_hide(da_f16v *s, uint32_t mine) {
+    if constexpr (R < 16) {
+        const uint32_t on = da_bit<8 * (R >> 2) + (R & 3)>(mine);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t][R] = __uint_as_float((__float_as_uint(s[t][R]) & on) | (0xff800000u & ~on));
+        da_hide<R + 1>(s, mine);
+    }
+}
 // Two floats to bf16 as a conversion the compiler sees (common.h's pack_bf16x2 is inline assembly): it has to put two wait states between the
 // conversion and a matrix instruction that reads it, which it does not do behind assembly.
 typedef __attribute__((ext_vector_type(2))) float da_f2;
@@ -139,6 +190,8 @@ template <typename T> __device__ __forceinline__ void da_load4(const T *p, float
     }
 }
 
+__device__ __forceinline__ int da_div_g(const DiffArgs &a, int n) { return (int)(__umulhi(2u * (uint32_t)n, a.g_mul) >> a.g_shift); }
+
 // sum over the 64 lanes, the same in every lane
 __device__ __forceinline__ float da_wave_sum(float v) {
 #define DA_DPP(ctrl) __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, true))
@@ -171,9 +224,10 @@ __device__ __forceinline__ float da_lambda(const DiffArgs &a, int h) {
     return e1 - e2 + a.init;
 }
 // l of each lane's own head, for a wave whose rows start at w0: its rows' heads are min(G, 32) in a row (a whole wave calls this)
-__device__ __forceinline__ float da_lambda_rows(const DiffArgs &a, int hk, int64_t w0, int head) {
+__device__ __forceinline__ float da_lambda_rows(const DiffArgs &a, int hk, int w0, int head) {
     if (a.lam_heads == 1) return da_lambda(a, 0);
-    const int g0 = (int)(w0 % a.G), n = min(a.G, 32);
+    if (a.G == 1) return da_lambda(a, hk);
+    const int g0 = w0 - da_div_g(a, w0) * a.G, n = min(a.G, 32);
     float lam = 0.f;
     for (int x = 0; x < n; ++x) {
         const int h = hk * a.G + (g0 + x) % a.G;
@@ -207,6 +261,13 @@ __device__ __forceinline__ void da_copy16(const void *src, uint32_t lds_addr) {
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(lds_addr) : "memory");
 }
 template <int N> __device__ __forceinline__ void da_wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void da_copies_done_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// Makes the compiler wait for a loaded value HERE: it does not see the waits above, and would put its own in front of the value's first use in the loop -
+// which is a wait for the copies that are on their way by then
+__device__ __forceinline__ void da_pin(uint4 &v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+__device__ __forceinline__ void da_pin(float &v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void da_pin(uint32_t &v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void da_pin(uint64_t &v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void da_lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 __device__ __attribute__((aligned(16))) uint32_t da_zero_page[4];            // what rows and channels that are not there are copied from
@@ -214,7 +275,7 @@ __device__ __attribute__((aligned(16))) uint32_t da_zero_page[4];            // 
 // One operand's way into LDS: `ROWS` rows of U units by NT threads (a workgroup or a wave), this thread's part
 template <typename T, int DK, int ROWS, int NT> struct DaCopy {
     using C = DaCfg<T, DK>;
-    static constexpr int J = ROWS * C::U / NT, STEP = NT / C::U, P = STEP >= 8 ? 1 : 8 / STEP;       // the swizzle repeats every 8 rows
+    static constexpr int J = ROWS * C::U / NT, STEP = NT / C::U, P = STEP >= 16 ? 1 : 16 / STEP;     // the swizzle repeats every 16 rows
     static_assert(J >= 1 && STEP >= 1 && J % P == 0, "");
     const T *base[P];                                   // row r0 of the tile at hand, this thread's channels
     bool ok[P];
@@ -223,7 +284,7 @@ template <typename T, int DK, int ROWS, int NT> struct DaCopy {
         r0 = t / C::U;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int u = (t % C::U) ^ da_swz<C::U>(r0 + p * STEP), half = maps ? u / (C::U / 2) : 0;
+            const int u = (t % C::U) ^ da_swz<T, C::U>(r0 + p * STEP), half = maps ? u / (C::U / 2) : 0;
             const int c = (maps ? u % (C::U / 2) : u) * (16 / C::ES);
             ok[p] = c < nch;
             base[p] = src + (int64_t)(r0 + p * STEP) * ld + half * map + c;
@@ -254,21 +315,19 @@ __device__ __forceinline__ float da_both_halves(float v) {
 
 // the rows of a wave: what the forward pass knows about the lane's row and the wave's range of queries
 struct DaRows {
-    int64_t row;
-    int i, head, limit, lim_lo, lim_hi, q_lo, q_hi;           // lim_*: ends of the first and last query's keys; q_*: their 64-query tiles
-    bool live, alive, ragged;                                 // this row / any row of the wave exists; some do not
+    int row, i, head, limit, lim_lo, lim_hi, q_lo, q_hi;           // lim_*: ends of the first and last query's keys; q_*: their 64-query tiles
+    bool live, alive;                                         // this row / any row of the wave exists
 };
-__device__ __forceinline__ DaRows da_rows(const DiffArgs &a, int hk, int64_t w0, int l32, int len, int64_t start) {
+__device__ __forceinline__ DaRows da_rows(const DiffArgs &a, int hk, int w0, int l32, int len, int64_t start) {
     DaRows w;
-    const int64_t R = (int64_t)a.N * a.G, wl = w0 + 31 < R - 1 ? w0 + 31 : R - 1;
+    const int R = a.N * a.G, wl = min(w0 + 31, R - 1);
     w.row = w0 + l32;
     w.live = w.row < R;
     w.alive = w0 < R;
-    w.ragged = wl - w0 < 31;
-    w.i = w.live ? (int)(w.row / a.G) : 0;
-    w.head = hk * a.G + (w.live ? (int)(w.row - (int64_t)w.i * a.G) : 0);
+    w.i = w.live ? da_div_g(a, w.row) : 0;
+    w.head = hk * a.G + (w.live ? w.row - w.i * a.G : 0);
     w.limit = w.live ? da_limit(a, len, start, w.i) : 0;
-    const int i_lo = w.alive ? (int)(w0 / a.G) : 0, i_hi = w.alive ? (int)(wl / a.G) : 0;
+    const int i_lo = w.alive ? da_div_g(a, w0) : 0, i_hi = w.alive ? da_div_g(a, wl) : 0;
     w.lim_lo = da_limit(a, len, start, i_lo);
     w.lim_hi = w.alive ? da_limit(a, len, start, i_hi) : 0;
     w.q_lo = i_lo >> 6; w.q_hi = i_hi >> 6;
@@ -352,32 +411,26 @@ template <typename T, int DK> __device__ __forceinline__ void da_load_q(const Di
 // The running maximum moves only when some row's grows by more than 2^8 (in the exp2 domain, 8): the accumulators are then rescaled; below that the
 // probabilities are at most 256 times what the true maximum would give, which 32-bit sums and bf16's exponent hold without loss.
 template <typename T, int DK>
-__device__ __forceinline__ void da_fwd_tile(DaState<T, DK> &st, const uint4 (*qf)[DaCfg<T, DK>::NF], const char *sK, const char *sV, int r0, bool masked, uint32_t vis,
-                                            float c, int lane) {
+__device__ __forceinline__ void da_fwd_tile(DaState<T, DK> &st, const uint4 (*qf)[DaCfg<T, DK>::NF], const DaLane<T, DK> &ln, uint32_t tk, uint32_t tv, bool masked, uint32_t vis, float c,
+                                            int lane) {
     using C = DaCfg<T, DK>;
-    const int h2 = lane >> 5, l32 = lane & 31;
-    uint4 pf[2][C::FPT];
-    vis >>= 4 * h2;
+    da_f16v s[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
+    da_ring<2 * C::NF, 4>([&](int i) { return ln.frag(tk, i); }, [&](int i, const uint4 &f) { s[i / C::NF] = Da<T>::mma(f, qf[i / C::NF][i % C::NF], s[i / C::NF]); });
+    if (masked) da_hide(s, vis >> (4 * (lane >> 5)));
+    float bm[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        da_f16v s;
+        bm[t] = s[t][0];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        for (int r = 1; r < 16; ++r) bm[t] = fmaxf(bm[t], s[t][r]);
+        bm[t] = da_other_half_max(bm[t]) * c;
+    }
+    if (__any(bm[0] > st.m[0] + 8.f || bm[1] > st.m[1] + 8.f)) {
 #pragma unroll
-        for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sK, r0 + l32, t * (C::U / 2) + 2 * f + h2), qf[t][f], s);
-        if (masked) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)vis, 8 * (r >> 2) + (r & 3), 1);
-                s[r] = __uint_as_float((__float_as_uint(s[r]) & on) | (0xff800000u & ~on));
-            }
-        }
-        float bm = s[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
-        bm = da_other_half_max(bm) * c;
-        if (__any(bm > st.m[t] + 8.f)) {
-            const float mn = fmaxf(st.m[t], bm), alpha = mn == -INFINITY ? 1.f : da_exp2(st.m[t] - mn);
+        for (int t = 0; t < 2; ++t) {
+            const float mn = fmaxf(st.m[t], bm[t]), alpha = mn == -INFINITY ? 1.f : da_exp2(st.m[t] - mn);
             st.m[t] = mn;
             st.l[t] *= alpha;
 #pragma unroll
@@ -385,27 +438,26 @@ __device__ __forceinline__ void da_fwd_tile(DaState<T, DK> &st, const uint4 (*qf
 #pragma unroll
                 for (int r = 0; r < 16; ++r) st.o[t][x][r] *= alpha;
         }
+    }
+    uint4 pf[2][C::FPT];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
         const float mu = st.m[t] == -INFINITY ? 0.f : st.m[t];
         float sum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[r] = da_exp2(fmaf(s[r], c, -mu));
-            sum += s[r];
+            s[t][r] = da_exp2(fmaf(s[t][r], c, -mu));
+            sum += s[t][r];
         }
         st.l[t] += sum;
 #pragma unroll
-        for (int f = 0; f < C::FPT; ++f) pf[t][f] = da_pack<T>(s, f);
-        if (C::ROWB > 256) __builtin_amdgcn_sched_barrier(0); // (fp32 heads of 64: all fragments asked for at once would not fit the registers)
+        for (int f = 0; f < C::FPT; ++f) pf[t][f] = da_pack<T>(s[t], f);
     }
-#pragma unroll
-    for (int f = 0; f < C::FPT; ++f)
-#pragma unroll
-        for (int x = 0; x < C::MT; ++x) {
-            if (C::ROWB > 256) __builtin_amdgcn_sched_barrier(0);
-            const uint4 vf = da_frag_tr<T, C::U>(sV, r0 + f * Da<T>::KPF, x * 32, lane);
-            st.o[0][x] = Da<T>::mma(vf, pf[0][f], st.o[0][x]);
-            st.o[1][x] = Da<T>::mma(vf, pf[1][f], st.o[1][x]);
-        }
+    da_ring<C::FPT * C::MT, 4>([&](int i) { return ln.frag_tr(tv, i / C::MT, i % C::MT); },
+                               [&](int i, const uint4 &f) {
+                                   st.o[0][i % C::MT] = Da<T>::mma(f, pf[0][i / C::MT], st.o[0][i % C::MT]);
+                                   st.o[1][i % C::MT] = Da<T>::mma(f, pf[1][i / C::MT], st.o[1][i % C::MT]);
+                               });
 }
 
 __device__ __forceinline__ float da_inv(float l) { return l > 0.f ? 1.f / l : l; }                 // an empty row: 0; not a number stays that
@@ -423,22 +475,27 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, nblk = gridDim.x / nbh, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int blk = a.causal ? nblk - 1 - (int)(blockIdx.x / nbh) : (int)(blockIdx.x / nbh);          // causal: the longest first
     const int len = da_len(a, b);
-    const int64_t start = da_start(a, b), R = (int64_t)a.N * a.G, blk0 = (int64_t)blk * 128;
+    const int64_t start = da_start(a, b);
+    const int R = a.N * a.G, blk0 = blk * 128;
     const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
     const int64_t mb = a.mask_b ? b : 0;
     const DaRows w = da_rows(a, hk, blk0 + wave * 32, l32, len, start);
-    const int i_end = (int)((blk0 + 127 < R - 1 ? blk0 + 127 : R - 1) / a.G);
-    const int wg_end = da_limit(a, len, start, i_end), qt0 = (int)(blk0 / a.G) >> 6, qt1 = i_end >> 6;
+    const int i_end = da_div_g(a, min(blk0 + 127, R - 1));
+    const int wg_end = da_limit(a, len, start, i_end), qt0 = da_div_g(a, blk0) >> 6, qt1 = i_end >> 6;
 
     uint4 qf[2][C::NF];
     da_load_q<T, DK>(a, w, b, h2, qf);
     DaState<T, DK> st;
     st.init();
+#pragma unroll
+    for (int f = 0; f < 2 * C::NF; ++f) da_pin(qf[f / C::NF][f % C::NF]);
     DaCopy<T, DK, KB, kDaThreads> ck, cv;
     ck.init(reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.ks[3], a.d, true, tid);
     cv.init(reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, a.dv, false, tid);
     const bool full = a.d == DK && a.dv == C::DV;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 1024;
+    const uint32_t tile0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds, lds0 = tile0 + wave * 1024;
+    DaLane<T, DK> ln;
+    ln.init(lane);
     DaWalk walk;
     walk.base = -1;
     auto next = [&](int k0) { return walk.next(a, w, mb, qt0, qt1, M64, N64, k0, wg_end); };
@@ -463,17 +520,19 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     while (k0 < wg_end) {
         const int kn = next(k0 + KB), code_n = kn < wg_end ? walk.code(a, kn) : 0;
         uint64_t vis_n = ~0ull;
-        da_wait_copies<0>();
-        da_lds_done();
-        __builtin_amdgcn_s_barrier();                         // block k0 is there for every wave, and every wave is done with the buffer in front
+        da_copies_done_barrier();                             // block k0 is there for every wave, and every wave is done with the buffer in front
+        da_pin(vis);
         if (code_n == 1) vis_n = bits(kn);                    // (in front of the copies: the wait for it is a wait for what comes before it)
         if (kn < wg_end) issue(kn, buf ^ 1);
         if (code != 2 && k0 < w.lim_hi) {
-            const bool cut = k0 + KB > w.lim_lo || w.ragged, masked = cut || code == 1;
+            const bool cut = k0 + KB > w.lim_lo, masked = cut || code == 1;
             if (cut) vis &= w.limit <= k0 ? 0ull : w.limit >= k0 + 64 ? ~0ull : (1ull << (w.limit - k0)) - 1;
-            const char *sK = lds + buf * 2 * TILE, *sV = sK + TILE;
+            const uint32_t tk = tile0 + buf * 2 * TILE, tv = tk + TILE;
 #pragma unroll 1
-            for (int nt = 0; nt < KB / 32; ++nt) da_fwd_tile<T, DK>(st, qf, sK, sV, nt * 32, masked, (uint32_t)(vis >> (32 * nt)), a.scale_log2e, lane);
+            for (int nt = 0; nt < KB / 32; ++nt) {
+                const uint32_t at = nt * 32 * C::ROWB;
+                da_fwd_tile<T, DK>(st, qf, ln, tk + at, tv + at, masked, (uint32_t)(vis >> (32 * nt)), a.scale_log2e, lane);
+            }
         }
         k0 = kn;
         code = code_n;
@@ -567,7 +626,7 @@ __device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, i
 // through two LDS buffers of its own (no barrier until the end).  The waves' sums meet in LDS; with one run the rows are finished here, else the run's sums
 // go to `part` (rows x nsplit x 2 DV, with maxima and sums in `ml`) for diff_attn_join_kernel.
 template <typename T, int DK>
-__global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(const DiffArgs a, int nsplit, float *__restrict__ part, float4 *__restrict__ ml) {
+__global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff_attn_fwd_split_kernel(const DiffArgs a, int nsplit, float *__restrict__ part, float4 *__restrict__ ml) {
     using C = DaCfg<T, DK>;
     constexpr int TILE = 32 * C::ROWB, NE = C::DV / 8, UO = 2 * C::DV / 4;
     constexpr int NBUF = C::ROWB > 256 ? 1 : 2;               // (fp32 heads of 64: two buffers for four waves would not fit LDS)
@@ -577,7 +636,7 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
     __shared__ float sM[2][4][32], sS[2][4][32], sLam[32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, rest = blockIdx.x / nbh, sp = rest % nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int64_t blk = rest / nsplit, R = (int64_t)a.N * a.G;
+    const int blk = rest / nsplit, R = a.N * a.G;
     const int len = da_len(a, b);
     const int64_t start = da_start(a, b);
     const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
@@ -589,6 +648,8 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
     da_load_q<T, DK>(a, w, b, h2, qf);
     DaState<T, DK> st;
     st.init();
+#pragma unroll
+    for (int f = 0; f < 2 * C::NF; ++f) da_pin(qf[f / C::NF][f % C::NF]);
     DaCopy<T, DK, 32, 64> ck, cv;
     constexpr int NCOPY = 2 * DaCopy<T, DK, 32, 64>::J;
     ck.init(reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.ks[3], a.d, true, lane);
@@ -596,6 +657,8 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
     const bool full = a.d == DK && a.dv == C::DV;
     char *mine = lds + wave * WBYTES;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)mine;
+    DaLane<T, DK> ln;
+    ln.init(lane);
     DaWalk walk;
     walk.base = -1;
     auto next = [&](int t) {
@@ -605,7 +668,11 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
         }
         return t;
     };
-    auto bits = [&](int t) { return w.live ? (uint32_t)(a.rowbits[(mb * a.N + w.i) * M64 + (t >> 1)] >> (t & 1 ? 32 : 0)) : 0u; };
+    auto bits = [&](int t) {
+        uint32_t v = w.live ? (uint32_t)(a.rowbits[(mb * a.N + w.i) * M64 + (t >> 1)] >> (t & 1 ? 32 : 0)) : 0u;
+        da_pin(v);
+        return v;
+    };
     auto issue = [&](int t, int buf) {
         const int k0 = t * 32, valid = len - k0;
         const uint64_t live = walk.live(a, mb, w.q_lo, w.q_hi, M64, N64, k0);
@@ -631,8 +698,7 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
         }
         const int tn = next(t + 4), code_n = tn < t_end ? walk.code(a, tn * 32) : 0, k0 = t * 32;
         uint32_t vis_n = ~0u;
-        if (code_n == 1) vis_n = bits(tn);                    // (in front of the copies: the wait for it is a wait for what comes before it)
-        asm volatile("" : "+v"(vis), "+v"(vis_n));
+        if (code_n == 1) vis_n = bits(tn);
         da_lds_done();                                        // the buffer in front has been read
         if (NBUF == 2 && tn < t_end) {
             issue(tn, buf ^ 1);
@@ -640,9 +706,10 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
         } else {
             da_wait_copies<0>();
         }
-        const bool cut = k0 + 32 > w.lim_lo || w.ragged, masked = cut || code == 1;
+        const bool cut = k0 + 32 > w.lim_lo, masked = cut || code == 1;
         if (cut) vis &= w.limit <= k0 ? 0u : w.limit >= k0 + 32 ? ~0u : (1u << (w.limit - k0)) - 1;
-        da_fwd_tile<T, DK>(st, qf, mine + buf * 2 * TILE, mine + buf * 2 * TILE + TILE, 0, masked, vis, a.scale_log2e, lane);
+        const uint32_t tk = lds0 + buf * 2 * TILE;
+        da_fwd_tile<T, DK>(st, qf, ln, tk, tk + TILE, masked, vis, a.scale_log2e, lane);
         t = tn;
         code = code_n;
         vis = vis_n;
@@ -673,7 +740,7 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
     }
     __syncthreads();
     const int r = tid >> 3, c0 = (tid & 7) * NE;
-    const int64_t row = blk * 32 + r;
+    const int row = blk * 32 + r;
     if (row >= R) return;
     float o[2][NE], lse[2], mx[2], sum[2];
 #pragma unroll
@@ -695,7 +762,7 @@ __global__ __launch_bounds__(kDaThreads, 1) void diff_attn_fwd_split_kernel(cons
             o[x][j] = s4.x; o[x][j + 1] = s4.y; o[x][j + 2] = s4.z; o[x][j + 3] = s4.w;
         }
     }
-    const int i = (int)(row / a.G), head = hk * a.G + (int)(row - (int64_t)i * a.G);
+    const int i = da_div_g(a, row), head = hk * a.G + row - i * a.G;
     if (nsplit == 1) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -719,11 +786,11 @@ template <typename T, int DV>
 __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffArgs a, int nsplit, const float *__restrict__ part, const float4 *__restrict__ ml) {
     constexpr int NE = DV / 8;
     const int lane = threadIdx.x & 63, sg = lane >> 3, c0 = (lane & 7) * NE;
-    const int64_t R = (int64_t)a.N * a.G, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= R * a.B * a.Hk) return;
+    const int R = a.N * a.G;
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= (int64_t)R * a.B * a.Hk) return;
     const int bh = (int)(at / R), b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int64_t row = at - (int64_t)bh * R;
-    const int i = (int)(row / a.G), head = hk * a.G + (int)(row - (int64_t)i * a.G);
+    const int row = (int)(at - (int64_t)bh * R), i = da_div_g(a, row), head = hk * a.G + row - i * a.G;
     const float lam = da_lambda(a, head);
     float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, o[2][NE];
     for (int s = lane; s < nsplit; s += 64) {
@@ -956,39 +1023,37 @@ __global__ __launch_bounds__(1024) void diff_attn_param_kernel(const DiffArgs a,
 // ------------------------------------------------------------------------------------------------------------------
 // backward, dQ: the forward's decomposition and copies; probabilities from the saved statistics
 template <typename T, int DK>
-__device__ __forceinline__ void da_dq_tile(const DiffArgs &a, da_f16v (*dq)[DaCfg<T, DK>::MTK], const uint4 (*qf)[DaCfg<T, DK>::NF], const uint4 *uf, const float *lse, const float *dl, float sign,
-                                           const char *sK, const char *sV, int r0, bool masked, uint32_t vis, int lane) {
+__device__ __forceinline__ void da_dq_tile(const DiffArgs &a, da_f16v (*dq)[DaCfg<T, DK>::MTK], const uint4 (*qf)[DaCfg<T, DK>::NF], const uint4 *uf, const float *lse, const float *dl,
+                                           float sign, const DaLane<T, DK> &ln, uint32_t tk, uint32_t tv, bool masked, uint32_t vis, int lane) {
     using C = DaCfg<T, DK>;
-    const int h2 = lane >> 5, l32 = lane & 31;
     const float c = a.scale_log2e;
-    vis >>= 4 * h2;
-    da_f16v dp;
+    da_f16v dp, s[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dp[r] = 0.f;
-#pragma unroll
-    for (int f = 0; f < C::NFV; ++f) dp = Da<T>::mma(da_frag<C::U>(sV, r0 + l32, 2 * f + h2), uf[f], dp);
+    for (int r = 0; r < 16; ++r) dp[r] = s[0][r] = s[1][r] = 0.f;
+    da_ring<C::NFV + 2 * C::NF, 4>([&](int i) { return i < C::NFV ? ln.frag(tv, i) : ln.frag(tk, i - C::NFV); },
+                                   [&](int i, const uint4 &f) {
+                                       if (i < C::NFV) { dp = Da<T>::mma(f, uf[i], dp); return; }
+                                       const int t = (i - C::NFV) / C::NF;
+                                       s[t] = Da<T>::mma(f, qf[t][(i - C::NFV) % C::NF], s[t]);
+                                   });
+    if (masked) da_hide(s, vis >> (4 * (lane >> 5)));
+    uint4 sf[2][C::FPT];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        da_f16v s;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-        for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sK, r0 + l32, t * (C::U / 2) + 2 * f + h2), qf[t][f], s);
         const float fac = t ? -sign : 1.f, dd = t ? dl[1] : -dl[0];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = da_exp2(fmaf(s[r], c, -lse[t])) * fmaf(dp[r], fac, dd);
-        if (masked) {
+        for (int r = 0; r < 16; ++r) s[t][r] = da_exp2(fmaf(s[t][r], c, -lse[t])) * (t ? fmaf(dp[r], fac, dd) : dp[r] + dd);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __uint_as_float(__float_as_uint(s[r]) & (uint32_t)__builtin_amdgcn_sbfe((int)vis, 8 * (r >> 2) + (r & 3), 1));
-        }
-#pragma unroll
-        for (int f = 0; f < C::FPT; ++f) {
-            const uint4 sf = da_pack<T>(s, f);
-#pragma unroll
-            for (int x = 0; x < C::MTK; ++x)
-                dq[t][x] = Da<T>::mma(da_frag_tr<T, C::U>(sK, r0 + f * Da<T>::KPF, DK < 32 ? 0 : t * DK + x * 32, lane), sf, dq[t][x]);
-        }
+        for (int f = 0; f < C::FPT; ++f) sf[t][f] = da_pack<T>(s[t], f);
     }
+    da_ring<2 * C::FPT * C::MTK, 4>([&](int i) {
+                                        const int t = i / (C::FPT * C::MTK), f = i / C::MTK % C::FPT, x = i % C::MTK;
+                                        return ln.frag_tr(tk, f, DK < 32 ? 0 : t * (DK / 32) + x);
+                                    },
+                                    [&](int i, const uint4 &fr) {
+                                        const int t = i / (C::FPT * C::MTK), f = i / C::MTK % C::FPT, x = i % C::MTK;
+                                        dq[t][x] = Da<T>::mma(fr, sf[t][f], dq[t][x]);
+                                    });
 }
 
 template <typename T, int DK>
@@ -1000,18 +1065,21 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, nblk = gridDim.x / nbh, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int blk = a.causal ? nblk - 1 - (int)(blockIdx.x / nbh) : (int)(blockIdx.x / nbh);          // causal: the longest first
     const int len = da_len(a, b);
-    const int64_t start = da_start(a, b), R = (int64_t)a.N * a.G, blk0 = (int64_t)blk * 128;
+    const int64_t start = da_start(a, b);
+    const int R = a.N * a.G, blk0 = blk * 128;
     const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
     const int64_t mb = a.mask_b ? b : 0;
     const DaRows w = da_rows(a, hk, blk0 + wave * 32, l32, len, start);
-    const int i_end = (int)((blk0 + 127 < R - 1 ? blk0 + 127 : R - 1) / a.G);
-    const int wg_end = da_limit(a, len, start, i_end), qt0 = (int)(blk0 / a.G) >> 6, qt1 = i_end >> 6;
+    const int i_end = da_div_g(a, min(blk0 + 127, R - 1));
+    const int wg_end = da_limit(a, len, start, i_end), qt0 = da_div_g(a, blk0) >> 6, qt1 = i_end >> 6;
 
     DaCopy<T, DK, KB, kDaThreads> ck, cv;
     ck.init(reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.ks[3], a.d, true, tid);
     cv.init(reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, a.dv, false, tid);
     const bool full = a.d == DK && a.dv == C::DV;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 1024;
+    const uint32_t tile0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds, lds0 = tile0 + wave * 1024;
+    DaLane<T, DK> ln;
+    ln.init(lane);
     DaWalk walk;
     walk.base = -1;
     auto next = [&](int k0) { return walk.next(a, w, mb, qt0, qt1, M64, N64, k0, wg_end); };
@@ -1059,27 +1127,35 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     }
     da_f16v dq[2][C::MTK];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+        da_pin(lse[t]);
+        da_pin(dl[t]);
+#pragma unroll
+        for (int f = 0; f < C::NF; ++f) da_pin(qf[t][f]);
 #pragma unroll
         for (int x = 0; x < C::MTK; ++x)
 #pragma unroll
             for (int r = 0; r < 16; ++r) dq[t][x][r] = 0.f;
+    }
+#pragma unroll
+    for (int f = 0; f < C::NFV; ++f) da_pin(uf[f]);
 
     while (k0 < wg_end) {
         const int kn = next(k0 + KB), code_n = kn < wg_end ? walk.code(a, kn) : 0;
         uint64_t vis_n = ~0ull;
-        da_wait_copies<0>();
-        da_lds_done();
-        __builtin_amdgcn_s_barrier();
+        da_copies_done_barrier();
+        da_pin(vis);
         if (code_n == 1) vis_n = bits(kn);
         if (kn < wg_end) issue(kn, buf ^ 1);
         if (code != 2 && k0 < w.lim_hi) {
-            const bool cut = k0 + KB > w.lim_lo || w.ragged, masked = cut || code == 1;
+            const bool cut = k0 + KB > w.lim_lo, masked = cut || code == 1;
             if (cut) vis &= w.limit <= k0 ? 0ull : w.limit >= k0 + 64 ? ~0ull : (1ull << (w.limit - k0)) - 1;
-            const char *sK = lds + buf * 2 * TILE, *sV = sK + TILE;
+            const uint32_t tk = tile0 + buf * 2 * TILE, tv = tk + TILE;
 #pragma unroll 1
-            for (int nt = 0; nt < KB / 32; ++nt)
-                da_dq_tile<T, DK>(a, dq, qf, uf, lse, dl, sign, sK, sV, nt * 32, masked, (uint32_t)(vis >> (32 * nt)), lane);
+            for (int nt = 0; nt < KB / 32; ++nt) {
+                const uint32_t at = nt * 32 * C::ROWB;
+                da_dq_tile<T, DK>(a, dq, qf, uf, lse, dl, sign, ln, tk + at, tv + at, masked, (uint32_t)(vis >> (32 * nt)), lane);
+            }
         }
         k0 = kn;
         code = code_n;
@@ -1109,53 +1185,55 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
 // backward, dK and dV: workgroup = (batch, key head, 128 keys, one of kvruns runs of the rows), a wave owns 32 keys with both operands in registers; the
 // queries of the group's heads stream through two LDS buffers of QB rows (Q | dU | four statistics), copied while the block in front is worked on
 template <typename T, int DK>
-__device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[DaCfg<T, DK>::MTK], da_f16v *dv, const uint4 (*kf)[DaCfg<T, DK>::NF], const uint4 *vf, float sign, const char *sQ,
-                                             const char *sU, const float *stat, int stat_ld, int r0, bool masked, uint32_t vis, int lane) {
+__device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[DaCfg<T, DK>::MTK], da_f16v *dv, const uint4 (*kf)[DaCfg<T, DK>::NF], const uint4 *vf, float sign,
+                                             const DaLane<T, DK> &ln, uint32_t tq, uint32_t tu, uint32_t stat, bool masked, uint32_t vis, int lane) {
     using C = DaCfg<T, DK>;
-    const int h2 = lane >> 5, l32 = lane & 31;
     const float c = a.scale_log2e;
-    vis >>= 4 * h2;
-    da_f16v dp, p;
+    const int h2 = lane >> 5;
+    da_f16v dp, s[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dp[r] = 0.f;
-#pragma unroll
-    for (int f = 0; f < C::NFV; ++f) dp = Da<T>::mma(da_frag<C::U>(sU, r0 + l32, 2 * f + h2), vf[f], dp);
+    for (int r = 0; r < 16; ++r) dp[r] = s[0][r] = s[1][r] = 0.f;
+    da_ring<C::NFV + 2 * C::NF, 4>([&](int i) { return i < C::NFV ? ln.frag(tu, i) : ln.frag(tq, i - C::NFV); },
+                                   [&](int i, const uint4 &f) {
+                                       if (i < C::NFV) { dp = Da<T>::mma(f, vf[i], dp); return; }
+                                       const int t = (i - C::NFV) / C::NF;
+                                       s[t] = Da<T>::mma(f, kf[t][(i - C::NFV) % C::NF], s[t]);
+                                   });
+    if (masked) da_hide(s, vis >> (4 * h2));
+    uint4 sf[2][C::FPT], pf[C::FPT];
+    da_f16v p;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        da_f16v s;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-        for (int f = 0; f < C::NF; ++f) s = Da<T>::mma(da_frag<C::U>(sQ, r0 + l32, t * (C::U / 2) + 2 * f + h2), kf[t][f], s);
         const float fac = t ? -sign : 1.f;
+        float lv[16], dl[16];                                 // this lane's 16 rows' statistics: QB floats of each kind in LDS
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-            const float4 ls = *reinterpret_cast<const float4 *>(stat + t * stat_ld + r0 + 8 * q4 + 4 * h2);
-            const float4 dd = *reinterpret_cast<const float4 *>(stat + (2 + t) * stat_ld + r0 + 8 * q4 + 4 * h2);
-            const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dl[4] = {dd.x, dd.y, dd.z, dd.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = 4 * q4 + j;
-                float e = da_exp2(fmaf(s[r], c, -lv[j]));
-                if (masked) e = __uint_as_float(__float_as_uint(e) & (uint32_t)__builtin_amdgcn_sbfe((int)vis, 8 * q4 + j, 1));
-                p[r] = t ? fmaf(e, fac, p[r]) : e;
-                s[r] = e * (t ? fmaf(dp[r], fac, dl[j]) : dp[r] - dl[j]);
-            }
+            const da_u4v x = *(da_lds_u4)(uintptr_t)(stat + (t * 64 + 8 * q4 + 4 * h2) * 4), y = *(da_lds_u4)(uintptr_t)(stat + ((2 + t) * 64 + 8 * q4 + 4 * h2) * 4);
+            lv[4 * q4] = __uint_as_float(x.x); lv[4 * q4 + 1] = __uint_as_float(x.y); lv[4 * q4 + 2] = __uint_as_float(x.z); lv[4 * q4 + 3] = __uint_as_float(x.w);
+            dl[4 * q4] = __uint_as_float(y.x); dl[4 * q4 + 1] = __uint_as_float(y.y); dl[4 * q4 + 2] = __uint_as_float(y.z); dl[4 * q4 + 3] = __uint_as_float(y.w);
         }
 #pragma unroll
-        for (int f = 0; f < C::FPT; ++f) {
-            const uint4 sf = da_pack<T>(s, f);
-#pragma unroll
-            for (int x = 0; x < C::MTK; ++x)
-                dk[t][x] = Da<T>::mma(da_frag_tr<T, C::U>(sQ, r0 + f * Da<T>::KPF, DK < 32 ? 0 : t * DK + x * 32, lane), sf, dk[t][x]);
+        for (int r = 0; r < 16; ++r) {
+            const float e = da_exp2(fmaf(s[t][r], c, -lv[r]));
+            p[r] = t ? fmaf(e, fac, p[r]) : e;
+            s[t][r] = e * (t ? fmaf(dp[r], fac, dl[r]) : dp[r] - dl[r]);
         }
+#pragma unroll
+        for (int f = 0; f < C::FPT; ++f) sf[t][f] = da_pack<T>(s[t], f);
     }
 #pragma unroll
-    for (int f = 0; f < C::FPT; ++f) {
-        const uint4 pf = da_pack<T>(p, f);
-#pragma unroll
-        for (int x = 0; x < C::MT; ++x) dv[x] = Da<T>::mma(da_frag_tr<T, C::U>(sU, r0 + f * Da<T>::KPF, x * 32, lane), pf, dv[x]);
-    }
+    for (int f = 0; f < C::FPT; ++f) pf[f] = da_pack<T>(p, f);
+    constexpr int NK = 2 * C::FPT * C::MTK;
+    da_ring<NK + C::FPT * C::MT, 4>([&](int i) {
+                                        if (i >= NK) return ln.frag_tr(tu, (i - NK) / C::MT, (i - NK) % C::MT);
+                                        const int t = i / (C::FPT * C::MTK), f = i / C::MTK % C::FPT, x = i % C::MTK;
+                                        return ln.frag_tr(tq, f, DK < 32 ? 0 : t * (DK / 32) + x);
+                                    },
+                                    [&](int i, const uint4 &fr) {
+                                        if (i >= NK) { dv[(i - NK) % C::MT] = Da<T>::mma(fr, pf[(i - NK) / C::MT], dv[(i - NK) % C::MT]); return; }
+                                        const int t = i / (C::FPT * C::MTK), f = i / C::MTK % C::FPT, x = i % C::MTK;
+                                        dk[t][x] = Da<T>::mma(fr, sf[t][f], dk[t][x]);
+                                    });
 }
 
 __device__ __attribute__((aligned(16))) float da_no_row[4] = {__builtin_huge_valf(), __builtin_huge_valf(), 0.f, 0.f};     // statistics of a row that is not there
@@ -1167,7 +1245,7 @@ __device__ __forceinline__ void da_copy4(const void *src, uint32_t lds_addr) {
 template <typename T, int DK>
 __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2) ? 2 : 1) void diff_attn_dkdv_kernel(const DiffArgs a) {
     using C = DaCfg<T, DK>;
-    constexpr int QB = 64, TILE = QB * C::ROWB, BUF = 2 * TILE + 4 * QB * 4;
+    constexpr int QB = 64, TILE = QB * C::ROWB, BUF = 2 * TILE + 4 * QB * 4;       // (BUF: a multiple of 512 bytes)
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, rest = blockIdx.x / nbh, run = rest % a.kvruns, blk = rest / a.kvruns, b = bh / a.Hk, hk = bh - b * a.Hk;
@@ -1195,6 +1273,10 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
         const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
         vf[f] = klive && c < a.dv ? *reinterpret_cast<const uint4 *>(vp + c) : make_uint4(0, 0, 0, 0);
     }
+#pragma unroll
+    for (int f = 0; f < 2 * C::NF; ++f) da_pin(kf[f / C::NF][f % C::NF]);
+#pragma unroll
+    for (int f = 0; f < C::NFV; ++f) da_pin(vf[f]);
     da_f16v dk[2][C::MTK], dv[C::MT];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -1216,6 +1298,8 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
     const int u0 = (int)((int64_t)total * run / a.kvruns), u1 = (int)((int64_t)total * (run + 1) / a.kvruns);
     const int kt0 = blk * 2, kt1 = min(kt0 + 1, M64 - 1);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    DaLane<T, DK> ln;
+    ln.init(lane);
     const bool full = a.d == DK && a.dv == C::DV;
     DaCopy<T, DK, QB, kDaThreads> cq, cu;
     cq.init(reinterpret_cast<const T *>(a.q) + b * a.qs[0], a.qs[1], a.qs[3], a.d, true, tid);
@@ -1281,16 +1365,15 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
             sign = da_lambda(a, hk * a.G + g) < 0.f ? -1.f : 1.f;
             g_now = g;
         }
+        da_copies_done_barrier();                             // block u is there for every wave, and every wave is done with the buffer in front
+        da_pin(vis);
+        da_pin(lse_n);
         const int unn = next(un + 1), code_nn = code_of(unn);
         const float lse_nn = row_lse(unn);                    // (one block ahead of its use: the rows that the next copies leave out)
         const uint64_t vis_n = code_n == 1 && un < u1 ? bits(un) : ~0ull;
-        da_wait_copies<0>();
-        da_lds_done();
-        __builtin_amdgcn_s_barrier();                         // block u is there for every wave, and every wave is done with the buffer in front
         if (un < u1) issue(un, buf ^ 1, lse_n);
         if (wlive && code != 2) {
-            const char *sQ = lds + buf * BUF, *sU = sQ + TILE;
-            const float *stat = reinterpret_cast<const float *>(sU + TILE);
+            const uint32_t tq = lds0 + buf * BUF, tu = tq + TILE, stat = tu + TILE;
 #pragma unroll 1
             for (int nt = 0; nt < QB / 32; ++nt) {
                 const int i1 = i0 + nt * 32;
@@ -1302,7 +1385,8 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
                     v &= n0 <= 0 ? ~0u : n0 >= 32 ? 0u : ~0u << n0;
                 }
                 seen = seen || v;
-                da_dkdv_tile<T, DK>(a, dk, dv, kf, vf, sign, sQ, sU, stat, QB, nt * 32, cut || code == 1, v, lane);
+                const uint32_t at = nt * 32 * C::ROWB;
+                da_dkdv_tile<T, DK>(a, dk, dv, kf, vf, sign, ln, tq + at, tu + at, stat + nt * 128, cut || code == 1, v, lane);
             }
         }
         u = un; un = unn; lse_n = lse_nn;
@@ -1375,8 +1459,11 @@ static int diff_attn_setup(DiffArgs &a, const int64_t *s, float scale, float ini
         dv > 128 || dv % 8 || (dt != 0 && dt != 1) || !(scale > 0.f) || !(eps >= 0.f))
         return DFINE_E_BADARG;
     if (s[8] != 1 && s[8] != H) return DFINE_E_BADARG;                               // heads of the learned vectors
-    if (N * (H / Hk) > (int64_t)1 << 36 || B * Hk > 0xffffff) return DFINE_E_BADARG;
+    if (N * (H / Hk) > 0x7fffff00 || B * Hk > 0xffffff) return DFINE_E_BADARG;       // (rows of a key head: 32-bit)
     a.B = (int)B; a.N = (int)N; a.M = (int)M; a.H = (int)H; a.Hk = (int)Hk; a.G = (int)(H / Hk); a.d = (int)d; a.dv = (int)dv;
+    a.g_shift = 0;
+    while ((1 << a.g_shift) < a.G) ++a.g_shift;
+    a.g_mul = (uint32_t)((((uint64_t)1 << (31 + a.g_shift)) + a.G - 1) / a.G);
     a.lam_heads = (int)s[8]; a.lam_bf16 = s[9] != 0; a.w_bf16 = s[10] != 0;
     a.causal = s[11] != 0; a.qstart = s[12]; a.mask_b = s[13];
     const int unit = dt == 0 ? 4 : 8;                                                // elements of a 16-byte load

@@ -2651,7 +2651,7 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
         _refuse(f"{op}: heads of 2 x {d} channels with values of {dv} (multiples of 8 up to 64, 128)")
     if not 1 <= Hk <= H <= 4096 or H % Hk:
         _refuse(f"{op}: {H} heads on {Hk} key heads")
-    if N >= 2 ** 30 or M >= 2 ** 30 or B * Hk >= 2 ** 24:
+    if N >= 2 ** 30 or M >= 2 ** 30 or N * (H // Hk) >= 2 ** 31 - 256 or B * Hk >= 2 ** 24:
         _refuse(f"{op}: {B} sequences of {N} queries and {M} keys")
     _float_operand(op, "lambda_vectors", lambda_vectors, device)
     if lambda_vectors.shape != (4, d) and lambda_vectors.shape != (4, H, d):
