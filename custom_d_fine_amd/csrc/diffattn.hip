@@ -460,6 +460,30 @@ __device__ __forceinline__ void da_fwd_tile(DaState<T, DK> &st, const uint4 (*qf
                                });
 }
 
+// A wave's 32 rows x W channels from accumulator order to memory in whole rows: four channels at a time into LDS (unit u of row r at u ^ r % units), then 16
+// bytes per lane, a row's units on neighbouring lanes.  (Stores straight from the accumulators are 8-byte pieces of 32 rows each: the forward pass of 32 x 492
+// tokens spent 15 of its 40 us in them.)
+template <typename T, int W> struct DaRowsOut {
+    static constexpr int UN = W * (int)sizeof(T) / 16, RP = 64 / UN;               // units of a row, rows of one round
+    char *buf;
+    __device__ __forceinline__ void put(int r, int c, float a, float b, float d, float e) const {
+        const int at = c * (int)sizeof(T);
+        da_store4(reinterpret_cast<T *>(buf + r * W * sizeof(T) + (((at >> 4) ^ (r & (UN < 16 ? UN - 1 : 15))) << 4) + (at & 15)), a, b, d, e);
+    }
+    // dst(row, channel): where the 16 bytes from `channel` on of row `row` go, or null
+    template <class F> __device__ __forceinline__ void flush(int lane, F dst) const {
+        da_lds_done();
+#pragma unroll
+        for (int n = 0; n < 32 / RP; ++n) {
+            const int r = n * RP + lane / UN, u = lane % UN;
+            const uint4 v = *reinterpret_cast<const uint4 *>(buf + r * W * sizeof(T) + ((u ^ (r & (UN < 16 ? UN - 1 : 15))) << 4));
+            T *p = dst(r, u * 16 / (int)sizeof(T));
+            if (p) *reinterpret_cast<uint4 *>(p) = v;
+        }
+        da_lds_done();
+    }
+};
+
 __device__ __forceinline__ float da_inv(float l) { return l > 0.f ? 1.f / l : l; }                 // an empty row: 0; not a number stays that
 __device__ __forceinline__ float da_lse(float m, float l) { return l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l; }
 
@@ -539,7 +563,6 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         vis = vis_n;
         buf ^= 1;
     }
-    if (!w.live) return;                                      // (both lanes of a row go together)
     const float l0 = da_both_halves(st.l[0]), l1 = da_both_halves(st.l[1]), inv0 = da_inv(l0), inv1 = da_inv(l1);
     float ss = 0.f, us = 0.f;
 #pragma unroll
@@ -555,32 +578,53 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     us = da_both_halves(us);
     const float beta = a.weight && ss > 0.f ? us / ss : 0.f;  // what is kept of A_1 V is its part at right angles to U (diff_attn_prep_kernel)
     const float rn = a.weight ? rsqrtf(ss / (float)a.dv + a.eps) : 1.f;
-    const int64_t orow = (((int64_t)b * a.N + w.i) * a.H + w.head) * a.dv;
-#pragma unroll
-    for (int x = 0; x < C::MT; ++x)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-            const int c = x * 32 + 8 * q4 + 4 * h2;
-            if (c >= a.dv) continue;
-            float g[4] = {1.f, 1.f, 1.f, 1.f};
-            if (a.weight)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) g[j] = da_load1(a.weight, c + j, a.w_bf16) * a.post * rn;
-            const float u0 = st.o[0][x][4 * q4], u1 = st.o[0][x][4 * q4 + 1], u2 = st.o[0][x][4 * q4 + 2], u3 = st.o[0][x][4 * q4 + 3];
-            da_store4(reinterpret_cast<T *>(a.out) + orow + c, u0 * g[0], u1 * g[1], u2 * g[2], u3 * g[3]);
-            if (a.o2) {
-                if (a.weight) da_store4(reinterpret_cast<T *>(a.u) + orow + c, u0, u1, u2, u3);
-                da_store4(reinterpret_cast<T *>(a.o2) + orow + c, st.o[1][x][4 * q4] - beta * u0, st.o[1][x][4 * q4 + 1] - beta * u1, st.o[1][x][4 * q4 + 2] - beta * u2,
-                          st.o[1][x][4 * q4 + 3] - beta * u3);
-            }
-        }
-    if (a.stats && h2 == 0) {
+    if (a.stats && h2 == 0 && w.live) {
         const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + w.head) * a.N + w.i;
         a.stats[at] = da_lse(st.m[0], l0);
         a.stats[bhn + at] = da_lse(st.m[1], l1);
         a.stats[2 * bhn + at] = rn;
         a.stats[3 * bhn + at] = beta;
     }
+    __syncthreads();                                          // every wave is done with the tiles
+    const DaRowsOut<T, C::DV> rows{lds + wave * 32 * C::DV * C::ES};
+    const int w0 = blk0 + wave * 32;
+    auto to = [&](void *base) {
+        rows.flush(lane, [&](int r, int c) -> T * {
+            const int row = w0 + r, i = da_div_g(a, min(row, R - 1));
+            return row < R && c < a.dv ? reinterpret_cast<T *>(base) + (((int64_t)b * a.N + i) * a.H + hk * a.G + row - i * a.G) * a.dv + c : nullptr;
+        });
+    };
+#pragma unroll
+    for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const int c = x * 32 + 8 * q4 + 4 * h2;
+            float g[4] = {1.f, 1.f, 1.f, 1.f};
+            if (a.weight && c < a.dv)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) g[j] = da_load1(a.weight, c + j, a.w_bf16) * a.post * rn;
+            rows.put(l32, c, st.o[0][x][4 * q4] * g[0], st.o[0][x][4 * q4 + 1] * g[1], st.o[0][x][4 * q4 + 2] * g[2], st.o[0][x][4 * q4 + 3] * g[3]);
+        }
+    to(a.out);
+    if (!a.o2) return;
+    if (a.weight) {
+#pragma unroll
+        for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                rows.put(l32, x * 32 + 8 * q4 + 4 * h2, st.o[0][x][4 * q4], st.o[0][x][4 * q4 + 1], st.o[0][x][4 * q4 + 2], st.o[0][x][4 * q4 + 3]);
+        to(a.u);
+    }
+#pragma unroll
+    for (int x = 0; x < C::MT; ++x)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            float o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = st.o[1][x][4 * q4 + j] - beta * st.o[0][x][4 * q4 + j];
+            rows.put(l32, x * 32 + 8 * q4 + 4 * h2, o[0], o[1], o[2], o[3]);
+        }
+    to(a.o2);
 }
 
 // One row of the result from its two maps' sums in plain order: LPR neighbouring lanes of NE channels each (c0: the lane's first), O normalised
@@ -835,39 +879,39 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// mask [Bm][N][M] bytes (strides sb, sn; non-zero = blocked) -> the forms the kernels read.  A wave per tile of 64 queries x 64 keys; lane = key, one ballot
-// per query, 32 loads in flight
-__global__ __launch_bounds__(64) void diff_attn_mask_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sn, int N, int M, uint64_t *__restrict__ rowbits,
-                                                            uint64_t *__restrict__ colbits, uint64_t *__restrict__ some_, uint8_t *__restrict__ tiles) {
+// mask [Bm][N][M] bytes (strides sb, sn; non-zero = blocked) -> the forms the kernels read.  Workgroup = tile of 64 queries x 64 keys, a wave takes 16 queries;
+// lane = key, one ballot per query, all 16 loads in flight
+__global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sn, int N, int M, uint64_t *__restrict__ rowbits,
+                                                             uint64_t *__restrict__ colbits, uint64_t *__restrict__ some_, uint8_t *__restrict__ tiles) {
     const int M64 = (M + 63) >> 6, N64 = (N + 63) >> 6;
-    const int kt = blockIdx.x % M64;
-    const int64_t rest = blockIdx.x / M64;
-    const int nt = (int)(rest % N64), lane = threadIdx.x, key = kt * 64 + lane, n1 = min(64, N - nt * 64);
+    const int kt = blockIdx.x % M64, rest = blockIdx.x / M64;
     const int64_t b = rest / N64;
+    const int nt = rest - (int)b * N64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, key = kt * 64 + lane, n0 = nt * 64 + wave * 16, n1 = min(16, N - n0);
     const uint64_t inside = M - kt * 64 >= 64 ? ~0ull : (1ull << (M - kt * 64)) - 1;
-    const uint8_t *p = mask + b * sb + (int64_t)nt * 64 * sn + min(key, M - 1);
+    const uint8_t *p = mask + b * sb + min(key, M - 1);
+    uint32_t v[16], c = 0;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) v[x] = p[(int64_t)min(n0 + x, N - 1) * sn];
     uint64_t all = inside, some = 0, mine = 0;
-    uint32_t col[2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        uint32_t v[32], c = 0;
-#pragma unroll
-        for (int x = 0; x < 32; ++x) v[x] = p[(int64_t)min(half * 32 + x, n1 - 1) * sn];
-#pragma unroll
-        for (int x = 0; x < 32; ++x) {
-            const int n = half * 32 + x;
-            const bool see = v[x] == 0 && key < M && n < n1;
-            const uint64_t bits = __ballot(see);
-            c |= see ? 1u << x : 0u;
-            mine = n == lane ? bits : mine;
-            all &= n < n1 ? bits : ~0ull;
-            some |= bits;
-        }
-        col[half] = c;
+    for (int x = 0; x < 16; ++x) {
+        const bool see = v[x] == 0 && key < M && x < n1;
+        const uint64_t bits = __ballot(see);
+        c |= see ? 1u << x : 0u;
+        mine = x == lane ? bits : mine;
+        all &= x < n1 ? bits : ~0ull;
+        some |= bits;
     }
-    if (lane < n1) rowbits[(b * N + nt * 64 + lane) * M64 + kt] = mine;
-    if (key < M) colbits[(b * M + key) * N64 + nt] = (uint64_t)col[1] << 32 | col[0];
-    if (lane == 0) {
+    __shared__ __attribute__((aligned(8))) uint16_t col[64][4];
+    __shared__ uint64_t s_all[4], s_some[4];
+    col[lane][wave] = (uint16_t)c;
+    if (lane == 0) { s_all[wave] = all; s_some[wave] = some; }
+    if (lane < n1) rowbits[(b * N + n0 + lane) * M64 + kt] = mine;
+    __syncthreads();
+    if (wave == 0 && key < M) colbits[(b * M + key) * N64 + nt] = *reinterpret_cast<const uint64_t *>(col[lane]);
+    if (threadIdx.x == 64) {
+        some = s_some[0] | s_some[1] | s_some[2] | s_some[3];
+        all = s_all[0] & s_all[1] & s_all[2] & s_all[3];
         some_[(b * N64 + nt) * M64 + kt] = some;
         tiles[(b * N64 + nt) * M64 + kt] = some == 0 ? 2 : all == inside ? 0 : 1;
     }
@@ -1162,23 +1206,25 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         vis = vis_n;
         buf ^= 1;
     }
-    if (!w.live) return;
-    T *dst = reinterpret_cast<T *>(a.dq) + (((int64_t)b * a.N + w.i) * a.H + w.head) * 2 * a.d;
+    __syncthreads();                                          // every wave is done with the tiles
+    const DaRowsOut<T, C::DV> rows{lds + wave * 32 * C::DV * C::ES};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int x = 0; x < C::MTK; ++x)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
-                int c = x * 32 + 8 * q4 + 4 * h2;
-                if (DK < 32) {                                // one tile holds both maps' channels: this map's half
-                    if (c / DK != t) continue;
-                    c -= t * DK;
-                }
-                if (c >= a.d) continue;
-                da_store4(dst + t * a.d + c, dq[t][x][4 * q4] * a.scale, dq[t][x][4 * q4 + 1] * a.scale, dq[t][x][4 * q4 + 2] * a.scale,
-                          dq[t][x][4 * q4 + 3] * a.scale);
+                const int c = x * 32 + 8 * q4 + 4 * h2;       // heads of up to 16 channels: one tile holds both maps' channels, this map's half counts
+                if (DK < 32 && c / DK != t) continue;
+                rows.put(l32, DK < 32 ? c : t * DK + c, dq[t][x][4 * q4] * a.scale, dq[t][x][4 * q4 + 1] * a.scale, dq[t][x][4 * q4 + 2] * a.scale,
+                         dq[t][x][4 * q4 + 3] * a.scale);
             }
+    const int w0 = blk0 + wave * 32;
+    rows.flush(lane, [&](int r, int c) -> T * {
+        const int row = w0 + r, i = da_div_g(a, min(row, R - 1)), t = c / DK;
+        c -= t * DK;
+        return row < R && c < a.d ? reinterpret_cast<T *>(a.dq) + (((int64_t)b * a.N + i) * a.H + hk * a.G + row - i * a.G) * 2 * a.d + t * a.d + c : nullptr;
+    });
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -1394,39 +1440,43 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
         vis = vis_n;
         buf ^= 1;
     }
-    if (key >= a.M) return;
-    const int64_t krow = ((int64_t)b * a.M + key) * a.Hk + hk;
-    const int w = 2 * a.d + a.dv;
-    float *part = a.kvpart ? a.kvpart + ((int64_t)run * a.B * a.M * a.Hk + krow) * w : nullptr;
-    T *dkp = reinterpret_cast<T *>(a.dk) + krow * 2 * a.d, *dvp = reinterpret_cast<T *>(a.dvv) + krow * a.dv;
+    __syncthreads();                                          // every wave is done with the tiles
     const bool keep = klive && seen;
+    const float f = keep ? a.scale : 0.f;
+    const int64_t k0 = (int64_t)b * a.M;
+    const int w = 2 * a.d + a.dv;
+    auto out = [&](auto rows, auto dkv) {                     // dV, then dK, as whole rows; dkv(key): where the key's dK row starts, dV behind it or in its own tensor
 #pragma unroll
-    for (int x = 0; x < C::MT; ++x)
+        for (int x = 0; x < C::MT; ++x)
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-            const int c = x * 32 + 8 * q4 + 4 * h2;
-            if (c >= a.dv) continue;
-            const float v0 = keep ? dv[x][4 * q4] : 0.f, v1 = keep ? dv[x][4 * q4 + 1] : 0.f, v2 = keep ? dv[x][4 * q4 + 2] : 0.f, v3 = keep ? dv[x][4 * q4 + 3] : 0.f;
-            if (part) da_store4(part + 2 * a.d + c, v0, v1, v2, v3);
-            else da_store4(dvp + c, v0, v1, v2, v3);
-        }
+            for (int q4 = 0; q4 < 4; ++q4)
+                rows.put(l32, x * 32 + 8 * q4 + 4 * h2, keep ? dv[x][4 * q4] : 0.f, keep ? dv[x][4 * q4 + 1] : 0.f, keep ? dv[x][4 * q4 + 2] : 0.f, keep ? dv[x][4 * q4 + 3] : 0.f);
+        rows.flush(lane, [&](int r, int c) { return kw0 + r < a.M && c < a.dv ? dkv(kw0 + r, 1) + c : nullptr; });
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int x = 0; x < C::MTK; ++x)
+            for (int x = 0; x < C::MTK; ++x)
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                int c = x * 32 + 8 * q4 + 4 * h2;
-                if (DK < 32) {
-                    if (c / DK != t) continue;
-                    c -= t * DK;
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const int c = x * 32 + 8 * q4 + 4 * h2;
+                    if (DK < 32 && c / DK != t) continue;
+                    rows.put(l32, DK < 32 ? c : t * DK + c, keep ? dk[t][x][4 * q4] * f : 0.f, keep ? dk[t][x][4 * q4 + 1] * f : 0.f, keep ? dk[t][x][4 * q4 + 2] * f : 0.f,
+                             keep ? dk[t][x][4 * q4 + 3] * f : 0.f);
                 }
-                if (c >= a.d) continue;
-                const float v0 = keep ? dk[t][x][4 * q4] * a.scale : 0.f, v1 = keep ? dk[t][x][4 * q4 + 1] * a.scale : 0.f, v2 = keep ? dk[t][x][4 * q4 + 2] * a.scale : 0.f,
-                            v3 = keep ? dk[t][x][4 * q4 + 3] * a.scale : 0.f;
-                if (part) da_store4(part + t * a.d + c, v0, v1, v2, v3);
-                else da_store4(dkp + t * a.d + c, v0, v1, v2, v3);
-            }
+        rows.flush(lane, [&](int r, int c) {
+            const int t = c / DK;
+            c -= t * DK;
+            return kw0 + r < a.M && c < a.d ? dkv(kw0 + r, 0) + t * a.d + c : nullptr;
+        });
+    };
+    if (a.kvpart) {
+        float *part = a.kvpart + (int64_t)run * a.B * a.M * a.Hk * w;
+        out(DaRowsOut<float, C::DV>{lds + wave * 32 * C::DV * 4}, [&](int key, int v) { return part + ((k0 + key) * a.Hk + hk) * w + v * 2 * a.d; });
+    } else {
+        out(DaRowsOut<T, C::DV>{lds + wave * 32 * C::DV * C::ES}, [&](int key, int v) {
+            return v ? reinterpret_cast<T *>(a.dvv) + ((k0 + key) * a.Hk + hk) * a.dv : reinterpret_cast<T *>(a.dk) + ((k0 + key) * a.Hk + hk) * 2 * a.d;
+        });
+    }
 }
 
 // dK and dV from the runs' sums, in order: a thread per 4 channels
@@ -1497,7 +1547,7 @@ int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_
     const int64_t M64 = (M + 63) / 64, N64 = (N + 63) / 64;
     if (batches * M64 * N64 > 0x7fffffff) return DFINE_E_BADARG;
     uint64_t *col = forms + batches * N * M64, *some = col + batches * M * N64;
-    hipLaunchKernelGGL(diff_attn_mask_kernel, dim3((unsigned)(batches * M64 * N64)), dim3(64), 0, (hipStream_t)stream, mask, stride_b, stride_n, (int)N, (int)M, forms, col,
+    hipLaunchKernelGGL(diff_attn_mask_kernel, dim3((unsigned)(batches * M64 * N64)), dim3(256), 0, (hipStream_t)stream, mask, stride_b, stride_n, (int)N, (int)M, forms, col,
                        some, reinterpret_cast<uint8_t *>(some + batches * N64 * M64));
     return check_launch();
 }

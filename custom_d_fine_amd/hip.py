@@ -1527,23 +1527,29 @@ _QKN_SHAPE, _DA_SHAPE = c_int64 * 25, c_int64 * 28
 
 def _rows16(t):
     """`t` as the kernels read it - unit stride in the last dimension, every row on a 16-byte border - and its other strides; a copy where it is not."""
-    unit = 16 // t.element_size()
     shape, st = t.shape, t.stride()
-    ok = (st[-1] == 1 or shape[-1] == 1) and t.data_ptr() % 16 == 0
-    out = []
-    for n, s in zip(shape[:-1], st[:-1]):
-        out.append(s if n > 1 else 0)                       # (a dimension of one row carries any stride)
-        ok = ok and (n <= 1 or s % unit == 0)
-    if ok:
-        return t, out
-    t = t.clone(memory_format=torch.contiguous_format)
-    return t, [s if n > 1 else 0 for n, s in zip(shape[:-1], t.stride()[:-1])]
+    unit = 4 if t.dtype is torch.float32 else 8
+    if t.data_ptr() % 16 or (st[-1] != 1 and shape[-1] > 1):
+        ok = False
+    else:
+        ok = True
+        for s in st[:-1]:
+            if s % unit:
+                ok = False
+    if not ok:
+        if t.data_ptr() % 16 == 0 and (st[-1] == 1 or shape[-1] == 1) and not any(s % unit for n, s in zip(shape[:-1], st[:-1]) if n > 1):
+            return t, [s if n > 1 else 0 for n, s in zip(shape[:-1], st[:-1])]       # (a dimension of one row carries any stride)
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = t.stride()
+    return t, st[:-1]
 
 
 def _on_device(fn):
     """The launcher on its first tensor's device: the stream and the new tensors are that device's."""
+    here = _raw_device or torch.cuda.current_device
+
     def launch(t, *args):
-        if t.device.index == torch.cuda.current_device():
+        if t.get_device() == here():
             return fn(t, *args)
         with torch.cuda.device(t.device):
             return fn(t, *args)

@@ -2508,6 +2508,11 @@ def _float_operand(op, name, t, device, dtypes=_ACT_DTYPES):
         _refuse(f"{op}: {name} is on {t.device}, the queries on {device}")
 
 
+def _no_double_backward(op):
+    if torch.is_grad_enabled():                # create_graph=True: the kernels' results would come back without a graph
+        raise RuntimeError(f"custom_d_fine_amd.kernels.{op}: no second derivative (create_graph=True)")
+
+
 class _QKNormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, paired):
@@ -2517,8 +2522,8 @@ class _QKNormRotate(torch.autograd.Function):
         return yq, yk
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
+        _no_double_backward("qk_norm_rotate")
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         need = ctx.needs_input_grad
         dq, dk, dwq, dwk = _hip().qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions, *ctx.meta, dyq, dyk, need[2] and wq is not None,
@@ -2605,8 +2610,8 @@ class _DiffAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _no_double_backward("diff_attention")
         q, k, v, lam, weight, forms, kv_len, at, out, u, o2, stats = ctx.saved_tensors
         mask_batches, causal, start, scale, init, eps = ctx.meta
         n = ctx.needs_input_grad

@@ -357,3 +357,14 @@ def test_offsets_past_32_bits(cuda):
         one, two = _run(q, far, v, lam, w, dy)[0], _run(q, k, v, lam, w, dy)[0]
         for a, b in zip(one, two):
             assert torch.equal(a, b)
+
+
+def test_no_second_derivative(cuda):
+    from custom_d_fine_amd import kernels
+    q, k, v, lam, w, dy, _ = _inputs(cuda, 1, 8, 8, 6, 6, 16, 32, torch.float32)
+    q.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(kernels.diff_attention(q, k, v, lam, INIT, w), q, dy, create_graph=True)
+    x = torch.randn(1, 4, 2, 16, device=cuda, requires_grad=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(kernels.qk_norm_rotate(x, None)[0].sum(), x, create_graph=True)
