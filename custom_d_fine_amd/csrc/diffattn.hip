@@ -91,7 +91,7 @@ typedef __attribute__((address_space(3))) const da_u4v *da_lds_u4;
 typedef __attribute__((address_space(3))) const uint32_t *da_lds_u1;
 
 // A lane's way through a tile of rows of U units (byte addresses in LDS; tiles start on 512-byte borders): everything that depends on the lane is one register
-// per kind of read, the fragment only flips bits of it
+// per kind of read, the fragment only flips bits of it (below 512: the tiles' own borders)
 template <typename T, int DK> struct DaLane {
     using C = DaCfg<T, DK>;
     uint32_t row, tr[sizeof(T) == 2 ? 1 : 4];
@@ -107,11 +107,11 @@ template <typename T, int DK> struct DaLane {
         }
     }
     // row-major operand: row lane % 32 of the 32 rows at `tile`, fragment f
-    __device__ __forceinline__ uint4 frag(uint32_t tile, int f) const { return __builtin_bit_cast(uint4, *(da_lds_u4)(uintptr_t)(tile + (row ^ (f << 5)))); }
+    __device__ __forceinline__ uint4 frag(uint32_t tile, int f) const { return __builtin_bit_cast(uint4, *(da_lds_u4)(uintptr_t)((tile + row) ^ (f << 5))); }
     // transposed operand: contraction over rows KPF f .. of the 32 rows at `tile` in the order 8 a + 4 h + b, column 32 x + lane % 32
     __device__ __forceinline__ uint4 frag_tr(uint32_t tile, int f, int x) const {
         if constexpr (sizeof(T) == 2) {
-            const uint32_t p = tile + (tr[0] ^ (x << 6)) + f * 16 * C::ROWB, q = tile + (tr[0] ^ (x << 6) ^ 32) + (f * 16 + 8) * C::ROWB;
+            const uint32_t p = ((tile + tr[0]) ^ (x << 6)) + f * 16 * C::ROWB, q = ((tile + tr[0]) ^ (x << 6) ^ 32) + (f * 16 + 8) * C::ROWB;
             const da_tr4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_tr4 __attribute__((address_space(3))) *)(uintptr_t)p);
             const da_tr4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_tr4 __attribute__((address_space(3))) *)(uintptr_t)q);
             return __builtin_bit_cast(uint4, (da_tr8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -119,7 +119,7 @@ template <typename T, int DK> struct DaLane {
             uint32_t r[4];
 #pragma unroll
             for (int b = 0; b < 4; ++b)
-                r[b] = *(da_lds_u1)(uintptr_t)(tile + (tr[b] ^ (x << 7) ^ (C::U >= 16 && (f & 1) ? 16 : 0) ^ (C::U == 8 && (f & 1) ? 64 : 0)) + f * 8 * C::ROWB);
+                r[b] = *(da_lds_u1)(uintptr_t)(((tile + tr[b]) ^ (x << 7) ^ (C::U >= 16 && (f & 1) ? 16 : 0) ^ (C::U == 8 && (f & 1) ? 64 : 0)) + f * 8 * C::ROWB);
             return make_uint4(r[0], r[1], r[2], r[3]);
         }
     }
@@ -140,6 +140,21 @@ template <int N, int D, class RD, class USE> __device__ __forceinline__ void da_
     }
 }
 
+// N products with the vector work of 16 elements between them: after product i the elements [16 i / N, 16 (i + 1) / N).  The matrix unit runs a product in 32 cycles of
+// which the wave issues for 4; vector work of the SAME wave that the products do not wait for fills the rest, and here it stands in that order.  fr: the first two
+// fragments, asked for in front.
+template <int N, class RD, class USE, class VEC> __device__ __forceinline__ void da_between(uint4 *fr, RD rd, USE use, VEC vec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        use(i, fr[i & 1]);
+        if (i + 2 < N) fr[i & 1] = rd(i + 2);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 16 * i / N; r < 16 * (i + 1) / N; ++r) vec(r);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 // -1 where bit `pos` of v is set, else 0 (assembly: written as an expression it becomes an and, a compare and a select for each use)
 template <int POS> __device__ __forceinline__ uint32_t da_bit(uint32_t v) {
     uint32_t r;
@@ -147,11 +162,10 @@ template <int POS> __device__ __forceinline__ uint32_t da_bit(uint32_t v) {
     return r;
 }
 // scores of keys (rows) that the lane's row (key) does not see: -inf
-template <int R = 0> __device__ __forceinline__ void da_hide(da_f16v *s, uint32_t mine) {
+template <int R = 0> __device__ __forceinline__ void da_hide(da_f16v &s, uint32_t mine) {
     if constexpr (R < 16) {
         const uint32_t on = da_bit<8 * (R >> 2) + (R & 3)>(mine);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) s[t][R] = __uint_as_float((__float_as_uint(s[t][R]) & on) | (0xff800000u & ~on));
+        s[R] = __uint_as_float((__float_as_uint(s[R]) & on) | (0xff800000u & ~on));
         da_hide<R + 1>(s, mine);
     }
 }
@@ -414,23 +428,19 @@ template <typename T, int DK>
 __device__ __forceinline__ void da_fwd_tile(DaState<T, DK> &st, const uint4 (*qf)[DaCfg<T, DK>::NF], const DaLane<T, DK> &ln, uint32_t tk, uint32_t tv, bool masked, uint32_t vis, float c,
                                             int lane) {
     using C = DaCfg<T, DK>;
+    const uint32_t mine = vis >> (4 * (lane >> 5));
     da_f16v s[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
-    da_ring<2 * C::NF, 4>([&](int i) { return ln.frag(tk, i); }, [&](int i, const uint4 &f) { s[i / C::NF] = Da<T>::mma(f, qf[i / C::NF][i % C::NF], s[i / C::NF]); });
-    if (masked) da_hide(s, vis >> (4 * (lane >> 5)));
-    float bm[2];
+    float mu[2], sum[2] = {0.f, 0.f};
+    auto scores = [&](int t) {                                // hides what is hidden, moves the maximum of map t where it has to
+        if (masked) da_hide(s[t], mine);
+        float bm = s[t][0];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        bm[t] = s[t][0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) bm[t] = fmaxf(bm[t], s[t][r]);
-        bm[t] = da_other_half_max(bm[t]) * c;
-    }
-    if (__any(bm[0] > st.m[0] + 8.f || bm[1] > st.m[1] + 8.f)) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const float mn = fmaxf(st.m[t], bm[t]), alpha = mn == -INFINITY ? 1.f : da_exp2(st.m[t] - mn);
+        for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[t][r]);
+        bm = da_other_half_max(bm) * c;
+        if (__any(bm > st.m[t] + 8.f)) {
+            const float mn = fmaxf(st.m[t], bm), alpha = mn == -INFINITY ? 1.f : da_exp2(st.m[t] - mn);
             st.m[t] = mn;
             st.l[t] *= alpha;
 #pragma unroll
@@ -438,26 +448,31 @@ __device__ __forceinline__ void da_fwd_tile(DaState<T, DK> &st, const uint4 (*qf
 #pragma unroll
                 for (int r = 0; r < 16; ++r) st.o[t][x][r] *= alpha;
         }
-    }
-    uint4 pf[2][C::FPT];
+        mu[t] = st.m[t] == -INFINITY ? 0.f : st.m[t];
+    };
+    auto vec = [&](int t, int r) {
+        s[t][r] = da_exp2(fmaf(s[t][r], c, -mu[t]));
+        sum[t] += s[t][r];
+    };
+    auto value = [&](int i) { return ln.frag_tr(tv, i / C::MT, i % C::MT); };
+    uint4 fr[2], pf[C::FPT];
+    da_ring<C::NF, 2>([&](int i) { return ln.frag(tk, i); }, [&](int i, const uint4 &f) { s[0] = Da<T>::mma(f, qf[0][i], s[0]); });
+    fr[0] = ln.frag(tk, C::NF);
+    if (C::NF > 1) fr[1] = ln.frag(tk, C::NF + 1);
+    scores(0);
+    // the first map's exponentials between the second's products, the second's between the first map's products with the values
+    da_between<C::NF>(fr, [&](int i) { return ln.frag(tk, C::NF + i); }, [&](int i, const uint4 &f) { s[1] = Da<T>::mma(f, qf[1][i], s[1]); }, [&](int r) { vec(0, r); });
+    fr[0] = value(0);
+    fr[1] = value(1);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const float mu = st.m[t] == -INFINITY ? 0.f : st.m[t];
-        float sum = 0.f;
+    for (int f = 0; f < C::FPT; ++f) pf[f] = da_pack<T>(s[0], f);
+    scores(1);
+    da_between<C::FPT * C::MT>(fr, value, [&](int i, const uint4 &f) { st.o[0][i % C::MT] = Da<T>::mma(f, pf[i / C::MT], st.o[0][i % C::MT]); }, [&](int r) { vec(1, r); });
+    st.l[0] += sum[0];
+    st.l[1] += sum[1];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[t][r] = da_exp2(fmaf(s[t][r], c, -mu));
-            sum += s[t][r];
-        }
-        st.l[t] += sum;
-#pragma unroll
-        for (int f = 0; f < C::FPT; ++f) pf[t][f] = da_pack<T>(s[t], f);
-    }
-    da_ring<C::FPT * C::MT, 4>([&](int i) { return ln.frag_tr(tv, i / C::MT, i % C::MT); },
-                               [&](int i, const uint4 &f) {
-                                   st.o[0][i % C::MT] = Da<T>::mma(f, pf[0][i / C::MT], st.o[0][i % C::MT]);
-                                   st.o[1][i % C::MT] = Da<T>::mma(f, pf[1][i / C::MT], st.o[1][i % C::MT]);
-                               });
+    for (int f = 0; f < C::FPT; ++f) pf[f] = da_pack<T>(s[1], f);
+    da_ring<C::FPT * C::MT, 2>(value, [&](int i, const uint4 &f) { st.o[1][i % C::MT] = Da<T>::mma(f, pf[i / C::MT], st.o[1][i % C::MT]); });
 }
 
 // A wave's 32 rows x W channels from accumulator order to memory in whole rows: four channels at a time into LDS (unit u of row r at u ^ r % units), then 16
@@ -494,7 +509,7 @@ template <typename T, int DK>
 __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) void diff_attn_fwd_kernel(const DiffArgs a) {
     using C = DaCfg<T, DK>;
     constexpr int KB = sizeof(T) == 2 ? 64 : 32, TILE = KB * C::ROWB;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];      // (512: DaLane)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, nblk = gridDim.x / nbh, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int blk = a.causal ? nblk - 1 - (int)(blockIdx.x / nbh) : (int)(blockIdx.x / nbh);          // causal: the longest first
@@ -540,7 +555,11 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         if (code == 1) vis = bits(k0);
         issue(k0, 0);
     }
-    const float lam = da_lambda_rows(a, hk, blk0 + wave * 32, w.head);
+    __shared__ float sLam[128];                               // (not held in registers over the loop)
+    {
+        const float l = da_lambda_rows(a, hk, blk0 + wave * 32, w.head);
+        if (h2 == 0) sLam[wave * 32 + l32] = l;
+    }
     while (k0 < wg_end) {
         const int kn = next(k0 + KB), code_n = kn < wg_end ? walk.code(a, kn) : 0;
         uint64_t vis_n = ~0ull;
@@ -563,7 +582,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         vis = vis_n;
         buf ^= 1;
     }
-    const float l0 = da_both_halves(st.l[0]), l1 = da_both_halves(st.l[1]), inv0 = da_inv(l0), inv1 = da_inv(l1);
+    const float lam = sLam[wave * 32 + l32], l0 = da_both_halves(st.l[0]), l1 = da_both_halves(st.l[1]), inv0 = da_inv(l0), inv1 = da_inv(l1);
     float ss = 0.f, us = 0.f;
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
@@ -578,8 +597,11 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     us = da_both_halves(us);
     const float beta = a.weight && ss > 0.f ? us / ss : 0.f;  // what is kept of A_1 V is its part at right angles to U (diff_attn_prep_kernel)
     const float rn = a.weight ? rsqrtf(ss / (float)a.dv + a.eps) : 1.f;
-    if (a.stats && h2 == 0 && w.live) {
-        const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + w.head) * a.N + w.i;
+    int row = blk0 + wave * 32 + l32;
+    asm volatile("" : "+v"(row));                             // (worked out again: the row's numbers are not held over the loop either)
+    if (a.stats && h2 == 0 && row < R) {
+        const int i = da_div_g(a, row);
+        const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + hk * a.G + row - i * a.G) * a.N + i;
         a.stats[at] = da_lse(st.m[0], l0);
         a.stats[bhn + at] = da_lse(st.m[1], l1);
         a.stats[2 * bhn + at] = rn;
@@ -676,7 +698,7 @@ __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff
     constexpr int NBUF = C::ROWB > 256 ? 1 : 2;               // (fp32 heads of 64: two buffers for four waves would not fit LDS)
     constexpr int WBYTES = NBUF * 2 * TILE;                   // a wave's buffers, later its sums
     static_assert(WBYTES >= 32 * 2 * C::DV * 4, "");
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];      // (512: DaLane)
     __shared__ float sM[2][4][32], sS[2][4][32], sLam[32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, rest = blockIdx.x / nbh, sp = rest % nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
@@ -1074,37 +1096,37 @@ __device__ __forceinline__ void da_dq_tile(const DiffArgs &a, da_f16v (*dq)[DaCf
     da_f16v dp, s[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] = s[0][r] = s[1][r] = 0.f;
-    da_ring<C::NFV + 2 * C::NF, 4>([&](int i) { return i < C::NFV ? ln.frag(tv, i) : ln.frag(tk, i - C::NFV); },
-                                   [&](int i, const uint4 &f) {
-                                       if (i < C::NFV) { dp = Da<T>::mma(f, uf[i], dp); return; }
-                                       const int t = (i - C::NFV) / C::NF;
-                                       s[t] = Da<T>::mma(f, qf[t][(i - C::NFV) % C::NF], s[t]);
-                                   });
-    if (masked) da_hide(s, vis >> (4 * (lane >> 5)));
-    uint4 sf[2][C::FPT];
+    const uint32_t mine = vis >> (4 * (lane >> 5));
+    da_ring<C::NFV + C::NF, 2>([&](int i) { return i < C::NFV ? ln.frag(tv, i) : ln.frag(tk, i - C::NFV); },
+                               [&](int i, const uint4 &f) {
+                                   if (i < C::NFV) dp = Da<T>::mma(f, uf[i], dp);
+                                   else s[0] = Da<T>::mma(f, qf[0][i - C::NFV], s[0]);
+                               });
+    uint4 fr[2], sf[C::FPT];
+    fr[0] = ln.frag(tk, C::NF);
+    if (C::NF > 1) fr[1] = ln.frag(tk, C::NF + 1);
+    if (masked) da_hide(s[0], mine);
+    // the first map's vector work between the second's scores, the second's between the first map's products with the keys
+    da_between<C::NF>(fr, [&](int i) { return ln.frag(tk, C::NF + i); }, [&](int i, const uint4 &f) { s[1] = Da<T>::mma(f, qf[1][i], s[1]); },
+                      [&](int r) { s[0][r] = da_exp2(fmaf(s[0][r], c, -lse[0])) * (dp[r] - dl[0]); });
+    auto key = [&](int t, int i) { return ln.frag_tr(tk, i / C::MTK, DK < 32 ? 0 : t * (DK / 32) + i % C::MTK); };
+    fr[0] = key(0, 0);
+    fr[1] = key(0, 1);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const float fac = t ? -sign : 1.f, dd = t ? dl[1] : -dl[0];
+    for (int f = 0; f < C::FPT; ++f) sf[f] = da_pack<T>(s[0], f);
+    if (masked) da_hide(s[1], mine);
+    da_between<C::FPT * C::MTK>(fr, [&](int i) { return key(0, i); }, [&](int i, const uint4 &f) { dq[0][i % C::MTK] = Da<T>::mma(f, sf[i / C::MTK], dq[0][i % C::MTK]); },
+                                [&](int r) { s[1][r] = da_exp2(fmaf(s[1][r], c, -lse[1])) * fmaf(dp[r], -sign, dl[1]); });
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = da_exp2(fmaf(s[t][r], c, -lse[t])) * (t ? fmaf(dp[r], fac, dd) : dp[r] + dd);
-#pragma unroll
-        for (int f = 0; f < C::FPT; ++f) sf[t][f] = da_pack<T>(s[t], f);
-    }
-    da_ring<2 * C::FPT * C::MTK, 4>([&](int i) {
-                                        const int t = i / (C::FPT * C::MTK), f = i / C::MTK % C::FPT, x = i % C::MTK;
-                                        return ln.frag_tr(tk, f, DK < 32 ? 0 : t * (DK / 32) + x);
-                                    },
-                                    [&](int i, const uint4 &fr) {
-                                        const int t = i / (C::FPT * C::MTK), f = i / C::MTK % C::FPT, x = i % C::MTK;
-                                        dq[t][x] = Da<T>::mma(fr, sf[t][f], dq[t][x]);
-                                    });
+    for (int f = 0; f < C::FPT; ++f) sf[f] = da_pack<T>(s[1], f);
+    da_ring<C::FPT * C::MTK, 2>([&](int i) { return key(1, i); }, [&](int i, const uint4 &f) { dq[1][i % C::MTK] = Da<T>::mma(f, sf[i / C::MTK], dq[1][i % C::MTK]); });
 }
 
 template <typename T, int DK>
 __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) void diff_attn_dq_kernel(const DiffArgs a) {
     using C = DaCfg<T, DK>;
     constexpr int KB = sizeof(T) == 2 ? 64 : 32, TILE = KB * C::ROWB;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];      // (512: DaLane)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, nblk = gridDim.x / nbh, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int blk = a.causal ? nblk - 1 - (int)(blockIdx.x / nbh) : (int)(blockIdx.x / nbh);          // causal: the longest first
@@ -1239,46 +1261,53 @@ __device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[Da
     da_f16v dp, s[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] = s[0][r] = s[1][r] = 0.f;
-    da_ring<C::NFV + 2 * C::NF, 4>([&](int i) { return i < C::NFV ? ln.frag(tu, i) : ln.frag(tq, i - C::NFV); },
-                                   [&](int i, const uint4 &f) {
-                                       if (i < C::NFV) { dp = Da<T>::mma(f, vf[i], dp); return; }
-                                       const int t = (i - C::NFV) / C::NF;
-                                       s[t] = Da<T>::mma(f, kf[t][(i - C::NFV) % C::NF], s[t]);
-                                   });
-    if (masked) da_hide(s, vis >> (4 * h2));
-    uint4 sf[2][C::FPT], pf[C::FPT];
+    const uint32_t mine = vis >> (4 * h2);
+    uint4 fr[2], sf[C::FPT], pf[C::FPT];
     da_f16v p;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const float fac = t ? -sign : 1.f;
-        float lv[16], dl[16];                                 // this lane's 16 rows' statistics: QB floats of each kind in LDS
+    float lv[16], dl[16];                                     // this lane's 16 rows' statistics (QB floats of each kind in LDS)
+    auto stats = [&](int t) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
             const da_u4v x = *(da_lds_u4)(uintptr_t)(stat + (t * 64 + 8 * q4 + 4 * h2) * 4), y = *(da_lds_u4)(uintptr_t)(stat + ((2 + t) * 64 + 8 * q4 + 4 * h2) * 4);
             lv[4 * q4] = __uint_as_float(x.x); lv[4 * q4 + 1] = __uint_as_float(x.y); lv[4 * q4 + 2] = __uint_as_float(x.z); lv[4 * q4 + 3] = __uint_as_float(x.w);
             dl[4 * q4] = __uint_as_float(y.x); dl[4 * q4 + 1] = __uint_as_float(y.y); dl[4 * q4 + 2] = __uint_as_float(y.z); dl[4 * q4 + 3] = __uint_as_float(y.w);
         }
+    };
+    stats(0);
+    da_ring<C::NFV + C::NF, 2>([&](int i) { return i < C::NFV ? ln.frag(tu, i) : ln.frag(tq, i - C::NFV); },
+                               [&](int i, const uint4 &f) {
+                                   if (i < C::NFV) dp = Da<T>::mma(f, vf[i], dp);
+                                   else s[0] = Da<T>::mma(f, kf[0][i - C::NFV], s[0]);
+                               });
+    fr[0] = ln.frag(tq, C::NF);
+    if (C::NF > 1) fr[1] = ln.frag(tq, C::NF + 1);
+    if (masked) da_hide(s[0], mine);
+    // the first map's vector work between the second's scores, the second's between the first map's products with the queries
+    da_between<C::NF>(fr, [&](int i) { return ln.frag(tq, C::NF + i); }, [&](int i, const uint4 &f) { s[1] = Da<T>::mma(f, kf[1][i], s[1]); },
+                      [&](int r) {
+                          p[r] = da_exp2(fmaf(s[0][r], c, -lv[r]));
+                          s[0][r] = p[r] * (dp[r] - dl[r]);
+                      });
+    auto query = [&](int t, int i) { return ln.frag_tr(tq, i / C::MTK, DK < 32 ? 0 : t * (DK / 32) + i % C::MTK); };
+    fr[0] = query(0, 0);
+    fr[1] = query(0, 1);
+    stats(1);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float e = da_exp2(fmaf(s[t][r], c, -lv[r]));
-            p[r] = t ? fmaf(e, fac, p[r]) : e;
-            s[t][r] = e * (t ? fmaf(dp[r], fac, dl[r]) : dp[r] - dl[r]);
-        }
+    for (int f = 0; f < C::FPT; ++f) sf[f] = da_pack<T>(s[0], f);
+    if (masked) da_hide(s[1], mine);
+    da_between<C::FPT * C::MTK>(fr, [&](int i) { return query(0, i); }, [&](int i, const uint4 &f) { dk[0][i % C::MTK] = Da<T>::mma(f, sf[i / C::MTK], dk[0][i % C::MTK]); },
+                                [&](int r) {
+                                    const float e = da_exp2(fmaf(s[1][r], c, -lv[r]));
+                                    p[r] = fmaf(e, -sign, p[r]);
+                                    s[1][r] = e * fmaf(dp[r], -sign, dl[r]);
+                                });
 #pragma unroll
-        for (int f = 0; f < C::FPT; ++f) sf[t][f] = da_pack<T>(s[t], f);
-    }
-#pragma unroll
-    for (int f = 0; f < C::FPT; ++f) pf[f] = da_pack<T>(p, f);
-    constexpr int NK = 2 * C::FPT * C::MTK;
-    da_ring<NK + C::FPT * C::MT, 4>([&](int i) {
-                                        if (i >= NK) return ln.frag_tr(tu, (i - NK) / C::MT, (i - NK) % C::MT);
-                                        const int t = i / (C::FPT * C::MTK), f = i / C::MTK % C::FPT, x = i % C::MTK;
-                                        return ln.frag_tr(tq, f, DK < 32 ? 0 : t * (DK / 32) + x);
-                                    },
-                                    [&](int i, const uint4 &fr) {
-                                        if (i >= NK) { dv[(i - NK) % C::MT] = Da<T>::mma(fr, pf[(i - NK) / C::MT], dv[(i - NK) % C::MT]); return; }
-                                        const int t = i / (C::FPT * C::MTK), f = i / C::MTK % C::FPT, x = i % C::MTK;
-                                        dk[t][x] = Da<T>::mma(fr, sf[t][f], dk[t][x]);
+    for (int f = 0; f < C::FPT; ++f) { sf[f] = da_pack<T>(s[1], f); pf[f] = da_pack<T>(p, f); }
+    constexpr int NK = C::FPT * C::MTK;
+    da_ring<NK + C::FPT * C::MT, 2>([&](int i) { return i < NK ? query(1, i) : ln.frag_tr(tu, (i - NK) / C::MT, (i - NK) % C::MT); },
+                                    [&](int i, const uint4 &f) {
+                                        if (i < NK) dk[1][i % C::MTK] = Da<T>::mma(f, sf[i / C::MTK], dk[1][i % C::MTK]);
+                                        else dv[(i - NK) % C::MT] = Da<T>::mma(f, pf[(i - NK) / C::MT], dv[(i - NK) % C::MT]);
                                     });
 }
 
@@ -1292,7 +1321,7 @@ template <typename T, int DK>
 __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2) ? 2 : 1) void diff_attn_dkdv_kernel(const DiffArgs a) {
     using C = DaCfg<T, DK>;
     constexpr int QB = 64, TILE = QB * C::ROWB, BUF = 2 * TILE + 4 * QB * 4;       // (BUF: a multiple of 512 bytes)
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];      // (512: DaLane)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, rest = blockIdx.x / nbh, run = rest % a.kvruns, blk = rest / a.kvruns, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int len = da_len(a, b);
