@@ -27,6 +27,7 @@ typedef short da_tr4 __attribute__((ext_vector_type(4)));
 typedef short da_tr8 __attribute__((ext_vector_type(8)));
 
 constexpr int kDaThreads = 256;
+constexpr int kDaSplitWgs = 256, kDaRunKeys = 512;
 
 struct DiffArgs {
     const void *q, *k, *v;                      // [B, N, H, 2, d], [B, M, Hk, 2, d], [B, M, Hk, dv]
@@ -522,12 +523,6 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     const int i_end = da_div_g(a, min(blk0 + 127, R - 1));
     const int wg_end = da_limit(a, len, start, i_end), qt0 = da_div_g(a, blk0) >> 6, qt1 = i_end >> 6;
 
-    uint4 qf[2][C::NF];
-    da_load_q<T, DK>(a, w, b, h2, qf);
-    DaState<T, DK> st;
-    st.init();
-#pragma unroll
-    for (int f = 0; f < 2 * C::NF; ++f) da_pin(qf[f / C::NF][f % C::NF]);
     DaCopy<T, DK, KB, kDaThreads> ck, cv;
     ck.init(reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.ks[3], a.d, true, tid);
     cv.init(reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, a.dv, false, tid);
@@ -555,6 +550,12 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         if (code == 1) vis = bits(k0);
         issue(k0, 0);
     }
+    uint4 qf[2][C::NF];
+    da_load_q<T, DK>(a, w, b, h2, qf);
+    DaState<T, DK> st;
+    st.init();
+#pragma unroll
+    for (int f = 0; f < 2 * C::NF; ++f) da_pin(qf[f / C::NF][f % C::NF]);
     __shared__ float sLam[128];                               // (not held in registers over the loop)
     {
         const float l = da_lambda_rows(a, hk, blk0 + wave * 32, w.head);
@@ -710,12 +711,6 @@ __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff
     const DaRows w = da_rows(a, hk, blk * 32, l32, len, start);
     const int tiles = (w.lim_hi + 31) >> 5, per = (tiles + nsplit - 1) / nsplit, t_end = min(tiles, (sp + 1) * per);
 
-    uint4 qf[2][C::NF];
-    da_load_q<T, DK>(a, w, b, h2, qf);
-    DaState<T, DK> st;
-    st.init();
-#pragma unroll
-    for (int f = 0; f < 2 * C::NF; ++f) da_pin(qf[f / C::NF][f % C::NF]);
     DaCopy<T, DK, 32, 64> ck, cv;
     constexpr int NCOPY = 2 * DaCopy<T, DK, 32, 64>::J;
     ck.init(reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.ks[3], a.d, true, lane);
@@ -753,6 +748,12 @@ __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff
         if (code == 1) vis = bits(t);
         if (NBUF == 2) issue(t, 0);
     }
+    uint4 qf[2][C::NF];
+    da_load_q<T, DK>(a, w, b, h2, qf);
+    DaState<T, DK> st;
+    st.init();
+#pragma unroll
+    for (int f = 0; f < 2 * C::NF; ++f) da_pin(qf[f / C::NF][f % C::NF]);
     if (wave == 0 && nsplit == 1) {
         const float lam = da_lambda_rows(a, hk, blk * 32, w.head);
         if (h2 == 0) sLam[l32] = lam;
@@ -1617,8 +1618,8 @@ static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <
 static int diff_attn_splits(const DiffArgs &a) {
     const int64_t R = (int64_t)a.N * a.G, bh = (int64_t)a.B * a.Hk;
     if ((R + 127) / 128 * bh >= 256) return 0;
-    const int64_t wgs = (R + 31) / 32 * bh, most = ((int64_t)a.M + 255) / 256;           // a run has 256 keys (two tiles per wave) at least
-    int64_t n = 1024 / wgs;
+    const int64_t wgs = (R + 31) / 32 * bh, most = ((int64_t)a.M + kDaRunKeys - 1) / kDaRunKeys;
+    int64_t n = kDaSplitWgs / wgs;
     if (n > most) n = most;
     if (n > 256) n = 256;
     return (int)(n < 1 ? 1 : n);

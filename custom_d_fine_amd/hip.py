@@ -6,7 +6,9 @@ current HIP stream, allocates outputs/workspaces with torch (device memory plumb
 raises RuntimeError on a non-zero status.
 """
 import ctypes
+import functools
 import os
+import struct
 from ctypes import c_float, c_int, c_int64, c_void_p
 
 import torch
@@ -1522,7 +1524,12 @@ def attn_backward(q, k, v, o, dout, lse2, num_heads, dq, dk, dv, mask=None):
 
 
 # ------------------------------------------------------------------------------------- attention block: norms + rotation, differential attention
-_QKN_SHAPE, _DA_SHAPE = c_int64 * 25, c_int64 * 28
+_QKN_SHAPE, _DA_SHAPE = struct.Struct("=25q").pack, struct.Struct("=28q").pack        # (host int64 arrays of the C entries)
+_EMPTY_LIKE = functools.partial(torch.empty_like, memory_format=torch.contiguous_format)
+
+
+def _is_bf16(t):
+    return t is not None and t.dtype is torch.bfloat16
 
 
 def _rows16(t):
@@ -1558,9 +1565,9 @@ def _on_device(fn):
 
 def _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks, dqs=(0, 0, 0), dks=(0, 0, 0)):
     B, L, Hq, D = q.shape
-    return _QKN_SHAPE(B, L, Hq, 0 if k is None else k.shape[2], D, 0 if cos is None else 2 * cos.shape[1], 0 if cos is None else cos.shape[0], _DTYPE[q.dtype],
-                      paired, positions is not None and positions.dtype == torch.int64, L if positions is not None and positions.dim() == 2 else 0,
-                      wq is not None and wq.dtype == torch.bfloat16, wk is not None and wk.dtype == torch.bfloat16, *qs, *ks, *dqs, *dks)
+    T, half = (0, 0) if cos is None else cos.shape
+    return _QKN_SHAPE(B, L, Hq, 0 if k is None else k.shape[2], D, 2 * half, T, _DTYPE[q.dtype], paired, positions is not None and positions.dtype is torch.int64,
+                      L if positions is not None and positions.dim() == 2 else 0, _is_bf16(wq), _is_bf16(wk), *qs, *ks, *dqs, *dks)
 
 
 @_on_device
@@ -1570,8 +1577,8 @@ def qk_norm_rotate_forward(q, k, wq, wk, cos, sin, positions, eps, paired):
     ks = (0, 0, 0)
     if k is not None:
         k, ks = _rows16(k)
-    yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    yk = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
+    yq = _EMPTY_LIKE(q)
+    yk = None if k is None else _EMPTY_LIKE(k)
     with _timed("qk_norm_rotate", 2.0 * q.element_size() * (q.numel() + (0 if k is None else k.numel()))):
         _check(_lib.dfine_qk_norm_rotate_fwd(_ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(yq), _ptr(yk),
                                              _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks), eps, _stream()), "dfine_qk_norm_rotate_fwd")
@@ -1586,8 +1593,8 @@ def qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions, eps, paired, dyq,
     if k is not None:
         k, ks = _rows16(k)
         dyk, dks = _rows16(dyk)
-    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    dk = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
+    dq = _EMPTY_LIKE(q)
+    dk = None if k is None else _EMPTY_LIKE(k)
     dwq = torch.empty_like(wq) if want_wq else None
     dwk = torch.empty_like(wk) if want_wk else None
     shape = _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks, dqs, dks)
@@ -1611,8 +1618,8 @@ def diff_attn_mask_forms(mask):
 
 def _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys=(0, 0, 0)):
     B, N, H, _, d = q.shape
-    return _DA_SHAPE(B, N, k.shape[1], H, k.shape[2], d, v.shape[3], _DTYPE[q.dtype], 1 if lam.dim() == 2 else H, lam.dtype == torch.bfloat16,
-                     weight is not None and weight.dtype == torch.bfloat16, causal, start if isinstance(start, int) else 0, mask_batches, *qs, *ks, *vs, *dys)
+    return _DA_SHAPE(B, N, k.shape[1], H, k.shape[2], d, v.shape[3], _DTYPE[q.dtype], 1 if lam.dim() == 2 else H, _is_bf16(lam), _is_bf16(weight), causal,
+                     start if isinstance(start, int) else 0, mask_batches, *qs, *ks, *vs, *dys)
 
 
 @_on_device
@@ -1626,8 +1633,8 @@ def diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal,
     out = torch.empty(B, N, H, dv, device=q.device, dtype=q.dtype)
     u = o2 = stats = None
     if keep:
-        u = torch.empty_like(out) if weight is not None else None
-        o2 = torch.empty_like(out)
+        u = _EMPTY_LIKE(out) if weight is not None else None
+        o2 = _EMPTY_LIKE(out)
         stats = torch.empty(4, B, H, N, device=q.device, dtype=torch.float32)
     shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs)
     nws = _lib.dfine_diff_attn_fwd_ws_bytes(shape)
@@ -1646,7 +1653,7 @@ def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal
     k, ks = _rows16(k)
     v, vs = _rows16(v)
     dy, dys = _rows16(dy)
-    new = lambda t, on: torch.empty(t.shape, device=t.device, dtype=t.dtype) if on else None  # noqa: E731
+    new = lambda t, on: _EMPTY_LIKE(t) if on else None  # noqa: E731
     dq, dk, dv, dlam = new(q, want[0]), new(k, want[1]), new(v, want[1]), new(lam, want[2])
     dweight = None if weight is None else new(weight, want[3])
     shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys)

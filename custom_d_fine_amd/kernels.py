@@ -2502,10 +2502,11 @@ def _refuse(what, kind=ValueError):
 
 
 def _float_operand(op, name, t, device, dtypes=_ACT_DTYPES):
+    """device: the queries' get_device() (an int: t.device makes an object)."""
     if not (isinstance(t, torch.Tensor) and t.dtype in dtypes):
         _refuse(f"{op}: {name} is a {' or '.join(str(d)[6:] for d in dtypes)} tensor, got {getattr(t, 'dtype', type(t).__name__)}", TypeError)
-    if t.device != device:
-        _refuse(f"{op}: {name} is on {t.device}, the queries on {device}")
+    if t.get_device() != device:
+        _refuse(f"{op}: {name} is on {t.device}, the queries are not")
 
 
 def _no_double_backward(op):
@@ -2540,7 +2541,7 @@ def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, posit
     pass.  positions: int32 / int64 [L] or [B, L]; a position outside the table gives NaN.  Gradients for q, k and the weights.
     -> (q', k'), contiguous, of q's type (k' None without k).  Under bf16 autocast q and k are cast to bfloat16 first."""
     op = "qk_norm_rotate"
-    device = q.device if isinstance(q, torch.Tensor) else None
+    device = q.get_device() if isinstance(q, torch.Tensor) else None
     _float_operand(op, "q", q, device)
     if k is not None:
         _float_operand(op, "k", k, device)
@@ -2560,11 +2561,17 @@ def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, posit
         _refuse(f"{op}: too many tokens or heads")
     if k is None and k_weight is not None:
         _refuse(f"{op}: k_weight without k")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            _float_operand(op, name, w, device)
-            if w.shape != (D,):
-                _refuse(f"{op}: {name} {tuple(w.shape)} for heads of {D} channels")
+    grad = q.requires_grad or (k is not None and k.requires_grad)
+    if q_weight is not None:
+        _float_operand(op, "q_weight", q_weight, device)
+        if q_weight.shape != (D,):
+            _refuse(f"{op}: q_weight {tuple(q_weight.shape)} for heads of {D} channels")
+        q_weight, grad = q_weight.contiguous(), grad or q_weight.requires_grad
+    if k_weight is not None:
+        _float_operand(op, "k_weight", k_weight, device)
+        if k_weight.shape != (D,):
+            _refuse(f"{op}: k_weight {tuple(k_weight.shape)} for heads of {D} channels")
+        k_weight, grad = k_weight.contiguous(), grad or k_weight.requires_grad
     if (cos is None) != (sin is None):
         _refuse(f"{op}: cos and sin come together")
     if cos is None:
@@ -2583,21 +2590,23 @@ def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, posit
         else:
             if not isinstance(positions, torch.Tensor) or positions.dtype not in _INDEX_DTYPES:
                 _refuse(f"{op}: positions are int32 or int64", TypeError)
-            if positions.device != device:
-                _refuse(f"{op}: positions are on {positions.device}, the queries on {device}")
+            if positions.get_device() != device:
+                _refuse(f"{op}: positions are on {positions.device}, the queries are not")
             if positions.shape != (B, L) and positions.shape != (L,):
                 _refuse(f"{op}: positions {tuple(positions.shape)} for {(B, L)} tokens")
             positions = positions.contiguous()
-        cos, sin = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+        if not cos.is_contiguous() or cos.data_ptr() % 16:
+            cos = cos.clone(memory_format=torch.contiguous_format)
+        if not sin.is_contiguous() or sin.data_ptr() % 16:
+            sin = sin.clone(memory_format=torch.contiguous_format)
     eps = float(eps)
     if not eps >= 0:
         _refuse(f"{op}: eps {eps}")
     if not q.is_cuda:
         return _backend_for_cpu(op)(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))
-    wq, wk = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, wq, wk)):
-        return _QKNormRotate.apply(q, k, wq, wk, cos, sin, positions, eps, bool(interleaved))
-    return _hip().qk_norm_rotate_forward(q, k, wq, wk, cos, sin, positions, eps, bool(interleaved))[:2]
+    if grad and torch.is_grad_enabled():
+        return _QKNormRotate.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))
+    return _hip().qk_norm_rotate_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))[:2]
 
 
 class _DiffAttention(torch.autograd.Function):
@@ -2635,7 +2644,7 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
     Gradients for q, k, v, lambda_vectors and norm_weight, added up in a fixed order.  -> [B, N, H, dv], contiguous, of q's type.  Under bf16 autocast
     q, k, v are cast to bfloat16 first.  scale: d ** -0.5 by default."""
     op = "diff_attention"
-    device = q.device if isinstance(q, torch.Tensor) else None
+    device = q.get_device() if isinstance(q, torch.Tensor) else None
     _float_operand(op, "q", q, device)
     _float_operand(op, "k", k, device)
     _float_operand(op, "v", v, device)
@@ -2668,8 +2677,8 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
     if attn_mask is not None:
         if not isinstance(attn_mask, torch.Tensor) or attn_mask.dtype != torch.bool:
             _refuse(f"{op}: attn_mask is a bool tensor, True = may not attend", TypeError)
-        if attn_mask.device != device:
-            _refuse(f"{op}: attn_mask is on {attn_mask.device}, the queries on {device}")
+        if attn_mask.get_device() != device:
+            _refuse(f"{op}: attn_mask is on {attn_mask.device}, the queries are not")
         if attn_mask.shape != (N, M) and attn_mask.shape != (B, N, M):
             _refuse(f"{op}: attn_mask {tuple(attn_mask.shape)} for {N} queries and {M} keys of {B} sequences")
     starts = isinstance(query_start, torch.Tensor)
@@ -2677,8 +2686,8 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
         if t is not None:
             if not isinstance(t, torch.Tensor) or t.dtype not in _INDEX_DTYPES:
                 _refuse(f"{op}: {name} is an int32 or int64 tensor", TypeError)
-            if t.device != device or t.shape != (B,):
-                _refuse(f"{op}: {name} {tuple(t.shape)} on {t.device} for {B} sequences on {device}")
+            if t.get_device() != device or t.shape != (B,):
+                _refuse(f"{op}: {name} {tuple(t.shape)} on {t.device} for {B} sequences on {q.device}")
     if not causal and (starts or query_start != 0):
         _refuse(f"{op}: query_start goes with causal")
     if not starts and not -(2 ** 31) < int(query_start) < 2 ** 31:
@@ -2697,7 +2706,7 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
     if attn_mask is not None:
         forms = _hip().diff_attn_mask_forms(attn_mask if attn_mask.dim() == 3 else attn_mask[None])
     batches = attn_mask is not None and attn_mask.dim() == 3 and B > 1
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, lam, weight)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad or (weight is not None and weight.requires_grad)):
         return _DiffAttention.apply(q, k, v, lam, weight, forms, batches, kv_len, bool(causal), start, scale, init, eps)
     return _hip().diff_attn_forward(q, k, v, lam, weight, forms, batches, kv_len, bool(causal), start, scale, init, eps, False)[0]
 

@@ -58,26 +58,26 @@ def test_no_cpu_kernels():
 def test_c_entries_refuse_without_a_gpu():
     """Bad arguments come back as a status before anything touches a device."""
     from custom_d_fine_amd import hip
-    shape = hip._DA_SHAPE(*([2, 5, 7, 4, 2, 16, 32, 1, 4, 1, 1, 0, 0, 0] + [8] * 14))
-    call = lambda s, scale=0.25, q=None: hip._lib.dfine_diff_attn_fwd(q, q, q, q, None, None, None, None, q, None, None, None, None, s, scale, 0.1, 1e-5, None)  # noqa: E731
+    pack = hip._DA_SHAPE
+    shape = [2, 5, 7, 4, 2, 16, 32, 1, 4, 1, 1, 0, 0, 0] + [8] * 14
+    call = lambda s, scale=0.25, q=None: hip._lib.dfine_diff_attn_fwd(q, q, q, q, None, None, None, None, q, None, None, None, None, s and pack(*s), scale, 0.1, 1e-5, None)  # noqa: E731
     assert call(shape) == -1                                                            # null pointers
     assert call(None) == -1
     for at, bad in ((3, 3), (5, 12), (5, 72), (6, 130), (7, 2), (8, 3), (14, 4)):
-        s = hip._DA_SHAPE(*shape)
+        s = list(shape)
         s[at] = bad
-        assert call(s, q=1 << 20) == -1 and hip._lib.dfine_diff_attn_bwd_ws_bytes(s) == -1
+        assert call(s, q=1 << 20) == -1 and hip._lib.dfine_diff_attn_bwd_ws_bytes(pack(*s)) == -1 and hip._lib.dfine_diff_attn_fwd_ws_bytes(pack(*s)) == -1
     assert call(shape, scale=0.0, q=1 << 20) == -1 and call(shape, q=(1 << 20) + 2) == -1
-    empty = hip._DA_SHAPE(*([0] + list(shape)[1:]))
-    assert call(empty) == 0
-    assert hip._lib.dfine_diff_attn_bwd_ws_bytes(shape) > 0 and hip._lib.dfine_diff_attn_mask_words(1, 65, 130) == 65 * 3 + 130 * 2 + 2 * 3 + 1
+    assert call([0] + shape[1:]) == 0
+    assert hip._lib.dfine_diff_attn_bwd_ws_bytes(pack(*shape)) > 0 and hip._lib.dfine_diff_attn_mask_words(1, 65, 130) == 65 * 3 + 130 * 2 + 2 * 3 + 1
     assert hip._lib.dfine_diff_attn_mask(None, 1, 5, 5, 0, 5, None, None) == -1
-    qkn = hip._QKN_SHAPE(*([2, 5, 4, 2, 16, 8, 9, 1, 0, 0, 0, 0, 0] + [0] * 12))
+    qkn = [2, 5, 4, 2, 16, 8, 9, 1, 0, 0, 0, 0, 0] + [0] * 12
     for at, bad in ((4, 12), (4, 264), (5, 12), (5, 24), (6, 4), (7, 3), (0, -1)):
-        s = hip._QKN_SHAPE(*qkn)
+        s = list(qkn)
         s[at] = bad
-        assert hip._lib.dfine_qk_norm_rotate_fwd(1 << 20, 1 << 20, None, None, 1 << 20, 1 << 20, None, 1 << 20, 1 << 20, s, 1e-6, None) == -1
-    assert hip._lib.dfine_qk_norm_rotate_fwd(None, None, None, None, 1 << 20, 1 << 20, None, None, None, qkn, 1e-6, None) == -1
-    none = hip._QKN_SHAPE(*([2, 5, 0, 0] + list(qkn)[4:]))
+        assert hip._lib.dfine_qk_norm_rotate_fwd(1 << 20, 1 << 20, None, None, 1 << 20, 1 << 20, None, 1 << 20, 1 << 20, hip._QKN_SHAPE(*s), 1e-6, None) == -1
+    assert hip._lib.dfine_qk_norm_rotate_fwd(None, None, None, None, 1 << 20, 1 << 20, None, None, None, hip._QKN_SHAPE(*qkn), 1e-6, None) == -1
+    none = hip._QKN_SHAPE(*([2, 5, 0, 0] + qkn[4:]))
     assert hip._lib.dfine_qk_norm_rotate_fwd(None, None, None, None, 1 << 20, 1 << 20, None, None, None, none, 1e-6, None) == 0
 
 
