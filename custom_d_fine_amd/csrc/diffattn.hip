@@ -292,32 +292,62 @@ template <typename T, int DK, int ROWS, int NT> struct DaCopy {
     using C = DaCfg<T, DK>;
     static constexpr int J = ROWS * C::U / NT, STEP = NT / C::U, P = STEP >= 16 ? 1 : 16 / STEP;     // the swizzle repeats every 16 rows
     static_assert(J >= 1 && STEP >= 1 && J % P == 0, "");
-    const T *base[P];                                   // row r0 of the tile at hand, this thread's channels
-    bool ok[P];
+    const T *at[P];                                     // row r0 (+ p STEP) of the block at hand, this thread's channels
+    int64_t hop;                                        // P STEP rows, in elements
+    uint32_t ok;                                        // bit p: the channels are there
     int r0;
     __device__ __forceinline__ void init(const T *src, int64_t ld, int64_t map, int nch, bool maps, int t) {
         r0 = t / C::U;
+        ok = 0;
+        hop = ld * (P * STEP);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const int u = (t % C::U) ^ da_swz<T, C::U>(r0 + p * STEP), half = maps ? u / (C::U / 2) : 0;
             const int c = (maps ? u % (C::U / 2) : u) * (16 / C::ES);
-            ok[p] = c < nch;
-            base[p] = src + (int64_t)(r0 + p * STEP) * ld + half * map + c;
+            ok |= c < nch ? 1u << p : 0u;
+            at[p] = src + (int64_t)(r0 + p * STEP) * ld + half * map + c;
         }
     }
-    // rows [row0, row0 + ROWS) of the source into the tile at lds (this wave's first byte); rows >= valid and rows whose live bit is 0 become zeros
-    __device__ __forceinline__ void run(uint32_t lds, int64_t row0, int64_t ld, int valid, uint64_t live, bool whole) const {
+    __device__ __forceinline__ void move(int64_t elements) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) at[p] += elements;
+    }
+    // the block into the tile at lds (this wave's first byte); rows >= valid, rows whose live bit is 0 and channels that are not there become zeros.
+    // rows: all ROWS rows are there and live; full: all channels are
+    __device__ __forceinline__ void run(uint32_t lds, int valid, uint64_t live, bool rows, bool full) const {
+        const T *p[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q) p[q] = at[q];
+        if (rows && full) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                da_copy16(p[j % P], __builtin_amdgcn_readfirstlane(lds + j * NT * 16));
+                p[j % P] += hop;
+            }
+            return;
+        }
+        const T *zero = reinterpret_cast<const T *>(da_zero_page);
+        uint32_t on = 0;                                // bit j: copy j is of a row and channels that are there
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const T *p = base[j % P] + (row0 + (j / P) * P * STEP) * ld;
-            if (!whole) {
-                const int r = r0 + j * STEP;
-                if (!(ok[j % P] && r < valid && ((live >> r) & 1))) p = reinterpret_cast<const T *>(da_zero_page);
-            }
-            da_copy16(p, __builtin_amdgcn_readfirstlane(lds + j * NT * 16));
+            const int r = r0 + j * STEP;
+            on |= ((ok >> (j % P)) & 1) && (rows || (r < valid && ((live >> r) & 1))) ? 1u << j : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            da_copy16((on >> j) & 1 ? p[j % P] : zero, __builtin_amdgcn_readfirstlane(lds + j * NT * 16));
+            p[j % P] += hop;
         }
     }
 };
+
+// The kernel's arguments read again: what a loop does not need is not held in scalar registers over it (held, it spills to vector registers and comes back lane by
+// lane, eight instructions for each copy).
+__device__ __forceinline__ const DiffArgs &da_again() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();    // (DiffArgs is the first argument of every kernel)
+    asm volatile("" : "+s"(p));
+    return *(const DiffArgs *)p;
+}
 
 __device__ __forceinline__ float da_other_half_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -357,7 +387,7 @@ struct DaWalk {
         const int kt = chunk * 64 + (threadIdx.x & 63);
         bool n = false, p = false, x = false, y = true;
         if (kt < M64) {
-            const uint8_t *tp = a.tiles + mb * N64 * M64 + kt;
+            const uint8_t *tp = da_again().tiles + mb * N64 * M64 + kt;
             for (int qt = qt0; qt <= qt1; ++qt) {
                 const int c = tp[(int64_t)qt * M64];
                 n = n || c != 2;
@@ -390,7 +420,8 @@ struct DaWalk {
     __device__ __forceinline__ uint64_t live(const DiffArgs &a, int64_t mb, int qt0, int qt1, int M64, int N64, int k0) const {
         if (!a.tiles || !((part >> ((k0 >> 6) & 63)) & 1)) return ~0ull;
         uint64_t m = 0;
-        for (int qt = qt0; qt <= qt1; ++qt) m |= a.some[(mb * N64 + qt) * M64 + (k0 >> 6)];
+        const uint64_t *some = da_again().some;
+        for (int qt = qt0; qt <= qt1; ++qt) m |= some[(mb * N64 + qt) * M64 + (k0 >> 6)];
         return m >> (k0 & 63);
     }
 };
@@ -533,15 +564,20 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     DaWalk walk;
     walk.base = -1;
     auto next = [&](int k0) { return walk.next(a, w, mb, qt0, qt1, M64, N64, k0, wg_end); };
+    const int64_t ldk = a.ks[1], ldv = a.vs[1];
+    int stand = 0;                                            // the block that the copies stand at
     auto issue = [&](int k0, int buf) {
         const int valid = len - k0;
         const uint64_t live = walk.live(a, mb, qt0, qt1, M64, N64, k0), all = KB == 64 ? ~0ull : 0xffffffffull;
-        const bool whole = full && valid >= KB && (live & all) == all;
-        ck.run(lds0 + buf * 2 * TILE, k0, a.ks[1], valid, live, whole);
-        cv.run(lds0 + buf * 2 * TILE + TILE, k0, a.vs[1], valid, live, whole);
+        const bool rows = valid >= KB && (live & all) == all;
+        ck.move((k0 - stand) * ldk);
+        cv.move((k0 - stand) * ldv);
+        stand = k0;
+        ck.run(lds0 + buf * 2 * TILE, valid, live, rows, full);
+        cv.run(lds0 + buf * 2 * TILE + TILE, valid, live, rows, full);
     };
     auto bits = [&](int k0) {                                 // a mixed tile's keys as this lane's row sees them
-        return w.live ? a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63) : 0ull;
+        return w.live ? da_again().rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63) : 0ull;
     };
     int k0 = next(0), buf = 0, code = 0;
     uint64_t vis = ~0ull;
@@ -583,6 +619,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         vis = vis_n;
         buf ^= 1;
     }
+    const DiffArgs &e = da_again();
     const float lam = sLam[wave * 32 + l32], l0 = da_both_halves(st.l[0]), l1 = da_both_halves(st.l[1]), inv0 = da_inv(l0), inv1 = da_inv(l1);
     float ss = 0.f, us = 0.f;
 #pragma unroll
@@ -596,25 +633,25 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         }
     ss = da_both_halves(ss);
     us = da_both_halves(us);
-    const float beta = a.weight && ss > 0.f ? us / ss : 0.f;  // what is kept of A_1 V is its part at right angles to U (diff_attn_prep_kernel)
-    const float rn = a.weight ? rsqrtf(ss / (float)a.dv + a.eps) : 1.f;
+    const float beta = e.weight && ss > 0.f ? us / ss : 0.f;  // what is kept of A_1 V is its part at right angles to U (diff_attn_prep_kernel)
+    const float rn = e.weight ? rsqrtf(ss / (float)e.dv + e.eps) : 1.f;
     int row = blk0 + wave * 32 + l32;
     asm volatile("" : "+v"(row));                             // (worked out again: the row's numbers are not held over the loop either)
-    if (a.stats && h2 == 0 && row < R) {
-        const int i = da_div_g(a, row);
-        const int64_t bhn = (int64_t)a.B * a.H * a.N, at = ((int64_t)b * a.H + hk * a.G + row - i * a.G) * a.N + i;
-        a.stats[at] = da_lse(st.m[0], l0);
-        a.stats[bhn + at] = da_lse(st.m[1], l1);
-        a.stats[2 * bhn + at] = rn;
-        a.stats[3 * bhn + at] = beta;
+    if (e.stats && h2 == 0 && row < R) {
+        const int i = da_div_g(e, row);
+        const int64_t bhn = (int64_t)e.B * e.H * e.N, at = ((int64_t)b * e.H + hk * e.G + row - i * e.G) * e.N + i;
+        e.stats[at] = da_lse(st.m[0], l0);
+        e.stats[bhn + at] = da_lse(st.m[1], l1);
+        e.stats[2 * bhn + at] = rn;
+        e.stats[3 * bhn + at] = beta;
     }
     __syncthreads();                                          // every wave is done with the tiles
     const DaRowsOut<T, C::DV> rows{lds + wave * 32 * C::DV * C::ES};
     const int w0 = blk0 + wave * 32;
     auto to = [&](void *base) {
         rows.flush(lane, [&](int r, int c) -> T * {
-            const int row = w0 + r, i = da_div_g(a, min(row, R - 1));
-            return row < R && c < a.dv ? reinterpret_cast<T *>(base) + (((int64_t)b * a.N + i) * a.H + hk * a.G + row - i * a.G) * a.dv + c : nullptr;
+            const int row = w0 + r, i = da_div_g(e, min(row, R - 1));
+            return row < R && c < e.dv ? reinterpret_cast<T *>(base) + (((int64_t)b * e.N + i) * e.H + hk * e.G + row - i * e.G) * e.dv + c : nullptr;
         });
     };
 #pragma unroll
@@ -623,20 +660,20 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         for (int q4 = 0; q4 < 4; ++q4) {
             const int c = x * 32 + 8 * q4 + 4 * h2;
             float g[4] = {1.f, 1.f, 1.f, 1.f};
-            if (a.weight && c < a.dv)
+            if (e.weight && c < e.dv)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) g[j] = da_load1(a.weight, c + j, a.w_bf16) * a.post * rn;
+                for (int j = 0; j < 4; ++j) g[j] = da_load1(e.weight, c + j, e.w_bf16) * e.post * rn;
             rows.put(l32, c, st.o[0][x][4 * q4] * g[0], st.o[0][x][4 * q4 + 1] * g[1], st.o[0][x][4 * q4 + 2] * g[2], st.o[0][x][4 * q4 + 3] * g[3]);
         }
-    to(a.out);
-    if (!a.o2) return;
-    if (a.weight) {
+    to(e.out);
+    if (!e.o2) return;
+    if (e.weight) {
 #pragma unroll
         for (int x = 0; x < C::MT; ++x)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
                 rows.put(l32, x * 32 + 8 * q4 + 4 * h2, st.o[0][x][4 * q4], st.o[0][x][4 * q4 + 1], st.o[0][x][4 * q4 + 2], st.o[0][x][4 * q4 + 3]);
-        to(a.u);
+        to(e.u);
     }
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
@@ -647,7 +684,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
             for (int j = 0; j < 4; ++j) o[j] = st.o[1][x][4 * q4 + j] - beta * st.o[0][x][4 * q4 + j];
             rows.put(l32, x * 32 + 8 * q4 + 4 * h2, o[0], o[1], o[2], o[3]);
         }
-    to(a.o2);
+    to(e.o2);
 }
 
 // One row of the result from its two maps' sums in plain order: LPR neighbouring lanes of NE channels each (c0: the lane's first), O normalised
@@ -729,17 +766,22 @@ __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff
         }
         return t;
     };
+    const int64_t ldk = a.ks[1], ldv = a.vs[1];
+    int stand = 0;                                            // the key that the copies stand at
     auto bits = [&](int t) {
-        uint32_t v = w.live ? (uint32_t)(a.rowbits[(mb * a.N + w.i) * M64 + (t >> 1)] >> (t & 1 ? 32 : 0)) : 0u;
+        uint32_t v = w.live ? (uint32_t)(da_again().rowbits[(mb * a.N + w.i) * M64 + (t >> 1)] >> (t & 1 ? 32 : 0)) : 0u;
         da_pin(v);
         return v;
     };
     auto issue = [&](int t, int buf) {
         const int k0 = t * 32, valid = len - k0;
         const uint64_t live = walk.live(a, mb, w.q_lo, w.q_hi, M64, N64, k0);
-        const bool whole = full && valid >= 32 && (uint32_t)live == ~0u;
-        ck.run(lds0 + buf * 2 * TILE, k0, a.ks[1], valid, live, whole);
-        cv.run(lds0 + buf * 2 * TILE + TILE, k0, a.vs[1], valid, live, whole);
+        const bool rows = valid >= 32 && (uint32_t)live == ~0u;
+        ck.move((k0 - stand) * ldk);
+        cv.move((k0 - stand) * ldv);
+        stand = k0;
+        ck.run(lds0 + buf * 2 * TILE, valid, live, rows, full);
+        cv.run(lds0 + buf * 2 * TILE + TILE, valid, live, rows, full);
     };
     int t = next(sp * per + wave), buf = 0, code = 0;
     uint32_t vis = ~0u;
@@ -1150,15 +1192,20 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     DaWalk walk;
     walk.base = -1;
     auto next = [&](int k0) { return walk.next(a, w, mb, qt0, qt1, M64, N64, k0, wg_end); };
+    const int64_t ldk = a.ks[1], ldv = a.vs[1];
+    int stand = 0;                                            // the block that the copies stand at
     auto issue = [&](int k0, int buf) {
         const int valid = len - k0;
         const uint64_t live = walk.live(a, mb, qt0, qt1, M64, N64, k0), all = KB == 64 ? ~0ull : 0xffffffffull;
-        const bool whole = full && valid >= KB && (live & all) == all;
-        ck.run(lds0 + buf * 2 * TILE, k0, a.ks[1], valid, live, whole);
-        cv.run(lds0 + buf * 2 * TILE + TILE, k0, a.vs[1], valid, live, whole);
+        const bool rows = valid >= KB && (live & all) == all;
+        ck.move((k0 - stand) * ldk);
+        cv.move((k0 - stand) * ldv);
+        stand = k0;
+        ck.run(lds0 + buf * 2 * TILE, valid, live, rows, full);
+        cv.run(lds0 + buf * 2 * TILE + TILE, valid, live, rows, full);
     };
     auto bits = [&](int k0) {                                 // a mixed tile's keys as this lane's row sees them
-        return w.live ? a.rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63) : 0ull;
+        return w.live ? da_again().rowbits[(mb * a.N + w.i) * M64 + (k0 >> 6)] >> (k0 & 63) : 0ull;
     };
     int k0 = next(0), buf = 0, code = 0;
     uint64_t vis = ~0ull;
@@ -1229,6 +1276,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         vis = vis_n;
         buf ^= 1;
     }
+    const DiffArgs &e = da_again();
     __syncthreads();                                          // every wave is done with the tiles
     const DaRowsOut<T, C::DV> rows{lds + wave * 32 * C::DV * C::ES};
 #pragma unroll
@@ -1239,14 +1287,14 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
             for (int q4 = 0; q4 < 4; ++q4) {
                 const int c = x * 32 + 8 * q4 + 4 * h2;       // heads of up to 16 channels: one tile holds both maps' channels, this map's half counts
                 if (DK < 32 && c / DK != t) continue;
-                rows.put(l32, DK < 32 ? c : t * DK + c, dq[t][x][4 * q4] * a.scale, dq[t][x][4 * q4 + 1] * a.scale, dq[t][x][4 * q4 + 2] * a.scale,
-                         dq[t][x][4 * q4 + 3] * a.scale);
+                rows.put(l32, DK < 32 ? c : t * DK + c, dq[t][x][4 * q4] * e.scale, dq[t][x][4 * q4 + 1] * e.scale, dq[t][x][4 * q4 + 2] * e.scale,
+                         dq[t][x][4 * q4 + 3] * e.scale);
             }
     const int w0 = blk0 + wave * 32;
     rows.flush(lane, [&](int r, int c) -> T * {
-        const int row = w0 + r, i = da_div_g(a, min(row, R - 1)), t = c / DK;
+        const int row = w0 + r, i = da_div_g(e, min(row, R - 1)), t = c / DK;
         c -= t * DK;
-        return row < R && c < a.d ? reinterpret_cast<T *>(a.dq) + (((int64_t)b * a.N + i) * a.H + hk * a.G + row - i * a.G) * 2 * a.d + t * a.d + c : nullptr;
+        return row < R && c < e.d ? reinterpret_cast<T *>(e.dq) + (((int64_t)b * e.N + i) * e.H + hk * e.G + row - i * e.G) * 2 * e.d + t * e.d + c : nullptr;
     });
 }
 
@@ -1274,12 +1322,12 @@ __device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[Da
             dl[4 * q4] = __uint_as_float(y.x); dl[4 * q4 + 1] = __uint_as_float(y.y); dl[4 * q4 + 2] = __uint_as_float(y.z); dl[4 * q4 + 3] = __uint_as_float(y.w);
         }
     };
-    stats(0);
     da_ring<C::NFV + C::NF, 2>([&](int i) { return i < C::NFV ? ln.frag(tu, i) : ln.frag(tq, i - C::NFV); },
                                [&](int i, const uint4 &f) {
                                    if (i < C::NFV) dp = Da<T>::mma(f, vf[i], dp);
                                    else s[0] = Da<T>::mma(f, kf[0][i - C::NFV], s[0]);
                                });
+    stats(0);
     fr[0] = ln.frag(tq, C::NF);
     if (C::NF > 1) fr[1] = ln.frag(tq, C::NF + 1);
     if (masked) da_hide(s[0], mine);
@@ -1391,7 +1439,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
                 const int qt = qt_first + base * 64 + lane;
                 bool n = false, p = false, y = true;
                 if (qt < N64) {
-                    const uint8_t *tp = a.tiles + (mb * N64 + qt) * M64;
+                    const uint8_t *tp = da_again().tiles + (mb * N64 + qt) * M64;
                     const int c = wlive ? tp[kw0 >> 6] : 2;
                     n = tp[kt0] != 2 || tp[kt1] != 2;
                     p = c == 1;
@@ -1410,22 +1458,24 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
         const int x = u % per_head & 63;
         return (int)((mixed >> x) & 1 ? 1 : (hide >> x) & 1 ? 2 : 0);
     };
-    auto bits = [&](int u) { return klive ? a.colbits[(mb * a.M + key) * N64 + qt_first + u % per_head] : 0ull; };
+    auto bits = [&](int u) { return klive ? da_again().colbits[(mb * a.M + key) * N64 + qt_first + u % per_head] : 0ull; };
     auto row_lse = [&](int u) {                               // lse of this lane's row of block u: +inf where it sees nothing or is not there
         if (u >= u1) return INFINITY;
         const int g = u / per_head, i = (qt_first + u - g * per_head) * QB + lane;
         return i < a.N ? a.rowstat[((int64_t)b * a.H + hk * a.G + g) * a.N + i] : INFINITY;
     };
+    const int64_t ldq = a.qs[1], ldh = a.qs[2], ldu = (int64_t)a.H * a.dv;
+    int at_i = 0, at_h = 0;                                   // query and head that the copies stand at
     auto issue = [&](int u, int buf, float lse) {
         const int g = u / per_head, i0 = (qt_first + u - g * per_head) * QB, head = hk * a.G + g, valid = a.N - i0;
         const uint64_t rows = __ballot(lse != INFINITY);      // rows that see nothing: their queries may hold anything, zeros are copied
-        const bool whole = full && rows == ~0ull;
         const uint32_t to = lds0 + buf * BUF;
-        DaCopy<T, DK, QB, kDaThreads> q2 = cq, u2 = cu;
-#pragma unroll
-        for (int p = 0; p < DaCopy<T, DK, QB, kDaThreads>::P; ++p) { q2.base[p] += head * a.qs[2]; u2.base[p] += (int64_t)head * a.dv; }
-        q2.run(to + wave * 1024, i0, a.qs[1], valid, rows, whole);
-        u2.run(to + TILE + wave * 1024, i0, (int64_t)a.H * a.dv, valid, rows, whole);
+        cq.move((i0 - at_i) * ldq + (head - at_h) * ldh);
+        cu.move((i0 - at_i) * ldu + (head - at_h) * (int64_t)a.dv);
+        at_i = i0;
+        at_h = head;
+        cq.run(to + wave * 1024, valid, rows, rows == ~0ull, full);
+        cu.run(to + TILE + wave * 1024, valid, rows, rows == ~0ull, full);
         const float *sp = i0 + lane < a.N ? a.rowstat + wave * bhn + ((int64_t)b * a.H + head) * a.N + i0 + lane : da_no_row + wave;     // wave = which statistic
         da_copy4(sp, __builtin_amdgcn_readfirstlane(to + 2 * TILE + wave * QB * 4));
     };
@@ -1470,18 +1520,19 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
         vis = vis_n;
         buf ^= 1;
     }
+    const DiffArgs &e = da_again();
     __syncthreads();                                          // every wave is done with the tiles
     const bool keep = klive && seen;
-    const float f = keep ? a.scale : 0.f;
-    const int64_t k0 = (int64_t)b * a.M;
-    const int w = 2 * a.d + a.dv;
+    const float f = keep ? e.scale : 0.f;
+    const int64_t k0 = (int64_t)b * e.M;
+    const int w = 2 * e.d + e.dv;
     auto out = [&](auto rows, auto dkv) {                     // dV, then dK, as whole rows; dkv(key): where the key's dK row starts, dV behind it or in its own tensor
 #pragma unroll
         for (int x = 0; x < C::MT; ++x)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
                 rows.put(l32, x * 32 + 8 * q4 + 4 * h2, keep ? dv[x][4 * q4] : 0.f, keep ? dv[x][4 * q4 + 1] : 0.f, keep ? dv[x][4 * q4 + 2] : 0.f, keep ? dv[x][4 * q4 + 3] : 0.f);
-        rows.flush(lane, [&](int r, int c) { return kw0 + r < a.M && c < a.dv ? dkv(kw0 + r, 1) + c : nullptr; });
+        rows.flush(lane, [&](int r, int c) { return kw0 + r < e.M && c < e.dv ? dkv(kw0 + r, 1) + c : nullptr; });
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -1496,15 +1547,15 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
         rows.flush(lane, [&](int r, int c) {
             const int t = c / DK;
             c -= t * DK;
-            return kw0 + r < a.M && c < a.d ? dkv(kw0 + r, 0) + t * a.d + c : nullptr;
+            return kw0 + r < e.M && c < e.d ? dkv(kw0 + r, 0) + t * e.d + c : nullptr;
         });
     };
-    if (a.kvpart) {
-        float *part = a.kvpart + (int64_t)run * a.B * a.M * a.Hk * w;
-        out(DaRowsOut<float, C::DV>{lds + wave * 32 * C::DV * 4}, [&](int key, int v) { return part + ((k0 + key) * a.Hk + hk) * w + v * 2 * a.d; });
+    if (e.kvpart) {
+        float *part = e.kvpart + (int64_t)run * e.B * e.M * e.Hk * w;
+        out(DaRowsOut<float, C::DV>{lds + wave * 32 * C::DV * 4}, [&](int key, int v) { return part + ((k0 + key) * e.Hk + hk) * w + v * 2 * e.d; });
     } else {
         out(DaRowsOut<T, C::DV>{lds + wave * 32 * C::DV * C::ES}, [&](int key, int v) {
-            return v ? reinterpret_cast<T *>(a.dvv) + ((k0 + key) * a.Hk + hk) * a.dv : reinterpret_cast<T *>(a.dk) + ((k0 + key) * a.Hk + hk) * 2 * a.d;
+            return v ? reinterpret_cast<T *>(e.dvv) + ((k0 + key) * e.Hk + hk) * e.dv : reinterpret_cast<T *>(e.dk) + ((k0 + key) * e.Hk + hk) * 2 * e.d;
         });
     }
 }
