@@ -900,39 +900,48 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
     if (at >= (int64_t)R * a.B * a.Hk) return;
     const int bh = (int)(at / R), b = bh / a.Hk, hk = bh - b * a.Hk;
     const int row = (int)(at - (int64_t)bh * R), i = da_div_g(a, row), head = hk * a.G + row - i * a.G;
-    const float lam = da_lambda(a, head);
     float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, o[2][NE];
-    for (int s = lane; s < nsplit; s += 64) {
-        const float4 v = ml[at * nsplit + s];
-        mx[0] = fmaxf(mx[0], v.x);
-        mx[1] = fmaxf(mx[1], v.z);
-    }
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) { mx[0] = fmaxf(mx[0], __shfl_xor(mx[0], x)); mx[1] = fmaxf(mx[1], __shfl_xor(mx[1], x)); }
 #pragma unroll
     for (int j = 0; j < NE; ++j) o[0][j] = o[1][j] = 0.f;
 #pragma unroll 2
-    for (int s = sg; s < nsplit; s += 8) {
+    for (int s = sg; s < nsplit; s += 8) {                    // (the sums come with their maximum: no load waits for another)
         const float4 v = ml[at * nsplit + s];
-        const float f[2] = {mx[0] == -INFINITY ? 1.f : da_exp2(v.x - mx[0]), mx[1] == -INFINITY ? 1.f : da_exp2(v.z - mx[1])};
-        sum[0] += v.y * f[0];
-        sum[1] += v.w * f[1];
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int j = 0; j < NE; j += 4) {
-                const float4 z = *reinterpret_cast<const float4 *>(part + ((at * nsplit + s) * 2 + x) * DV + c0 + j);
-                o[x][j] += z.x * f[x]; o[x][j + 1] += z.y * f[x]; o[x][j + 2] += z.z * f[x]; o[x][j + 3] += z.w * f[x];
-            }
-    }
-#pragma unroll
-    for (int y = 8; y < 64; y <<= 1)
+        const float m[2] = {v.x, v.z}, l[2] = {v.y, v.w};
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
+            float4 z[NE / 4];
+#pragma unroll
+            for (int j = 0; j < NE / 4; ++j) z[j] = *reinterpret_cast<const float4 *>(part + ((at * nsplit + s) * 2 + x) * DV + c0 + 4 * j);
+            const float mn = fmaxf(mx[x], m[x]), f = mn == -INFINITY ? 1.f : da_exp2(mx[x] - mn), g = mn == -INFINITY ? 1.f : da_exp2(m[x] - mn);
+            mx[x] = mn;
+            sum[x] = sum[x] * f + l[x] * g;
+#pragma unroll
+            for (int j = 0; j < NE / 4; ++j) {
+                o[x][4 * j] = o[x][4 * j] * f + z[j].x * g;
+                o[x][4 * j + 1] = o[x][4 * j + 1] * f + z[j].y * g;
+                o[x][4 * j + 2] = o[x][4 * j + 2] * f + z[j].z * g;
+                o[x][4 * j + 3] = o[x][4 * j + 3] * f + z[j].w * g;
+            }
+        }
+    }
+    const float lam = da_lambda(a, head);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {                             // the 8 groups, in order of their distance
+        float m = mx[x];
+#pragma unroll
+        for (int y = 8; y < 64; y <<= 1) m = fmaxf(m, __shfl_xor(m, y));
+        const float f = m == -INFINITY ? 1.f : da_exp2(mx[x] - m);
+        mx[x] = m;
+        sum[x] *= f;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) o[x][j] *= f;
+#pragma unroll
+        for (int y = 8; y < 64; y <<= 1) {
             sum[x] += __shfl_xor(sum[x], y);
 #pragma unroll
             for (int j = 0; j < NE; ++j) o[x][j] += __shfl_xor(o[x][j], y);
         }
+    }
     if (sg) return;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {

@@ -2518,17 +2518,20 @@ class _QKNormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, paired):
         yq, yk, qr, kr = _hip().qk_norm_rotate_forward(q, k, wq, wk, cos, sin, positions, eps, paired)
-        ctx.save_for_backward(qr, kr, wq, wk, cos, sin, positions)
+        if positions is None:                      # (each tensor costs a microsecond on its way through the graph)
+            ctx.save_for_backward(qr, kr, wq, wk, cos, sin)
+        else:
+            ctx.save_for_backward(qr, kr, wq, wk, cos, sin, positions)
         ctx.meta = (eps, paired)
         return yq, yk
 
     @staticmethod
     def backward(ctx, dyq, dyk):
         _no_double_backward("qk_norm_rotate")
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+        q, k, wq, wk, cos, sin, *positions = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dwq, dwk = _hip().qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions, *ctx.meta, dyq, dyk, need[2] and wq is not None,
-                                                         need[3] and wk is not None)
+        eps, paired = ctx.meta
+        dq, dk, dwq, dwk = _hip().qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions[0] if positions else None, eps, paired, dyq, dyk, need[2], need[3])
         return dq, dk, dwq, dwk, None, None, None, None, None
 
 
@@ -2613,20 +2616,30 @@ class _DiffAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps):
         out, qr, kr, vr, u, o2, stats = _hip().diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, True)
-        at = None if isinstance(start, int) else start
-        ctx.save_for_backward(qr, kr, vr, lam, weight, forms, kv_len, at, out if weight is None else None, u, o2, stats)
-        ctx.meta = (mask_batches, causal, start if at is None else None, scale, init, eps)
+        # what the caller holds too goes through the graph, which notices a change of it; what is made here only hangs on the node
+        users = [t for t in (kv_len, start) if isinstance(t, torch.Tensor)]
+        if weight is None:
+            ctx.save_for_backward(qr, kr, vr, lam, out, *users)
+        else:
+            ctx.save_for_backward(qr, kr, vr, lam, weight, *users)
+        ctx.kept = (forms, u, o2, stats)
+        ctx.meta = (weight is not None, kv_len is not None, mask_batches, causal, None if isinstance(start, torch.Tensor) else start, scale, init, eps)
         return out
 
     @staticmethod
     def backward(ctx, dy):
         _no_double_backward("diff_attention")
-        q, k, v, lam, weight, forms, kv_len, at, out, u, o2, stats = ctx.saved_tensors
-        mask_batches, causal, start, scale, init, eps = ctx.meta
+        q, k, v, lam, weight, *users = ctx.saved_tensors
+        forms, u, o2, stats = ctx.kept
+        normed, has_len, mask_batches, causal, start, scale, init, eps = ctx.meta
+        out = u
+        if not normed:
+            out, weight = weight, None
+        kv_len = users.pop(0) if has_len else None
         n = ctx.needs_input_grad
-        dq, dk, dv, dlam, dw = _hip().diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start if at is None else at, scale, init, eps,
-                                                         u if out is None else out, u, o2, stats, dy, (n[0], n[1] or n[2], n[3], n[4]))
-        return (dq, dk if n[1] else None, dv if n[2] else None, dlam, dw) + (None,) * 8
+        dq, dk, dv, dlam, dw = _hip().diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, users[0] if users else start, scale, init, eps,
+                                                         out, u, o2, stats, dy, (n[0], n[1] or n[2], n[3], n[4]))
+        return (dq, dk if n[1] else None, dv if n[2] else None, dlam, dw, None, None, None, None, None, None, None, None)
 
 
 def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None, norm_eps: float = 1e-5, attn_mask=None, kv_lengths=None, causal: bool = False,
