@@ -27,7 +27,7 @@ typedef short da_tr4 __attribute__((ext_vector_type(4)));
 typedef short da_tr8 __attribute__((ext_vector_type(8)));
 
 constexpr int kDaThreads = 256;
-constexpr int kDaSplitWgs = 256, kDaRunKeys = 512;
+constexpr int kDaSplitWgs = 256, kDaRunKeys = 512, kDaManyRows = 256;
 
 struct DiffArgs {
     const void *q, *k, *v;                      // [B, N, H, 2, d], [B, M, Hk, 2, d], [B, M, Hk, dv]
@@ -1677,7 +1677,7 @@ static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <
 // workgroup, n runs).
 static int diff_attn_splits(const DiffArgs &a) {
     const int64_t R = (int64_t)a.N * a.G, bh = (int64_t)a.B * a.Hk;
-    if ((R + 127) / 128 * bh >= 256) return 0;
+    if ((R + 127) / 128 * bh >= kDaManyRows) return 0;
     const int64_t wgs = (R + 31) / 32 * bh, most = ((int64_t)a.M + kDaRunKeys - 1) / kDaRunKeys;
     int64_t n = kDaSplitWgs / wgs;
     if (n > most) n = most;
@@ -1770,8 +1770,8 @@ int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void 
     if (int e = diff_attn_setup(a, shape, scale, init, eps)) return e;
     if (!lam || !ws || ((uintptr_t)ws & 255)) return DFINE_E_BADARG;
     const bool rows_ = a.B && a.N, keys_ = a.B && a.M;
-    if (rows_ && (!diff_attn_aligned(q) || !diff_attn_aligned(out) || !diff_attn_aligned(o2) || !stats || !diff_attn_aligned(dy) || (dq && !diff_attn_aligned(dq)) ||
-                  (weight && !diff_attn_aligned(u))))
+    if (rows_ && (!diff_attn_aligned(q) || !diff_attn_aligned(weight ? u : out) || !diff_attn_aligned(o2) || !stats || !diff_attn_aligned(dy) ||
+                  (dq && !diff_attn_aligned(dq))))
         return DFINE_E_BADARG;
     if ((dk == nullptr) != (dv == nullptr)) return DFINE_E_BADARG;
     if (keys_ && (!diff_attn_aligned(k) || !diff_attn_aligned(v) || (dk && (!diff_attn_aligned(dk) || !diff_attn_aligned(dv))))) return DFINE_E_BADARG;

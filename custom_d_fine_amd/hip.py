@@ -1622,33 +1622,42 @@ def _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys
                      start if isinstance(start, int) else 0, mask_batches, *qs, *ks, *vs, *dys)
 
 
+def _da_kept(out, normed):
+    """What the forward pass keeps for the backward, in one buffer (each tensor costs microseconds to make and on its way through the graph): the rows'
+    statistics, then W, then with a norm U -> bytes in all, where W and U begin (U: None without a norm)."""
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    B, N, H, dv = out.shape
+    stats, rows = up(16 * B * N * H), up(out.element_size() * out.numel())
+    return (stats + 2 * rows, stats, stats + rows) if normed else (stats + rows, stats, None)
+
+
 @_on_device
 def diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, keep):
-    """-> out [B, N, H, dv], and with `keep` what the backward pass reads: q, k, v as the kernel read them, u, o2, stats (else None)."""
+    """-> out [B, N, H, dv], q, k, v as the kernel read them, and with `keep` what else the backward pass reads, one buffer (else None)."""
     q, qs = _rows16(q)
     k, ks = _rows16(k)
     v, vs = _rows16(v)
     B, N, H, _, d = q.shape
     M, dv = k.shape[1], v.shape[3]
     out = torch.empty(B, N, H, dv, device=q.device, dtype=q.dtype)
-    u = o2 = stats = None
+    kept = o2 = stats = u = None
     if keep:
-        u = _EMPTY_LIKE(out) if weight is not None else None
-        o2 = _EMPTY_LIKE(out)
-        stats = torch.empty(4, B, H, N, device=q.device, dtype=torch.float32)
+        size, o2_at, u_at = _da_kept(out, weight is not None)
+        kept = torch.empty(size, device=q.device, dtype=torch.uint8)
+        stats, o2, u = kept.data_ptr(), kept.data_ptr() + o2_at, u_at and kept.data_ptr() + u_at
     shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs)
     nws = _lib.dfine_diff_attn_fwd_ws_bytes(shape)
     ws = torch.empty(nws, device=q.device, dtype=torch.uint8) if nws > 0 else None
     with _timed("diff_attention", 4.0 * B * H * N * M * (d + dv), io=float(q.element_size()) * (q.numel() + k.numel() + v.numel() + out.numel())):
         _check(_lib.dfine_diff_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(weight), _ptr(forms), _ptr(kv_len),
-                                        None if isinstance(start, int) else _ptr(start), _ptr(out), _ptr(u), _ptr(o2), _ptr(stats), _ptr(ws), shape, scale, init,
-                                        eps, _stream()), "dfine_diff_attn_fwd")
-    return out, q, k, v, u, o2, stats
+                                        None if isinstance(start, int) else _ptr(start), _ptr(out), u, o2, stats, _ptr(ws), shape, scale, init, eps, _stream()),
+               "dfine_diff_attn_fwd")
+    return out, q, k, v, kept
 
 
 @_on_device
-def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, out, u, o2, stats, dy, want):
-    """`want`: which of dq, (dk, dv), dlam, dweight are needed -> (dq, dk, dv, dlam, dweight)."""
+def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, out, kept, dy, want):
+    """`out`: the forward pass's (needed without a norm weight); `want`: which of dq, (dk, dv), dlam, dweight are needed -> (dq, dk, dv, dlam, dweight)."""
     q, qs = _rows16(q)
     k, ks = _rows16(k)
     v, vs = _rows16(v)
@@ -1659,10 +1668,12 @@ def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal
     shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys)
     ws = torch.empty(max(256, int(_lib.dfine_diff_attn_bwd_ws_bytes(shape))), device=q.device, dtype=torch.uint8)
     B, N, H, _, d = q.shape
-    with _timed("diff_attention", 4.0 * B * H * N * k.shape[1] * (3 * d + 2 * v.shape[3]), io=2.0 * q.element_size() * (q.numel() + k.numel() + v.numel() + out.numel())):
+    _, o2_at, u_at = _da_kept(dy, weight is not None)
+    stats = kept.data_ptr()
+    with _timed("diff_attention", 4.0 * B * H * N * k.shape[1] * (3 * d + 2 * v.shape[3]), io=2.0 * q.element_size() * (q.numel() + k.numel() + v.numel() + dy.numel())):
         _check(_lib.dfine_diff_attn_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(weight), _ptr(forms), _ptr(kv_len),
-                                        None if isinstance(start, int) else _ptr(start), _ptr(out), _ptr(u), _ptr(o2), _ptr(stats), _ptr(dy), _ptr(dq), _ptr(dk),
-                                        _ptr(dv), _ptr(dlam), _ptr(dweight), _ptr(ws), shape, scale, init, eps, _stream()), "dfine_diff_attn_bwd")
+                                        None if isinstance(start, int) else _ptr(start), _ptr(out), u_at and stats + u_at, stats + o2_at, stats, _ptr(dy), _ptr(dq),
+                                        _ptr(dk), _ptr(dv), _ptr(dlam), _ptr(dweight), _ptr(ws), shape, scale, init, eps, _stream()), "dfine_diff_attn_bwd")
     return dq, dk, dv, dlam, dweight
 
 

@@ -2612,33 +2612,36 @@ def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, posit
     return _hip().qk_norm_rotate_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))[:2]
 
 
+def _index32(t):
+    """Lengths or positions as the kernels read them (which cut them to the keys there are): beyond 32 bits the nearest that fits."""
+    if t.dtype is not torch.int32:
+        t = t.clamp(-(2 ** 31) + 1, 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
+
+
 class _DiffAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps):
-        out, qr, kr, vr, u, o2, stats = _hip().diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, True)
-        # what the caller holds too goes through the graph, which notices a change of it; what is made here only hangs on the node
-        users = [t for t in (kv_len, start) if isinstance(t, torch.Tensor)]
-        if weight is None:
-            ctx.save_for_backward(qr, kr, vr, lam, out, *users)
-        else:
-            ctx.save_for_backward(qr, kr, vr, lam, weight, *users)
-        ctx.kept = (forms, u, o2, stats)
-        ctx.meta = (weight is not None, kv_len is not None, mask_batches, causal, None if isinstance(start, torch.Tensor) else start, scale, init, eps)
+        out, qr, kr, vr, kept = _hip().diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, True)
+        users = [t for t in (forms, kv_len, start) if isinstance(t, torch.Tensor)]               # (each costs a microsecond on its way through the graph)
+        ctx.save_for_backward(qr, kr, vr, lam, out if weight is None else weight, kept, *users)
+        ctx.meta = (weight is not None, forms is not None, kv_len is not None, mask_batches, causal, None if isinstance(start, torch.Tensor) else start, scale, init,
+                    eps)
         return out
 
     @staticmethod
     def backward(ctx, dy):
         _no_double_backward("diff_attention")
-        q, k, v, lam, weight, *users = ctx.saved_tensors
-        forms, u, o2, stats = ctx.kept
-        normed, has_len, mask_batches, causal, start, scale, init, eps = ctx.meta
-        out = u
+        q, k, v, lam, weight, kept, *users = ctx.saved_tensors
+        normed, has_forms, has_len, mask_batches, causal, start, scale, init, eps = ctx.meta
+        out = None
         if not normed:
             out, weight = weight, None
+        forms = users.pop(0) if has_forms else None
         kv_len = users.pop(0) if has_len else None
         n = ctx.needs_input_grad
         dq, dk, dv, dlam, dw = _hip().diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, users[0] if users else start, scale, init, eps,
-                                                         out, u, o2, stats, dy, (n[0], n[1] or n[2], n[3], n[4]))
+                                                         out, kept, dy, (n[0], n[1] or n[2], n[3], n[4]))
         return (dq, dk if n[1] else None, dv if n[2] else None, dlam, dw, None, None, None, None, None, None, None, None)
 
 
@@ -2713,8 +2716,8 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
     if not q.is_cuda:
         return _backend_for_cpu(op)(q, k, v, lambda_vectors, init, norm_weight, eps, attn_mask, kv_lengths, bool(causal), query_start, scale)
     lam, weight = lambda_vectors.contiguous(), None if norm_weight is None else norm_weight.contiguous()
-    kv_len = None if kv_lengths is None else kv_lengths.to(torch.int32).contiguous()
-    start = query_start.to(torch.int32).contiguous() if starts else int(query_start)
+    kv_len = None if kv_lengths is None else _index32(kv_lengths)
+    start = _index32(query_start) if starts else int(query_start)
     forms = None
     if attn_mask is not None:
         forms = _hip().diff_attn_mask_forms(attn_mask if attn_mask.dim() == 3 else attn_mask[None])

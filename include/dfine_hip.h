@@ -836,7 +836,7 @@ int dfine_qk_norm_rotate_bwd(const void *q, const void *k, const void *wq, const
  * shape (host int64): B, N, M, H, Hk, d, dv, dtype (0 fp32, 1 bf16), heads of lam, lam bf16, weight bf16, causal, q_start, mask has batches, then the
  * strides (batch, token, head, map) of q, of k, (batch, token, head) of v, of dy (elements; 16-byte rows).
  * Forward ws: dfine_diff_attn_fwd_ws_bytes(shape) bytes, 256-byte aligned (0: NULL): few queries over many keys are cut into runs of the keys.
- * Backward: dq, dk, dv contiguous (dq, or dk and dv, NULL: not wanted), dlam, dweight of lam's and weight's types (NULL: not wanted);
+ * Backward: reads u with a weight, out without (the other may be NULL); dq, dk, dv contiguous (dq, or dk and dv, NULL: not wanted), dlam, dweight of lam's and weight's types (NULL: not wanted);
  * ws: dfine_diff_attn_bwd_ws_bytes(shape) bytes, 256-byte aligned.  Deterministic. */
 int64_t dfine_diff_attn_mask_words(int64_t batches, int64_t N, int64_t M);
 int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_t M, int64_t stride_b, int64_t stride_n, uint64_t *forms,
