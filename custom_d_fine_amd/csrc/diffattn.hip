@@ -48,7 +48,7 @@ struct DiffArgs {
     const void *dy;
     int64_t dys[3];
     void *du, *dq, *dk, *dvv;
-    float *rowstat;                             // [4][B, H, N]: lse_0, lse_1 - log2 |l|, D_0, sign(l) D_1 (diff_attn_prep_kernel)
+    float *rowstat;                             // [4][B, H, N]: -lse_0 / c, -(lse_1 - log2 |l|) / c, -D_0, sign(l) (D_1 - D_0) or -D_1 (da_pair), c = scale_log2e
     float *lpart, *wpart;                       // per workgroup of the first kernel: sum of D_1, sums of dg
     float *kvpart;                              // dK | dV sums of each run of the rows, fp32 [runs][B, M, Hk, 2 d + dv] (null: one run)
     int kvruns;
@@ -77,6 +77,9 @@ template <typename T, int DK> struct DaCfg {
                          MTK = DK / 32 ? DK / 32 : 1, FPT = 32 / Da<T>::KPF;      // fragments per 32 keys
     static_assert(DV % 32 == 0, "a value tile is 32 channels");
 };
+
+// dK and dV by two waves per 32 keys, one map each (diff_attn_dkdv_kernel)
+template <typename T, int DK> constexpr bool da_pair() { return DK == 64 && sizeof(T) == 2; }
 
 // f(row): a b128 read serves 16 lanes at a time (rows 16 apart in some order, one u), a transposed read 32 lanes (4 rows from a multiple of 4 on, 4 units from a
 // multiple of 4 on): f takes all values over 16 rows and, in its bits from 2 on, over 4 (256 bytes = all banks; rows shorter than that share them).
@@ -998,14 +1001,15 @@ __global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__re
 // near the mean of the values where the maps are flat), so dU . (A_1 V) of rounded vectors would be a small difference of large products.  The forward
 // pass therefore keeps W = A_1 V - beta U, beta = (A_1 V . U) / (U . U), and D_1 = r (t . W) + beta (dU . U), D_0 = dU . U + l D_1 (long rows, bf16: error of dl
 // and dq against 64 bits 0.0046 with A_1 V itself).  dP is made from the ROUNDED dU: what the rounding adds to D is added here too.
-// The other kernels read the rows' statistics with l worked in: exp2(s - (lse_1 - log2 |l|)) is |l| A_1, and its sign goes with D_1 and dP.
+// The other kernels read the rows' statistics with l worked in - exp2(c s - (lse_1 - log2 |l|)) is |l| A_1, and its sign goes with D_1 and dP - and as the
+// numbers that dK's and dV's products start from: S_t at -lse_t / c, dP at -D_0.
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, int nrun) {
     constexpr int RW = 256 / LPR;                                                              // rows at a time, LPR lanes of 8 channels each
     const int head = blockIdx.x % a.H, run = blockIdx.x / a.H;
     const int tid = threadIdx.x, lane = tid % LPR, rr = tid / LPR, c = lane * 8;
     const bool ok = c < a.dv;
-    const float lam = da_lambda(a, head), log2l = log2f(fabsf(lam)), sign = lam < 0.f ? -1.f : 1.f;
+    const float lam = da_lambda(a, head), log2l = log2f(fabsf(lam)), sign = lam < 0.f ? -1.f : 1.f, inv_c = 1.f / a.scale_log2e;
     float w[8], dw[8], dsum = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -1068,10 +1072,11 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
             da_store4(dp + 4, du[4], du[5], du[6], du[7]);
         }
         if (lane == 0) {
-            a.rowstat[at] = lse0;
-            a.rowstat[bhn + at] = lse1 - log2l;
-            a.rowstat[2 * bhn + at] = d0 + e1r + lam * e2r;
-            a.rowstat[3 * bhn + at] = (d1 + e2r) * sign;
+            const float dd0 = d0 + e1r + lam * e2r;
+            a.rowstat[at] = -lse0 * inv_c;
+            a.rowstat[bhn + at] = (log2l - lse1) * inv_c;
+            a.rowstat[2 * bhn + at] = -dd0;
+            a.rowstat[3 * bhn + at] = da_pair<T, LPR * 4>() ? -(d1 + e2r) : (d1 + e2r - dd0) * sign;
             dsum += d1;
         }
     }
@@ -1232,9 +1237,11 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     const T *up = reinterpret_cast<const T *>(a.du) + (((int64_t)b * a.N + w.i) * a.H + w.head) * a.dv;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        lse[t] = w.live ? a.rowstat[t * bhn + at] : INFINITY;
+        lse[t] = w.live ? a.rowstat[t * bhn + at] * -a.scale_log2e : INFINITY;
         dl[t] = w.live ? a.rowstat[(2 + t) * bhn + at] : 0.f;
     }
+    dl[1] = da_pair<T, DK>() ? -sign * dl[1] : dl[1] - sign * dl[0];
+    dl[0] = -dl[0];
     const bool empty = lse[0] == INFINITY;                    // sees no key: its query may hold anything
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -1316,46 +1323,44 @@ __device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[Da
     using C = DaCfg<T, DK>;
     const float c = a.scale_log2e;
     const int h2 = lane >> 5;
-    da_f16v dp, s[2];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) dp[r] = s[0][r] = s[1][r] = 0.f;
-    const uint32_t mine = vis >> (4 * h2);
-    uint4 fr[2], sf[C::FPT], pf[C::FPT];
-    da_f16v p;
-    float lv[16], dl[16];                                     // this lane's 16 rows' statistics (QB floats of each kind in LDS)
-    auto stats = [&](int t) {
+    // a lane's 16 rows' statistics (64 floats of each kind in LDS) are where the sums start: c S_t - lse_t and dP - D_0 come out of the products
+    auto stat16 = [&](int kind, da_f16v &x) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-            const da_u4v x = *(da_lds_u4)(uintptr_t)(stat + (t * 64 + 8 * q4 + 4 * h2) * 4), y = *(da_lds_u4)(uintptr_t)(stat + ((2 + t) * 64 + 8 * q4 + 4 * h2) * 4);
-            lv[4 * q4] = __uint_as_float(x.x); lv[4 * q4 + 1] = __uint_as_float(x.y); lv[4 * q4 + 2] = __uint_as_float(x.z); lv[4 * q4 + 3] = __uint_as_float(x.w);
-            dl[4 * q4] = __uint_as_float(y.x); dl[4 * q4 + 1] = __uint_as_float(y.y); dl[4 * q4 + 2] = __uint_as_float(y.z); dl[4 * q4 + 3] = __uint_as_float(y.w);
+            const da_u4v y = *(da_lds_u4)(uintptr_t)(stat + (kind * 64 + 8 * q4 + 4 * h2) * 4);
+            x[4 * q4] = __uint_as_float(y.x); x[4 * q4 + 1] = __uint_as_float(y.y); x[4 * q4 + 2] = __uint_as_float(y.z); x[4 * q4 + 3] = __uint_as_float(y.w);
         }
     };
+    da_f16v dp, s[2], p, dl;
+    const uint32_t mine = vis >> (4 * h2);
+    uint4 fr[2], sf[C::FPT], pf[C::FPT];
+    stat16(2, dp);
+    stat16(0, s[0]);
     da_ring<C::NFV + C::NF, 2>([&](int i) { return i < C::NFV ? ln.frag(tu, i) : ln.frag(tq, i - C::NFV); },
                                [&](int i, const uint4 &f) {
                                    if (i < C::NFV) dp = Da<T>::mma(f, vf[i], dp);
                                    else s[0] = Da<T>::mma(f, kf[0][i - C::NFV], s[0]);
                                });
-    stats(0);
+    stat16(1, s[1]);
     fr[0] = ln.frag(tq, C::NF);
     if (C::NF > 1) fr[1] = ln.frag(tq, C::NF + 1);
     if (masked) da_hide(s[0], mine);
     // the first map's vector work between the second's scores, the second's between the first map's products with the queries
     da_between<C::NF>(fr, [&](int i) { return ln.frag(tq, C::NF + i); }, [&](int i, const uint4 &f) { s[1] = Da<T>::mma(f, kf[1][i], s[1]); },
                       [&](int r) {
-                          p[r] = da_exp2(fmaf(s[0][r], c, -lv[r]));
-                          s[0][r] = p[r] * (dp[r] - dl[r]);
+                          p[r] = da_exp2(s[0][r] * c);
+                          s[0][r] = p[r] * dp[r];
                       });
     auto query = [&](int t, int i) { return ln.frag_tr(tq, i / C::MTK, DK < 32 ? 0 : t * (DK / 32) + i % C::MTK); };
     fr[0] = query(0, 0);
     fr[1] = query(0, 1);
-    stats(1);
+    stat16(3, dl);
 #pragma unroll
     for (int f = 0; f < C::FPT; ++f) sf[f] = da_pack<T>(s[0], f);
     if (masked) da_hide(s[1], mine);
     da_between<C::FPT * C::MTK>(fr, [&](int i) { return query(0, i); }, [&](int i, const uint4 &f) { dk[0][i % C::MTK] = Da<T>::mma(f, sf[i / C::MTK], dk[0][i % C::MTK]); },
                                 [&](int r) {
-                                    const float e = da_exp2(fmaf(s[1][r], c, -lv[r]));
+                                    const float e = da_exp2(s[1][r] * c);
                                     p[r] = fmaf(e, -sign, p[r]);
                                     s[1][r] = e * fmaf(dp[r], -sign, dl[r]);
                                 });
@@ -1369,37 +1374,75 @@ __device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[Da
                                     });
 }
 
-__device__ __attribute__((aligned(16))) float da_no_row[4] = {__builtin_huge_valf(), __builtin_huge_valf(), 0.f, 0.f};     // statistics of a row that is not there
+// One map's part of it (da_pair): f = 1 for map 0, -sign(l) for map 1
+template <typename T, int DK>
+__device__ __forceinline__ void da_dkdv_pair_tile(float c, da_f16v *dk, da_f16v *dv, const uint4 *kf, const uint4 *vf, float f, const DaLane<T, DK> &lq, const DaLane<T, DK> &lu,
+                                                  uint32_t tq, uint32_t tu, uint32_t stat, bool masked, uint32_t vis, int lane) {
+    using C = DaCfg<T, DK>;
+    const int h2 = lane >> 5;
+    da_f16v dp, s;
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+        const da_u4v x = *(da_lds_u4)(uintptr_t)(stat + 512 + (8 * q4 + 4 * h2) * 4), y = *(da_lds_u4)(uintptr_t)(stat + (8 * q4 + 4 * h2) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { dp[4 * q4 + j] = __uint_as_float(x[j]); s[4 * q4 + j] = __uint_as_float(y[j]); }
+    }
+    da_ring<C::NFV + C::NF, 2>([&](int i) { return i < C::NFV ? lu.frag(tu, i) : lq.frag(tq, i - C::NFV); },
+                               [&](int i, const uint4 &x) {
+                                   if (i < C::NFV) dp = Da<T>::mma(x, vf[i], dp);
+                                   else s = Da<T>::mma(x, kf[i - C::NFV], s);
+                               });
+    if (masked) da_hide(s, vis >> (4 * h2));
+    uint4 sf[C::FPT], pf[C::FPT];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        s[r] = da_exp2(s[r] * c) * f;
+        dp[r] *= s[r];
+    }
+#pragma unroll
+    for (int x = 0; x < C::FPT; ++x) { sf[x] = da_pack<T>(dp, x); pf[x] = da_pack<T>(s, x); }
+    constexpr int NK = C::FPT * C::MTK;
+    da_ring<NK + C::FPT * C::MT, 2>([&](int i) { return i < NK ? lq.frag_tr(tq, i / C::MTK, i % C::MTK) : lu.frag_tr(tu, (i - NK) / C::MT, (i - NK) % C::MT); },
+                                    [&](int i, const uint4 &x) {
+                                        if (i < NK) dk[i % C::MTK] = Da<T>::mma(x, sf[i / C::MTK], dk[i % C::MTK]);
+                                        else dv[(i - NK) % C::MT] = Da<T>::mma(x, pf[(i - NK) / C::MT], dv[(i - NK) % C::MT]);
+                                    });
+}
+
+__device__ __attribute__((aligned(16))) float da_no_row[4] = {-__builtin_huge_valf(), -__builtin_huge_valf(), 0.f, 0.f};     // statistics of a row that is not there
 __device__ __forceinline__ void da_copy4(const void *src, uint32_t lds_addr) {
     unsigned keep;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(lds_addr) : "memory");
 }
 
 template <typename T, int DK>
-__global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2) ? 2 : 1) void diff_attn_dkdv_kernel(const DiffArgs a) {
+__global__ __launch_bounds__((da_pair<T, DK>() ? 2 : 1) * kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) void diff_attn_dkdv_kernel(const DiffArgs a) {
     using C = DaCfg<T, DK>;
+    constexpr bool PAIR = da_pair<T, DK>();
+    constexpr int NT = (PAIR ? 2 : 1) * kDaThreads, NM = PAIR ? 1 : 2;              // maps of a wave
     constexpr int QB = 64, TILE = QB * C::ROWB, BUF = 2 * TILE + 4 * QB * 4;       // (BUF: a multiple of 512 bytes)
     extern __shared__ __attribute__((aligned(512))) char lds[];      // (512: DaLane)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
+    const int kw = wave & 3, map = wave >> 2;                 // 32 of the workgroup's keys; PAIR: the wave's map
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, rest = blockIdx.x / nbh, run = rest % a.kvruns, blk = rest / a.kvruns, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int len = da_len(a, b);
     const int64_t start = da_start(a, b);
     const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
-    const int kw0 = blk * 128 + wave * 32, key = kw0 + l32;
+    const int kw0 = blk * 128 + kw * 32, key = kw0 + l32;
     const int64_t mb = a.mask_b ? b : 0, bhn = (int64_t)a.B * a.H * a.N;
     const bool klive = key < len;
     bool seen = false;                                        // some row of this run sees the key; else zeros are written, whatever its lanes met
     const bool wlive = kw0 < len;
 
-    uint4 kf[2][C::NF], vf[C::NFV];
+    uint4 kf[NM][C::NF], vf[C::NFV];
     const T *kp = reinterpret_cast<const T *>(a.k) + b * a.ks[0] + (int64_t)key * a.ks[1] + hk * a.ks[2];
     const T *vp = reinterpret_cast<const T *>(a.v) + b * a.vs[0] + (int64_t)key * a.vs[1] + hk * a.vs[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < NM; ++t)
 #pragma unroll
         for (int f = 0; f < C::NF; ++f) {
             const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
-            kf[t][f] = klive && c < a.d ? *reinterpret_cast<const uint4 *>(kp + t * a.ks[3] + c) : make_uint4(0, 0, 0, 0);
+            kf[t][f] = klive && c < a.d ? *reinterpret_cast<const uint4 *>(kp + (PAIR ? map : t) * a.ks[3] + c) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
     for (int f = 0; f < C::NFV; ++f) {
@@ -1407,14 +1450,14 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
         vf[f] = klive && c < a.dv ? *reinterpret_cast<const uint4 *>(vp + c) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int f = 0; f < 2 * C::NF; ++f) da_pin(kf[f / C::NF][f % C::NF]);
+    for (int f = 0; f < NM * C::NF; ++f) da_pin(kf[f / C::NF][f % C::NF]);
 #pragma unroll
     for (int f = 0; f < C::NFV; ++f) da_pin(vf[f]);
-    da_f16v dk[2][C::MTK], dv[C::MT];
+    da_f16v dk[NM][C::MTK], dv[C::MT];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NM; ++t)
 #pragma unroll
             for (int x = 0; x < C::MTK; ++x) dk[t][x][r] = 0.f;
 #pragma unroll
@@ -1431,82 +1474,104 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
     const int u0 = (int)((int64_t)total * run / a.kvruns), u1 = (int)((int64_t)total * (run + 1) / a.kvruns);
     const int kt0 = blk * 2, kt1 = min(kt0 + 1, M64 - 1);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    DaLane<T, DK> ln;
+    DaLane<T, DK> ln, lq;
     ln.init(lane);
+    lq = ln;
+    if (PAIR) {                                               // the wave's map: 128 bytes on in a row of Q
+        lq.row ^= map << 7;
+        lq.tr[0] ^= map << 7;
+    }
     const bool full = a.d == DK && a.dv == C::DV;
-    DaCopy<T, DK, QB, kDaThreads> cq, cu;
+    DaCopy<T, DK, QB, NT> cq, cu;
     cq.init(reinterpret_cast<const T *>(a.q) + b * a.qs[0], a.qs[1], a.qs[3], a.d, true, tid);
     cu.init(reinterpret_cast<const T *>(a.du) + (int64_t)b * a.N * a.H * a.dv, (int64_t)a.H * a.dv, 0, a.dv, false, tid);
     // the mask's tiles along the queries as bit sets, 64 query blocks from qt_first + 64 base on (one per lane): workgroup and wave
     uint64_t need = ~0ull, mixed = 0, hide = 0;
     int base = -1;
-    auto next = [&](int u) {
-        while (u < u1 && a.tiles) {
-            const int x = u % per_head;
-            if (x >> 6 != base) {
-                base = x >> 6;
+    struct Block { int u, g, x; };                            // the run's block u: query block x of the group's head g
+    auto skip = [&](Block p, int n) {                         // n blocks on, and on to one that the mask does not leave out
+        for (;;) {
+            p.u += n;
+            p.x += n;
+            if (p.x >= per_head) {
+                p.x = 0;
+                ++p.g;
+            }
+            if (p.u >= u1 || !a.tiles) return p;
+            if (p.x >> 6 != base) {
+                base = p.x >> 6;
                 const int qt = qt_first + base * 64 + lane;
-                bool n = false, p = false, y = true;
+                bool n = false, m = false, y = true;
                 if (qt < N64) {
                     const uint8_t *tp = da_again().tiles + (mb * N64 + qt) * M64;
                     const int c = wlive ? tp[kw0 >> 6] : 2;
                     n = tp[kt0] != 2 || tp[kt1] != 2;
-                    p = c == 1;
+                    m = c == 1;
                     y = c == 2;
                 }
-                need = __ballot(n); mixed = __ballot(p); hide = __ballot(y);
+                need = __ballot(n); mixed = __ballot(m); hide = __ballot(y);
             }
-            const uint64_t m = need >> (x & 63);
-            if (m & 1) break;
-            u += m ? __builtin_ctzll(m) : min(64 - (x & 63), per_head - x);
+            const uint64_t m = need >> (p.x & 63);
+            if (m & 1) return p;
+            n = m ? __builtin_ctzll(m) : min(64 - (p.x & 63), per_head - p.x);
         }
-        return u;
     };
-    auto code_of = [&](int u) {
-        if (!a.tiles || u >= u1) return 0;
-        const int x = u % per_head & 63;
+    auto code_of = [&](const Block &p) {
+        if (!a.tiles || p.u >= u1) return 0;
+        const int x = p.x & 63;
         return (int)((mixed >> x) & 1 ? 1 : (hide >> x) & 1 ? 2 : 0);
     };
-    auto bits = [&](int u) { return klive ? da_again().colbits[(mb * a.M + key) * N64 + qt_first + u % per_head] : 0ull; };
-    auto row_lse = [&](int u) {                               // lse of this lane's row of block u: +inf where it sees nothing or is not there
-        if (u >= u1) return INFINITY;
-        const int g = u / per_head, i = (qt_first + u - g * per_head) * QB + lane;
-        return i < a.N ? a.rowstat[((int64_t)b * a.H + hk * a.G + g) * a.N + i] : INFINITY;
+    auto bits = [&](const Block &p) { return klive ? da_again().colbits[(mb * a.M + key) * N64 + qt_first + p.x] : 0ull; };
+    const float *stat0 = a.rowstat + ((int64_t)b * a.H + hk * a.G) * a.N, *stat_w = stat0 + kw * bhn;       // of the group's first head; kw: which kind the wave copies
+    auto row_lse = [&](const Block &p) {                      // -lse of this lane's row of the block: -inf where it sees nothing or is not there
+        if (p.u >= u1) return -INFINITY;
+        const int i = (qt_first + p.x) * QB + lane;
+        return i < a.N ? stat0[p.g * a.N + i] : -INFINITY;
     };
-    const int64_t ldq = a.qs[1], ldh = a.qs[2], ldu = (int64_t)a.H * a.dv;
-    int at_i = 0, at_h = 0;                                   // query and head that the copies stand at
-    auto issue = [&](int u, int buf, float lse) {
-        const int g = u / per_head, i0 = (qt_first + u - g * per_head) * QB, head = hk * a.G + g, valid = a.N - i0;
-        const uint64_t rows = __ballot(lse != INFINITY);      // rows that see nothing: their queries may hold anything, zeros are copied
+    const int64_t step_q = QB * a.qs[1], step_u = QB * (int64_t)a.H * a.dv;
+    Block at{0, 0, 0};                                        // the block that the copies stand at, from the head's first query block that counts
+    cq.move((int64_t)qt_first * step_q + hk * a.G * a.qs[2]);
+    cu.move((int64_t)qt_first * step_u + hk * a.G * (int64_t)a.dv);
+    auto issue = [&](const Block &p, int buf, float lse) {
+        const int i0 = (qt_first + p.x) * QB, valid = a.N - i0;
+        const uint64_t rows = __ballot(lse != -INFINITY);     // rows that see nothing: their queries may hold anything, zeros are copied
         const uint32_t to = lds0 + buf * BUF;
-        cq.move((i0 - at_i) * ldq + (head - at_h) * ldh);
-        cu.move((i0 - at_i) * ldu + (head - at_h) * (int64_t)a.dv);
-        at_i = i0;
-        at_h = head;
+        if (p.g == at.g && p.x == at.x + 1) {
+            cq.move(step_q);
+            cu.move(step_u);
+        } else {
+            const DiffArgs &e = da_again();
+            cq.move((p.x - at.x) * step_q + (p.g - at.g) * e.qs[2]);
+            cu.move((p.x - at.x) * step_u + (p.g - at.g) * (int64_t)e.dv);
+        }
+        at = p;
         cq.run(to + wave * 1024, valid, rows, rows == ~0ull, full);
         cu.run(to + TILE + wave * 1024, valid, rows, rows == ~0ull, full);
-        const float *sp = i0 + lane < a.N ? a.rowstat + wave * bhn + ((int64_t)b * a.H + head) * a.N + i0 + lane : da_no_row + wave;     // wave = which statistic
-        da_copy4(sp, __builtin_amdgcn_readfirstlane(to + 2 * TILE + wave * QB * 4));
+        if (!PAIR || map == 0)
+            da_copy4(lane < valid ? stat_w + (p.g * a.N + i0 + lane) : da_no_row + kw, __builtin_amdgcn_readfirstlane(to + 2 * TILE + kw * QB * 4));
     };
-    int u = next(u0), buf = 0, g_now = -1, code = code_of(u);
+    Block now = skip(Block{u0, per_head ? u0 / per_head : 0, per_head ? u0 % per_head : 0}, 0);
+    int buf = 0, g_now = -1, code = code_of(now);
     float sign = 1.f;
-    uint64_t vis = code == 1 ? bits(u) : ~0ull;
-    if (u < u1) issue(u, 0, row_lse(u));
-    int un = next(u + 1), code_n = code_of(un);
-    float lse_n = row_lse(un);
-    while (u < u1) {
-        const int g = u / per_head, i0 = (qt_first + u - g * per_head) * QB;
-        if (g != g_now) {
-            sign = da_lambda(a, hk * a.G + g) < 0.f ? -1.f : 1.f;
-            g_now = g;
+    uint64_t vis = code == 1 ? bits(now) : ~0ull;
+    if (now.u < u1) issue(now, 0, row_lse(now));
+    Block then = skip(now, 1);
+    int code_n = code_of(then);
+    float lse_n = row_lse(then);
+    while (now.u < u1) {
+        const int i0 = (qt_first + now.x) * QB;
+        if (now.g != g_now) {
+            g_now = now.g;
+            sign = da_lambda(a, hk * a.G + g_now) < 0.f ? -1.f : 1.f;
         }
-        da_copies_done_barrier();                             // block u is there for every wave, and every wave is done with the buffer in front
+        da_copies_done_barrier();                             // the block is there for every wave, and every wave is done with the buffer in front
         da_pin(vis);
         da_pin(lse_n);
-        const int unn = next(un + 1), code_nn = code_of(unn);
-        const float lse_nn = row_lse(unn);                    // (one block ahead of its use: the rows that the next copies leave out)
-        const uint64_t vis_n = code_n == 1 && un < u1 ? bits(un) : ~0ull;
-        if (un < u1) issue(un, buf ^ 1, lse_n);
+        const Block third = skip(then, 1);
+        const int code_nn = code_of(third);
+        const float lse_nn = row_lse(third);                  // (one block ahead of its use: the rows that the next copies leave out)
+        const uint64_t vis_n = code_n == 1 && then.u < u1 ? bits(then) : ~0ull;
+        if (then.u < u1) issue(then, buf ^ 1, lse_n);
         if (wlive && code != 2) {
             const uint32_t tq = lds0 + buf * BUF, tu = tq + TILE, stat = tu + TILE;
 #pragma unroll 1
@@ -1521,10 +1586,13 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
                 }
                 seen = seen || v;
                 const uint32_t at = nt * 32 * C::ROWB;
-                da_dkdv_tile<T, DK>(a, dk, dv, kf, vf, sign, ln, tq + at, tu + at, stat + nt * 128, cut || code == 1, v, lane);
+                if constexpr (PAIR)
+                    da_dkdv_pair_tile<T, DK>(a.scale_log2e, dk[0], dv, kf[0], vf, map ? -sign : 1.f, lq, ln, tq + at, tu + at, stat + nt * 128 + map * 256, cut || code == 1, v, lane);
+                else
+                    da_dkdv_tile<T, DK>(a, dk, dv, kf, vf, sign, ln, tq + at, tu + at, stat + nt * 128, cut || code == 1, v, lane);
             }
         }
-        u = un; un = unn; lse_n = lse_nn;
+        now = then; then = third; lse_n = lse_nn;
         code = code_n; code_n = code_nn;
         vis = vis_n;
         buf ^= 1;
@@ -1535,15 +1603,17 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
     const float f = keep ? e.scale : 0.f;
     const int64_t k0 = (int64_t)b * e.M;
     const int w = 2 * e.d + e.dv;
-    auto out = [&](auto rows, auto dkv) {                     // dV, then dK, as whole rows; dkv(key): where the key's dK row starts, dV behind it or in its own tensor
+    auto put_dv = [&](auto rows, auto dkv) {                  // as whole rows; dkv(key, v): where the key's dK (dV) starts
 #pragma unroll
         for (int x = 0; x < C::MT; ++x)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
                 rows.put(l32, x * 32 + 8 * q4 + 4 * h2, keep ? dv[x][4 * q4] : 0.f, keep ? dv[x][4 * q4 + 1] : 0.f, keep ? dv[x][4 * q4 + 2] : 0.f, keep ? dv[x][4 * q4 + 3] : 0.f);
         rows.flush(lane, [&](int r, int c) { return kw0 + r < e.M && c < e.dv ? dkv(kw0 + r, 1) + c : nullptr; });
+    };
+    auto put_dk = [&](auto rows, auto dkv) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NM; ++t)
 #pragma unroll
             for (int x = 0; x < C::MTK; ++x)
 #pragma unroll
@@ -1554,18 +1624,46 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
                              keep ? dk[t][x][4 * q4 + 3] * f : 0.f);
                 }
         rows.flush(lane, [&](int r, int c) {
-            const int t = c / DK;
-            c -= t * DK;
+            const int t = PAIR ? map : c / DK;
+            if (!PAIR) c -= t * DK;
             return kw0 + r < e.M && c < e.d ? dkv(kw0 + r, 0) + t * e.d + c : nullptr;
         });
     };
-    if (e.kvpart) {
-        float *part = e.kvpart + (int64_t)run * e.B * e.M * e.Hk * w;
-        out(DaRowsOut<float, C::DV>{lds + wave * 32 * C::DV * 4}, [&](int key, int v) { return part + ((k0 + key) * e.Hk + hk) * w + v * 2 * e.d; });
+    auto part = [&](int key, int v) { return e.kvpart + ((int64_t)run * e.B * e.M * e.Hk + (k0 + key) * e.Hk + hk) * w + v * 2 * e.d; };
+    auto whole = [&](int key, int v) {
+        return v ? reinterpret_cast<T *>(e.dvv) + ((k0 + key) * e.Hk + hk) * e.dv : reinterpret_cast<T *>(e.dk) + ((k0 + key) * e.Hk + hk) * 2 * e.d;
+    };
+    char *own = lds + kw * 32 * C::DV * 4;
+    if constexpr (PAIR) {                                     // dV: the second map's waves hand theirs over; dK: every wave has its map's
+        da_u4v *other = reinterpret_cast<da_u4v *>(own) + lane;
+        if (map) {
+#pragma unroll
+            for (int x = 0; x < C::MT * 4; ++x) {
+                const int r = x % 4 * 4;
+                other[x * 64] = da_u4v{__float_as_uint(dv[x / 4][r]), __float_as_uint(dv[x / 4][r + 1]), __float_as_uint(dv[x / 4][r + 2]), __float_as_uint(dv[x / 4][r + 3])};
+            }
+        }
+        __syncthreads();
+        if (!map) {
+#pragma unroll
+            for (int x = 0; x < C::MT * 4; ++x) {
+                const da_u4v v = other[x * 64];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dv[x / 4][x % 4 * 4 + j] += __uint_as_float(v[j]);
+            }
+            if (e.kvpart) put_dv(DaRowsOut<float, C::DV>{own}, part);
+            else put_dv(DaRowsOut<T, C::DV>{own}, whole);
+        }
+        __syncthreads();
+        own = lds + wave * 32 * DK * 4;
+        if (e.kvpart) put_dk(DaRowsOut<float, DK>{own}, part);
+        else put_dk(DaRowsOut<T, DK>{own}, whole);
+    } else if (e.kvpart) {
+        put_dv(DaRowsOut<float, C::DV>{own}, part);
+        put_dk(DaRowsOut<float, C::DV>{own}, part);
     } else {
-        out(DaRowsOut<T, C::DV>{lds + wave * 32 * C::DV * C::ES}, [&](int key, int v) {
-            return v ? reinterpret_cast<T *>(e.dvv) + ((k0 + key) * e.Hk + hk) * e.dv : reinterpret_cast<T *>(e.dk) + ((k0 + key) * e.Hk + hk) * 2 * e.d;
-        });
+        put_dv(DaRowsOut<T, C::DV>{own}, whole);
+        put_dk(DaRowsOut<T, C::DV>{own}, whole);
     }
 }
 
@@ -1657,10 +1755,11 @@ static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <
         }                                                                                                                                                        \
         hipLaunchKernelGGL(K_, grid_, block_, by_, st_, DA_ARGS);                                                                                                \
     }
-#define DA_DISPATCH(KERNEL, GRID, ROWS16, ROWS32, MORE)                                                                                                                \
+#define DA_DISPATCH(KERNEL, GRID, ROWS16, ROWS32, MORE, WIDE)                                                                                                                \
     {                                                                                                                                                            \
         const int dk_ = diff_attn_size(a.d, a.dv);                                                                                                               \
-        const dim3 grid_(GRID), block_(kDaThreads);                                                                                                              \
+        const bool wide_ = (WIDE) && dk_ == 64 && shape[7] != 0;                                                                                                 \
+        const dim3 grid_(GRID), block_(wide_ ? 2 * kDaThreads : kDaThreads);                                                                                                              \
         hipStream_t st_ = (hipStream_t)stream;                                                                                                                   \
         if (shape[7] == 0) {                                                                                                                                     \
             if (dk_ == 16) DA_LAUNCH((KERNEL<float, 16>), (ROWS32) * 128 + (MORE))                                                                                        \
@@ -1712,7 +1811,7 @@ int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void 
     if (blocks > 0x7fffffff) return DFINE_E_BADARG;
     if (n == 0) {
         #define DA_ARGS a
-        DA_DISPATCH(diff_attn_fwd_kernel, (unsigned)blocks, 256, 128, 0)
+        DA_DISPATCH(diff_attn_fwd_kernel, (unsigned)blocks, 256, 128, 0, false)
 #undef DA_ARGS
         return check_launch();
     }
@@ -1720,7 +1819,7 @@ int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void 
     float4 *ml = reinterpret_cast<float4 *>(ws);
     float *part = n > 1 ? reinterpret_cast<float *>(reinterpret_cast<char *>(ws) + da_up(diff_attn_rows(a) * n * 16)) : nullptr;
 #define DA_ARGS a, n, part, ml
-    DA_DISPATCH(diff_attn_fwd_split_kernel, (unsigned)blocks, 512, dk_ == 64 ? 256 : 512, 0)
+    DA_DISPATCH(diff_attn_fwd_split_kernel, (unsigned)blocks, 512, dk_ == 64 ? 256 : 512, 0, false)
 #undef DA_ARGS
     if (int e = check_launch()) return e;
     if (n == 1) return DFINE_OK;
@@ -1805,13 +1904,13 @@ int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void 
     if (rows_ && dq) {
         const int64_t blocks = ((int64_t)a.N * a.G + 127) / 128 * a.B * a.Hk;
         if (blocks > 0x7fffffff) return DFINE_E_BADARG;
-        DA_DISPATCH(diff_attn_dq_kernel, (unsigned)blocks, 256, 128, 0)
+        DA_DISPATCH(diff_attn_dq_kernel, (unsigned)blocks, 256, 128, 0, false)
         if (int e = check_launch()) return e;
     }
     if (keys_ && dk) {
         const int64_t blocks = ((int64_t)a.M + 127) / 128 * a.B * a.Hk * a.kvruns;
         if (blocks > 0x7fffffff) return DFINE_E_BADARG;
-        DA_DISPATCH(diff_attn_dkdv_kernel, (unsigned)blocks, 256, 256, 2 * 4 * 64 * 4)
+        DA_DISPATCH(diff_attn_dkdv_kernel, (unsigned)blocks, 256, 256, 2 * 4 * 64 * 4, true)
         if (int e = check_launch()) return e;
         if (a.kvruns > 1) {
             const int64_t grid = ((int64_t)a.B * a.M * a.Hk * (2 * a.d + a.dv) / 4 + 255) / 256;
