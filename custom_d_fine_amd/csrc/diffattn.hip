@@ -48,7 +48,7 @@ struct DiffArgs {
     const void *dy;
     int64_t dys[3];
     void *du, *dq, *dk, *dvv;
-    float *rowstat;                             // [4][B, H, N]: -lse_0 / c, -(lse_1 - log2 |l|) / c, -D_0, sign(l) (D_1 - D_0) or -D_1 (da_pair), c = scale_log2e
+    float *rowstat;                             // [4][B, H, N]: -lse_0 / c, -(lse_1 - log2 |l|) / c, -D_0, sign(l) (D_1 - D_0), c = scale_log2e (diff_attn_prep_kernel)
     float *lpart, *wpart;                       // per workgroup of the first kernel: sum of D_1, sums of dg
     float *kvpart;                              // dK | dV sums of each run of the rows, fp32 [runs][B, M, Hk, 2 d + dv] (null: one run)
     int kvruns;
@@ -77,9 +77,6 @@ template <typename T, int DK> struct DaCfg {
                          MTK = DK / 32 ? DK / 32 : 1, FPT = 32 / Da<T>::KPF;      // fragments per 32 keys
     static_assert(DV % 32 == 0, "a value tile is 32 channels");
 };
-
-// dK and dV by two waves per 32 keys, one map each (diff_attn_dkdv_kernel)
-template <typename T, int DK> constexpr bool da_pair() { return DK == 64 && sizeof(T) == 2; }
 
 // f(row): a b128 read serves 16 lanes at a time (rows 16 apart in some order, one u), a transposed read 32 lanes (4 rows from a multiple of 4 on, 4 units from a
 // multiple of 4 on): f takes all values over 16 rows and, in its bits from 2 on, over 4 (256 bytes = all banks; rows shorter than that share them).
@@ -223,23 +220,41 @@ __device__ __forceinline__ float da_wave_sum(float v) {
 }
 
 // exp(x0 . x1) and exp(x2 . x3) of a head, by a whole wave: one channel per lane
-__device__ __forceinline__ void da_lambda_parts(const DiffArgs &a, int h, float &e1, float &e2) {
+__device__ __forceinline__ float4 da_lambda_vectors(const DiffArgs &a, int h) {
     const int j = threadIdx.x & 63;
     const int64_t st = (int64_t)a.lam_heads * a.d, o = (a.lam_heads == 1 ? 0 : (int64_t)h * a.d) + j;
-    float s1 = 0.f, s2 = 0.f;
-    if (j < a.d) {
-        const float x0 = da_load1(a.lam, o, a.lam_bf16), x1 = da_load1(a.lam, st + o, a.lam_bf16), x2 = da_load1(a.lam, 2 * st + o, a.lam_bf16),
-                    x3 = da_load1(a.lam, 3 * st + o, a.lam_bf16);
-        s1 = x0 * x1;
-        s2 = x2 * x3;
+    if (j >= a.d) return make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.lam_bf16) {
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(a.lam) + o;
+        return make_float4(bf16_to_f32(p[0]), bf16_to_f32(p[st]), bf16_to_f32(p[2 * st]), bf16_to_f32(p[3 * st]));
     }
-    e1 = expf(da_wave_sum(s1));
-    e2 = expf(da_wave_sum(s2));
+    const float *p = reinterpret_cast<const float *>(a.lam) + o;
+    return make_float4(p[0], p[st], p[2 * st], p[3 * st]);
 }
-__device__ __forceinline__ float da_lambda(const DiffArgs &a, int h) {
+__device__ __forceinline__ void da_lambda_parts(const float4 &x, float &e1, float &e2) {
+    e1 = expf(da_wave_sum(x.x * x.y));
+    e2 = expf(da_wave_sum(x.z * x.w));
+}
+__device__ __forceinline__ float da_lambda(const DiffArgs &a, const float4 &x) {
     float e1, e2;
-    da_lambda_parts(a, h, e1, e2);
+    da_lambda_parts(x, e1, e2);
     return e1 - e2 + a.init;
+}
+__device__ __forceinline__ float da_lambda(const DiffArgs &a, int h) { return da_lambda(a, da_lambda_vectors(a, h)); }
+// (1 - init) g of N channels from c0 on (1 without a norm), channels from dv on 0: one test of the type, all loads at once
+template <int N> __device__ __forceinline__ void da_weights(const DiffArgs &a, int c0, float *w) {
+    if (!a.weight) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = c0 + j < a.dv ? 1.f : 0.f;
+    } else if (a.w_bf16) {
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(a.weight) + c0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = c0 + j < a.dv ? bf16_to_f32(p[j]) * a.post : 0.f;
+    } else {
+        const float *p = reinterpret_cast<const float *>(a.weight) + c0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = c0 + j < a.dv ? p[j] * a.post : 0.f;
+    }
 }
 // l of each lane's own head, for a wave whose rows start at w0: its rows' heads are min(G, 32) in a row (a whole wave calls this)
 __device__ __forceinline__ float da_lambda_rows(const DiffArgs &a, int hk, int w0, int head) {
@@ -595,7 +610,8 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     st.init();
 #pragma unroll
     for (int f = 0; f < 2 * C::NF; ++f) da_pin(qf[f / C::NF][f % C::NF]);
-    __shared__ float sLam[128];                               // (not held in registers over the loop)
+    __shared__ __attribute__((aligned(16))) float sLam[128], sW[C::DV];         // (not held in registers over the loop)
+    if (tid < C::DV) da_weights<1>(a, tid, sW + tid);
     {
         const float l = da_lambda_rows(a, hk, blk0 + wave * 32, w.head);
         if (h2 == 0) sLam[wave * 32 + l32] = l;
@@ -662,11 +678,8 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
             const int c = x * 32 + 8 * q4 + 4 * h2;
-            float g[4] = {1.f, 1.f, 1.f, 1.f};
-            if (e.weight && c < e.dv)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) g[j] = da_load1(e.weight, c + j, e.w_bf16) * e.post * rn;
-            rows.put(l32, c, st.o[0][x][4 * q4] * g[0], st.o[0][x][4 * q4 + 1] * g[1], st.o[0][x][4 * q4 + 2] * g[2], st.o[0][x][4 * q4 + 3] * g[3]);
+            const float4 g = *reinterpret_cast<const float4 *>(sW + c);
+            rows.put(l32, c, st.o[0][x][4 * q4] * g.x * rn, st.o[0][x][4 * q4 + 1] * g.y * rn, st.o[0][x][4 * q4 + 2] * g.z * rn, st.o[0][x][4 * q4 + 3] * g.w * rn);
         }
     to(e.out);
     if (!e.o2) return;
@@ -692,7 +705,8 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
 
 // One row of the result from its two maps' sums in plain order: LPR neighbouring lanes of NE channels each (c0: the lane's first), O normalised
 template <typename T, int NE, int LPR>
-__device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, int head, float lam, int c0, float *o0, float *o1, float lse0, float lse1, bool first) {
+__device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, int head, float lam, int c0, const float *g, float *o0, float *o1, float lse0,
+                                              float lse1, bool first) {
     float ss = 0.f, us = 0.f;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
@@ -709,11 +723,7 @@ __device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, i
     for (int j = 0; j < NE; j += 4) {
         const int c = c0 + j;
         if (c >= a.dv) continue;
-        float g[4] = {1.f, 1.f, 1.f, 1.f};
-        if (a.weight)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) g[x] = da_load1(a.weight, c + x, a.w_bf16) * a.post * rn;
-        da_store4(reinterpret_cast<T *>(a.out) + orow + c, o0[j] * g[0], o0[j + 1] * g[1], o0[j + 2] * g[2], o0[j + 3] * g[3]);
+        da_store4(reinterpret_cast<T *>(a.out) + orow + c, o0[j] * g[j] * rn, o0[j + 1] * g[j + 1] * rn, o0[j + 2] * g[j + 2] * rn, o0[j + 3] * g[j + 3] * rn);
         if (a.o2) {
             if (a.weight) da_store4(reinterpret_cast<T *>(a.u) + orow + c, o0[j], o0[j + 1], o0[j + 2], o0[j + 3]);
             da_store4(reinterpret_cast<T *>(a.o2) + orow + c, o1[j] - beta * o0[j], o1[j + 1] - beta * o0[j + 1], o1[j + 2] - beta * o0[j + 2], o1[j + 3] - beta * o0[j + 3]);
@@ -854,6 +864,8 @@ __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff
     const int r = tid >> 3, c0 = (tid & 7) * NE;
     const int row = blk * 32 + r;
     if (row >= R) return;
+    float g[NE];
+    if (nsplit == 1) da_weights<NE>(a, c0, g);
     float o[2][NE], lse[2], mx[2], sum[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -882,7 +894,7 @@ __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff
 #pragma unroll
             for (int j = 0; j < NE; ++j) o[x][j] *= inv;
         }
-        da_finish_row<T, NE, 8>(a, b, i, head, sLam[r], c0, o[0], o[1], lse[0], lse[1], (tid & 7) == 0);
+        da_finish_row<T, NE, 8>(a, b, i, head, sLam[r], c0, g, o[0], o[1], lse[0], lse[1], (tid & 7) == 0);
         return;
     }
     const int64_t at = ((int64_t)bh * R + row) * nsplit + sp;
@@ -903,7 +915,9 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
     if (at >= (int64_t)R * a.B * a.Hk) return;
     const int bh = (int)(at / R), b = bh / a.Hk, hk = bh - b * a.Hk;
     const int row = (int)(at - (int64_t)bh * R), i = da_div_g(a, row), head = hk * a.G + row - i * a.G;
-    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, o[2][NE];
+    const float4 vectors = da_lambda_vectors(a, head);        // (asked for in front of the sums)
+    float g[NE], mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, o[2][NE];
+    da_weights<NE>(a, c0, g);
 #pragma unroll
     for (int j = 0; j < NE; ++j) o[0][j] = o[1][j] = 0.f;
 #pragma unroll 2
@@ -927,7 +941,7 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
             }
         }
     }
-    const float lam = da_lambda(a, head);
+    const float lam = da_lambda(a, vectors);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {                             // the 8 groups, in order of their distance
         float m = mx[x];
@@ -952,7 +966,7 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
 #pragma unroll
         for (int j = 0; j < NE; ++j) o[x][j] *= inv;
     }
-    da_finish_row<T, NE, 8>(a, b, i, head, lam, c0, o[0], o[1], da_lse(mx[0], sum[0]), da_lse(mx[1], sum[1]), lane == 0);
+    da_finish_row<T, NE, 8>(a, b, i, head, lam, c0, g, o[0], o[1], da_lse(mx[0], sum[0]), da_lse(mx[1], sum[1]), lane == 0);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -1011,11 +1025,9 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
     const bool ok = c < a.dv;
     const float lam = da_lambda(a, head), log2l = log2f(fabsf(lam)), sign = lam < 0.f ? -1.f : 1.f, inv_c = 1.f / a.scale_log2e;
     float w[8], dw[8], dsum = 0.f;
+    da_weights<8>(a, c, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        w[j] = !ok ? 0.f : a.weight ? a.post * da_load1(a.weight, c + j, a.w_bf16) : 1.f;
-        dw[j] = 0.f;
-    }
+    for (int j = 0; j < 8; ++j) dw[j] = 0.f;
     const int64_t rows = (int64_t)a.B * a.N, bhn = rows * a.H;
     for (int64_t r = (int64_t)run * RW + rr; r < rows; r += (int64_t)nrun * RW) {
         const int b = (int)(r / a.N), i = (int)(r - (int64_t)b * a.N);
@@ -1076,7 +1088,7 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
             a.rowstat[at] = -lse0 * inv_c;
             a.rowstat[bhn + at] = (log2l - lse1) * inv_c;
             a.rowstat[2 * bhn + at] = -dd0;
-            a.rowstat[3 * bhn + at] = da_pair<T, LPR * 4>() ? -(d1 + e2r) : (d1 + e2r - dd0) * sign;
+            a.rowstat[3 * bhn + at] = (d1 + e2r - dd0) * sign;
             dsum += d1;
         }
     }
@@ -1114,7 +1126,7 @@ __global__ __launch_bounds__(1024) void diff_attn_param_kernel(const DiffArgs a,
         v = da_wave_sum(v);
         if ((tid & 63) == 0) s[0][tid >> 6] = v;
         float e1, e2;
-        da_lambda_parts(a, h0, e1, e2);
+        da_lambda_parts(da_lambda_vectors(a, h0), e1, e2);
         __syncthreads();
         float dl = 0.f;
 #pragma unroll
@@ -1240,7 +1252,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         lse[t] = w.live ? a.rowstat[t * bhn + at] * -a.scale_log2e : INFINITY;
         dl[t] = w.live ? a.rowstat[(2 + t) * bhn + at] : 0.f;
     }
-    dl[1] = da_pair<T, DK>() ? -sign * dl[1] : dl[1] - sign * dl[0];
+    dl[1] -= sign * dl[0];
     dl[0] = -dl[0];
     const bool empty = lse[0] == INFINITY;                    // sees no key: its query may hold anything
 #pragma unroll
@@ -1374,41 +1386,6 @@ __device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[Da
                                     });
 }
 
-// One map's part of it (da_pair): f = 1 for map 0, -sign(l) for map 1
-template <typename T, int DK>
-__device__ __forceinline__ void da_dkdv_pair_tile(float c, da_f16v *dk, da_f16v *dv, const uint4 *kf, const uint4 *vf, float f, const DaLane<T, DK> &lq, const DaLane<T, DK> &lu,
-                                                  uint32_t tq, uint32_t tu, uint32_t stat, bool masked, uint32_t vis, int lane) {
-    using C = DaCfg<T, DK>;
-    const int h2 = lane >> 5;
-    da_f16v dp, s;
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-        const da_u4v x = *(da_lds_u4)(uintptr_t)(stat + 512 + (8 * q4 + 4 * h2) * 4), y = *(da_lds_u4)(uintptr_t)(stat + (8 * q4 + 4 * h2) * 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { dp[4 * q4 + j] = __uint_as_float(x[j]); s[4 * q4 + j] = __uint_as_float(y[j]); }
-    }
-    da_ring<C::NFV + C::NF, 2>([&](int i) { return i < C::NFV ? lu.frag(tu, i) : lq.frag(tq, i - C::NFV); },
-                               [&](int i, const uint4 &x) {
-                                   if (i < C::NFV) dp = Da<T>::mma(x, vf[i], dp);
-                                   else s = Da<T>::mma(x, kf[i - C::NFV], s);
-                               });
-    if (masked) da_hide(s, vis >> (4 * h2));
-    uint4 sf[C::FPT], pf[C::FPT];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        s[r] = da_exp2(s[r] * c) * f;
-        dp[r] *= s[r];
-    }
-#pragma unroll
-    for (int x = 0; x < C::FPT; ++x) { sf[x] = da_pack<T>(dp, x); pf[x] = da_pack<T>(s, x); }
-    constexpr int NK = C::FPT * C::MTK;
-    da_ring<NK + C::FPT * C::MT, 2>([&](int i) { return i < NK ? lq.frag_tr(tq, i / C::MTK, i % C::MTK) : lu.frag_tr(tu, (i - NK) / C::MT, (i - NK) % C::MT); },
-                                    [&](int i, const uint4 &x) {
-                                        if (i < NK) dk[i % C::MTK] = Da<T>::mma(x, sf[i / C::MTK], dk[i % C::MTK]);
-                                        else dv[(i - NK) % C::MT] = Da<T>::mma(x, pf[(i - NK) / C::MT], dv[(i - NK) % C::MT]);
-                                    });
-}
-
 __device__ __attribute__((aligned(16))) float da_no_row[4] = {-__builtin_huge_valf(), -__builtin_huge_valf(), 0.f, 0.f};     // statistics of a row that is not there
 __device__ __forceinline__ void da_copy4(const void *src, uint32_t lds_addr) {
     unsigned keep;
@@ -1416,33 +1393,30 @@ __device__ __forceinline__ void da_copy4(const void *src, uint32_t lds_addr) {
 }
 
 template <typename T, int DK>
-__global__ __launch_bounds__((da_pair<T, DK>() ? 2 : 1) * kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) void diff_attn_dkdv_kernel(const DiffArgs a) {
+__global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2) ? 2 : 1) void diff_attn_dkdv_kernel(const DiffArgs a) {
     using C = DaCfg<T, DK>;
-    constexpr bool PAIR = da_pair<T, DK>();
-    constexpr int NT = (PAIR ? 2 : 1) * kDaThreads, NM = PAIR ? 1 : 2;              // maps of a wave
     constexpr int QB = 64, TILE = QB * C::ROWB, BUF = 2 * TILE + 4 * QB * 4;       // (BUF: a multiple of 512 bytes)
     extern __shared__ __attribute__((aligned(512))) char lds[];      // (512: DaLane)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h2 = lane >> 5, l32 = lane & 31;
-    const int kw = wave & 3, map = wave >> 2;                 // 32 of the workgroup's keys; PAIR: the wave's map
     const int nbh = a.B * a.Hk, bh = blockIdx.x % nbh, rest = blockIdx.x / nbh, run = rest % a.kvruns, blk = rest / a.kvruns, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int len = da_len(a, b);
     const int64_t start = da_start(a, b);
     const int M64 = (a.M + 63) >> 6, N64 = (a.N + 63) >> 6;
-    const int kw0 = blk * 128 + kw * 32, key = kw0 + l32;
+    const int kw0 = blk * 128 + wave * 32, key = kw0 + l32;
     const int64_t mb = a.mask_b ? b : 0, bhn = (int64_t)a.B * a.H * a.N;
     const bool klive = key < len;
     bool seen = false;                                        // some row of this run sees the key; else zeros are written, whatever its lanes met
     const bool wlive = kw0 < len;
 
-    uint4 kf[NM][C::NF], vf[C::NFV];
+    uint4 kf[2][C::NF], vf[C::NFV];
     const T *kp = reinterpret_cast<const T *>(a.k) + b * a.ks[0] + (int64_t)key * a.ks[1] + hk * a.ks[2];
     const T *vp = reinterpret_cast<const T *>(a.v) + b * a.vs[0] + (int64_t)key * a.vs[1] + hk * a.vs[2];
 #pragma unroll
-    for (int t = 0; t < NM; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int f = 0; f < C::NF; ++f) {
             const int c = f * Da<T>::KPF + h2 * (Da<T>::KPF / 2);
-            kf[t][f] = klive && c < a.d ? *reinterpret_cast<const uint4 *>(kp + (PAIR ? map : t) * a.ks[3] + c) : make_uint4(0, 0, 0, 0);
+            kf[t][f] = klive && c < a.d ? *reinterpret_cast<const uint4 *>(kp + t * a.ks[3] + c) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
     for (int f = 0; f < C::NFV; ++f) {
@@ -1450,14 +1424,14 @@ __global__ __launch_bounds__((da_pair<T, DK>() ? 2 : 1) * kDaThreads, DK == 16 |
         vf[f] = klive && c < a.dv ? *reinterpret_cast<const uint4 *>(vp + c) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int f = 0; f < NM * C::NF; ++f) da_pin(kf[f / C::NF][f % C::NF]);
+    for (int f = 0; f < 2 * C::NF; ++f) da_pin(kf[f / C::NF][f % C::NF]);
 #pragma unroll
     for (int f = 0; f < C::NFV; ++f) da_pin(vf[f]);
-    da_f16v dk[NM][C::MTK], dv[C::MT];
+    da_f16v dk[2][C::MTK], dv[C::MT];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
 #pragma unroll
-        for (int t = 0; t < NM; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int x = 0; x < C::MTK; ++x) dk[t][x][r] = 0.f;
 #pragma unroll
@@ -1474,15 +1448,10 @@ __global__ __launch_bounds__((da_pair<T, DK>() ? 2 : 1) * kDaThreads, DK == 16 |
     const int u0 = (int)((int64_t)total * run / a.kvruns), u1 = (int)((int64_t)total * (run + 1) / a.kvruns);
     const int kt0 = blk * 2, kt1 = min(kt0 + 1, M64 - 1);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    DaLane<T, DK> ln, lq;
+    DaLane<T, DK> ln;
     ln.init(lane);
-    lq = ln;
-    if (PAIR) {                                               // the wave's map: 128 bytes on in a row of Q
-        lq.row ^= map << 7;
-        lq.tr[0] ^= map << 7;
-    }
     const bool full = a.d == DK && a.dv == C::DV;
-    DaCopy<T, DK, QB, NT> cq, cu;
+    DaCopy<T, DK, QB, kDaThreads> cq, cu;
     cq.init(reinterpret_cast<const T *>(a.q) + b * a.qs[0], a.qs[1], a.qs[3], a.d, true, tid);
     cu.init(reinterpret_cast<const T *>(a.du) + (int64_t)b * a.N * a.H * a.dv, (int64_t)a.H * a.dv, 0, a.dv, false, tid);
     // the mask's tiles along the queries as bit sets, 64 query blocks from qt_first + 64 base on (one per lane): workgroup and wave
@@ -1522,7 +1491,7 @@ __global__ __launch_bounds__((da_pair<T, DK>() ? 2 : 1) * kDaThreads, DK == 16 |
         return (int)((mixed >> x) & 1 ? 1 : (hide >> x) & 1 ? 2 : 0);
     };
     auto bits = [&](const Block &p) { return klive ? da_again().colbits[(mb * a.M + key) * N64 + qt_first + p.x] : 0ull; };
-    const float *stat0 = a.rowstat + ((int64_t)b * a.H + hk * a.G) * a.N, *stat_w = stat0 + kw * bhn;       // of the group's first head; kw: which kind the wave copies
+    const float *stat0 = a.rowstat + ((int64_t)b * a.H + hk * a.G) * a.N, *stat_w = stat0 + wave * bhn;     // of the group's first head; the wave's kind
     auto row_lse = [&](const Block &p) {                      // -lse of this lane's row of the block: -inf where it sees nothing or is not there
         if (p.u >= u1) return -INFINITY;
         const int i = (qt_first + p.x) * QB + lane;
@@ -1547,8 +1516,7 @@ __global__ __launch_bounds__((da_pair<T, DK>() ? 2 : 1) * kDaThreads, DK == 16 |
         at = p;
         cq.run(to + wave * 1024, valid, rows, rows == ~0ull, full);
         cu.run(to + TILE + wave * 1024, valid, rows, rows == ~0ull, full);
-        if (!PAIR || map == 0)
-            da_copy4(lane < valid ? stat_w + (p.g * a.N + i0 + lane) : da_no_row + kw, __builtin_amdgcn_readfirstlane(to + 2 * TILE + kw * QB * 4));
+        da_copy4(lane < valid ? stat_w + (p.g * a.N + i0 + lane) : da_no_row + wave, __builtin_amdgcn_readfirstlane(to + 2 * TILE + wave * QB * 4));
     };
     Block now = skip(Block{u0, per_head ? u0 / per_head : 0, per_head ? u0 % per_head : 0}, 0);
     int buf = 0, g_now = -1, code = code_of(now);
@@ -1586,10 +1554,7 @@ __global__ __launch_bounds__((da_pair<T, DK>() ? 2 : 1) * kDaThreads, DK == 16 |
                 }
                 seen = seen || v;
                 const uint32_t at = nt * 32 * C::ROWB;
-                if constexpr (PAIR)
-                    da_dkdv_pair_tile<T, DK>(a.scale_log2e, dk[0], dv, kf[0], vf, map ? -sign : 1.f, lq, ln, tq + at, tu + at, stat + nt * 128 + map * 256, cut || code == 1, v, lane);
-                else
-                    da_dkdv_tile<T, DK>(a, dk, dv, kf, vf, sign, ln, tq + at, tu + at, stat + nt * 128, cut || code == 1, v, lane);
+                da_dkdv_tile<T, DK>(a, dk, dv, kf, vf, sign, ln, tq + at, tu + at, stat + nt * 128, cut || code == 1, v, lane);
             }
         }
         now = then; then = third; lse_n = lse_nn;
@@ -1603,17 +1568,15 @@ __global__ __launch_bounds__((da_pair<T, DK>() ? 2 : 1) * kDaThreads, DK == 16 |
     const float f = keep ? e.scale : 0.f;
     const int64_t k0 = (int64_t)b * e.M;
     const int w = 2 * e.d + e.dv;
-    auto put_dv = [&](auto rows, auto dkv) {                  // as whole rows; dkv(key, v): where the key's dK (dV) starts
+    auto out = [&](auto rows, auto dkv) {                     // dV, then dK, as whole rows; dkv(key): where the key's dK row starts, dV behind it or in its own tensor
 #pragma unroll
         for (int x = 0; x < C::MT; ++x)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
                 rows.put(l32, x * 32 + 8 * q4 + 4 * h2, keep ? dv[x][4 * q4] : 0.f, keep ? dv[x][4 * q4 + 1] : 0.f, keep ? dv[x][4 * q4 + 2] : 0.f, keep ? dv[x][4 * q4 + 3] : 0.f);
         rows.flush(lane, [&](int r, int c) { return kw0 + r < e.M && c < e.dv ? dkv(kw0 + r, 1) + c : nullptr; });
-    };
-    auto put_dk = [&](auto rows, auto dkv) {
 #pragma unroll
-        for (int t = 0; t < NM; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int x = 0; x < C::MTK; ++x)
 #pragma unroll
@@ -1624,46 +1587,18 @@ __global__ __launch_bounds__((da_pair<T, DK>() ? 2 : 1) * kDaThreads, DK == 16 |
                              keep ? dk[t][x][4 * q4 + 3] * f : 0.f);
                 }
         rows.flush(lane, [&](int r, int c) {
-            const int t = PAIR ? map : c / DK;
-            if (!PAIR) c -= t * DK;
+            const int t = c / DK;
+            c -= t * DK;
             return kw0 + r < e.M && c < e.d ? dkv(kw0 + r, 0) + t * e.d + c : nullptr;
         });
     };
-    auto part = [&](int key, int v) { return e.kvpart + ((int64_t)run * e.B * e.M * e.Hk + (k0 + key) * e.Hk + hk) * w + v * 2 * e.d; };
-    auto whole = [&](int key, int v) {
-        return v ? reinterpret_cast<T *>(e.dvv) + ((k0 + key) * e.Hk + hk) * e.dv : reinterpret_cast<T *>(e.dk) + ((k0 + key) * e.Hk + hk) * 2 * e.d;
-    };
-    char *own = lds + kw * 32 * C::DV * 4;
-    if constexpr (PAIR) {                                     // dV: the second map's waves hand theirs over; dK: every wave has its map's
-        da_u4v *other = reinterpret_cast<da_u4v *>(own) + lane;
-        if (map) {
-#pragma unroll
-            for (int x = 0; x < C::MT * 4; ++x) {
-                const int r = x % 4 * 4;
-                other[x * 64] = da_u4v{__float_as_uint(dv[x / 4][r]), __float_as_uint(dv[x / 4][r + 1]), __float_as_uint(dv[x / 4][r + 2]), __float_as_uint(dv[x / 4][r + 3])};
-            }
-        }
-        __syncthreads();
-        if (!map) {
-#pragma unroll
-            for (int x = 0; x < C::MT * 4; ++x) {
-                const da_u4v v = other[x * 64];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) dv[x / 4][x % 4 * 4 + j] += __uint_as_float(v[j]);
-            }
-            if (e.kvpart) put_dv(DaRowsOut<float, C::DV>{own}, part);
-            else put_dv(DaRowsOut<T, C::DV>{own}, whole);
-        }
-        __syncthreads();
-        own = lds + wave * 32 * DK * 4;
-        if (e.kvpart) put_dk(DaRowsOut<float, DK>{own}, part);
-        else put_dk(DaRowsOut<T, DK>{own}, whole);
-    } else if (e.kvpart) {
-        put_dv(DaRowsOut<float, C::DV>{own}, part);
-        put_dk(DaRowsOut<float, C::DV>{own}, part);
+    if (e.kvpart) {
+        float *part = e.kvpart + (int64_t)run * e.B * e.M * e.Hk * w;
+        out(DaRowsOut<float, C::DV>{lds + wave * 32 * C::DV * 4}, [&](int key, int v) { return part + ((k0 + key) * e.Hk + hk) * w + v * 2 * e.d; });
     } else {
-        put_dv(DaRowsOut<T, C::DV>{own}, whole);
-        put_dk(DaRowsOut<T, C::DV>{own}, whole);
+        out(DaRowsOut<T, C::DV>{lds + wave * 32 * C::DV * C::ES}, [&](int key, int v) {
+            return v ? reinterpret_cast<T *>(e.dvv) + ((k0 + key) * e.Hk + hk) * e.dv : reinterpret_cast<T *>(e.dk) + ((k0 + key) * e.Hk + hk) * 2 * e.d;
+        });
     }
 }
 
@@ -1755,11 +1690,10 @@ static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <
         }                                                                                                                                                        \
         hipLaunchKernelGGL(K_, grid_, block_, by_, st_, DA_ARGS);                                                                                                \
     }
-#define DA_DISPATCH(KERNEL, GRID, ROWS16, ROWS32, MORE, WIDE)                                                                                                                \
+#define DA_DISPATCH(KERNEL, GRID, ROWS16, ROWS32, MORE)                                                                                                                \
     {                                                                                                                                                            \
         const int dk_ = diff_attn_size(a.d, a.dv);                                                                                                               \
-        const bool wide_ = (WIDE) && dk_ == 64 && shape[7] != 0;                                                                                                 \
-        const dim3 grid_(GRID), block_(wide_ ? 2 * kDaThreads : kDaThreads);                                                                                                              \
+        const dim3 grid_(GRID), block_(kDaThreads);                                                                                                              \
         hipStream_t st_ = (hipStream_t)stream;                                                                                                                   \
         if (shape[7] == 0) {                                                                                                                                     \
             if (dk_ == 16) DA_LAUNCH((KERNEL<float, 16>), (ROWS32) * 128 + (MORE))                                                                                        \
@@ -1811,7 +1745,7 @@ int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void 
     if (blocks > 0x7fffffff) return DFINE_E_BADARG;
     if (n == 0) {
         #define DA_ARGS a
-        DA_DISPATCH(diff_attn_fwd_kernel, (unsigned)blocks, 256, 128, 0, false)
+        DA_DISPATCH(diff_attn_fwd_kernel, (unsigned)blocks, 256, 128, 0)
 #undef DA_ARGS
         return check_launch();
     }
@@ -1819,7 +1753,7 @@ int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void 
     float4 *ml = reinterpret_cast<float4 *>(ws);
     float *part = n > 1 ? reinterpret_cast<float *>(reinterpret_cast<char *>(ws) + da_up(diff_attn_rows(a) * n * 16)) : nullptr;
 #define DA_ARGS a, n, part, ml
-    DA_DISPATCH(diff_attn_fwd_split_kernel, (unsigned)blocks, 512, dk_ == 64 ? 256 : 512, 0, false)
+    DA_DISPATCH(diff_attn_fwd_split_kernel, (unsigned)blocks, 512, dk_ == 64 ? 256 : 512, 0)
 #undef DA_ARGS
     if (int e = check_launch()) return e;
     if (n == 1) return DFINE_OK;
@@ -1904,13 +1838,13 @@ int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void 
     if (rows_ && dq) {
         const int64_t blocks = ((int64_t)a.N * a.G + 127) / 128 * a.B * a.Hk;
         if (blocks > 0x7fffffff) return DFINE_E_BADARG;
-        DA_DISPATCH(diff_attn_dq_kernel, (unsigned)blocks, 256, 128, 0, false)
+        DA_DISPATCH(diff_attn_dq_kernel, (unsigned)blocks, 256, 128, 0)
         if (int e = check_launch()) return e;
     }
     if (keys_ && dk) {
         const int64_t blocks = ((int64_t)a.M + 127) / 128 * a.B * a.Hk * a.kvruns;
         if (blocks > 0x7fffffff) return DFINE_E_BADARG;
-        DA_DISPATCH(diff_attn_dkdv_kernel, (unsigned)blocks, 256, 256, 2 * 4 * 64 * 4, true)
+        DA_DISPATCH(diff_attn_dkdv_kernel, (unsigned)blocks, 256, 256, 2 * 4 * 64 * 4)
         if (int e = check_launch()) return e;
         if (a.kvruns > 1) {
             const int64_t grid = ((int64_t)a.B * a.M * a.Hk * (2 * a.d + a.dv) / 4 + 255) / 256;
