@@ -27,7 +27,7 @@ typedef short da_tr4 __attribute__((ext_vector_type(4)));
 typedef short da_tr8 __attribute__((ext_vector_type(8)));
 
 constexpr int kDaThreads = 256;
-constexpr int kDaSplitWgs = 256, kDaRunKeys = 512, kDaManyRows = 256;
+constexpr int kDaSplitWgs = 256, kDaRunKeys = 256, kDaOneRun = 1024, kDaManyRows = 256;      // diff_attn_splits
 
 struct DiffArgs {
     const void *q, *k, *v;                      // [B, N, H, 2, d], [B, M, Hk, 2, d], [B, M, Hk, dv]
@@ -287,7 +287,8 @@ __device__ __forceinline__ int da_len(const DiffArgs &a, int b) {
     return len;
 }
 
-// 16 bytes global -> LDS without registers; the LDS side is lane-linear from lds_addr (wave-uniform).  Inline assembly, waited for by hand (da_wait_copies):
+// 16 bytes global -> LDS without registers; the LDS side is lane-linear from lds_addr (wave-uniform).  Inline assembly, waited for by hand (da_wait_copies,
+// da_copies_done_barrier):
 // behind the builtin the compiler waits for every copy in front of the next LDS read, which would end the overlap of copies and products.
 __device__ __forceinline__ void da_copy16(const void *src, uint32_t lds_addr) {
     unsigned keep;
@@ -401,7 +402,7 @@ __device__ __forceinline__ DaRows da_rows(const DiffArgs &a, int hk, int w0, int
 struct DaWalk {
     uint64_t need, part, mixed, hide;                         // workgroup: not all hidden, not all free; wave: mixed, all hidden
     int base;
-    __device__ __forceinline__ void load(const DiffArgs &a, const DaRows &w, int64_t mb, int qt0, int qt1, int chunk, int M64, int N64) {
+    __device__ __forceinline__ void load(const DaRows &w, int64_t mb, int qt0, int qt1, int chunk, int M64, int N64) {
         const int kt = chunk * 64 + (threadIdx.x & 63);
         bool n = false, p = false, x = false, y = true;
         if (kt < M64) {
@@ -423,7 +424,7 @@ struct DaWalk {
         if (!a.tiles) return k0;
         while (k0 < end) {
             const int kt = k0 >> 6;
-            if (kt >> 6 != base) load(a, w, mb, qt0, qt1, kt >> 6, M64, N64);
+            if (kt >> 6 != base) load(w, mb, qt0, qt1, kt >> 6, M64, N64);
             const uint64_t m = need >> (kt & 63);
             if (m & 1) break;
             k0 = m ? (kt + __builtin_ctzll(m)) << 6 : ((kt >> 6) + 1) << 12;
@@ -554,7 +555,11 @@ __device__ __forceinline__ float da_lse(float m, float l) { return l > 0.f ? m +
 
 // ------------------------------------------------------------------------------------------------------------------
 // forward, many rows: workgroup = (batch, key head, 128 rows), a wave owns 32 rows; the keys stream through two LDS buffers of KB, copied while the block
-// in front is worked on (one barrier per block)
+// in front is worked on (one barrier per block).
+// 128 rows read a key once from L2 for 4 waves; two waves per SIMD (registers: DK = 64) hide each other's LDS and matrix latencies.  Bound: the vector unit for
+// heads up to 32 channels (16 exponentials, maxima, sums and conversions per 12 products of 32 cycles), vector and matrix unit about alike at 64.
+// Measured: 8192 causal tokens, 16 heads on 4, 2 x 64 channels bf16 522 us (790 TFLOP/s; a plain 8192^3 product reaches 1177 here); 32 x 492 tokens with their group
+// mask, 4 heads of 2 x 32, results for the backward kept, 31 us; 8 x 900 tokens, 8 heads of 2 x 24, 51 us; 16 x 396 tokens of 4 heads in fp32 64 us.
 template <typename T, int DK>
 __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) void diff_attn_fwd_kernel(const DiffArgs a) {
     using C = DaCfg<T, DK>;
@@ -742,6 +747,8 @@ __device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, i
 // forward, few rows: workgroup = (batch, key head, 32 rows, one of nsplit runs of the keys), its waves take every fourth tile of 32 keys of the run, each
 // through two LDS buffers of its own (no barrier until the end).  The waves' sums meet in LDS; with one run the rows are finished here, else the run's sums
 // go to `part` (rows x nsplit x 2 DV, with maxima and sums in `ml`) for diff_attn_join_kernel.
+// Bound: HBM, every key and value once for all heads of the group.  Measured: one token of 16 heads over 16 caches of up to 32768 keys (835 MB) 165 us, 5.1 TB/s;
+// 17 tokens over 4 x 10001 keys 22 us (41 MB: 11 us of it are the first loads, the joins in LDS and the last stores); 300 tokens of one image 10.6 us.
 template <typename T, int DK>
 __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff_attn_fwd_split_kernel(const DiffArgs a, int nsplit, float *__restrict__ part, float4 *__restrict__ ml) {
     using C = DaCfg<T, DK>;
@@ -774,7 +781,7 @@ __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff
     walk.base = -1;
     auto next = [&](int t) {
         for (; a.tiles && t < t_end; t += 4) {
-            if (t >> 7 != walk.base) walk.load(a, w, mb, w.q_lo, w.q_hi, t >> 7, M64, N64);
+            if (t >> 7 != walk.base) walk.load(w, mb, w.q_lo, w.q_hi, t >> 7, M64, N64);
             if (walk.code(a, t * 32) != 2) break;
         }
         return t;
@@ -905,7 +912,8 @@ __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff
     if ((tid & 7) == 0) ml[at] = make_float4(mx[0], sum[0], mx[1], sum[1]);
 }
 
-// joins the runs of a row: a wave per row, 8 lanes x DV / 8 channels, 8 runs side by side, in a fixed order
+// joins the runs of a row: a wave per row, 8 lanes x DV / 8 channels, 8 runs side by side, in a fixed order.  Bound: latency (a launch, one round of loads, the
+// reduction); 9 - 10 us for the two cases above.
 template <typename T, int DV>
 __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffArgs a, int nsplit, const float *__restrict__ part, const float4 *__restrict__ ml) {
     constexpr int NE = DV / 8;
@@ -971,7 +979,7 @@ __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffAr
 
 // ------------------------------------------------------------------------------------------------------------------
 // mask [Bm][N][M] bytes (strides sb, sn; non-zero = blocked) -> the forms the kernels read.  Workgroup = tile of 64 queries x 64 keys, a wave takes 16 queries;
-// lane = key, one ballot per query, all 16 loads in flight
+// lane = key, one ballot per query, all 16 loads in flight.  4 us for 492 x 492 (a launch and its latency).
 __global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sn, int N, int M, uint64_t *__restrict__ rowbits,
                                                              uint64_t *__restrict__ colbits, uint64_t *__restrict__ some_, uint8_t *__restrict__ tiles) {
     const int M64 = (M + 63) >> 6, N64 = (N + 63) >> 6;
@@ -1015,6 +1023,8 @@ __global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__re
 // near the mean of the values where the maps are flat), so dU . (A_1 V) of rounded vectors would be a small difference of large products.  The forward
 // pass therefore keeps W = A_1 V - beta U, beta = (A_1 V . U) / (U . U), and D_1 = r (t . W) + beta (dU . U), D_0 = dU . U + l D_1 (long rows, bf16: error of dl
 // and dq against 64 bits 0.0046 with A_1 V itself).  dP is made from the ROUNDED dU: what the rounding adds to D is added here too.
+// Bound: HBM (dY, U, W read, dU written: 33 MB and 13.4 us at 32 x 492 tokens of 4 heads, 134 MB and 33 us at 8192 of 16; two rounds of rows per workgroup leave
+// latency in the small case; loading a row ahead of its use changed nothing, 14.0 and 34 us).
 // The other kernels read the rows' statistics with l worked in - exp2(c s - (lse_1 - log2 |l|)) is |l| A_1, and its sign goes with D_1 and dP - and as the
 // numbers that dK's and dV's products start from: S_t at -lse_t / c, dP at -D_0.
 template <typename T, int LPR>
@@ -1112,7 +1122,7 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
 }
 
 // gradients of the learned vectors and of the norm weight from the first kernel's partial sums, in a fixed order: one workgroup per head (or one for shared
-// vectors), then one per 32 channels of the weight (32 interleaved runs of the partial rows, 8 loads in flight)
+// vectors), then one per 32 channels of the weight (32 interleaved runs of the partial rows, 8 loads in flight).  4 - 5 us, latency.
 __global__ __launch_bounds__(1024) void diff_attn_param_kernel(const DiffArgs a, int nrun, void *dlam, void *dw) {
     const int tid = threadIdx.x;
     __shared__ float s[32][33];
@@ -1156,7 +1166,10 @@ __global__ __launch_bounds__(1024) void diff_attn_param_kernel(const DiffArgs a,
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// backward, dQ: the forward's decomposition and copies; probabilities from the saved statistics
+// backward, dQ: the forward's decomposition and copies; probabilities from the saved statistics, nothing to rescale.  dS is rounded to bf16 for its product with K (as the keys it meets
+// are), dU for its product with V: each adds 0.0017 to dq's relative error, 0.0030 in all with the result's own 0.0017.  Keeping either in two bf16 terms would
+// cost a third more products for 0.0025.
+// Bound as the forward: 495 us and 835 TFLOP/s at 8192 causal tokens, 27 us at 32 x 492, 58 us in fp32 at 16 x 396.
 template <typename T, int DK>
 __device__ __forceinline__ void da_dq_tile(const DiffArgs &a, da_f16v (*dq)[DaCfg<T, DK>::MTK], const uint4 (*qf)[DaCfg<T, DK>::NF], const uint4 *uf, const float *lse, const float *dl,
                                            float sign, const DaLane<T, DK> &ln, uint32_t tk, uint32_t tv, bool masked, uint32_t vis, int lane) {
@@ -1328,7 +1341,11 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
 
 // ------------------------------------------------------------------------------------------------------------------
 // backward, dK and dV: workgroup = (batch, key head, 128 keys, one of kvruns runs of the rows), a wave owns 32 keys with both operands in registers; the
-// queries of the group's heads stream through two LDS buffers of QB rows (Q | dU | four statistics), copied while the block in front is worked on
+// queries of the group's heads stream through two LDS buffers of QB rows (Q | dU | four statistics), copied while the block in front is worked on.
+// The rows' statistics are what the products start from (S at -lse / c, dP at -D_0): they come from LDS straight into the accumulators.
+// Both operands and both results of 64-channel heads are 385 registers, one wave per SIMD: vector and matrix work of a tile follow each other, which bounds it.
+// Measured: 900 us at 8192 causal tokens (610 TFLOP/s), 37 us at 32 x 492, 77 us in fp32 at 16 x 396.  Two waves for the same 32 keys, one map each (two waves per
+// SIMD, dP worked out twice), took 942 us where this took 901; both mask forms of a tile as code of their own 1140 (the accumulators change places between them).
 template <typename T, int DK>
 __device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[DaCfg<T, DK>::MTK], da_f16v *dv, const uint4 (*kf)[DaCfg<T, DK>::NF], const uint4 *vf, float sign,
                                              const DaLane<T, DK> &ln, uint32_t tq, uint32_t tu, uint32_t stat, bool masked, uint32_t vis, int lane) {
@@ -1602,7 +1619,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || (DK == 32 && sizeof(T) == 2
     }
 }
 
-// dK and dV from the runs' sums, in order: a thread per 4 channels
+// dK and dV from the runs' sums, in order: a thread per 4 channels.  Bound: HBM (14 us for 67 MB at 8192 tokens).
 template <typename T> __global__ __launch_bounds__(256) void diff_attn_kv_sum_kernel(const DiffArgs a) {
     const int w4 = (2 * a.d + a.dv) / 4;
     const int64_t rows = (int64_t)a.B * a.M * a.Hk, n = rows * w4;
@@ -1629,7 +1646,7 @@ static int diff_attn_setup(DiffArgs &a, const int64_t *s, float scale, float ini
     // shape: see include/dfine_hip.h
     const int64_t B = s[0], N = s[1], M = s[2], H = s[3], Hk = s[4], d = s[5], dv = s[6], dt = s[7];
     if (B < 0 || N < 0 || M < 0 || B > 0xffffff || N > 0x3fffffff || M > 0x3fffffff || H < 1 || Hk < 1 || H > 4096 || H % Hk || d < 8 || d > 64 || d % 8 || dv < 8 ||
-        dv > 128 || dv % 8 || (dt != 0 && dt != 1) || !(scale > 0.f) || !(eps >= 0.f))
+        dv > 128 || dv % 8 || (dt != 0 && dt != 1) || !(scale >= 1e-30f) || !(eps >= 0.f))
         return DFINE_E_BADARG;
     if (s[8] != 1 && s[8] != H) return DFINE_E_BADARG;                               // heads of the learned vectors
     if (N * (H / Hk) > 0x7fffff00 || B * Hk > 0xffffff) return DFINE_E_BADARG;       // (rows of a key head: 32-bit)
@@ -1708,9 +1725,17 @@ static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <
 
 // Runs of the keys a forward pass is cut into: 0 = the kernel for many rows (128 rows per workgroup, all keys), n >= 1 = the kernel for few (32 rows per
 // workgroup, n runs).
+// kDaManyRows: many rows are those that make 256 workgroups (one per CU).  At 256 of them (16 x 396 tokens of 4 heads, fp32) the kernel for many takes 69 us and
+// the one for few 92, at 512 (32 x 492, bf16) 35 and 56; at 12 (300 tokens of one image) 20 and 16.
+// kDaSplitWgs: the runs fill the chip once, 256 workgroups.  One token over 16 caches of 32768 keys (4 key heads): 170 / 177 / 184 / 212 us with 256 / 512 / 1024 /
+// 2048 workgroups; 17 tokens over 4 x 10001 keys 36 / 46 / 66 us with 256 / 512 / 1024: every run costs a prologue, its sums and a share of the join.
+// kDaRunKeys: a run has 256 keys at least (two tiles for each of its four waves): one token of 16 heads over 4096 keys, runs + join, 19.4 / 19.5 / 21.5 / 26.8 / 35.9 us
+// with runs of 128 / 256 / 512 / 1024 / 2048 keys.
+// kDaOneRun: up to 1024 keys stay one run (8 us and 4.9 for every 512 keys, against 10.7 and a join of 8): 300 tokens of one image 10.6 us, in two runs 15.0.
 static int diff_attn_splits(const DiffArgs &a) {
     const int64_t R = (int64_t)a.N * a.G, bh = (int64_t)a.B * a.Hk;
     if ((R + 127) / 128 * bh >= kDaManyRows) return 0;
+    if (a.M <= kDaOneRun) return 1;
     const int64_t wgs = (R + 31) / 32 * bh, most = ((int64_t)a.M + kDaRunKeys - 1) / kDaRunKeys;
     int64_t n = kDaSplitWgs / wgs;
     if (n > most) n = most;
@@ -1769,23 +1794,28 @@ int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void 
     return check_launch();
 }
 
-static int diff_attn_runs(const DiffArgs &a) {                  // workgroups per head of the first backward kernel: 1024 in all, one pass each at least
+// Workgroups per head of the first backward kernel: 1024 in all, one pass over their rows each at least.  Kernel us at 512 / 1024 / 2048 / 4096: 42 / 33 / 38 / 44 for
+// 8192 tokens of 16 heads of 128 channels, 14.2 / 13.5 / 17.2 / 17.4 for 32 x 492 tokens of 4 heads of 64, 11.2 / 11.9 / 10.6 / 11.6 for 16 x 396 in fp32.
+static int diff_attn_runs(const DiffArgs &a) {
     const int64_t rw = 2048 / (2 * diff_attn_size(a.d, a.dv)), rows = ((int64_t)a.B * a.N + rw - 1) / rw;       // rows of one pass of a workgroup
     int64_t n = 1024 / a.H;
     if (n < 1) n = 1;
     return (int)(n < rows ? n : rows < 1 ? 1 : rows);
 }
 
-// workspace of the backward pass in bytes: dU, D_0 and D_1, the partial sums
-// runs of the rows that dK and dV are summed in: more where (batch, key head, 128 keys) are fewer workgroups than the chip holds at once
+// Runs of the rows that dK and dV are summed in, about 512 workgroups in all, each with four blocks of queries at least.  Measured, kernel + sum kernel in us:
+// 8192 causal tokens of 4 key heads, bf16 (256 workgroups of very unequal work) 1543 with one run, 898 + 14 with 2, 905 + 23 with 4, 945 + 54 with 8;
+// 32 x 492 tokens of 4 heads (512 workgroups) 37 with one, 45 + 13 with 2; 16 x 396 tokens of 4 heads in fp32 (256 workgroups, 7 blocks of queries) 77 with
+// one, 89 + 8 with 2, 105 + 12 with 4.
 static int diff_attn_kvruns(const DiffArgs &a) {
     const int64_t wgs = ((int64_t)a.M + 127) / 128 * a.B * a.Hk, units = ((int64_t)a.N + 63) / 64 * a.G;
-    if (wgs == 0 || wgs >= 512) return 1;
-    int64_t n = 1024 / wgs;
+    if (wgs == 0) return 1;
+    int64_t n = 512 / wgs;
     if (n > 8) n = 8;
     if (n > units / 4) n = units / 4;
     return (int)(n < 1 ? 1 : n);
 }
+// workspace of the backward pass: dU, the rows' statistics, the partial sums of dl and dg, the runs' sums of dK and dV
 int64_t dfine_diff_attn_bwd_ws_bytes(const int64_t *shape) {
     DiffArgs a{};
     if (!shape || diff_attn_setup(a, shape, 1.f, 0.f, 0.f)) return -1;

@@ -10,6 +10,8 @@
 // next to each other (a power of two of them), and a wave walks through the heads of its tokens with the table row and the weights in registers, so the
 // table - 4 bytes per channel against 2 of data - is read once per token and not once per head.  The partner of a pair comes from its lane as raw
 // storage (a shuffle of 16 bytes) and is normed again here: cheaper than exchanging the 32-bit results.
+// Measured: 4 x 8192 tokens of 32 + 8 heads of 128 channels, bf16, forward 163 us (671 MB, 4.1 TB/s; a large copy reaches 4.9), backward 200 us (1007 MB, 5.0 TB/s)
+// and 5 us for the weights' sums; 32 x 492 tokens of 8 + 8 heads of 32 channels 14, 19 and 4 us (32 MB, 48 MB); one token each of 16 sequences 4.6 us (a launch).
 // All arithmetic is in 32 bits; the one rounding is the store.  The weight gradients leave as one partial row per workgroup, added up in order.
 #include "common.h"
 
@@ -293,7 +295,7 @@ using namespace dfine;
 
 extern "C" {
 
-// shape: the DFINE_QKN_* slots of include/dfine_hip.h
+// shape: see include/dfine_hip.h
 static int qk_norm_setup(QkNormArgs &a, const int64_t *s, const float *cosv, const float *sinv, const void *pos, float eps, int *vec, int *gx, int *gy,
                          bool bwd) {
     const int64_t B = s[0], L = s[1], Hq = s[2], Hk = s[3], D = s[4], R = s[5], T = s[6], dt = s[7];
@@ -317,12 +319,15 @@ static int qk_norm_setup(QkNormArgs &a, const int64_t *s, const float *cosv, con
     while (hs < slots && hs < hmax) hs <<= 1;
     a.lpr = lpr; a.hs = hs;
     const int64_t per_wave = slots / hs, waves = (B * L + per_wave - 1) / per_wave, groups = (waves + 3) / 4;
-    // few tokens: the heads go over workgroups too, down to one load per lane; many: a wave takes all heads of its tokens (one read of the table row)
+    // few tokens: the heads go over workgroups too, down to one load per lane; many: a wave takes all heads of its tokens (one read of the table row).
+    // All heads in a wave / up to 1024 / up to 4096 workgroups: 16 tokens of 32 heads 6.1 / 4.7 / 4.6 us, one token of 64 heads 14.5 / 4.8 / 4.8, 160 tokens of 32
+    // heads 11.5 / 6.0 / 6.0, 16 x 900 tokens of 16 heads (fp32) 21 / 21 / 24.
     int chunk = hmax;
     while (chunk > hs && groups * ((hmax + chunk - 1) / chunk) < 1024) chunk = (chunk / 2 + hs - 1) / hs * hs;
     a.hchunk = chunk < hs ? hs : chunk;
     *gy = hmax ? (hmax + a.hchunk - 1) / a.hchunk : 1;
-    // backward: at most 1024 partial rows of weight gradients
+    // backward: at most 1024 partial rows of weight gradients.  512 / 1024 / 2048 rows: 267 / 200 / 201 us and 4.9 / 4.9 / 8.0 for their sums at 4 x 8192 tokens of
+    // 40 heads, 20.6 / 17.8 / 24.1 and 3.8 / 3.8 / 6.2 at 32 x 492 of 16
     const int64_t most = bwd ? 1024 / (*gy < 1024 ? *gy : 1024) : 65536;
     *gx = (int)(groups < most ? groups : most);
     return DFINE_OK;

@@ -2658,7 +2658,7 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
     of the first query among the keys).  A query that sees no key gives 0 and takes no gradient.  Keys that some query sees hold finite numbers; keys that
     the mask hides from every query, and keys behind kv_lengths or the last causal position, may hold anything.
     Gradients for q, k, v, lambda_vectors and norm_weight, added up in a fixed order.  -> [B, N, H, dv], contiguous, of q's type.  Under bf16 autocast
-    q, k, v are cast to bfloat16 first.  scale: d ** -0.5 by default."""
+    q, k, v are cast to bfloat16 first.  scale: d ** -0.5 by default, at least 1e-30."""
     op = "diff_attention"
     device = q.get_device() if isinstance(q, torch.Tensor) else None
     _float_operand(op, "q", q, device)
@@ -2709,7 +2709,7 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
     if not starts and not -(2 ** 31) < int(query_start) < 2 ** 31:
         _refuse(f"{op}: query_start {query_start}")
     scale, init, eps = d ** -0.5 if scale is None else float(scale), float(lambda_init), float(norm_eps)
-    if not 0 < scale < float("inf"):
+    if not 1e-30 <= scale < float("inf"):              # (the backward pass divides the rows' statistics by it)
         _refuse(f"{op}: scale {scale}")
     if not eps >= 0:
         _refuse(f"{op}: norm_eps {eps}")

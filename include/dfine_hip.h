@@ -827,7 +827,7 @@ int dfine_qk_norm_rotate_bwd(const void *q, const void *k, const void *wq, const
 
 /* Differential attention of the token streams: out = (1 - init) norm((A_0 - l A_1) V) weight per head, A_t = softmax(scale q_t k_t^T +
  * mask), l = exp(x0 . x1) - exp(x2 . x3) + init from lam [4, H or 1, d]; without weight: out = (A_0 - l A_1) V.  A query that sees no key
- * gives 0 and takes no gradient.
+ * gives 0 and takes no gradient.  scale at least 1e-30.
  * q [B, N, H, 2, d], k [B, M, Hk, 2, d], v [B, M, Hk, dv] (H a multiple of Hk), out [B, N, H, dv] contiguous; d <= 64, dv <= 128, multiples of 8.
  * What query i of batch b sees: keys j < kv_len[b] (NULL: M; keys from there on are not read), j <= q_start[b] + i when causal (q_start NULL:
  * one start for all in shape), and where the mask lets it: mask_forms = the dfine_diff_attn_mask_words(batches, N, M) words that

@@ -36,7 +36,7 @@ def _diff():
     (dict(attn_mask=torch.zeros(5, 7)), TypeError), (dict(attn_mask=torch.zeros(7, 5, dtype=torch.bool)), ValueError),
     (dict(kv_lengths=torch.tensor([1.0, 2.0])), TypeError), (dict(kv_lengths=torch.tensor([1, 2, 3])), ValueError), (dict(query_start=3), ValueError),
     (dict(query_start=torch.tensor([1, 2])), ValueError), (dict(causal=True, query_start=2 ** 40), ValueError), (dict(scale=0.0), ValueError),
-    (dict(scale=-1.0), ValueError), (dict(scale=float("nan")), ValueError), (dict(norm_eps=-1.0), ValueError)])
+    (dict(scale=-1.0), ValueError), (dict(scale=1e-31), ValueError), (dict(scale=float("nan")), ValueError), (dict(norm_eps=-1.0), ValueError)])
 def test_diff_attention_refuses(oracle_backend, change, kind):
     with pytest.raises(kind, match="diff_attention"):
         kernels.diff_attention(**{**_diff(), **change})

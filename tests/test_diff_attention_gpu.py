@@ -37,23 +37,23 @@ def _inputs(cuda, B, N, M, H, Hk, d, dv, dtype, shared=False, seed=1):
     return q, k, v, lam, w, dy, g
 
 
-def _run(q, k, v, lam, w, dy, **kw):
+def _run(q, k, v, lam, w, dy, init=INIT, **kw):
     from custom_d_fine_amd import kernels
     leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam) + (() if w is None else (w,))]
-    y = kernels.diff_attention(*leaves[:4], INIT, norm_weight=None if w is None else leaves[4], norm_eps=EPS, **kw)
+    y = kernels.diff_attention(*leaves[:4], init, norm_weight=None if w is None else leaves[4], norm_eps=EPS, **kw)
     return (y,) + torch.autograd.grad(y, leaves, dy), leaves
 
 
-def _check(cuda, q, k, v, lam, w, dy, **kw):
+def _check(cuda, q, k, v, lam, w, dy, init=INIT, **kw):
     from custom_d_fine_amd import kernels
     B, N, H, _, d = q.shape
     M = k.shape[1]
-    got, _ = _run(q, k, v, lam, w, dy, **kw)
+    got, _ = _run(q, k, v, lam, w, dy, init, **kw)
     seen = ref.visible(B, N, M, kw.get("attn_mask"), kw.get("kv_lengths"), kw.get("causal", False), kw.get("query_start", 0), cuda)
     dl = [t.detach().double().requires_grad_(True) for t in (q, k, v, lam) + (() if w is None else (w,))]
-    y = ref.diff_attention(*dl[:4], INIT, None if w is None else dl[4], EPS, seen, kw.get("scale") or d ** -0.5)
+    y = ref.diff_attention(*dl[:4], init, None if w is None else dl[4], EPS, seen, kw.get("scale") or d ** -0.5)
     want = (y,) + torch.autograd.grad(y, dl, dy.double())
-    spread = ref.diff_attention_spread(*[t.detach() for t in dl[:4]], INIT, None if w is None else dl[4].detach(), EPS, seen, kw.get("scale") or d ** -0.5, dy.double())
+    spread = ref.diff_attention_spread(*[t.detach() for t in dl[:4]], init, None if w is None else dl[4].detach(), EPS, seen, kw.get("scale") or d ** -0.5, dy.double())
     for name, a, b in zip(("out", "dq", "dk", "dv", "dlam", "dweight"), got, want):
         assert a.dtype == q.dtype or name in ("dlam", "dweight")
         assert a.shape == b.shape and torch.isfinite(a).all(), name
@@ -61,7 +61,7 @@ def _check(cuda, q, k, v, lam, w, dy, **kw):
         print(name, "%.2e of %.2e" % (err, tol))
         assert err <= tol, name
     with torch.no_grad():
-        z = kernels.diff_attention(q, k, v, lam, INIT, norm_weight=w, norm_eps=EPS, **kw)
+        z = kernels.diff_attention(q, k, v, lam, init, norm_weight=w, norm_eps=EPS, **kw)
     assert _off(z, y, spread["out"]) <= _tol("out", q.dtype, M, d)
     return got
 
@@ -357,6 +357,79 @@ def test_offsets_past_32_bits(cuda):
         one, two = _run(q, far, v, lam, w, dy)[0], _run(q, k, v, lam, w, dy)[0]
         for a, b in zip(one, two):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hk,d,dv", [(6, 2, 16, 32), (6, 6, 32, 64), (4, 2, 64, 128)])
+def test_negative_and_zero_lambda(cuda, dtype, H, Hk, d, dv):
+    """l < 0 for every second head (exp(d x^2) = 2.2 taken away from 1 + init); then l = 1 - 1 + 0 exactly: nothing comes through the second map."""
+    q, k, v, lam, w, dy, _ = _inputs(cuda, 2, 70, 101, H, Hk, d, dv, dtype)
+    lam[2:, ::2] = (0.8 / d) ** 0.5
+    _check(cuda, q, k, v, lam, w, dy)
+    _check(cuda, q, k, v, lam, None, dy)
+    lam = torch.zeros_like(lam)
+    _check(cuda, q, k, v, lam, w, dy, 0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,N,M,H,Hk,d,dv", [(2, 3, 70, 40, 1, 16, 32), (1, 130, 130, 66, 2, 8, 16), (3, 1, 300, 64, 1, 64, 128)])
+def test_many_heads_of_one_key_head(cuda, dtype, B, N, M, H, Hk, d, dv):
+    """More heads to a key head than a wave has rows, and numbers of them that no power of two divides."""
+    q, k, v, lam, w, dy, _ = _inputs(cuda, B, N, M, H, Hk, d, dv, dtype)
+    _check(cuda, q, k, v, lam, w, dy, causal=True, query_start=M - N)
+
+
+def test_masks_as_they_come(cuda):
+    """An expanded mask, a transposed one, one batch's own, and lengths in 64 bits that do not fit 32."""
+    from custom_d_fine_amd import kernels
+    B, N, M = 3, 70, 90
+    q, k, v, lam, w, _, g = _inputs(cuda, B, N, M, 6, 2, 32, 64, torch.bfloat16)
+    mask = (torch.rand(N, M, generator=g) < 0.4).to(cuda)
+
+    def run(m, n=B, lengths=None, **kw):
+        return kernels.diff_attention(q[:n], k[:n], v[:n], lam, INIT, w, attn_mask=m, kv_lengths=lengths, **kw)
+
+    base = run(mask)
+    assert torch.equal(run(mask.expand(B, N, M)), base)
+    assert torch.equal(run(mask.t().contiguous().t()), base)
+    assert torch.equal(run(mask[None].repeat(B, 1, 1).transpose(0, 1).contiguous().transpose(0, 1)), base)
+    assert torch.equal(run(mask[None], 1), base[:1])
+    far = torch.tensor([2 ** 40, 2 ** 32 + 5, -2 ** 40], device=cuda)
+    assert torch.equal(run(None, lengths=far), run(None, lengths=torch.tensor([M, M, 0], device=cuda, dtype=torch.int32)))
+    assert torch.equal(run(None, causal=True, query_start=far), run(None, causal=True, query_start=torch.tensor([M, M, -M - N], device=cuda, dtype=torch.int32)))
+
+
+def test_two_streams_at_once(cuda):
+    """Calls on two streams that may run side by side, few rows (runs of the keys) and many, with their backward passes: nothing of one call is another's."""
+    sets = [_inputs(cuda, 2, n, m, 8, 2, 32, 64, torch.bfloat16, seed=n) for n, m in ((4, 3000), (300, 300))]
+    base = [_run(*s[:6])[0] for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for j, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[j].append(_run(*sets[j][:6])[0])
+    torch.cuda.synchronize()
+    for j in range(2):
+        for one in got[j]:
+            for a, b in zip(one, base[j]):
+                assert torch.equal(a, b)
+
+
+def test_small_scales(cuda):
+    """scale = 1e-20: both maps are flat, and the row statistics over scale still fit 32 bits."""
+    q, k, v, lam, w, dy, _ = _inputs(cuda, 2, 50, 60, 6, 2, 16, 32, torch.float32)
+    got, _ = _run(q, k, v, lam, w, dy, scale=1e-20)
+    dl = [t.detach().double().requires_grad_(True) for t in (v, lam, w)]
+    G = 3
+    x = torch.exp((dl[1][0] * dl[1][1]).sum(-1)) - torch.exp((dl[1][2] * dl[1][3]).sum(-1)) + INIT
+    u = ((1 - x)[None, :, None] * dl[0].mean(1).repeat_interleave(G, 1))[:, None].expand(2, 50, 6, 32)
+    y = (1 - INIT) * dl[2] * u / (u.pow(2).mean(-1, keepdim=True) + EPS).sqrt()
+    want = (y,) + torch.autograd.grad(y, dl, dy.double())
+    for name, a, b in zip(("out", "dv", "dweight"), (got[0], got[3], got[5]), (want[0], want[1], want[3])):
+        assert ref.rel(a, b) <= (60 + 8 * 16 + 64) * 2 ** -24, name
+    assert torch.isfinite(torch.stack([g.double().abs().max() for g in got])).all()
 
 
 def test_no_second_derivative(cuda):
