@@ -35,7 +35,8 @@ struct DiffArgs {
     const uint64_t *rowbits, *colbits, *some;   // mask forms (1 = may attend): [Bm][N][M64], [Bm][M][N64], any of 64 queries [Bm][N64][M64]; null: no mask
     const uint8_t *tiles;                       // [Bm][N64][M64] 0 free, 1 mixed, 2 blocked
     const int *kvlen, *qstart_dev;              // [B] or null
-    void *out, *u, *o2;                         // [B, N, H, dv]; u, o2 (null: not kept) are read by the backward pass
+    void *out, *o2;                             // [B, N, H, dv]; o2 = W and u = U (null: not kept) are read by the backward pass
+    float *u;
     float *stats;                               // [4][B, H, N]: lse of the two maps in the exp2 domain (+inf: an empty row), r, beta
     int64_t qs[4], ks[4], vs[3];                // strides (batch, token, head, map)
     int64_t mask_b;                             // 0: one mask for the batch
@@ -670,12 +671,13 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
         e.stats[3 * bhn + at] = beta;
     }
     __syncthreads();                                          // every wave is done with the tiles
-    const DaRowsOut<T, C::DV> rows{lds + wave * 32 * C::DV * C::ES};
+    char *own = lds + wave * 32 * C::DV * 4;
+    const DaRowsOut<T, C::DV> rows{own};
     const int w0 = blk0 + wave * 32;
-    auto to = [&](void *base) {
-        rows.flush(lane, [&](int r, int c) -> T * {
+    auto to = [&](auto rows, auto *base) {
+        rows.flush(lane, [&](int r, int c) {
             const int row = w0 + r, i = da_div_g(e, min(row, R - 1));
-            return row < R && c < e.dv ? reinterpret_cast<T *>(base) + (((int64_t)b * e.N + i) * e.H + hk * e.G + row - i * e.G) * e.dv + c : nullptr;
+            return row < R && c < e.dv ? base + (((int64_t)b * e.N + i) * e.H + hk * e.G + row - i * e.G) * e.dv + c : nullptr;
         });
     };
 #pragma unroll
@@ -686,15 +688,16 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
             const float4 g = *reinterpret_cast<const float4 *>(sW + c);
             rows.put(l32, c, st.o[0][x][4 * q4] * g.x * rn, st.o[0][x][4 * q4 + 1] * g.y * rn, st.o[0][x][4 * q4 + 2] * g.z * rn, st.o[0][x][4 * q4 + 3] * g.w * rn);
         }
-    to(e.out);
+    to(rows, reinterpret_cast<T *>(e.out));
     if (!e.o2) return;
-    if (e.weight) {
+    {
+        const DaRowsOut<float, C::DV> rows{own};
 #pragma unroll
         for (int x = 0; x < C::MT; ++x)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
                 rows.put(l32, x * 32 + 8 * q4 + 4 * h2, st.o[0][x][4 * q4], st.o[0][x][4 * q4 + 1], st.o[0][x][4 * q4 + 2], st.o[0][x][4 * q4 + 3]);
-        to(e.u);
+        to(rows, e.u);
     }
 #pragma unroll
     for (int x = 0; x < C::MT; ++x)
@@ -705,7 +708,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
             for (int j = 0; j < 4; ++j) o[j] = st.o[1][x][4 * q4 + j] - beta * st.o[0][x][4 * q4 + j];
             rows.put(l32, x * 32 + 8 * q4 + 4 * h2, o[0], o[1], o[2], o[3]);
         }
-    to(e.o2);
+    to(rows, reinterpret_cast<T *>(e.o2));
 }
 
 // One row of the result from its two maps' sums in plain order: LPR neighbouring lanes of NE channels each (c0: the lane's first), O normalised
@@ -730,7 +733,7 @@ __device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, i
         if (c >= a.dv) continue;
         da_store4(reinterpret_cast<T *>(a.out) + orow + c, o0[j] * g[j] * rn, o0[j + 1] * g[j + 1] * rn, o0[j + 2] * g[j + 2] * rn, o0[j + 3] * g[j + 3] * rn);
         if (a.o2) {
-            if (a.weight) da_store4(reinterpret_cast<T *>(a.u) + orow + c, o0[j], o0[j + 1], o0[j + 2], o0[j + 3]);
+            da_store4(a.u + orow + c, o0[j], o0[j + 1], o0[j + 2], o0[j + 3]);
             da_store4(reinterpret_cast<T *>(a.o2) + orow + c, o1[j] - beta * o0[j], o1[j + 1] - beta * o0[j + 1], o1[j + 2] - beta * o0[j + 2], o1[j + 3] - beta * o0[j + 3]);
         }
     }
@@ -1022,8 +1025,9 @@ __global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__re
 // With a norm dU stands at right angles to U up to eps: dU . U = r (t . U) eps r^2 with t = (1 - init) g dY.  A_1 V mostly points along U (both are
 // near the mean of the values where the maps are flat), so dU . (A_1 V) of rounded vectors would be a small difference of large products.  The forward
 // pass therefore keeps W = A_1 V - beta U, beta = (A_1 V . U) / (U . U), and D_1 = r (t . W) + beta (dU . U), D_0 = dU . U + l D_1 (long rows, bf16: error of dl
-// and dq against 64 bits 0.0046 with A_1 V itself).  dP is made from the ROUNDED dU: what the rounding adds to D is added here too.
-// Bound: HBM (dY, U, W read, dU written: 33 MB and 13.4 us at 32 x 492 tokens of 4 heads, 134 MB and 33 us at 8192 of 16; two rounds of rows per workgroup leave
+// and dq against 64 bits 0.0046 with A_1 V itself), and U in 32 bits: dU . U is small for the same reason (with U in bf16 dq was 0.0042 off instead of 0.0030).
+// dP is made from the ROUNDED dU: what the rounding adds to D is added here too.
+// Bound: HBM (dY, U, W read, dU written: 41 MB and 15 us at 32 x 492 tokens of 4 heads, 168 MB and 35 us at 8192 of 16; two rounds of rows per workgroup leave
 // latency in the small case; loading a row ahead of its use changed nothing, 14.0 and 34 us).
 // The other kernels read the rows' statistics with l worked in - exp2(c s - (lse_1 - log2 |l|)) is |l| A_1, and its sign goes with D_1 and dP - and as the
 // numbers that dK's and dV's products start from: S_t at -lse_t / c, dP at -D_0.
@@ -1047,7 +1051,8 @@ __global__ __launch_bounds__(256) void diff_attn_prep_kernel(const DiffArgs a, i
         for (int j = 0; j < 8; ++j) dy[j] = u[j] = o2[j] = 0.f;
         if (ok) {
             const T *yp = reinterpret_cast<const T *>(a.dy) + b * a.dys[0] + i * a.dys[1] + head * a.dys[2] + c;
-            const T *up = reinterpret_cast<const T *>(a.weight ? a.u : a.out) + orow, *op = reinterpret_cast<const T *>(a.o2) + orow;
+            const float *up = a.u + orow;
+            const T *op = reinterpret_cast<const T *>(a.o2) + orow;
             da_load4(yp, dy); da_load4(yp + 4, dy + 4);
             da_load4(up, u); da_load4(up + 4, u + 4);
             da_load4(op, o2); da_load4(op + 4, o2 + 4);
@@ -1754,13 +1759,13 @@ int64_t dfine_diff_attn_fwd_ws_bytes(const int64_t *shape) {
 }
 
 int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms, const int *kv_len,
-                        const int *q_start, void *out, void *u, void *o2, float *stats, void *ws, const int64_t *shape, float scale, float init, float eps, void *stream) {
+                        const int *q_start, void *out, float *u, void *o2, float *stats, void *ws, const int64_t *shape, float scale, float init, float eps, void *stream) {
     if (!shape) return DFINE_E_BADARG;
     DiffArgs a{};
     if (int e = diff_attn_setup(a, shape, scale, init, eps)) return e;
     if (a.B == 0 || a.N == 0) return DFINE_OK;
     if (!diff_attn_aligned(q) || !diff_attn_aligned(out) || !lam || (a.M && (!diff_attn_aligned(k) || !diff_attn_aligned(v)))) return DFINE_E_BADARG;
-    if ((o2 != nullptr) != (stats != nullptr) || (u && !o2) || (o2 && weight && !u)) return DFINE_E_BADARG;
+    if ((o2 != nullptr) != (stats != nullptr) || (o2 != nullptr) != (u != nullptr) || (o2 && (!diff_attn_aligned(o2) || !diff_attn_aligned(u)))) return DFINE_E_BADARG;
     a.q = q; a.k = k; a.v = v; a.lam = lam; a.weight = weight; a.kvlen = kv_len; a.qstart_dev = q_start;
     a.out = out; a.u = u; a.o2 = o2; a.stats = stats;
     a.post = weight ? 1.f - init : 1.f;
@@ -1826,20 +1831,20 @@ int64_t dfine_diff_attn_bwd_ws_bytes(const int64_t *shape) {
 
 #define DA_ARGS a
 int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms, const int *kv_len,
-                        const int *q_start, const void *out, const void *u, const void *o2, const float *stats, const void *dy, void *dq, void *dk, void *dv,
+                        const int *q_start, const float *u, const void *o2, const float *stats, const void *dy, void *dq, void *dk, void *dv,
                         void *dlam, void *dweight, void *ws, const int64_t *shape, float scale, float init, float eps, void *stream) {
     if (!shape) return DFINE_E_BADARG;
     DiffArgs a{};
     if (int e = diff_attn_setup(a, shape, scale, init, eps)) return e;
     if (!lam || !ws || ((uintptr_t)ws & 255)) return DFINE_E_BADARG;
     const bool rows_ = a.B && a.N, keys_ = a.B && a.M;
-    if (rows_ && (!diff_attn_aligned(q) || !diff_attn_aligned(weight ? u : out) || !diff_attn_aligned(o2) || !stats || !diff_attn_aligned(dy) ||
+    if (rows_ && (!diff_attn_aligned(q) || !diff_attn_aligned(u) || !diff_attn_aligned(o2) || !stats || !diff_attn_aligned(dy) ||
                   (dq && !diff_attn_aligned(dq))))
         return DFINE_E_BADARG;
     if ((dk == nullptr) != (dv == nullptr)) return DFINE_E_BADARG;
     if (keys_ && (!diff_attn_aligned(k) || !diff_attn_aligned(v) || (dk && (!diff_attn_aligned(dk) || !diff_attn_aligned(dv))))) return DFINE_E_BADARG;
     a.q = q; a.k = k; a.v = v; a.lam = lam; a.weight = weight; a.kvlen = kv_len; a.qstart_dev = q_start;
-    a.out = const_cast<void *>(out); a.u = const_cast<void *>(u); a.o2 = const_cast<void *>(o2); a.stats = const_cast<float *>(stats);
+    a.u = const_cast<float *>(u); a.o2 = const_cast<void *>(o2); a.stats = const_cast<float *>(stats);
     a.dy = dy; a.dq = dq; a.dk = dk; a.dvv = dv;
     a.post = weight ? 1.f - init : 1.f;
     diff_attn_forms(a, mask_forms, a.mask_b ? a.B : 1);

@@ -127,7 +127,7 @@ _SIGNATURES = {
     "dfine_diff_attn_fwd_ws_bytes": (_L, [_P]),
     "dfine_diff_attn_bwd_ws_bytes": (_L, [_P]),
     "dfine_diff_attn_fwd": (c_int, [_P] * 14 + [_F, _F, _F, _P]),
-    "dfine_diff_attn_bwd": (c_int, [_P] * 20 + [_F, _F, _F, _P]),
+    "dfine_diff_attn_bwd": (c_int, [_P] * 19 + [_F, _F, _F, _P]),
     "dfine_attn_mask_bits": (c_int, [_P, _I, _P, _P]),
     "dfine_groupnorm_ws_floats": (_L, [_I, _I, _I]),
     "dfine_groupnorm_fwd": (c_int, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P]),
@@ -1622,13 +1622,14 @@ def _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys
                      start if isinstance(start, int) else 0, mask_batches, *qs, *ks, *vs, *dys)
 
 
-def _da_kept(out, normed):
+def _da_kept(out):
     """What the forward pass keeps for the backward, in one buffer (each tensor costs microseconds to make and on its way through the graph): the rows'
-    statistics, then W, then with a norm U -> bytes in all, where W and U begin (U: None without a norm)."""
-    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    statistics, then W, then U in 32 bits -> bytes in all, where W and U begin."""
     B, N, H, dv = out.shape
-    stats, rows = up(16 * B * N * H), up(out.element_size() * out.numel())
-    return (stats + 2 * rows, stats, stats + rows) if normed else (stats + rows, stats, None)
+    rows = B * N * H
+    o2 = (16 * rows + 255) // 256 * 256
+    u = o2 + (out.element_size() * rows * dv + 255) // 256 * 256
+    return u + 4 * rows * dv, o2, u
 
 
 @_on_device
@@ -1642,9 +1643,10 @@ def diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal,
     out = torch.empty(B, N, H, dv, device=q.device, dtype=q.dtype)
     kept = o2 = stats = u = None
     if keep:
-        size, o2_at, u_at = _da_kept(out, weight is not None)
+        size, o2_at, u_at = _da_kept(out)
         kept = torch.empty(size, device=q.device, dtype=torch.uint8)
-        stats, o2, u = kept.data_ptr(), kept.data_ptr() + o2_at, u_at and kept.data_ptr() + u_at
+        stats = kept.data_ptr()
+        o2, u = stats + o2_at, stats + u_at
     shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs)
     nws = _lib.dfine_diff_attn_fwd_ws_bytes(shape)
     ws = torch.empty(nws, device=q.device, dtype=torch.uint8) if nws > 0 else None
@@ -1656,8 +1658,8 @@ def diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal,
 
 
 @_on_device
-def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, out, kept, dy, want):
-    """`out`: the forward pass's (needed without a norm weight); `want`: which of dq, (dk, dv), dlam, dweight are needed -> (dq, dk, dv, dlam, dweight)."""
+def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, kept, dy, want):
+    """`want`: which of dq, (dk, dv), dlam, dweight are needed -> (dq, dk, dv, dlam, dweight)."""
     q, qs = _rows16(q)
     k, ks = _rows16(k)
     v, vs = _rows16(v)
@@ -1668,11 +1670,11 @@ def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal
     shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys)
     ws = torch.empty(max(256, int(_lib.dfine_diff_attn_bwd_ws_bytes(shape))), device=q.device, dtype=torch.uint8)
     B, N, H, _, d = q.shape
-    _, o2_at, u_at = _da_kept(dy, weight is not None)
+    _, o2_at, u_at = _da_kept(dy)
     stats = kept.data_ptr()
     with _timed("diff_attention", 4.0 * B * H * N * k.shape[1] * (3 * d + 2 * v.shape[3]), io=2.0 * q.element_size() * (q.numel() + k.numel() + v.numel() + dy.numel())):
         _check(_lib.dfine_diff_attn_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(weight), _ptr(forms), _ptr(kv_len),
-                                        None if isinstance(start, int) else _ptr(start), _ptr(out), u_at and stats + u_at, stats + o2_at, stats, _ptr(dy), _ptr(dq),
+                                        None if isinstance(start, int) else _ptr(start), stats + u_at, stats + o2_at, stats, _ptr(dy), _ptr(dq),
                                         _ptr(dk), _ptr(dv), _ptr(dlam), _ptr(dweight), _ptr(ws), shape, scale, init, eps, _stream()), "dfine_diff_attn_bwd")
     return dq, dk, dv, dlam, dweight
 

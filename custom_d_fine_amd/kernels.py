@@ -2624,8 +2624,8 @@ class _DiffAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps):
         out, qr, kr, vr, kept = _hip().diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, True)
         users = [t for t in (forms, kv_len, start) if isinstance(t, torch.Tensor)]               # (each costs a microsecond on its way through the graph)
-        ctx.save_for_backward(qr, kr, vr, lam, out if weight is None else weight, kept, *users)
-        ctx.meta = (weight is not None, forms is not None, kv_len is not None, mask_batches, causal, None if isinstance(start, torch.Tensor) else start, scale, init,
+        ctx.save_for_backward(qr, kr, vr, lam, weight, kept, *users)
+        ctx.meta = (forms is not None, kv_len is not None, mask_batches, causal, None if isinstance(start, torch.Tensor) else start, scale, init,
                     eps)
         return out
 
@@ -2633,15 +2633,12 @@ class _DiffAttention(torch.autograd.Function):
     def backward(ctx, dy):
         _no_double_backward("diff_attention")
         q, k, v, lam, weight, kept, *users = ctx.saved_tensors
-        normed, has_forms, has_len, mask_batches, causal, start, scale, init, eps = ctx.meta
-        out = None
-        if not normed:
-            out, weight = weight, None
+        has_forms, has_len, mask_batches, causal, start, scale, init, eps = ctx.meta
         forms = users.pop(0) if has_forms else None
         kv_len = users.pop(0) if has_len else None
         n = ctx.needs_input_grad
         dq, dk, dv, dlam, dw = _hip().diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, users[0] if users else start, scale, init, eps,
-                                                         out, kept, dy, (n[0], n[1] or n[2], n[3], n[4]))
+                                                         kept, dy, (n[0], n[1] or n[2], n[3], n[4]))
         return (dq, dk if n[1] else None, dv if n[2] else None, dlam, dw, None, None, None, None, None, None, None, None)
 
 

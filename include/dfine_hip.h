@@ -832,11 +832,11 @@ int dfine_qk_norm_rotate_bwd(const void *q, const void *k, const void *wq, const
  * What query i of batch b sees: keys j < kv_len[b] (NULL: M; keys from there on are not read), j <= q_start[b] + i when causal (q_start NULL:
  * one start for all in shape), and where the mask lets it: mask_forms = the dfine_diff_attn_mask_words(batches, N, M) words that
  * dfine_diff_attn_mask makes of bytes [batches, N, M] (non-zero = may not attend; strides in bytes), batches 1 or B.
- * Forward for training keeps u, o2 (out's shape and type; u NULL without weight) and stats fp32 [4, B, H, N].
+ * Forward for training keeps u (out's shape, fp32), o2 (out's shape and type) and stats fp32 [4, B, H, N]; all NULL: not kept.
  * shape (host int64): B, N, M, H, Hk, d, dv, dtype (0 fp32, 1 bf16), heads of lam, lam bf16, weight bf16, causal, q_start, mask has batches, then the
  * strides (batch, token, head, map) of q, of k, (batch, token, head) of v, of dy (elements; 16-byte rows).
  * Forward ws: dfine_diff_attn_fwd_ws_bytes(shape) bytes, 256-byte aligned (0: NULL): few queries over many keys are cut into runs of the keys.
- * Backward: reads u with a weight, out without (the other may be NULL); dq, dk, dv contiguous (dq, or dk and dv, NULL: not wanted), dlam, dweight of lam's and weight's types (NULL: not wanted);
+ * Backward: dq, dk, dv contiguous (dq, or dk and dv, NULL: not wanted), dlam, dweight of lam's and weight's types (NULL: not wanted);
  * ws: dfine_diff_attn_bwd_ws_bytes(shape) bytes, 256-byte aligned.  Deterministic. */
 int64_t dfine_diff_attn_mask_words(int64_t batches, int64_t N, int64_t M);
 int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_t M, int64_t stride_b, int64_t stride_n, uint64_t *forms,
@@ -844,11 +844,11 @@ int dfine_diff_attn_mask(const uint8_t *mask, int64_t batches, int64_t N, int64_
 int64_t dfine_diff_attn_fwd_ws_bytes(const int64_t *shape);
 int64_t dfine_diff_attn_bwd_ws_bytes(const int64_t *shape);
 int dfine_diff_attn_fwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms,
-                        const int *kv_len, const int *q_start, void *out, void *u, void *o2, float *stats, void *ws,
+                        const int *kv_len, const int *q_start, void *out, float *u, void *o2, float *stats, void *ws,
                         const int64_t *shape, float scale, float init, float eps, void *stream);
 int dfine_diff_attn_bwd(const void *q, const void *k, const void *v, const void *lam, const void *weight, const uint64_t *mask_forms,
-                        const int *kv_len, const int *q_start, const void *out, const void *u, const void *o2, const float *stats,
-                        const void *dy, void *dq, void *dk, void *dv, void *dlam, void *dweight, void *ws, const int64_t *shape,
+                        const int *kv_len, const int *q_start, const float *u, const void *o2, const float *stats, const void *dy,
+                        void *dq, void *dk, void *dv, void *dlam, void *dweight, void *ws, const int64_t *shape,
                         float scale, float init, float eps, void *stream);
 
 #ifdef __cplusplus

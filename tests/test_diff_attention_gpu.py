@@ -1,7 +1,7 @@
 """csrc/diffattn.hip through kernels.diff_attention against a 64-bit restatement.
 
-Tolerances, in the 2-norm.  A rounding to bf16 is off by at most 2^-8 of the value; the probabilities (forward), U, A_1 V, dU and dS (backward) and the
-result are rounded once each.  out: 2 roundings; dV: P, U, A_1 V, dU, result = 5; dq, dk: also dS = 6; parameters: U, A_1 V, P, result = 4.  What such a
+Tolerances, in the 2-norm.  A rounding to bf16 is off by at most 2^-8 of the value; the probabilities (forward), A_1 V, dU and dS (backward) and the
+result are rounded once each.  out: 2 roundings; dV: P, A_1 V, dU, result = 4; dq, dk: also dS = 5; parameters: A_1 V, P, result = 3.  What such a
 rounding is 2^-8 of are the TERMS of the sums that follow it, and their errors add up as terms of random signs do: the larger of the result's 2-norm and of
 attention_block_ref.diff_attention_spread's.  (A row that sees ONE key shows why: dS = 0 there, and dl of a normed head is eps-small, while dP and D are not.)
 fp32: sums of n = M (N for dk, dv) terms in 32 bits, at most (n + 8 d + 64) 2^-24 with scores up to 8 * sqrt(d) * scale in the exponent, of the same."""
@@ -13,7 +13,7 @@ from . import attention_block_ref as ref
 pytestmark = pytest.mark.gpu
 
 INIT, EPS = 0.35, 1e-5
-ROUNDINGS = {"out": 2, "dq": 6, "dk": 6, "dv": 5, "dlam": 4, "dweight": 4}
+ROUNDINGS = {"out": 2, "dq": 5, "dk": 5, "dv": 4, "dlam": 3, "dweight": 3}
 
 
 def _tol(name, dtype, n, d):
