@@ -1551,6 +1551,11 @@ def _rows16(t):
     return t, st[:-1]
 
 
+def _plain(t):
+    """Contiguous on a 16-byte border."""
+    return t.is_contiguous() and not t.data_ptr() % 16
+
+
 def _on_device(fn):
     """The launcher on its first tensor's device: the stream and the new tensors are that device's."""
     here = _raw_device or torch.cuda.current_device
@@ -1572,34 +1577,41 @@ def _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks, dqs=(0, 0, 0), dks=
 
 @_on_device
 def qk_norm_rotate_forward(q, k, wq, wk, cos, sin, positions, eps, paired):
-    """q [B, L, Hq, D], k [B, L, Hk, D] or None -> the normed and rotated queries and keys (contiguous), and q, k as the kernel read them."""
+    """q [B, L, Hq, D], k [B, L, Hk, D] or None -> the normed and rotated queries and keys (contiguous), q, k as the kernel read them, and what the backward
+    pass need not work out again where its operands come as these did and the gradients contiguous (it runs on autograd's own thread, where Python is slow)."""
     q, qs = _rows16(q)
     ks = (0, 0, 0)
     if k is not None:
         k, ks = _rows16(k)
     yq = _EMPTY_LIKE(q)
     yk = None if k is None else _EMPTY_LIKE(k)
-    with _timed("qk_norm_rotate", 2.0 * q.element_size() * (q.numel() + (0 if k is None else k.numel()))):
+    B, L, Hq, D = q.shape
+    Hk = 0 if k is None else k.shape[2]
+    shape = _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks, (L * Hq * D, Hq * D, D), (L * Hk * D, Hk * D, D))
+    work = 2.0 * q.element_size() * B * L * (Hq + Hk) * D
+    with _timed("qk_norm_rotate", work):
         _check(_lib.dfine_qk_norm_rotate_fwd(_ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(yq), _ptr(yk),
-                                             _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks), eps, _stream()), "dfine_qk_norm_rotate_fwd")
-    return yq, yk, q, k
+                                             shape, eps, _stream()), "dfine_qk_norm_rotate_fwd")
+    return yq, yk, q, k, (shape, q.stride(), None if k is None else k.stride(), 1.5 * work)
 
 
 @_on_device
-def qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions, eps, paired, dyq, dyk, want_wq, want_wk):
-    q, qs = _rows16(q)
-    dyq, dqs = _rows16(dyq)
-    ks = dks = (0, 0, 0)
-    if k is not None:
-        k, ks = _rows16(k)
-        dyk, dks = _rows16(dyk)
+def qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions, eps, paired, dyq, dyk, want_wq, want_wk, plan):
+    shape, q_stride, k_stride, work = plan
+    if not (_plain(dyq) and q.stride() == q_stride and (k is None or (_plain(dyk) and k.stride() == k_stride))):
+        q, qs = _rows16(q)
+        dyq, dqs = _rows16(dyq)
+        ks = dks = (0, 0, 0)
+        if k is not None:
+            k, ks = _rows16(k)
+            dyk, dks = _rows16(dyk)
+        shape = _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks, dqs, dks)
     dq = _EMPTY_LIKE(q)
     dk = None if k is None else _EMPTY_LIKE(k)
     dwq = torch.empty_like(wq) if want_wq else None
     dwk = torch.empty_like(wk) if want_wk else None
-    shape = _qkn_shape(q, k, wq, wk, cos, positions, paired, qs, ks, dqs, dks)
     ws = torch.empty(max(1, int(_lib.dfine_qk_norm_rotate_ws_floats(shape))), device=q.device, dtype=torch.float32)
-    with _timed("qk_norm_rotate", 3.0 * q.element_size() * (q.numel() + (0 if k is None else k.numel()))):
+    with _timed("qk_norm_rotate", work):
         _check(_lib.dfine_qk_norm_rotate_bwd(_ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(dyq), _ptr(dyk), _ptr(dq),
                                              _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(ws), shape, eps, _stream()), "dfine_qk_norm_rotate_bwd")
     return dq, dk, dwq, dwk
@@ -1634,7 +1646,8 @@ def _da_kept(out):
 
 @_on_device
 def diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, keep):
-    """-> out [B, N, H, dv], q, k, v as the kernel read them, and with `keep` what else the backward pass reads, one buffer (else None)."""
+    """-> out [B, N, H, dv], q, k, v as the kernel read them, and with `keep` what else the backward pass reads, one buffer, and what it need not work out
+    again (else None)."""
     q, qs = _rows16(q)
     k, ks = _rows16(k)
     v, vs = _rows16(v)
@@ -1647,32 +1660,34 @@ def diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal,
         kept = torch.empty(size, device=q.device, dtype=torch.uint8)
         stats = kept.data_ptr()
         o2, u = stats + o2_at, stats + u_at
-    shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs)
+    shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, (N * H * dv, H * dv, dv))
     nws = _lib.dfine_diff_attn_fwd_ws_bytes(shape)
     ws = torch.empty(nws, device=q.device, dtype=torch.uint8) if nws > 0 else None
-    with _timed("diff_attention", 4.0 * B * H * N * M * (d + dv), io=float(q.element_size()) * (q.numel() + k.numel() + v.numel() + out.numel())):
+    pairs, io = 4.0 * B * H * N * M, float(q.element_size()) * (q.numel() + k.numel() + v.numel() + out.numel())
+    with _timed("diff_attention", pairs * (d + dv), io=io):
         _check(_lib.dfine_diff_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(weight), _ptr(forms), _ptr(kv_len),
                                         None if isinstance(start, int) else _ptr(start), _ptr(out), u, o2, stats, _ptr(ws), shape, scale, init, eps, _stream()),
                "dfine_diff_attn_fwd")
-    return out, q, k, v, kept
+    plan = (shape, o2_at, u_at, int(_lib.dfine_diff_attn_bwd_ws_bytes(shape)), q.stride(), k.stride(), v.stride(), pairs * (3 * d + 2 * dv), 2.0 * io) if keep else None
+    return out, q, k, v, kept, plan
 
 
 @_on_device
-def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, kept, dy, want):
-    """`want`: which of dq, (dk, dv), dlam, dweight are needed -> (dq, dk, dv, dlam, dweight)."""
-    q, qs = _rows16(q)
-    k, ks = _rows16(k)
-    v, vs = _rows16(v)
-    dy, dys = _rows16(dy)
+def diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, kept, dy, want, plan):
+    """`want`: which of dq, (dk, dv), dlam, dweight are needed; kept, plan: diff_attn_forward's -> (dq, dk, dv, dlam, dweight)."""
+    shape, o2_at, u_at, nws, q_stride, k_stride, v_stride, work, io = plan
+    if not (_plain(dy) and q.stride() == q_stride and k.stride() == k_stride and v.stride() == v_stride):
+        q, qs = _rows16(q)
+        k, ks = _rows16(k)
+        v, vs = _rows16(v)
+        dy, dys = _rows16(dy)
+        shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys)
     new = lambda t, on: _EMPTY_LIKE(t) if on else None  # noqa: E731
     dq, dk, dv, dlam = new(q, want[0]), new(k, want[1]), new(v, want[1]), new(lam, want[2])
     dweight = None if weight is None else new(weight, want[3])
-    shape = _da_shape(q, k, v, lam, weight, mask_batches, causal, start, qs, ks, vs, dys)
-    ws = torch.empty(max(256, int(_lib.dfine_diff_attn_bwd_ws_bytes(shape))), device=q.device, dtype=torch.uint8)
-    B, N, H, _, d = q.shape
-    _, o2_at, u_at = _da_kept(dy)
+    ws = torch.empty(max(256, nws), device=q.device, dtype=torch.uint8)
     stats = kept.data_ptr()
-    with _timed("diff_attention", 4.0 * B * H * N * k.shape[1] * (3 * d + 2 * v.shape[3]), io=2.0 * q.element_size() * (q.numel() + k.numel() + v.numel() + dy.numel())):
+    with _timed("diff_attention", work, io=io):
         _check(_lib.dfine_diff_attn_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(weight), _ptr(forms), _ptr(kv_len),
                                         None if isinstance(start, int) else _ptr(start), stats + u_at, stats + o2_at, stats, _ptr(dy), _ptr(dq),
                                         _ptr(dk), _ptr(dv), _ptr(dlam), _ptr(dweight), _ptr(ws), shape, scale, init, eps, _stream()), "dfine_diff_attn_bwd")

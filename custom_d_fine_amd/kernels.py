@@ -2516,13 +2516,14 @@ def _no_double_backward(op):
 
 class _QKNormRotate(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, paired):
-        yq, yk, qr, kr = _hip().qk_norm_rotate_forward(q, k, wq, wk, cos, sin, positions, eps, paired)
+    def forward(ctx, q, k, wq, wk, rest):
+        cos, sin, positions, eps, paired = rest    # (one operand: what takes no gradient costs its way through the graph all the same)
+        yq, yk, qr, kr, plan = _hip().qk_norm_rotate_forward(q, k, wq, wk, cos, sin, positions, eps, paired)
         if positions is None:                      # (each tensor costs a microsecond on its way through the graph)
             ctx.save_for_backward(qr, kr, wq, wk, cos, sin)
         else:
             ctx.save_for_backward(qr, kr, wq, wk, cos, sin, positions)
-        ctx.meta = (eps, paired)
+        ctx.meta = (eps, paired, plan)
         return yq, yk
 
     @staticmethod
@@ -2530,9 +2531,9 @@ class _QKNormRotate(torch.autograd.Function):
         _no_double_backward("qk_norm_rotate")
         q, k, wq, wk, cos, sin, *positions = ctx.saved_tensors
         need = ctx.needs_input_grad
-        eps, paired = ctx.meta
-        dq, dk, dwq, dwk = _hip().qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions[0] if positions else None, eps, paired, dyq, dyk, need[2], need[3])
-        return dq, dk, dwq, dwk, None, None, None, None, None
+        eps, paired, plan = ctx.meta
+        dq, dk, dwq, dwk = _hip().qk_norm_rotate_backward(q, k, wq, wk, cos, sin, positions[0] if positions else None, eps, paired, dyq, dyk, need[2], need[3], plan)
+        return dq, dk, dwq, dwk, None
 
 
 def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, positions=None, eps: float = 1e-6, interleaved: bool = False):
@@ -2608,7 +2609,7 @@ def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, posit
     if not q.is_cuda:
         return _backend_for_cpu(op)(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))
     if grad and torch.is_grad_enabled():
-        return _QKNormRotate.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))
+        return _QKNormRotate.apply(q, k, q_weight, k_weight, (cos, sin, positions, eps, bool(interleaved)))
     return _hip().qk_norm_rotate_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))[:2]
 
 
@@ -2621,25 +2622,25 @@ def _index32(t):
 
 class _DiffAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps):
-        out, qr, kr, vr, kept = _hip().diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, True)
+    def forward(ctx, q, k, v, lam, weight, rest):
+        forms, mask_batches, kv_len, causal, start, scale, init, eps = rest
+        out, qr, kr, vr, kept, plan = _hip().diff_attn_forward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, start, scale, init, eps, True)
         users = [t for t in (forms, kv_len, start) if isinstance(t, torch.Tensor)]               # (each costs a microsecond on its way through the graph)
         ctx.save_for_backward(qr, kr, vr, lam, weight, kept, *users)
-        ctx.meta = (forms is not None, kv_len is not None, mask_batches, causal, None if isinstance(start, torch.Tensor) else start, scale, init,
-                    eps)
+        ctx.meta = (forms is not None, kv_len is not None, mask_batches, causal, None if isinstance(start, torch.Tensor) else start, scale, init, eps, plan)
         return out
 
     @staticmethod
     def backward(ctx, dy):
         _no_double_backward("diff_attention")
         q, k, v, lam, weight, kept, *users = ctx.saved_tensors
-        has_forms, has_len, mask_batches, causal, start, scale, init, eps = ctx.meta
+        has_forms, has_len, mask_batches, causal, start, scale, init, eps, plan = ctx.meta
         forms = users.pop(0) if has_forms else None
         kv_len = users.pop(0) if has_len else None
         n = ctx.needs_input_grad
         dq, dk, dv, dlam, dw = _hip().diff_attn_backward(q, k, v, lam, weight, forms, mask_batches, kv_len, causal, users[0] if users else start, scale, init, eps,
-                                                         kept, dy, (n[0], n[1] or n[2], n[3], n[4]))
-        return (dq, dk if n[1] else None, dv if n[2] else None, dlam, dw, None, None, None, None, None, None, None, None)
+                                                         kept, dy, (n[0], n[1] or n[2], n[3], n[4]), plan)
+        return dq, dk if n[1] else None, dv if n[2] else None, dlam, dw, None
 
 
 def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None, norm_eps: float = 1e-5, attn_mask=None, kv_lengths=None, causal: bool = False,
@@ -2720,7 +2721,7 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
         forms = _hip().diff_attn_mask_forms(attn_mask if attn_mask.dim() == 3 else attn_mask[None])
     batches = attn_mask is not None and attn_mask.dim() == 3 and B > 1
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad or (weight is not None and weight.requires_grad)):
-        return _DiffAttention.apply(q, k, v, lam, weight, forms, batches, kv_len, bool(causal), start, scale, init, eps)
+        return _DiffAttention.apply(q, k, v, lam, weight, (forms, batches, kv_len, bool(causal), start, scale, init, eps))
     return _hip().diff_attn_forward(q, k, v, lam, weight, forms, batches, kv_len, bool(causal), start, scale, init, eps, False)[0]
 
 
