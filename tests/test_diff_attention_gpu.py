@@ -344,6 +344,89 @@ def test_attention_block_of_a_token_stream(cuda):
         assert ref.rel(a, b) <= 2.5 * 12 * 2 ** -8, i
 
 
+def test_decoding_steps_captured(cuda):
+    """One token at a time: norms + rotation at the token's position, the cache written, attention over the filled part.  The step is captured once and replayed
+    for every token, eager work between the replays; each equals the eager step, and the last the whole sequence at once within the roundings of both."""
+    from custom_d_fine_amd import kernels
+    B, M, H, Hk, d, dv, steps = 3, 1500, 4, 2, 32, 64, 6
+    g = torch.Generator().manual_seed(21)
+    mk = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    toks = [[t.bfloat16().to(cuda) for t in (mk(B, 1, 2 * H, d), mk(B, 1, 2 * Hk, d), mk(B, 1, Hk, dv))] for _ in range(steps)]
+    wq, wk, wn, lam = (1 + 0.1 * mk(d)).to(cuda), (1 + 0.1 * mk(d)).to(cuda), (1 + 0.1 * mk(dv)).to(cuda), (0.1 * mk(4, H, d)).to(cuda)
+    angle = torch.arange(M)[:, None] * 100.0 ** (-torch.arange(d // 2) / (d // 2))
+    cos, sin = angle.cos().to(cuda), angle.sin().to(cuda)
+    first = torch.tensor([3, 1200, 700], device=cuda)
+    batch = torch.arange(B, device=cuda)
+
+    def state():
+        gg = torch.Generator().manual_seed(22)
+        k0, v0 = torch.randn(B, M, Hk, 2, d, generator=gg).bfloat16().to(cuda), torch.randn(B, M, Hk, dv, generator=gg).bfloat16().to(cuda)
+        return {"k": k0, "v": v0, "len": first.clone(), "in": [t.clone() for t in toks[0]]}
+
+    def step(s):
+        q, k = kernels.qk_norm_rotate(s["in"][0], s["in"][1], wq, wk, cos, sin, s["len"][:, None])
+        s["k"][batch, s["len"]] = k.view(B, Hk, 2, d)
+        s["v"][batch, s["len"]] = s["in"][2][:, 0]
+        s["len"] += 1
+        return kernels.diff_attention(q.view(B, 1, H, 2, d), s["k"], s["v"], lam, INIT, wn, EPS, kv_lengths=s["len"])
+
+    with torch.no_grad():
+        side, cap, eager = torch.cuda.Stream(), state(), state()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(cap)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(cap)
+        fresh = state()
+        for a, b in zip((cap["k"], cap["v"], cap["len"]), (fresh["k"], fresh["v"], fresh["len"])):
+            a.copy_(b)
+        for t in toks:
+            for s in (cap, eager):
+                for a, b in zip(s["in"], t):
+                    a.copy_(b)
+            want = step(eager)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        # the tokens at once, behind each sequence's own prefix
+        q, k = kernels.qk_norm_rotate(torch.cat([t[0] for t in toks], 1), torch.cat([t[1] for t in toks], 1), wq, wk, cos, sin,
+                                      first[:, None] + torch.arange(steps, device=cuda))
+        whole = kernels.diff_attention(q.view(B, steps, H, 2, d), eager["k"], eager["v"], lam, INIT, wn, EPS, causal=True, query_start=first)
+        assert torch.equal(eager["k"][1, 1200:1200 + steps], k.view(B, steps, Hk, 2, d)[1])
+        assert ref.rel(whole[:, -1:], want) <= 2 * 2.5 * _tol("out", torch.bfloat16, M, d)
+
+
+def test_saved_tensors_that_moved_and_a_second_backward(cuda):
+    """What the graph saved comes back from the host with other strides; a graph that is kept gives its gradients again; operands that are recomputed."""
+    from torch.utils.checkpoint import checkpoint
+
+    from custom_d_fine_amd import kernels
+    B, N, H, d, dv = 2, 90, 4, 32, 64
+    g = torch.Generator().manual_seed(5)
+    packed = torch.randn(B, N, H * (4 * d + dv), generator=g).bfloat16().to(cuda)
+    lam, w = (0.1 * torch.randn(4, H, d, generator=g)).to(cuda), torch.ones(dv, device=cuda)
+    mask = (torch.rand(N, N, generator=g) < 0.3).to(cuda)
+    dy = torch.randn(B, N, H, dv, generator=g).bfloat16().to(cuda)
+
+    def f(p, l, n):
+        q, k = kernels.qk_norm_rotate(p[..., :2 * H * d].view(B, N, 2 * H, d), p[..., 2 * H * d:4 * H * d].view(B, N, 2 * H, d))
+        return kernels.diff_attention(q.view(B, N, H, 2, d), k.view(B, N, H, 2, d), p[..., 4 * H * d:].view(B, N, H, dv), l, INIT, n, EPS, attn_mask=mask)
+
+    leaves = [t.clone().requires_grad_(True) for t in (packed, lam, w)]
+    y = f(*leaves)
+    base = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        z = f(*leaves)
+    moved = torch.autograd.grad(z, leaves, dy)
+    redone = torch.autograd.grad(checkpoint(f, *leaves, use_reentrant=False), leaves, dy)
+    for one in (again, moved, redone):
+        for a, b in zip(one, base):
+            assert torch.equal(a, b)
+
+
 def test_offsets_past_32_bits(cuda):
     """A cache of 4.3 GB whose second sequence and last tokens lie past 2^31 elements: sequence stride 2^30 + 512, token stride 2^24 and 64 tokens."""
     from custom_d_fine_amd import kernels
