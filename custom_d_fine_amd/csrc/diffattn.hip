@@ -559,8 +559,8 @@ __device__ __forceinline__ float da_lse(float m, float l) { return l > 0.f ? m +
 // in front is worked on (one barrier per block).
 // 128 rows read a key once from L2 for 4 waves; two waves per SIMD (registers: DK = 64) hide each other's LDS and matrix latencies.  Bound: the vector unit for
 // heads up to 32 channels (16 exponentials, maxima, sums and conversions per 12 products of 32 cycles), vector and matrix unit about alike at 64.
-// Measured: 8192 causal tokens, 16 heads on 4, 2 x 64 channels bf16 522 us (790 TFLOP/s; a plain 8192^3 product reaches 1177 here); 32 x 492 tokens with their group
-// mask, 4 heads of 2 x 32, results for the backward kept, 31 us; 8 x 900 tokens, 8 heads of 2 x 24, 51 us; 16 x 396 tokens of 4 heads in fp32 64 us.
+// Measured: 8192 causal tokens, 16 heads on 4, 2 x 64 channels bf16 494 - 520 us (790 - 830 TFLOP/s; a plain 8192^3 product reaches 1177 here); 32 x 492 tokens with their group
+// mask, 4 heads of 2 x 32, results for the backward kept, 32 us; 8 x 900 tokens, 8 heads of 2 x 24, 51 us; 16 x 396 tokens of 4 heads in fp32 64 us.
 template <typename T, int DK>
 __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) void diff_attn_fwd_kernel(const DiffArgs a) {
     using C = DaCfg<T, DK>;
@@ -1174,7 +1174,7 @@ __global__ __launch_bounds__(1024) void diff_attn_param_kernel(const DiffArgs a,
 // backward, dQ: the forward's decomposition and copies; probabilities from the saved statistics, nothing to rescale.  dS is rounded to bf16 for its product with K (as the keys it meets
 // are), dU for its product with V: each adds 0.0017 to dq's relative error, 0.0030 in all with the result's own 0.0017.  Keeping either in two bf16 terms would
 // cost a third more products for 0.0025.
-// Bound as the forward: 495 us and 835 TFLOP/s at 8192 causal tokens, 27 us at 32 x 492, 58 us in fp32 at 16 x 396.
+// Bound as the forward: 473 - 495 us (835 - 870 TFLOP/s) at 8192 causal tokens, 27 us at 32 x 492, 58 us in fp32 at 16 x 396.
 template <typename T, int DK>
 __device__ __forceinline__ void da_dq_tile(const DiffArgs &a, da_f16v (*dq)[DaCfg<T, DK>::MTK], const uint4 (*qf)[DaCfg<T, DK>::NF], const uint4 *uf, const float *lse, const float *dl,
                                            float sign, const DaLane<T, DK> &ln, uint32_t tk, uint32_t tv, bool masked, uint32_t vis, int lane) {
@@ -1349,7 +1349,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
 // queries of the group's heads stream through two LDS buffers of QB rows (Q | dU | four statistics), copied while the block in front is worked on.
 // The rows' statistics are what the products start from (S at -lse / c, dP at -D_0): they come from LDS straight into the accumulators.
 // Both operands and both results of 64-channel heads are 385 registers, one wave per SIMD: vector and matrix work of a tile follow each other, which bounds it.
-// Measured: 900 us at 8192 causal tokens (610 TFLOP/s), 37 us at 32 x 492, 77 us in fp32 at 16 x 396.  Two waves for the same 32 keys, one map each (two waves per
+// Measured: 844 - 900 us at 8192 causal tokens (610 - 650 TFLOP/s), 37 us at 32 x 492, 77 us in fp32 at 16 x 396.  Two waves for the same 32 keys, one map each (two waves per
 // SIMD, dP worked out twice), took 942 us where this took 901; both mask forms of a tile as code of their own 1140 (the accumulators change places between them).
 template <typename T, int DK>
 __device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[DaCfg<T, DK>::MTK], da_f16v *dv, const uint4 (*kf)[DaCfg<T, DK>::NF], const uint4 *vf, float sign,
