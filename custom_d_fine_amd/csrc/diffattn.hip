@@ -1348,7 +1348,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
 // backward, dK and dV: workgroup = (batch, key head, 128 keys, one of kvruns runs of the rows), a wave owns 32 keys with both operands in registers; the
 // queries of the group's heads stream through two LDS buffers of QB rows (Q | dU | four statistics), copied while the block in front is worked on.
 // The rows' statistics are what the products start from (S at -lse / c, dP at -D_0): they come from LDS straight into the accumulators.
-// Both operands and both results of 64-channel heads are 385 registers, one wave per SIMD: vector and matrix work of a tile follow each other, which bounds it.
+// Both operands and both results of 64-channel heads are 192 registers of 323, one wave per SIMD: vector and matrix work of a tile follow each other, which bounds it.
 // Measured: 844 - 900 us at 8192 causal tokens (610 - 650 TFLOP/s), 37 us at 32 x 492, 77 us in fp32 at 16 x 396.  Two waves for the same 32 keys, one map each (two waves per
 // SIMD, dP worked out twice), took 942 us where this took 901; both mask forms of a tile as code of their own 1140 (the accumulators change places between them).
 template <typename T, int DK>
