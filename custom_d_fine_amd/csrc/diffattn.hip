@@ -552,6 +552,8 @@ template <typename T, int W> struct DaRowsOut {
 };
 
 __device__ __forceinline__ float da_inv(float l) { return l > 0.f ? 1.f / l : l; }                 // an empty row: 0; not a number stays that
+// the norm's factor from sum U^2; a row that sees no key: 0, so that its result is 0 with eps = 0 too (1 / sqrt(0) times 0 is not a number)
+__device__ __forceinline__ float da_norm(float ss, const DiffArgs &a, bool empty) { return empty ? 0.f : rsqrtf(ss / (float)a.dv + a.eps); }
 __device__ __forceinline__ float da_lse(float m, float l) { return l > 0.f ? m + log2f(l) : l == 0.f ? INFINITY : l; }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -659,7 +661,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
     ss = da_both_halves(ss);
     us = da_both_halves(us);
     const float beta = e.weight && ss > 0.f ? us / ss : 0.f;  // what is kept of A_1 V is its part at right angles to U (diff_attn_prep_kernel)
-    const float rn = e.weight ? rsqrtf(ss / (float)e.dv + e.eps) : 1.f;
+    const float rn = e.weight ? da_norm(ss, e, l0 == 0.f) : 1.f;
     int row = blk0 + wave * 32 + l32;
     asm volatile("" : "+v"(row));                             // (worked out again: the row's numbers are not held over the loop either)
     if (e.stats && h2 == 0 && row < R) {
@@ -725,7 +727,7 @@ __device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, i
 #pragma unroll
     for (int x = 1; x < LPR; x <<= 1) { ss += __shfl_xor(ss, x); us += __shfl_xor(us, x); }
     const float beta = a.weight && ss > 0.f ? us / ss : 0.f;
-    const float rn = a.weight ? rsqrtf(ss / (float)a.dv + a.eps) : 1.f;
+    const float rn = a.weight ? da_norm(ss, a, lse0 == INFINITY) : 1.f;
     const int64_t orow = (((int64_t)b * a.N + i) * a.H + head) * a.dv;
 #pragma unroll
     for (int j = 0; j < NE; j += 4) {

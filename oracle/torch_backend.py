@@ -158,7 +158,8 @@ def diff_attention(q, k, v, lam, init, weight, eps, mask, kv_lengths, causal, st
     l = (x[0] * x[1]).sum(-1).exp() - (x[2] * x[3]).sum(-1).exp() + init
     u = ((a[:, :, 0] - l[:, None, None] * a[:, :, 1]) @ vh).transpose(1, 2)
     if weight is not None:
-        u = (1 - init) * u / torch.sqrt((u ** 2).mean(-1, keepdim=True) + eps) * weight.float()
+        empty = ~seen.any(2)[:, :, None, None]                        # (eps may be 0)
+        u = (1 - init) * u / torch.sqrt(torch.where(empty, 1.0, (u ** 2).mean(-1, keepdim=True) + eps)) * weight.float()
     return u.to(q.dtype)
 
 

@@ -1,0 +1,39 @@
+"""Calls of qk_norm_rotate and diff_attention at the border of what they take: no epsilon under rows that see nothing."""
+import pytest
+import torch
+
+from . import attention_block_ref as ref
+from .test_diff_attention_gpu import EPS, INIT, _inputs, _off, _tol
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float32]
+
+
+# one run of the keys, runs that are joined, many rows
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,N,M,H,Hk,d,dv", [(2, 70, 140, 6, 3, 32, 64), (3, 3, 3000, 8, 2, 64, 128), (16, 130, 130, 8, 8, 16, 32)])
+@pytest.mark.parametrize("eps", [0.0, 1e-60])                        # (1e-60: 0 in 32 bits)
+def test_rows_that_see_nothing_without_epsilon(cuda, dtype, eps, B, N, M, H, Hk, d, dv):
+    from custom_d_fine_amd import kernels
+    q, k, v, lam, w, dy, g = _inputs(cuda, B, N, M, H, Hk, d, dv, dtype)
+    mask = torch.rand(N, M, generator=g) < 0.3
+    mask[::3] = True
+    mask = mask.to(cuda)
+    lens = torch.full((B,), M, device=cuda)
+    lens[-1] = 0
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam, w)]
+    y = kernels.diff_attention(*leaves[:4], INIT, norm_weight=leaves[4], norm_eps=eps, attn_mask=mask, kv_lengths=lens)
+    grads = torch.autograd.grad(y, leaves, dy)
+    seen = ref.visible(B, N, M, mask, lens, device=cuda)
+    none = ~seen.any(2)
+    assert (y[none] == 0).all() and (grads[0][none] == 0).all()
+    assert all(torch.isfinite(t).all() for t in grads)
+    full = [t.double() for t in (q, k, v, lam)]
+    want = ref.diff_attention(*full, INIT, w.double(), eps, seen, d ** -0.5)
+    spread = ref.diff_attention_spread(*full, INIT, w.double(), EPS, seen, d ** -0.5, dy.double())["out"]
+    assert _off(y[~none], want[~none], spread) <= _tol("out", dtype, M, d)
+    with torch.no_grad():                                            # no key at all
+        y = kernels.diff_attention(q, k, v, lam, INIT, w, eps, attn_mask=torch.ones(N, M, dtype=torch.bool, device=cuda))
+        z = kernels.diff_attention(q, k[:, :0], v[:, :0], lam, INIT, w, eps)
+    assert (y == 0).all() and (z == 0).all()
