@@ -2509,6 +2509,19 @@ def _float_operand(op, name, t, device, dtypes=_ACT_DTYPES):
         _refuse(f"{op}: {name} is on {t.device}, the queries are not")
 
 
+_FORWARD_AD, _TRACING = torch.autograd.forward_ad, torch._C._get_tracing_state
+
+
+def _only_reverse_mode(op, *operands):
+    """A tangent or a trace would be lost on the way past the autograd function (and a trace would keep the addresses of its own run)."""
+    if _FORWARD_AD._current_level >= 0:        # inside a dual level
+        for t in operands:
+            if t is not None and _FORWARD_AD.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"custom_d_fine_amd.kernels.{op}: no forward-mode derivative")
+    if _TRACING() is not None:
+        raise RuntimeError(f"custom_d_fine_amd.kernels.{op}: not under torch.jit.trace")
+
+
 def _no_double_backward(op):
     if torch.is_grad_enabled():                # create_graph=True: the kernels' results would come back without a graph
         raise RuntimeError(f"custom_d_fine_amd.kernels.{op}: no second derivative (create_graph=True)")
@@ -2542,7 +2555,8 @@ def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, posit
     q [B, L, heads, D], k [B, L, key heads, D] or None, float32 / bfloat16, any strides (rows that are not on 16-byte borders are copied);
     D and 2 * cos.shape[1] multiples of 8, D <= 256.  q_weight, k_weight [D] (None: ones).  cos, sin float32 [T, R / 2] (None: no rotation):
     channels (j, j + R / 2) - with `interleaved` (2j, 2j + 1) - turn by row positions[.., l] of the table (None: row l); channels from R on
-    pass.  positions: int32 / int64 [L] or [B, L]; a position outside the table gives NaN.  Gradients for q, k and the weights.
+    pass.  positions: int32 / int64 [L] or [B, L]; a position outside the table gives NaN.  Gradients for q, k and the weights (first derivatives, not
+    under create_graph=True; forward-mode derivatives and torch.jit.trace are refused).
     -> (q', k'), contiguous, of q's type (k' None without k).  Under bf16 autocast q and k are cast to bfloat16 first."""
     op = "qk_norm_rotate"
     device = q.get_device() if isinstance(q, torch.Tensor) else None
@@ -2608,6 +2622,7 @@ def qk_norm_rotate(q, k, q_weight=None, k_weight=None, cos=None, sin=None, posit
         _refuse(f"{op}: eps {eps}")
     if not q.is_cuda:
         return _backend_for_cpu(op)(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))
+    _only_reverse_mode(op, q, k, q_weight, k_weight, cos, sin)
     if grad and torch.is_grad_enabled():
         return _QKNormRotate.apply(q, k, q_weight, k_weight, (cos, sin, positions, eps, bool(interleaved)))
     return _hip().qk_norm_rotate_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, bool(interleaved))[:2]
@@ -2655,7 +2670,8 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
     padded batch or a cache that is not full; keys from there on are never read), and when `causal` j <= query_start + i (an int, or int [B]: the position
     of the first query among the keys).  A query that sees no key gives 0 and takes no gradient.  Keys that some query sees hold finite numbers; keys that
     the mask hides from every query, and keys behind kv_lengths or the last causal position, may hold anything.
-    Gradients for q, k, v, lambda_vectors and norm_weight, added up in a fixed order.  -> [B, N, H, dv], contiguous, of q's type.  Under bf16 autocast
+    Gradients for q, k, v, lambda_vectors and norm_weight, added up in a fixed order (first derivatives, not under create_graph=True; forward-mode
+    derivatives and torch.jit.trace are refused).  -> [B, N, H, dv], contiguous, of q's type.  Under bf16 autocast
     q, k, v are cast to bfloat16 first.  scale: d ** -0.5 by default, at least 1e-30."""
     op = "diff_attention"
     device = q.get_device() if isinstance(q, torch.Tensor) else None
@@ -2713,6 +2729,7 @@ def diff_attention(q, k, v, lambda_vectors, lambda_init: float, norm_weight=None
         _refuse(f"{op}: norm_eps {eps}")
     if not q.is_cuda:
         return _backend_for_cpu(op)(q, k, v, lambda_vectors, init, norm_weight, eps, attn_mask, kv_lengths, bool(causal), query_start, scale)
+    _only_reverse_mode(op, q, k, v, lambda_vectors, norm_weight)
     lam, weight = lambda_vectors.contiguous(), None if norm_weight is None else norm_weight.contiguous()
     kv_len = None if kv_lengths is None else _index32(kv_lengths)
     start = _index32(query_start) if starts else int(query_start)

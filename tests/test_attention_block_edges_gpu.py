@@ -1,4 +1,5 @@
-"""Calls of qk_norm_rotate and diff_attention at the border of what they take: no epsilon under rows that see nothing."""
+"""Calls of qk_norm_rotate and diff_attention at the border of what they take: no epsilon under rows that see nothing, derivatives and traces that go past the
+autograd functions."""
 import pytest
 import torch
 
@@ -37,3 +38,41 @@ def test_rows_that_see_nothing_without_epsilon(cuda, dtype, eps, B, N, M, H, Hk,
         y = kernels.diff_attention(q, k, v, lam, INIT, w, eps, attn_mask=torch.ones(N, M, dtype=torch.bool, device=cuda))
         z = kernels.diff_attention(q, k[:, :0], v[:, :0], lam, INIT, w, eps)
     assert (y == 0).all() and (z == 0).all()
+
+
+def _norm_inputs(cuda):
+    g = torch.Generator().manual_seed(4)
+    q, k = torch.randn(2, 5, 4, 16, generator=g).to(cuda), torch.randn(2, 5, 2, 16, generator=g).to(cuda)
+    wq, wk = (1 + 0.2 * torch.randn(16, generator=g)).to(cuda), (1 + 0.2 * torch.randn(16, generator=g)).to(cuda)
+    angle = torch.rand(5, 4, generator=g)
+    return [q, k, wq, wk, angle.cos().to(cuda), angle.sin().to(cuda)]
+
+
+def test_forward_mode_derivatives_are_refused(cuda):
+    """An operand with a tangent is refused, with and without gradients; without one a call inside a dual level is as it is outside."""
+    import torch.autograd.forward_ad as fw
+
+    from custom_d_fine_amd import kernels
+    heads = list(_inputs(cuda, 1, 9, 9, 6, 6, 16, 32, torch.float32)[:5])
+    attend = lambda q, k, v, lam, w: kernels.diff_attention(q, k, v, lam, INIT, norm_weight=w)  # noqa: E731
+    for call, args in ((attend, heads), (lambda *a: kernels.qk_norm_rotate(*a)[0], _norm_inputs(cuda))):
+        base = call(*args)
+        with fw.dual_level():
+            assert torch.equal(call(*args), base)
+            for at in range(len(args)):
+                dual = [fw.make_dual(t, torch.ones_like(t)) if j == at else t for j, t in enumerate(args)]
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*dual)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*dual)
+        assert torch.equal(call(*args), base)
+
+
+def test_traces_are_refused(cuda):
+    from custom_d_fine_amd import kernels
+    q, k, v, lam, w, _, _ = _inputs(cuda, 1, 9, 9, 6, 6, 16, 32, torch.float32)
+    with pytest.raises(RuntimeError, match="torch.jit.trace"):
+        torch.jit.trace(lambda x: kernels.diff_attention(x, k, v, lam, INIT, w), (q,), check_trace=False)
+    args = _norm_inputs(cuda)
+    with pytest.raises(RuntimeError, match="torch.jit.trace"):
+        torch.jit.trace(lambda x: kernels.qk_norm_rotate(x, *args[1:])[0], (args[0],), check_trace=False)
