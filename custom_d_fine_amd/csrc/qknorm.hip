@@ -208,8 +208,8 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rotate_kernel(const QkNorm
                     if (a.paired) {
 #pragma unroll
                         for (int j = 0; j < V; j += 2) {
-                            out[j] = n[j] * c[j] - n[j + 1] * s[j];
-                            out[j + 1] = n[j + 1] * c[j] + n[j] * s[j];
+                            out[j] = turns ? n[j] * c[j] - n[j + 1] * s[j] : n[j];       // (not n 1 - n' 0: a channel that passes takes nothing of its neighbour)
+                            out[j + 1] = turns ? n[j + 1] * c[j] + n[j] * s[j] : n[j + 1];
                         }
                     } else {
                         float xp[V];
@@ -223,8 +223,8 @@ __global__ __launch_bounds__(kQkThreads) void qk_norm_rotate_kernel(const QkNorm
                     if (a.paired) {
 #pragma unroll
                         for (int j = 0; j < V; j += 2) {
-                            dn[j] = g[j] * c[j] + g[j + 1] * s[j];
-                            dn[j + 1] = g[j + 1] * c[j] - g[j] * s[j];
+                            dn[j] = turns ? g[j] * c[j] + g[j + 1] * s[j] : g[j];
+                            dn[j + 1] = turns ? g[j + 1] * c[j] - g[j] * s[j] : g[j + 1];
                         }
                     } else {
                         float gp[V];

@@ -1,5 +1,5 @@
 """Calls of qk_norm_rotate and diff_attention at the border of what they take: no epsilon under rows that see nothing, derivatives and traces that go past the
-autograd functions."""
+autograd functions, channels that the rotation leaves alone."""
 import pytest
 import torch
 
@@ -76,3 +76,28 @@ def test_traces_are_refused(cuda):
     args = _norm_inputs(cuda)
     with pytest.raises(RuntimeError, match="torch.jit.trace"):
         torch.jit.trace(lambda x: kernels.qk_norm_rotate(x, *args[1:])[0], (args[0],), check_trace=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_channels_that_pass_know_nothing_of_their_neighbours(cuda, dtype, what):
+    """Channels from 8 on are not rotated: what channel 12 holds, its weight or its gradient, stays out of channel 13, in either order of the pairs."""
+    from custom_d_fine_amd import kernels
+    q, _, w, _, cos, sin = _norm_inputs(cuda)
+    q = q.to(dtype)
+    others = [c for c in range(16) if c != 12]
+    for interleaved in (True, False):
+        base = kernels.qk_norm_rotate(q, None, w, None, cos, sin, interleaved=interleaved)[0]
+        bad = w.clone()
+        bad[12] = what
+        y = kernels.qk_norm_rotate(q, None, bad, None, cos, sin, interleaved=interleaved)[0]
+        assert torch.equal(y[..., others], base[..., others]) and not torch.isfinite(y[..., 12]).any()
+        wl = w.clone().requires_grad_(True)
+        dy = torch.ones_like(base)
+        dy[..., 12] = what
+        (dw,) = torch.autograd.grad(kernels.qk_norm_rotate(q, None, wl, None, cos, sin, interleaved=interleaved)[0], wl, dy)
+        assert torch.isfinite(dw[others]).all() and not torch.isfinite(dw[12])
+    x = q.clone()
+    x[..., 12] = float("inf")                                         # a norm of 1 / infinity: the head's other channels are 0
+    y = kernels.qk_norm_rotate(x, None, None, None, cos, sin, interleaved=True)[0]
+    assert (y[..., others] == 0).all()
