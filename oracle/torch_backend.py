@@ -146,10 +146,9 @@ def diff_attention(q, k, v, lam, init, weight, eps, mask, kv_lengths, causal, st
         first = start.long()[:, None, None] if isinstance(start, torch.Tensor) else start
         seen &= torch.arange(M) <= first + torch.arange(N)[:, None]
     share = torch.arange(H) // (H // Hk)
-    kh, vh = k.float()[:, :, share], v.float()[:, :, share].transpose(1, 2)
-    used = seen.any(1)[:, None, :, None]
-    vh = torch.where(used, vh, 0.0)
-    score = torch.where(seen[:, None, None], torch.einsum("bnhtd,bmhtd->bhtnm", q.float(), kh) * scale, -torch.inf)
+    used, asks = seen.any(1)[:, :, None, None], seen.any(2)[:, :, None, None, None]      # the others may hold anything
+    kh, vh = torch.where(used[..., None], k.float(), 0.0)[:, :, share], torch.where(used, v.float(), 0.0)[:, :, share].transpose(1, 2)
+    score = torch.where(seen[:, None, None], torch.einsum("bnhtd,bmhtd->bhtnm", torch.where(asks, q.float(), 0.0), kh) * scale, -torch.inf)
     top = score.detach().amax(-1, keepdim=True)
     p = torch.exp(score - torch.where(torch.isinf(top), 0.0, top))
     total = p.sum(-1, keepdim=True)
@@ -160,7 +159,7 @@ def diff_attention(q, k, v, lam, init, weight, eps, mask, kv_lengths, causal, st
     if weight is not None:
         empty = ~seen.any(2)[:, :, None, None]                        # (eps may be 0)
         u = (1 - init) * u / torch.sqrt(torch.where(empty, 1.0, (u ** 2).mean(-1, keepdim=True) + eps)) * weight.float()
-    return u.to(q.dtype)
+    return torch.where(seen.any(2)[:, :, None, None], u, 0.0).to(q.dtype)
 
 
 def install():

@@ -25,3 +25,24 @@ def test_oracle_rows_that_see_nothing_without_epsilon(oracle_backend, eps):
     assert ref.rel(y[~none], want[~none]) < 512 * 2 ** -24
     for t in torch.autograd.grad(y.sum(), args):
         assert torch.isfinite(t).all()
+
+
+def test_oracle_what_is_hidden_may_hold_anything(oracle_backend):
+    """Keys that no query sees and queries that see no key: no value, no gradient."""
+    mask = torch.rand(5, 7, generator=torch.Generator().manual_seed(3)) < 0.3
+    mask[2] = mask[:, 4] = True
+    lens = torch.tensor([6, 5])
+    dy = torch.randn(2, 5, 4, 32, generator=torch.Generator().manual_seed(4))
+
+    def run(args, dy):
+        args = [t.detach().clone().requires_grad_(True) for t in args]
+        y = kernels.diff_attention(*args[:4], 0.3, args[4], attn_mask=mask, kv_lengths=lens)
+        return (y.detach(),) + torch.autograd.grad(y, args, dy)
+
+    args = _heads()
+    clean = run(args, dy)
+    for t, what in ((args[1], float("nan")), (args[2], float("inf"))):
+        t[0, 6:] = t[1, 5:] = t[:, 4] = what
+    args[0][:, 2] = dy[:, 2] = float("nan")
+    for a, b in zip(clean, run(args, dy)):
+        assert torch.equal(a, b)
