@@ -122,7 +122,9 @@ def qk_norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps, interleav
             y = y * w.float()
         if cos is not None:
             rows = torch.arange(x.shape[1]) if positions is None else positions.long()
-            c, s = cos[rows].unsqueeze(-2), sin[rows].unsqueeze(-2)
+            inside = ((rows >= 0) & (rows < len(cos))).unsqueeze(-1)      # outside the table: not a number
+            rows = rows.clamp(0, len(cos) - 1)
+            c, s = (torch.where(inside, t[rows], torch.nan).unsqueeze(-2) for t in (cos, sin))
             r = 2 * cos.shape[1]
             first, second = (slice(0, r, 2), slice(1, r, 2)) if interleaved else (slice(0, r // 2), slice(r // 2, r))
             out = y.clone()

@@ -46,3 +46,15 @@ def test_oracle_what_is_hidden_may_hold_anything(oracle_backend):
     args[0][:, 2] = dy[:, 2] = float("nan")
     for a, b in zip(clean, run(args, dy)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_oracle_position_outside_the_table_is_nan_there_only(oracle_backend, interleaved):
+    g = torch.Generator().manual_seed(1)
+    q, angle = torch.randn(1, 6, 2, 32, generator=g), torch.rand(8, 8, generator=g)
+    p = torch.tensor([0, 7, 8, -1, 3, 2 ** 40])
+    y, _ = kernels.qk_norm_rotate(q, None, None, None, angle.cos(), angle.sin(), p, interleaved=interleaved)
+    bad = torch.tensor([False, False, True, True, False, True])
+    assert torch.isnan(y[0, bad][..., :16]).all() and torch.isfinite(y[0, ~bad]).all() and torch.isfinite(y[0, bad][..., 16:]).all()
+    z, _ = kernels.qk_norm_rotate(q[:, ~bad], None, None, None, angle.cos(), angle.sin(), p[~bad], interleaved=interleaved)
+    assert torch.equal(y[:, ~bad], z)
