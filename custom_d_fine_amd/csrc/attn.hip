@@ -54,6 +54,8 @@ __device__ __forceinline__ a_bf16x8 tr_frag(const uint16_t *p, int pitch) {
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_bf16x2(a, b); }
+// four of them as an operand of the second product
+__device__ __forceinline__ a_bf16x8 frag_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(a_bf16x8, mfma_operand(make_uint4(a, b, c, d))); }
 
 __device__ __forceinline__ float xor_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16));
@@ -208,7 +210,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(const uint16_t *
                 for (int r = 0; r < 4; ++r) oacc[t][d][r] *= alpha;
 #pragma unroll
             for (int ks = 0; ks < kKB / 32; ++ks) {
-                const a_bf16x8 pf = __builtin_bit_cast(a_bf16x8, make_uint4(pk[2 * ks][0], pk[2 * ks][1], pk[2 * ks + 1][0], pk[2 * ks + 1][1]));
+                const a_bf16x8 pf = frag_of(pk[2 * ks][0], pk[2 * ks][1], pk[2 * ks + 1][0], pk[2 * ks + 1][1]);
 #pragma unroll
                 for (int d = 0; d < 2 * DS; ++d)
                     oacc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(tr_frag(sV + ks * 32 * PT + tr_off + 16 * d, PT), pf,
@@ -337,7 +339,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_dq_kernel(const uint16_
             }
 #pragma unroll
             for (int ks = 0; ks < kKB / 32; ++ks) {
-                const a_bf16x8 pf = __builtin_bit_cast(a_bf16x8, make_uint4(pk[2 * ks][0], pk[2 * ks][1], pk[2 * ks + 1][0], pk[2 * ks + 1][1]));
+                const a_bf16x8 pf = frag_of(pk[2 * ks][0], pk[2 * ks][1], pk[2 * ks + 1][0], pk[2 * ks + 1][1]);
 #pragma unroll
                 for (int d = 0; d < 2 * DS; ++d)
                     dacc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(tr_frag(sK + ks * 32 * PT + tr_off + 16 * d, PT), pf,
@@ -517,16 +519,20 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_dkdv_kernel(const uint16_t *
                 else { pp2[kt][0] = pack2(p[0], p[1]); pp2[kt][1] = pack2(p[2], p[3]); dsp2[kt][0] = pack2(ds[0], ds[1]); dsp2[kt][1] = pack2(ds[2], ds[3]); }
             }
         }
+        a_bf16x8 pb[KT], db[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            pb[kt] = frag_of(pp[kt][0], pp[kt][1], pp2[kt][0], pp2[kt][1]);
+            db[kt] = frag_of(dsp[kt][0], dsp[kt][1], dsp2[kt][0], dsp2[kt][1]);
+        }
 #pragma unroll
         for (int d = 0; d < 2 * DS; ++d) {
             const a_bf16x8 dot = tr_frag(tdo + tr_off + 16 * d, PT);         // dO^T[d][q slots of g]
             const a_bf16x8 qtf = tr_frag(tq + tr_off + 16 * d, PT);          // Q^T
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                const a_bf16x8 pb = __builtin_bit_cast(a_bf16x8, make_uint4(pp[kt][0], pp[kt][1], pp2[kt][0], pp2[kt][1]));
-                const a_bf16x8 db = __builtin_bit_cast(a_bf16x8, make_uint4(dsp[kt][0], dsp[kt][1], dsp2[kt][0], dsp2[kt][1]));
-                dva[d][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dot, pb, dva[d][kt], 0, 0, 0);
-                dka[d][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qtf, db, dka[d][kt], 0, 0, 0);
+                dva[d][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dot, pb[kt], dva[d][kt], 0, 0, 0);
+                dka[d][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qtf, db[kt], dka[d][kt], 0, 0, 0);
             }
         }
         if (more) stage_store(buf ^ 1);

@@ -44,6 +44,20 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
     return r;
 }
+// Registers that pack_bf16x2 filled, as a matrix instruction's operand: a matrix instruction may read a register two wait states after a vector
+// instruction wrote it at the earliest, and behind inline assembly the compiler does not count them.
+typedef __attribute__((ext_vector_type(4))) uint32_t mfma_u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t mfma_u32x2;
+__device__ __forceinline__ uint4 mfma_operand(uint4 v) {
+    mfma_u32x4 r = __builtin_bit_cast(mfma_u32x4, v);
+    asm("s_nop 1" : "+v"(r));
+    return __builtin_bit_cast(uint4, r);
+}
+__device__ __forceinline__ uint2 mfma_operand(uint2 v) {
+    mfma_u32x2 r = __builtin_bit_cast(mfma_u32x2, v);
+    asm("s_nop 1" : "+v"(r));
+    return __builtin_bit_cast(uint2, r);
+}
 __device__ __forceinline__ uint16_t f32_to_bf16(float f) { return (uint16_t)(pack_bf16x2(f, f) & 0xffffu); }
 
 struct f32x4 { float x, y, z, w; };

@@ -242,8 +242,8 @@ __global__ __launch_bounds__(kStemThreads) void stem_mfma_s1_kernel(const uint16
                 const int ci = cig * 8 + j;
                 wv[j] = (qv && co < COUT && ci < CIN) ? wp[((ci * KS + ky) * KS + kx) * COUT + co] : 0.f;
             }
-            wreg[ks][nt] = make_uint4(pack_bf16x2(wv[0], wv[1]), pack_bf16x2(wv[2], wv[3]), pack_bf16x2(wv[4], wv[5]),
-                                      pack_bf16x2(wv[6], wv[7]));
+            wreg[ks][nt] = mfma_operand(make_uint4(pack_bf16x2(wv[0], wv[1]), pack_bf16x2(wv[2], wv[3]), pack_bf16x2(wv[4], wv[5]),
+                                                   pack_bf16x2(wv[6], wv[7])));
         }
     }
     uint4 pf[NPF][8];

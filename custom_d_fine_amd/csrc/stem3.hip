@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kS3Threads) void stem3_fwd_rows_kernel(const S3FwdA
                     const float w0 = a.wp[(ci * 9 + t) * COUT + coc], w1 = a.wp[((ci + 1) * 9 + t) * COUT + coc];
                     p[e] = cok ? pack_bf16x2(w0, w1) : 0u;
                 }
-                aw[t][s][nt] = make_uint4(p[0], p[1], p[2], p[3]);
+                aw[t][s][nt] = mfma_operand(make_uint4(p[0], p[1], p[2], p[3]));
             }
 #pragma unroll
             for (int s = 0; s < K16; ++s) {
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kS3Threads) void stem3_fwd_rows_kernel(const S3FwdA
                     const float w0 = a.wp[(ci * 9 + t) * COUT + coc], w1 = a.wp[((ci + 1) * 9 + t) * COUT + coc];
                     p[e] = cok ? pack_bf16x2(w0, w1) : 0u;
                 }
-                at[t][s][nt] = make_uint2(p[0], p[1]);
+                at[t][s][nt] = mfma_operand(make_uint2(p[0], p[1]));
             }
         }
 
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(kS3Threads) void stem3_bwd_rows_kernel(const S3BwdA
                 const float w0 = a.wq[(c0c * 9 + t) * CIN + ci], w1 = a.wq[(c1c * 9 + t) * CIN + ci];
                 p[e] = pack_bf16x2(co < COUT ? w0 : 0.f, co + 1 < COUT ? w1 : 0.f);
             }
-            aw[t][nt] = make_uint4(p[0], p[1], p[2], p[3]);
+            aw[t][nt] = mfma_operand(make_uint4(p[0], p[1], p[2], p[3]));
         }
 
     // ---- staging of dy rows: task = (channel group of 8, 8-pixel chunk); dy row j lives in slot j & 3 -----------------------------
