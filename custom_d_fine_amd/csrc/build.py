@@ -48,6 +48,7 @@ def needs_build():
     t = os.path.getmtime(LIB)
     deps = [os.path.join(HERE, f) for f in os.listdir(HERE) if f.endswith((".hip", ".cpp", ".h"))]
     deps.append(os.path.join(HERE, "..", "..", "include", "dfine_hip.h"))
+    deps.append(os.path.join(HERE, "build.py"))          # the flags
     return any(os.path.getmtime(d) > t for d in deps)
 
 
