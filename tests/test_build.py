@@ -17,3 +17,12 @@ def test_library_is_out_of_date(tmp_path, monkeypatch, newer):
     assert not build.needs_build()
     times[newer] = 3
     assert build.needs_build()
+
+
+def test_the_build_entry_compiles_each_time(monkeypatch):
+    import __graft_entry__ as entry
+    asked = []
+    monkeypatch.setattr(build, "build", lambda force=False, verbose=True: asked.append(force) or build.LIB)
+    monkeypatch.setattr(entry.subprocess, "check_call", lambda *a, **k: 0)
+    entry.build()
+    assert asked == [True]
