@@ -561,8 +561,9 @@ __device__ __forceinline__ float da_lse(float m, float l) { return l > 0.f ? m +
 // in front is worked on (one barrier per block).
 // 128 rows read a key once from L2 for 4 waves; two waves per SIMD (registers: DK = 64) hide each other's LDS and matrix latencies.  Bound: the vector unit for
 // heads up to 32 channels (16 exponentials, maxima, sums and conversions per 12 products of 32 cycles), vector and matrix unit about alike at 64.
-// Measured: 8192 causal tokens, 16 heads on 4, 2 x 64 channels bf16 494 - 520 us (790 - 830 TFLOP/s; a plain 8192^3 product reaches 1177 here); 32 x 492 tokens with their group
-// mask, 4 heads of 2 x 32, results for the backward kept, 32 us; 8 x 900 tokens, 8 heads of 2 x 24, 51 us; 16 x 396 tokens of 4 heads in fp32 64 us.
+// Measured (kernel alone under the tracer, several cards): 8192 causal tokens, 16 heads on 4, 2 x 64 channels bf16 470 - 520 us (790 - 880 TFLOP/s; a plain 8192^3 product
+// reaches 1177 here); 32 x 492 tokens with their group mask, 4 heads of 2 x 32, results for the backward kept, 30 - 33 us; 8 x 900 tokens, 8 heads of 2 x 24, 46 - 51 us;
+// 16 x 396 tokens of 4 heads in fp32, results kept, 60 - 64 us.
 template <typename T, int DK>
 __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) void diff_attn_fwd_kernel(const DiffArgs a) {
     using C = DaCfg<T, DK>;
@@ -752,8 +753,9 @@ __device__ __forceinline__ void da_finish_row(const DiffArgs &a, int b, int i, i
 // forward, few rows: workgroup = (batch, key head, 32 rows, one of nsplit runs of the keys), its waves take every fourth tile of 32 keys of the run, each
 // through two LDS buffers of its own (no barrier until the end).  The waves' sums meet in LDS; with one run the rows are finished here, else the run's sums
 // go to `part` (rows x nsplit x 2 DV, with maxima and sums in `ml`) for diff_attn_join_kernel.
-// Bound: HBM, every key and value once for all heads of the group.  Measured: one token of 16 heads over 16 caches of up to 32768 keys (835 MB) 165 us, 5.1 TB/s;
-// 17 tokens over 4 x 10001 keys 22 us (41 MB: 11 us of it are the first loads, the joins in LDS and the last stores); 300 tokens of one image 10.6 us.
+// Bound: HBM, every key and value once for all heads of the group.  Measured: one token of 16 heads over 16 caches of up to 32768 keys (835 MB) 161 - 165 us, 5.1 - 5.2 TB/s,
+// in fp32 (1670 MB) 507 - 520 us: one buffer per wave there, so a wave's copies (340 us at a large copy's rate) and fp32 products (260 us) follow each other;
+// 17 tokens over 4 x 10001 keys 21 - 23 us (41 MB: 11 us of it are the first loads, the joins in LDS and the last stores); 300 tokens of one image 10.2 - 10.6 us.
 template <typename T, int DK>
 __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff_attn_fwd_split_kernel(const DiffArgs a, int nsplit, float *__restrict__ part, float4 *__restrict__ ml) {
     using C = DaCfg<T, DK>;
@@ -918,7 +920,7 @@ __global__ __launch_bounds__(kDaThreads, DK * sizeof(T) <= 64 ? 2 : 1) void diff
 }
 
 // joins the runs of a row: a wave per row, 8 lanes x DV / 8 channels, 8 runs side by side, in a fixed order.  Bound: latency (a launch, one round of loads, the
-// reduction); 9 - 10 us for the two cases above.
+// reduction); 9 - 10 us for the two bf16 cases above.
 template <typename T, int DV>
 __global__ __launch_bounds__(kDaThreads) void diff_attn_join_kernel(const DiffArgs a, int nsplit, const float *__restrict__ part, const float4 *__restrict__ ml) {
     constexpr int NE = DV / 8;
@@ -1029,7 +1031,7 @@ __global__ __launch_bounds__(256) void diff_attn_mask_kernel(const uint8_t *__re
 // pass therefore keeps W = A_1 V - beta U, beta = (A_1 V . U) / (U . U), and D_1 = r (t . W) + beta (dU . U), D_0 = dU . U + l D_1 (long rows, bf16: error of dl
 // and dq against 64 bits 0.0046 with A_1 V itself), and U in 32 bits: dU . U is small for the same reason (with U in bf16 dq was 0.0042 off instead of 0.0030).
 // dP is made from the ROUNDED dU: what the rounding adds to D is added here too.
-// Bound: HBM (dY, U, W read, dU written: 41 MB and 15 us at 32 x 492 tokens of 4 heads, 168 MB and 35 us at 8192 of 16; two rounds of rows per workgroup leave
+// Bound: HBM (dY, U, W read, dU written: 41 MB and 14 - 15 us at 32 x 492 tokens of 4 heads, 168 MB and 34 - 35 us at 8192 of 16; two rounds of rows per workgroup leave
 // latency in the small case; loading a row ahead of its use changed nothing, 14.0 and 34 us).
 // The other kernels read the rows' statistics with l worked in - exp2(c s - (lse_1 - log2 |l|)) is |l| A_1, and its sign goes with D_1 and dP - and as the
 // numbers that dK's and dV's products start from: S_t at -lse_t / c, dP at -D_0.
@@ -1176,7 +1178,7 @@ __global__ __launch_bounds__(1024) void diff_attn_param_kernel(const DiffArgs a,
 // backward, dQ: the forward's decomposition and copies; probabilities from the saved statistics, nothing to rescale.  dS is rounded to bf16 for its product with K (as the keys it meets
 // are), dU for its product with V: each adds 0.0017 to dq's relative error, 0.0030 in all with the result's own 0.0017.  Keeping either in two bf16 terms would
 // cost a third more products for 0.0025.
-// Bound as the forward: 473 - 495 us (835 - 870 TFLOP/s) at 8192 causal tokens, 27 us at 32 x 492, 58 us in fp32 at 16 x 396.
+// Bound as the forward: 453 - 495 us (830 - 910 TFLOP/s) at 8192 causal tokens, 25 - 27 us at 32 x 492, 56 - 59 us in fp32 at 16 x 396.
 template <typename T, int DK>
 __device__ __forceinline__ void da_dq_tile(const DiffArgs &a, da_f16v (*dq)[DaCfg<T, DK>::MTK], const uint4 (*qf)[DaCfg<T, DK>::NF], const uint4 *uf, const float *lse, const float *dl,
                                            float sign, const DaLane<T, DK> &ln, uint32_t tk, uint32_t tv, bool masked, uint32_t vis, int lane) {
@@ -1351,7 +1353,7 @@ __global__ __launch_bounds__(kDaThreads, DK == 16 || sizeof(T) == 2 ? 2 : 1) voi
 // queries of the group's heads stream through two LDS buffers of QB rows (Q | dU | four statistics), copied while the block in front is worked on.
 // The rows' statistics are what the products start from (S at -lse / c, dP at -D_0): they come from LDS straight into the accumulators.
 // Both operands and both results of 64-channel heads are 192 registers of 323, one wave per SIMD: vector and matrix work of a tile follow each other, which bounds it.
-// Measured: 844 - 900 us at 8192 causal tokens (610 - 650 TFLOP/s), 37 us at 32 x 492, 77 us in fp32 at 16 x 396.  Two waves for the same 32 keys, one map each (two waves per
+// Measured: 765 - 900 us at 8192 causal tokens (610 - 720 TFLOP/s), 34 - 37 us at 32 x 492, 73 - 77 us in fp32 at 16 x 396.  Two waves for the same 32 keys, one map each (two waves per
 // SIMD, dP worked out twice), took 942 us where this took 901; both mask forms of a tile as code of their own 1140 (the accumulators change places between them).
 template <typename T, int DK>
 __device__ __forceinline__ void da_dkdv_tile(const DiffArgs &a, da_f16v (*dk)[DaCfg<T, DK>::MTK], da_f16v *dv, const uint4 (*kf)[DaCfg<T, DK>::NF], const uint4 *vf, float sign,
@@ -1732,8 +1734,11 @@ static int diff_attn_size(int d, int dv) { return d <= 16 && dv <= 32 ? 16 : d <
 
 // Runs of the keys a forward pass is cut into: 0 = the kernel for many rows (128 rows per workgroup, all keys), n >= 1 = the kernel for few (32 rows per
 // workgroup, n runs).
-// kDaManyRows: many rows are those that make 256 workgroups (one per CU).  At 256 of them (16 x 396 tokens of 4 heads, fp32) the kernel for many takes 69 us and
-// the one for few 92, at 512 (32 x 492, bf16) 35 and 56; at 12 (300 tokens of one image) 20 and 16.
+// kDaManyRows: many rows are those that make 256 workgroups (one per CU).  us of the kernel for many and the one for few, forward without results for the backward,
+// 4 heads, at 64 / 128 / 160 / 192 / 224 / 256 / 512 workgroups of 128 rows: 492 tokens of 2 x 32 bf16 19 and 11 / 20 and 14 / 20 and 21 / 20 and 21 / 20 and 24 / 20 and
+// 24 / 27 and 45; 512 tokens of 2 x 64 bf16 24 and 15 / 24 and 28 / 24 and 40 / 24 and 40 / 25 and 52 / 25 and 53 / 41 and 111; 396 tokens of 2 x 32 fp32 54 and 24 / 55
+// and 46 / 54 and 67 / 55 and 68 / 55 and 68 / 55 and 89 / 94 and 161.  The choice holds from 256 on and up to 64; from about 150 on (wide heads: from
+// fewer than 128) the kernel for many is the faster already.
 // kDaSplitWgs: the runs fill the chip once, 256 workgroups.  One token over 16 caches of 32768 keys (4 key heads): 170 / 177 / 184 / 212 us with 256 / 512 / 1024 /
 // 2048 workgroups; 17 tokens over 4 x 10001 keys 36 / 46 / 66 us with 256 / 512 / 1024: every run costs a prologue, its sums and a share of the join.
 // kDaRunKeys: a run has 256 keys at least (two tiles for each of its four waves): one token of 16 heads over 4096 keys, runs + join, 19.4 / 19.5 / 21.5 / 26.8 / 35.9 us
@@ -1811,7 +1816,7 @@ static int diff_attn_runs(const DiffArgs &a) {
 }
 
 // Runs of the rows that dK and dV are summed in, about 512 workgroups in all, each with four blocks of queries at least.  Measured, kernel + sum kernel in us:
-// 8192 causal tokens of 4 key heads, bf16 (256 workgroups of very unequal work) 1543 with one run, 898 + 14 with 2, 905 + 23 with 4, 945 + 54 with 8;
+// 8192 causal tokens of 4 key heads, bf16 (256 workgroups of very unequal work) 1543 with one run, 898 + 14 with 2, 905 + 23 with 4, 945 + 54 with 8 (one card);
 // 32 x 492 tokens of 4 heads (512 workgroups) 37 with one, 45 + 13 with 2; 16 x 396 tokens of 4 heads in fp32 (256 workgroups, 7 blocks of queries) 77 with
 // one, 89 + 8 with 2, 105 + 12 with 4.
 static int diff_attn_kvruns(const DiffArgs &a) {

@@ -10,8 +10,9 @@
 // next to each other (a power of two of them), and a wave walks through the heads of its tokens with the table row and the weights in registers, so the
 // table - 4 bytes per channel against 2 of data - is read once per token and not once per head.  The partner of a pair comes from its lane as raw
 // storage (a shuffle of 16 bytes) and is normed again here: cheaper than exchanging the 32-bit results.
-// Measured: 4 x 8192 tokens of 32 + 8 heads of 128 channels, bf16, forward 163 us (671 MB, 4.1 TB/s; a large copy reaches 4.9), backward 200 us (1007 MB, 5.0 TB/s)
-// and 5 us for the weights' sums; 32 x 492 tokens of 8 + 8 heads of 32 channels 14, 19 and 4 us (32 MB, 48 MB); one token each of 16 sequences 4.6 us (a launch).
+// Measured: 4 x 8192 tokens of 32 + 8 heads of 128 channels, bf16, forward 145 - 165 us (671 MB, 4.1 - 4.6 TB/s; a large copy reaches 4.9), backward 199 - 202 us (1007 MB,
+// 5.0 TB/s) and 5 us for the weights' sums; 32 x 492 tokens of 8 + 8 heads of 32 channels 13 - 16, 17 - 18 and 4 us (32 MB, 48 MB); 16 x 900 tokens of 16 + 16 heads of 24
+// channels in fp32 20 - 22, 29 and 4 us (88 MB, 133 MB); one token each of 16 sequences 4.5 us (a launch).
 // All arithmetic is in 32 bits; the one rounding is the store.  The weight gradients leave as one partial row per workgroup, added up in order.
 #include "common.h"
 
