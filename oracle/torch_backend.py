@@ -151,7 +151,7 @@ def diff_attention(q, k, v, lam, init, weight, eps, mask, kv_lengths, causal, st
     used, asks = seen.any(1)[:, :, None, None], seen.any(2)[:, :, None, None, None]      # the others may hold anything
     kh, vh = torch.where(used[..., None], k.float(), 0.0)[:, :, share], torch.where(used, v.float(), 0.0)[:, :, share].transpose(1, 2)
     score = torch.where(seen[:, None, None], torch.einsum("bnhtd,bmhtd->bhtnm", torch.where(asks, q.float(), 0.0), kh) * scale, -torch.inf)
-    top = score.detach().amax(-1, keepdim=True)
+    top = score.detach().amax(-1, keepdim=True) if M else torch.full_like(score.detach().sum(-1, keepdim=True), -torch.inf)
     p = torch.exp(score - torch.where(torch.isinf(top), 0.0, top))
     total = p.sum(-1, keepdim=True)
     a = p / torch.where(total == 0, 1.0, total)

@@ -58,3 +58,12 @@ def test_oracle_position_outside_the_table_is_nan_there_only(oracle_backend, int
     assert torch.isnan(y[0, bad][..., :16]).all() and torch.isfinite(y[0, ~bad]).all() and torch.isfinite(y[0, bad][..., 16:]).all()
     z, _ = kernels.qk_norm_rotate(q[:, ~bad], None, None, None, angle.cos(), angle.sin(), p[~bad], interleaved=interleaved)
     assert torch.equal(y[:, ~bad], z)
+
+
+@pytest.mark.parametrize("N,M", [(5, 0), (0, 7)])
+def test_oracle_without_keys_or_queries(oracle_backend, N, M):
+    args = [torch.randn(*s, requires_grad=True) for s in ((2, N, 4, 2, 16), (2, M, 2, 2, 16), (2, M, 2, 32), (4, 16), (32,))]
+    y = kernels.diff_attention(*args[:4], 0.3, args[4])
+    assert y.shape == (2, N, 4, 32) and (y == 0).all()
+    for t in torch.autograd.grad(y.sum(), args):
+        assert (t == 0).all()
